@@ -56,7 +56,10 @@ typedef enum {
     NXQ_ERR_NCCL = -8,        /* NCCL unavailable or a collective failed       */
     NXQ_ERR_UNSUPPORTED = -9, /* no GPU of the required architecture           */
     NXQ_ERR_FORMAT = -10,     /* a GGUF / NXF file that is malformed or truncated */
-    NXQ_ERR_RANGE = -11       /* an activation outside the f16 range (see below) */
+    NXQ_ERR_RANGE = -11,      /* an activation outside the f16 range (see below) */
+    NXQ_ERR_INDEX = -12       /* an index in device memory outside its range: a token
+                               * id, an expert offset, a row or slot index (reported by
+                               * nxq_stream_sync; that access was skipped) */
 } nxq_status;
 
 /* Numeric range of the tensor-core kernels.  The decode GEMV and the prefill
@@ -268,6 +271,89 @@ NXQ_API int nxq_qmatmul_residual(nxq_weight_t w, const void* x_dev, int x_dtype,
 NXQ_API int nxq_rmsnorm_qmatmul(const nxq_weight_t* w, int count, const void* x_dev, int x_dtype,
                                 const float* norm_dev, float eps, void* const* y_dev, int y_dtype,
                                 int64_t M, void* stream);
+
+/* ---- embedding lookup --------------------------------------------------------- */
+
+/* y_dev[t][0..K) = scale * decode(row ids_dev[t]) for t < T: the token
+ * embedding from a registered table [N][K] of any block type (the engine
+ * decodes the whole table to fp32 at load time and copies rows of it).  The
+ * decode is exact (as nxq_dequant), the product is formed in fp32 and rounded
+ * once to y_dtype.  ids_type: NXQ_I32 or NXQ_I64.  An id outside [0, N) gives
+ * a row of zeros and NXQ_ERR_INDEX at the next nxq_stream_sync.  y_dev must be
+ * 16-byte aligned; T = 0 does nothing.  Allocates nothing; may be captured. */
+typedef enum { NXQ_I32 = 0, NXQ_I64 = 1 } nxq_index_type;
+NXQ_API int nxq_embedding(nxq_weight_t table, const void* ids_dev, int ids_type, int64_t T, float scale, void* y_dev,
+                          int y_dtype, void* stream);
+
+/* ---- mixture of experts -------------------------------------------------------
+ * The feed-forward block of a mixture-of-experts layer with every decision on
+ * the device, so a step needs no host round trip and can be captured into a
+ * CUDA graph (the reference routes on the host, MoERouter::route,
+ * moe_router.h:47, and hands the active experts to batched_moe_ffn,
+ * compute_dispatch.cpp:211-275):
+ *   nxq_moe_route           logits -> experts of every token, sorted by expert
+ *   nxq_qmatmul_ragged_swiglu  gate and up projections of the sorted rows
+ *   nxq_qmatmul_ragged      down projection
+ *   nxq_moe_combine         weighted sum per token, plus the residual
+ * A "slot" is one (token, expert) pair in sorted order.  Calls of one stream
+ * run in order; calls on different streams share nothing and may overlap.
+ * Their workspaces are stream-ordered allocations (cudaMallocAsync) of each
+ * call, so a captured call owns its own inside the graph. */
+
+/* Experts of one projection: `count` (1 .. 1024) registered weights of one
+ * block type and shape, expert e = w[e] (a weight may appear more than once).
+ * The table holds references: nxq_weight_release refuses (NXQ_ERR_STATE) a
+ * weight that a live table uses.  nxq_experts_release waits for the device. */
+typedef struct nxq_experts_s* nxq_experts_t;
+NXQ_API int nxq_experts_create(const nxq_weight_t* w, int count, nxq_experts_t* out);
+NXQ_API int nxq_experts_release(nxq_experts_t e);
+NXQ_API int nxq_experts_info(nxq_experts_t e, int* count, int* type, int64_t* N, int64_t* K);
+
+/* Top-k routing of logits_dev [T][E] (row-major; 1 <= E <= 1024, 1 <= k <=
+ * min(E, 32), T * k < 2^31).  Token t takes the k experts of its largest
+ * logits, in descending order, ties to the lowest index; an expert whose
+ * logit is -inf or NaN is never taken, so a token may take fewer than k, or
+ * none (a padded row).
+ *   ids_dev     [T][k] int32   the experts; -1 for choices not taken
+ *   weights_dev [T][k] fp32    exp(l - max) / sum, the sum over the taken
+ *                              experts (normalize != 0) or over all E (0); 0
+ *                              for choices not taken.  Logits of +inf share
+ *                              the weight equally.
+ *   offsets_dev [E + 1] int32  slots offsets[e] .. offsets[e + 1] - 1 belong to
+ *                              expert e, ordered by token
+ *   rows_dev    [T * k] int32  the token of each slot; -1 from offsets[E] on
+ *   slots_dev   [T][k] int32   the slot of each choice; -1 if not taken
+ * T = 0 writes the offsets (zeros). */
+NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, int k, int normalize, int32_t* ids_dev,
+                          float* weights_dev, int32_t* offsets_dev, int32_t* rows_dev, int32_t* slots_dev,
+                          void* stream);
+
+/* Products grouped by expert with ragged sizes that are known on the device
+ * only: for every expert e and offsets_dev[e] <= s < offsets_dev[e + 1],
+ *   y_dev[s][0..N) = x_dev[rows_dev ? rows_dev[s] : s][0..K) * W_e^T,
+ * fp32 accumulation.  offsets_dev: E + 1 ascending int32 values in [0, R]; y_dev
+ * has R rows (rows before offsets[0] and from offsets[E] on are left as they
+ * were), x_dev has X rows (without rows_dev, slot s reads row s and X must be
+ * at least R).  Offsets outside [0, R] or descending, and row indices outside
+ * [0, X), are skipped (rows of a bad index give zeros) and reported as
+ * NXQ_ERR_INDEX.  Weight and activation rounding as in nxq_qmatmul.
+ * The _swiglu form takes gate and up tables of the same count, type and shape:
+ *   h_dev[s] = silu(x Wg_e^T) * (x Wu_e^T), silu(g) = g / (1 + exp(-g)).
+ * R < 2^31. */
+NXQ_API int nxq_qmatmul_ragged(nxq_experts_t e, const void* x_dev, int x_dtype, int64_t X, const int32_t* rows_dev,
+                               void* y_dev, int y_dtype, int64_t R, const int32_t* offsets_dev, void* stream);
+NXQ_API int nxq_qmatmul_ragged_swiglu(nxq_experts_t gate, nxq_experts_t up, const void* x_dev, int x_dtype, int64_t X,
+                                      const int32_t* rows_dev, void* h_dev, int h_dtype, int64_t R,
+                                      const int32_t* offsets_dev, void* stream);
+
+/* y_dev[t][n] = sum_j weights_dev[t][j] * h_dev[slots_dev[t][j]][n] (+ res_dev
+ * [t][n] if given, fp32), for t < T, n < N; j in ascending order, fp32.  Negative
+ * slots are skipped whatever their weight (a token without experts gives its
+ * residual, or zeros); a slot >= R is skipped and reported as NXQ_ERR_INDEX.
+ * y_dev may be res_dev when y_dtype is NXQ_F32.  1 <= k <= 32. */
+NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N, const int32_t* slots_dev,
+                            const float* weights_dev, int64_t T, int k, const float* res_dev, void* y_dev,
+                            int y_dtype, void* stream);
 
 /* Host-buffer form, synchronous: the drop-in for ComputeDispatch::gemm_int4
  * (compute_dispatch.h:59-61, .cpp:142-176) - fp32 activations [M][K] in, fp32

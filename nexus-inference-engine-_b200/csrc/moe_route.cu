@@ -1,0 +1,443 @@
+// Top-k routing of a mixture of experts, and the weighted sum of its outputs
+// (nxq_moe_route, nxq_moe_combine).  The reference routes on the host, token
+// by token (MoERouter::route, moe_router.h:47); here the choices, their
+// weights and their order by expert stay on the device.
+//
+// Routing has three steps.  (1) One warp per token: lane l holds the logits of
+// experts l, l + 32, ... as order-preserving integer keys; k rounds of a warp
+// maximum (redux on the key, then on the index among equals, so ties go to
+// the lowest index) pick the choices.  (2) An exclusive scan, over blocks of
+// tokens, of each expert's count.  (3) Every block ranks its own choices: a warp
+// walks a contiguous run of choices in order, equal experts among 32 lanes
+// ranked by their lane (match), so slots are ordered by (expert, token) and do
+// not depend on timing - the counts are integers and no atomic decides a place.
+// Up to kSmallT tokens one CTA does all three.
+#include "nxq_internal.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace nxq {
+
+namespace {
+
+constexpr int kMaxE = 1024, kMaxK = 32;
+constexpr int kRankWarps = 8;        // contiguous runs a block's choices are ranked in
+constexpr int kThreads = 32 * kRankWarps;
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallT = 128;
+constexpr float kInf = __builtin_huge_valf();
+
+struct RouteParams {
+    const void* logits;
+    int dtype;
+    int64_t T;
+    int E, k, normalize;
+    int tb;  // tokens per block
+    int blocks;
+    int32_t* ids;
+    float* weights;
+    int32_t* offsets;
+    int32_t* rows;
+    int32_t* slots;
+    int32_t* hist;   // [blocks][E]: counts, then their exclusive scan over blocks
+    int32_t* total;  // [E]
+};
+
+__device__ __forceinline__ float load_logit(const void* p, int dt, int64_t i) {
+    if (dt == NXQ_F32) return static_cast<const float*>(p)[i];
+    if (dt == NXQ_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Larger value, larger key; -0 and +0 equal; 0 for -inf and NaN (never taken).
+__device__ __forceinline__ uint32_t key_of(float v) {
+    if (!(v > -kInf)) return 0u;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float((key >> 31) ? (key & 0x7FFFFFFFu) : ~key);
+}
+// exp(v - m), with the limit for m = +inf.
+__device__ __forceinline__ float share_of(float v, float m) { return m == kInf ? (v == kInf ? 1.0f : 0.0f) : expf(v - m); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// The choices of token t by one warp; counts them in hist (shared, [E]).
+template <int V>
+__device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int lane, int32_t* hist) {
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = e < p.E ? key_of(load_logit(p.logits, p.dtype, t * p.E + e)) : 0u;
+    }
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = key[i] > top ? key[i] : top;
+    const uint32_t first = __reduce_max_sync(0xFFFFFFFFu, top);
+    const float m = value_of(first);
+    float all = 0.0f;  // sum over every expert
+    if (!p.normalize && first) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (key[i]) all += share_of(value_of(key[i]), m);
+        all = warp_sum(all);
+    }
+    int my_id = -1;
+    float my_p = 0.0f;
+    for (int j = 0; j < p.k; ++j) {
+        const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, top);
+        if (!best) break;
+        int at = 0x7FFFFFFF;
+        if (top == best) {
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i)
+                if (key[i] == best) at = lane + 32 * i;
+        }
+        const int e = __reduce_min_sync(0xFFFFFFFFu, at);
+        if (at == e) {
+            top = 0u;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (lane + 32 * i == e) key[i] = 0u;
+                top = key[i] > top ? key[i] : top;
+            }
+        }
+        if (lane == j) {
+            my_id = e;
+            my_p = share_of(value_of(best), m);
+        }
+    }
+    const float z = p.normalize ? warp_sum(my_p) : all;
+    if (lane < p.k) {
+        p.ids[t * p.k + lane] = my_id;
+        p.weights[t * p.k + lane] = my_id >= 0 ? my_p / z : 0.0f;
+        if (my_id >= 0) atomicAdd(&hist[my_id], 1);
+    }
+}
+
+// Ranks the choices of tokens [t0, t1): warp w < kRankWarps takes the w-th run
+// of them.  start[w][e] (shared) holds, on entry, nothing; base[e] is the
+// first slot of the block's choices of expert e.
+__device__ __forceinline__ void rank_choices(const RouteParams& p, int64_t t0, int64_t t1, int32_t* start,
+                                             const int32_t* base, int threads) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t c0 = t0 * p.k, n = (t1 - t0) * p.k;
+    const int64_t per = ((n + kRankWarps - 1) / kRankWarps + 31) & ~(int64_t)31;
+    const int64_t a = c0 + (warp * per < n ? warp * per : n), z = c0 + ((warp + 1) * per < n ? (warp + 1) * per : n);
+    for (int i = tid; i < kRankWarps * p.E; i += threads) start[i] = 0;
+    __syncthreads();
+    if (warp < kRankWarps)
+        for (int64_t c = a + lane; c < z; c += 32) {
+            const int e = p.ids[c];
+            if (e >= 0) atomicAdd(&start[warp * p.E + e], 1);
+        }
+    __syncthreads();
+    for (int e = tid; e < p.E; e += threads) {
+        int at = base[e];
+#pragma unroll
+        for (int w = 0; w < kRankWarps; ++w) {
+            const int cnt = start[w * p.E + e];
+            start[w * p.E + e] = at;
+            at += cnt;
+        }
+    }
+    __syncthreads();
+    if (warp >= kRankWarps) return;
+    for (int64_t c = a; c < z; c += 32) {
+        const bool in = c + lane < z;
+        const int e = in ? p.ids[c + lane] : -1;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+        const int rank = __popc(same & ((1u << lane) - 1u));
+        int slot = -1;
+        if (e >= 0) slot = start[warp * p.E + e] + rank;
+        __syncwarp();
+        if (e >= 0 && rank == 0) start[warp * p.E + e] += __popc(same);
+        __syncwarp();
+        if (in) {
+            p.slots[c + lane] = slot;
+            if (slot >= 0) p.rows[slot] = (int32_t)((c + lane) / p.k);
+        }
+    }
+}
+
+// Exclusive scan of cnt[0 .. E) (shared) into out[0 .. E) (shared) by warp 0;
+// returns nothing, out[E] = total.
+__device__ __forceinline__ void scan_experts(const int32_t* cnt, int32_t* out, int E) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, per = (E + 31) / 32, b = lane * per;
+        int s = 0;
+        for (int i = 0; i < per; ++i)
+            if (b + i < E) s += cnt[b + i];
+        int at = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, at, o);
+            if (lane >= o) at += v;
+        }
+        if (lane == 31) out[E] = at;
+        at -= s;
+        for (int i = 0; i < per; ++i)
+            if (b + i < E) {
+                const int c = cnt[b + i];
+                out[b + i] = at;
+                at += c;
+            }
+    }
+    __syncthreads();
+}
+
+template <int V>
+__global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteParams p) {
+    extern __shared__ int32_t sm[];
+    int32_t* hist = sm;                // [E]
+    int32_t* base = hist + p.E;        // [E + 1]
+    int32_t* start = base + p.E + 1;   // [kRankWarps][E]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int e = tid; e < p.E; e += kSmallThreads) hist[e] = 0;
+    __syncthreads();
+    for (int64_t t = warp; t < p.T; t += kSmallThreads / 32) choose<V>(p, t, lane, hist);
+    __syncthreads();
+    scan_experts(hist, base, p.E);
+    for (int e = tid; e <= p.E; e += kSmallThreads) p.offsets[e] = base[e];
+    for (int64_t s = base[p.E] + tid; s < p.T * p.k; s += kSmallThreads) p.rows[s] = -1;
+    rank_choices(p, 0, p.T, start, base, kSmallThreads);
+}
+
+template <int V>
+__global__ void __launch_bounds__(kThreads) route_choose_kernel(const RouteParams p) {
+    extern __shared__ int32_t hist[];  // [E]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int e = tid; e < p.E; e += kThreads) hist[e] = 0;
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
+    for (int64_t t = t0 + warp; t < t1; t += kThreads / 32) choose<V>(p, t, lane, hist);
+    __syncthreads();
+    for (int e = tid; e < p.E; e += kThreads) p.hist[(int64_t)blockIdx.x * p.E + e] = hist[e];
+}
+
+// 32 experts per CTA, lane = expert; the 32 warps scan a run of blocks each.
+__global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
+    __shared__ int32_t part[32][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int e = blockIdx.x * 32 + lane;
+    const int per = (p.blocks + 31) / 32, b0 = warp * per, b1 = b0 + per < p.blocks ? b0 + per : p.blocks;
+    int s = 0;
+    if (e < p.E)
+        for (int b = b0; b < b1; ++b) s += p.hist[(int64_t)b * p.E + e];
+    part[warp][lane] = s;
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+        const int v = part[w][lane];
+        if (w < warp) at += v;
+        all += v;
+    }
+    if (e >= p.E) return;
+    if (warp == 0) p.total[e] = all;
+    for (int b = b0; b < b1; ++b) {
+        const int c = p.hist[(int64_t)b * p.E + e];
+        p.hist[(int64_t)b * p.E + e] = at;
+        at += c;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams p) {
+    extern __shared__ int32_t sm[];
+    int32_t* cnt = sm;
+    int32_t* base = cnt + p.E;        // [E + 1]
+    int32_t* start = base + p.E + 1;  // [kRankWarps][E]
+    const int tid = threadIdx.x;
+    for (int e = tid; e < p.E; e += kThreads) cnt[e] = p.total[e];
+    __syncthreads();
+    scan_experts(cnt, base, p.E);
+    const int64_t n = p.T * p.k;
+    if (blockIdx.x == 0)
+        for (int e = tid; e <= p.E; e += kThreads) p.offsets[e] = base[e];
+    for (int64_t s = base[p.E] + (int64_t)blockIdx.x * kThreads + tid; s < n; s += (int64_t)gridDim.x * kThreads) p.rows[s] = -1;
+    __syncthreads();
+    for (int e = tid; e < p.E; e += kThreads) base[e] += p.hist[(int64_t)blockIdx.x * p.E + e];
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
+    rank_choices(p, t0, t1, start, base, kThreads);
+}
+
+template <int V>
+cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
+    if (small)
+        route_small_kernel<V><<<1, kSmallThreads, smem, st>>>(p);
+    else
+        route_choose_kernel<V><<<(unsigned)p.blocks, kThreads, p.E * sizeof(int32_t), st>>>(p);
+    note_launches(1);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
+    const int v = (p.E + 31) / 32;
+    return v <= 1    ? launch_choose<1>(p, small, smem, st)
+           : v <= 2  ? launch_choose<2>(p, small, smem, st)
+           : v <= 4  ? launch_choose<4>(p, small, smem, st)
+           : v <= 8  ? launch_choose<8>(p, small, smem, st)
+           : v <= 16 ? launch_choose<16>(p, small, smem, st)
+                     : launch_choose<32>(p, small, smem, st);
+}
+
+// ---- combine -------------------------------------------------------------------
+
+constexpr int kCombThreads = 128;
+
+__device__ __forceinline__ float load_h(const void* p, int dt, int64_t i) { return load_logit(p, dt, i); }
+
+// Eight consecutive values of h at element i (16-byte aligned).
+__device__ __forceinline__ void load_h8(const void* p, int dt, int64_t i, float (&v)[8]) {
+    if (dt == NXQ_F32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = __ldg(q), b = __ldg(q + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return;
+    }
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (dt == NXQ_F16) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        } else {
+            v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+    }
+}
+
+__device__ __forceinline__ void store_as(void* p, int dt, int64_t i, float v) {
+    if (dt == NXQ_F32)
+        static_cast<float*>(p)[i] = v;
+    else if (dt == NXQ_F16)
+        static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// grid = T * segs CTAs (walked with a stride); a thread sums VEC consecutive
+// columns of one token.  VEC = 8 needs N % 8 == 0 and 16-byte aligned arrays.
+template <int VEC>
+__global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __restrict__ h, int h_dtype, int64_t R, int64_t N,
+                                                               const int32_t* __restrict__ slots,
+                                                               const float* __restrict__ weights, int64_t T, int k,
+                                                               const float* res, void* y, int y_dtype, int64_t segs,
+                                                               DeviceStatus* status) {
+    for (int64_t b = blockIdx.x; b < T * segs; b += gridDim.x) {
+        const int64_t t = b / segs;
+        const int64_t n = ((b - t * segs) * kCombThreads + threadIdx.x) * VEC;
+        if (n >= N) continue;
+        float acc[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+        for (int j = 0; j < k; ++j) {
+            const int s = slots[t * k + j];
+            if (s < 0) continue;
+            if (s >= R) {
+                if (n == 0) raise_index(status, kIndexSlot);
+                continue;
+            }
+            const float w = weights[t * k + j];
+            float v[VEC];
+            if constexpr (VEC == 8)
+                load_h8(h, h_dtype, (int64_t)s * N + n, v);
+            else
+                v[0] = load_h(h, h_dtype, (int64_t)s * N + n);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float r = res ? res[t * N + n + i] : 0.0f;
+            store_as(y, y_dtype, t * N + n + i, acc[i] + r);
+        }
+    }
+}
+
+}  // namespace
+
+}  // namespace nxq
+
+using namespace nxq;
+
+extern "C" {
+
+NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, int k, int normalize, int32_t* ids_dev,
+                          float* weights_dev, int32_t* offsets_dev, int32_t* rows_dev, int32_t* slots_dev,
+                          void* stream) {
+    if (E < 1 || E > kMaxE) return fail(NXQ_ERR_ARG, "route: E=%d (1 to %d experts)", E, kMaxE);
+    if (k < 1 || k > kMaxK || k > E) return fail(NXQ_ERR_ARG, "route: k=%d of %d experts (at most %d)", k, E, kMaxK);
+    if (T < 0 || T > (int64_t)0x7FFFFFFF / k) return fail(NXQ_ERR_ARG, "route: T=%lld, k=%d", (long long)T, k);
+    if (!dtype_valid(dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
+    if (!offsets_dev) return fail(NXQ_ERR_ARG, "route: null offsets");
+    if (T > 0 && (!logits_dev || !ids_dev || !weights_dev || !rows_dev || !slots_dev))
+        return fail(NXQ_ERR_ARG, "route: null array");
+    if (int rc = context_ready()) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T == 0) {
+        NXQ_CUDA(cudaMemsetAsync(offsets_dev, 0, (size_t)(E + 1) * sizeof(int32_t), st));
+        return NXQ_OK;
+    }
+    RouteParams p{logits_dev, dtype, T, E, k, normalize, 0, 0, ids_dev, weights_dev, offsets_dev, rows_dev, slots_dev, nullptr, nullptr};
+    const size_t smem = (size_t)(2 * E + 1 + kRankWarps * E) * sizeof(int32_t);
+    if (T <= kSmallT) {
+        cudaError_t e = launch_choose(p, true, smem, st);
+        return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "route launch");
+    }
+    // At most 1024 blocks of tokens.
+    p.tb = (int)((T + 1023) / 1024);
+    if (p.tb < 64) p.tb = 64;
+    p.blocks = (int)((T + p.tb - 1) / p.tb);
+    cudaError_t e = cudaMallocAsync((void**)&p.hist, ((size_t)p.blocks + 1) * E * sizeof(int32_t), st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (route workspace)");
+    p.total = p.hist + (size_t)p.blocks * E;
+    e = launch_choose(p, false, smem, st);
+    if (e == cudaSuccess) {
+        route_scan_kernel<<<(unsigned)((E + 31) / 32), 1024, 0, st>>>(p);
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) {
+        route_rank_kernel<<<(unsigned)p.blocks, kThreads, smem, st>>>(p);
+        e = cudaGetLastError();
+    }
+    note_launches(2);
+    cudaFreeAsync(p.hist, st);
+    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "route launch");
+}
+
+NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N, const int32_t* slots_dev,
+                            const float* weights_dev, int64_t T, int k, const float* res_dev, void* y_dev,
+                            int y_dtype, void* stream) {
+    if (T < 0 || N < 0 || R < 0 || R > 0x7FFFFFFF || k < 1 || k > kMaxK)
+        return fail(NXQ_ERR_ARG, "combine: T=%lld N=%lld R=%lld k=%d", (long long)T, (long long)N, (long long)R, k);
+    if (!dtype_valid(h_dtype) || !dtype_valid(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
+    if (T == 0 || N == 0) return NXQ_OK;
+    if (!slots_dev || !weights_dev || !y_dev || (R > 0 && !h_dev)) return fail(NXQ_ERR_ARG, "combine: null array");
+    if ((const void*)y_dev == (const void*)res_dev && y_dtype != NXQ_F32)
+        return fail(NXQ_ERR_ARG, "combine: y may be the residual only as fp32");
+    if (int rc = context_ready()) return rc;
+    const bool vec = N % 8 == 0 && (((uintptr_t)h_dev | (uintptr_t)y_dev | (uintptr_t)res_dev) % 16) == 0;
+    const int64_t segs = (N + (int64_t)kCombThreads * (vec ? 8 : 1) - 1) / ((int64_t)kCombThreads * (vec ? 8 : 1));
+    if (T > ((int64_t)1 << 62) / segs) return fail(NXQ_ERR_ARG, "combine: T=%lld N=%lld", (long long)T, (long long)N);
+    const int64_t grid = T * segs < (1 << 30) ? T * segs : (1 << 30);
+    if (vec)
+        combine_kernel<8><<<(unsigned)grid, kCombThreads, 0, (cudaStream_t)stream>>>(
+            h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
+    else
+        combine_kernel<1><<<(unsigned)grid, kCombThreads, 0, (cudaStream_t)stream>>>(
+            h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
+    note_launches(1);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "combine launch");
+}
+
+}  // extern "C"

@@ -115,16 +115,6 @@ int check_ready() {
     return NXQ_OK;
 }
 
-int check_weight(nxq_weight_t h, Weight** out) {
-    Weight* w = reinterpret_cast<Weight*>(h);
-    if (!w) return fail(NXQ_ERR_ARG, "null weight handle");
-    std::lock_guard<std::mutex> lk(g_ctx.mu);
-    if (!g_ctx.live.count(w) || w->magic != kWeightMagic)
-        return fail(NXQ_ERR_ARG, "weight handle is not live (released or foreign)");
-    *out = w;
-    return NXQ_OK;
-}
-
 bool dtype_ok(int d) { return d == NXQ_F32 || d == NXQ_F16 || d == NXQ_BF16; }
 size_t dtype_size(int d) { return d == NXQ_F32 ? 4 : 2; }
 
@@ -141,7 +131,8 @@ int grow(void** buf, size_t* have, size_t need) {
 
 // Reads the device status word after a synchronize: a bounded wait that
 // gave up (NXQ_ERR_TIMEOUT), or an activation too large for f16
-// (NXQ_ERR_RANGE).  The word is cleared once reported.
+// (NXQ_ERR_RANGE), or an index outside its range (NXQ_ERR_INDEX).  The word is
+// cleared once reported.
 int report_status(const DeviceStatus& st) {
     if (!st.code) return NXQ_OK;
     // Clear the error (code and where); the settings after it stay.
@@ -153,6 +144,12 @@ int report_status(const DeviceStatus& st) {
                     "an activation of magnitude >= 65520 reached %s: it is outside the f16 range the "
                     "tensor-core kernels compute in (results of that call are not finite)",
                     what[st.where < 4 ? st.where : 0]);
+    }
+    if (st.code == kStatusIndex) {
+        static const char* const what[] = {"an index", "a token id of an embedding lookup",
+                                           "an expert offset of a ragged product", "a row index of a ragged product",
+                                           "a slot index of a combine"};
+        return fail(NXQ_ERR_INDEX, "%s was outside its range (that access was skipped)", what[st.where < 5 ? st.where : 0]);
     }
     scratch_reset_counters();
     return fail(NXQ_ERR_TIMEOUT, "device-side bounded wait expired (code %u at %u)", st.code, st.where);
@@ -241,6 +238,25 @@ int register_impl(const void* src, bool is_host, int type, int64_t N, int64_t K,
 }
 
 }  // namespace
+
+int check_weight(nxq_weight_t h, Weight** out) {
+    Weight* w = reinterpret_cast<Weight*>(h);
+    if (!w) return fail(NXQ_ERR_ARG, "null weight handle");
+    std::lock_guard<std::mutex> lk(g_ctx.mu);
+    if (!g_ctx.live.count(w) || w->magic != kWeightMagic)
+        return fail(NXQ_ERR_ARG, "weight handle is not live (released or foreign)");
+    *out = w;
+    return NXQ_OK;
+}
+
+int weight_table_ref(nxq_weight_t h, int delta) {
+    Weight* w = reinterpret_cast<Weight*>(h);
+    std::lock_guard<std::mutex> lk(g_ctx.mu);
+    if (!g_ctx.live.count(w) || w->magic != kWeightMagic)
+        return fail(NXQ_ERR_ARG, "weight handle is not live (released or foreign)");
+    w->tables += delta;
+    return NXQ_OK;
+}
 
 int fail(int status, const char* fmt, ...) {
     va_list ap;
@@ -386,6 +402,7 @@ NXQ_API int nxq_shutdown(void) {
     if (!g_ctx.ready) return NXQ_OK;
     cudaSetDevice(g_ctx.device);
     cudaDeviceSynchronize();
+    experts_shutdown();
     {
         std::lock_guard<std::mutex> lk2(g_ctx.mu);
         for (Weight* w : g_ctx.live) {
@@ -526,6 +543,8 @@ NXQ_API int nxq_weight_release(nxq_weight_t h) {
     rc = check_ready();
     if (rc) return rc;
     std::lock_guard<std::mutex> lk(g_ctx.mu);
+    if (w->tables)
+        return fail(NXQ_ERR_STATE, "the weight belongs to %d live expert table(s): release them first", w->tables);
     g_ctx.live.erase(w);
     w->magic = 0;
     // Work queued on other streams may still read the weight.
@@ -558,6 +577,23 @@ NXQ_API int nxq_dequant(nxq_weight_t h, float* y_dev, void* stream) {
     cudaError_t e = launch_dequant(w->dev, w->shape, y_dev, (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(e, "dequant launch");
     return NXQ_OK;
+}
+
+NXQ_API int nxq_embedding(nxq_weight_t h, const void* ids_dev, int ids_type, int64_t T, float scale, void* y_dev,
+                          int y_dtype, void* stream) {
+    Weight* w = nullptr;
+    int rc = check_weight(h, &w);
+    if (rc) return rc;
+    if (T < 0) return fail(NXQ_ERR_ARG, "T=%lld", (long long)T);
+    if (ids_type != NXQ_I32 && ids_type != NXQ_I64) return fail(NXQ_ERR_ARG, "bad index type %d", ids_type);
+    if (!dtype_ok(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
+    if (T == 0) return NXQ_OK;
+    if (!ids_dev || !y_dev) return fail(NXQ_ERR_ARG, "null ids or output");
+    if ((uintptr_t)y_dev % 16) return fail(NXQ_ERR_ARG, "output must be 16-byte aligned");
+    if ((uintptr_t)ids_dev % (ids_type == NXQ_I64 ? 8 : 4)) return fail(NXQ_ERR_ARG, "ids are not aligned to their type");
+    if ((rc = check_ready())) return rc;
+    cudaError_t e = launch_embedding(w->dev, w->shape, ids_dev, ids_type, T, scale, y_dev, y_dtype, (cudaStream_t)stream);
+    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "embedding launch");
 }
 
 NXQ_API int nxq_qmatmul(nxq_weight_t h, const void* x_dev, int x_dtype, void* y_dev, int y_dtype,

@@ -19,6 +19,7 @@ struct Weight {
     uint8_t* dev = nullptr;   // tiled copy (shape.total_bytes() + kTailPad)
     size_t dev_bytes = 0;
     size_t packed_bytes = 0;  // N * K/QK * block_bytes (the algorithmic bytes)
+    int tables = 0;           // live expert tables that refer to it
 };
 constexpr uint32_t kWeightMagic = 0x4E58514Bu;  // "NXQK"
 constexpr size_t kTailPad = 256;                 // slack after the last tile-chunk
@@ -36,7 +37,8 @@ int cuda_fail(cudaError_t e, const char* what);
 
 // Device-side error word of the context: 0 = ok, else the first error a
 // kernel raised (kStatusTimeout: a bounded wait ran out; kStatusRange: a
-// finite activation was too large for f16).  `where` says which wait or
+// finite activation was too large for f16; kStatusIndex: an index in device
+// memory lay outside its range).  `where` says which wait or
 // conversion.  Read by the host after a synchronize (nxq_stream_sync,
 // nxq_qmatmul_host).
 // The same device allocation also holds the settings kernels read on their
@@ -56,6 +58,7 @@ struct DeviceStatus {
 };
 constexpr unsigned kStatusTimeout = 1u;
 constexpr unsigned kStatusRange = 2u;
+constexpr unsigned kStatusIndex = 3u;
 constexpr long long kDefaultWaitCycles = 4000000000LL;  // ~2 s at 2 GHz
 constexpr long long kDrainWaitCycles = 4000000000LL;
 // Test hook: CTAs of a stream-K launch that publish a partial sum for a tile
@@ -86,12 +89,30 @@ __device__ __forceinline__ void raise_range(DeviceStatus* st, unsigned where) {
     }
 }
 
+// Records an index error (first error wins; `where`: kIndex*).
+constexpr unsigned kIndexToken = 1u, kIndexOffset = 2u, kIndexRow = 3u, kIndexSlot = 4u;
+__device__ __forceinline__ void raise_index(DeviceStatus* st, unsigned where) {
+    if (st && atomicCAS(&st->code, 0u, kStatusIndex) == 0u) {
+        st->where = where;
+        raise_host_flag(st);
+    }
+}
+
 // The context's device status word and SM count (nxq_api.cu).
 DeviceStatus* context_status();
 // NXQ_OK once nxq_init has run, with the context's device made current on the
 // calling thread; else the status (and message) the C ABI returns.
 int context_ready();
 int context_sm_count();
+
+// NXQ_OK and the weight behind a live handle, else the status the C ABI returns.
+int check_weight(nxq_weight_t h, Weight** out);
+// Adds `delta` references of expert tables to the weight behind a live handle.
+int weight_table_ref(nxq_weight_t h, int delta);
+// Releases every expert table (nxq_shutdown; the weights go after it).
+void experts_shutdown();
+
+inline bool dtype_valid(int d) { return d == NXQ_F32 || d == NXQ_F16 || d == NXQ_BF16; }
 
 // Process-wide count of kernels launched by the library (nxq_launch_count).
 void note_launches(unsigned n);
@@ -101,6 +122,9 @@ cudaError_t launch_repack(const uint8_t* src, uint8_t* dst, const TiledShape& s,
                           int64_t row0, int64_t rows, int64_t blk0, int64_t src_row_blocks,
                           cudaStream_t st);
 cudaError_t launch_dequant(const uint8_t* tiled, const TiledShape& s, float* y, cudaStream_t st);
+// y[t] = scale * decode(row ids[t]) (embedding.cu).
+cudaError_t launch_embedding(const uint8_t* tiled, const TiledShape& s, const void* ids, int ids_type, int64_t T,
+                             float scale, void* y, int y_dtype, cudaStream_t st);
 
 // CUDA-core fused dequant-GEMV/GEMM with exact fp32 decode; any M (chunked by 32).
 // `partials` must hold splits * M * N floats when splits > 1.

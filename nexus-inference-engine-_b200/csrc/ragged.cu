@@ -1,0 +1,325 @@
+// Products grouped by expert with ragged sizes: y[s] = x[rows[s]] W_e^T for the
+// slots s of expert e, with the sizes known on the device only.
+//
+// A call is a plan kernel, which turns the offsets into a list of the experts
+// that have rows (ragged.h), and a product kernel that walks it.  The kernel
+// here is the exact one: fp32 decode (formats.cuh, decode8) and fp32
+// products on the CUDA cores, for every block type and any size.
+#include "ragged.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+#include <new>
+#include <unordered_set>
+
+namespace nxq {
+
+namespace {
+
+std::mutex g_tables_mu;
+std::unordered_set<ExpertTable*> g_tables;
+
+int check_experts(nxq_experts_t h, const ExpertTable** out) {
+    ExpertTable* t = reinterpret_cast<ExpertTable*>(h);
+    if (!t) return fail(NXQ_ERR_ARG, "null expert table");
+    std::lock_guard<std::mutex> lk(g_tables_mu);
+    if (!g_tables.count(t)) return fail(NXQ_ERR_ARG, "expert table is not live (released or foreign)");
+    *out = t;
+    return NXQ_OK;
+}
+
+// One CTA, thread = expert: writes the experts that have rows.  An expert's
+// range is taken only if it lies in [0, R] and starts at or behind every offset
+// before it, so the ranges taken never overlap and hold at most R slots
+// whatever the offsets are; anything else is reported and left out.
+__global__ void __launch_bounds__(kMaxExperts) ragged_plan_kernel(const int32_t* __restrict__ offsets, int E, int64_t R,
+                                                                  int blk, RaggedPlan* plan, DeviceStatus* status) {
+    __shared__ int warp_n[32], warp_b[32], warp_m[32];
+    const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
+    const int o0 = e < E ? offsets[e] : 0, o1 = e < E ? offsets[e + 1] : 0;
+    int before = o0;  // the largest offset up to and including o0
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, before, o);
+        if (lane >= o && v > before) before = v;
+    }
+    if (lane == 31) warp_m[warp] = before;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before = warp_m[w] > before ? warp_m[w] : before;
+    int a = 0, n = 0;
+    if (e < E) {
+        if (o0 < 0 || o0 < before || o1 < o0 || o1 > R)
+            raise_index(status, kIndexOffset);
+        else
+            a = o0, n = o1 - o0;
+    }
+    const int has = n > 0, nb = (n + blk - 1) / blk;
+    const unsigned act = __ballot_sync(0xFFFFFFFFu, has);
+    int bs = nb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, bs, o);
+        if (lane >= o) bs += v;
+    }
+    if (lane == 31) {
+        warp_n[warp] = __popc(act);
+        warp_b[warp] = bs;
+    }
+    __syncthreads();
+    int n0 = 0, b0 = 0;
+    for (int w = 0; w < warp; ++w) {
+        n0 += warp_n[w];
+        b0 += warp_b[w];
+    }
+    if (has) plan->it[n0 + __popc(act & ((1u << lane) - 1u))] = RaggedEntry{e, a, n, b0 + bs - nb};
+    if (e == kMaxExperts - 1) {
+        plan->entries = n0 + __popc(act);
+        plan->blocks = b0 + bs;
+    }
+}
+
+__device__ __forceinline__ float load_x(const void* x, int dt, int64_t i) {
+    if (dt == NXQ_F16) return __half2float(static_cast<const __half*>(x)[i]);
+    if (dt == NXQ_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]);
+    return static_cast<const float*>(x)[i];
+}
+__device__ __forceinline__ void store_y(void* y, int dt, int64_t i, float v) {
+    if (dt == NXQ_F16)
+        static_cast<__half*>(y)[i] = __float2half_rn(v);
+    else if (dt == NXQ_BF16)
+        static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+    else
+        static_cast<float*>(y)[i] = v;
+}
+
+constexpr int kSimtBlk = 8;  // rows per work tile
+
+struct SimtParams {
+    const uint8_t* const* w;
+    const uint8_t* const* up;
+    TiledShape s;
+    const void* x;
+    int x_dtype;
+    int64_t X;
+    const int32_t* rows;
+    void* y;
+    int y_dtype;
+    const RaggedPlan* plan;
+    DeviceStatus* status;
+};
+
+// Thread r owns weight row r of the tile for up to kSimtBlk slots.
+template <bool PAIR>
+__global__ void __launch_bounds__(TILE_ROWS) ragged_simt_kernel(const SimtParams p) {
+    __shared__ float xs[kSimtBlk][CHUNK_K];
+    __shared__ int64_t src[kSimtBlk];
+    const int r = threadIdx.x;
+    const int tiles = (int)p.s.tiles;
+    const int64_t total = (int64_t)p.plan->blocks * tiles;
+    for (int64_t g = blockIdx.x; g < total; g += gridDim.x) {
+        const RaggedTile t = ragged_tile(p.plan, kSimtBlk, tiles, g);
+        __syncthreads();
+        if (r < kSimtBlk) {
+            int64_t row = -1;
+            if (r < t.rows) {
+                row = p.rows ? p.rows[t.row0 + r] : t.row0 + r;
+                if (row < 0 || row >= p.X) {
+                    raise_index(p.status, kIndexRow);
+                    row = -1;
+                }
+            }
+            src[r] = row;
+        }
+        float acc[kSimtBlk], accu[PAIR ? kSimtBlk : 1];
+#pragma unroll
+        for (int m = 0; m < kSimtBlk; ++m) {
+            acc[m] = 0.0f;
+            if constexpr (PAIR) accu[m] = 0.0f;
+        }
+        for (int64_t c = 0; c < p.s.chunks; ++c) {
+            const int64_t k0 = c * CHUNK_K;
+            __syncthreads();
+            for (int i = r; i < kSimtBlk * CHUNK_K; i += TILE_ROWS) {
+                const int m = i / CHUNK_K, kk = i % CHUNK_K;
+                xs[m][kk] = src[m] >= 0 && k0 + kk < p.s.K ? load_x(p.x, p.x_dtype, src[m] * p.s.K + k0 + kk) : 0.0f;
+            }
+            __syncthreads();
+            const int kmax = (int)(p.s.K - k0 < CHUNK_K ? p.s.K - k0 : CHUNK_K);
+            auto add = [&](const uint8_t* w, float* a) {
+                const uint8_t* chunk = w + p.s.chunk_offset(t.tile, c);
+                for (int e0 = 0; e0 < kmax; e0 += 8) {
+                    float v[8];
+                    decode8(p.s.type, chunk, r, e0, v);
+#pragma unroll
+                    for (int m = 0; m < kSimtBlk; ++m)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) a[m] = fmaf(v[i], xs[m][e0 + i], a[m]);
+                }
+            };
+            add(p.w[t.e], acc);
+            if constexpr (PAIR) add(p.up[t.e], accu);
+        }
+        const int64_t n = (int64_t)t.tile * TILE_ROWS + r;
+        if (n >= p.s.N) continue;
+#pragma unroll
+        for (int m = 0; m < kSimtBlk; ++m)
+            if (m < t.rows) {
+                float v = acc[m];
+                if constexpr (PAIR) v = v / (1.0f + expf(-v)) * accu[m];
+                store_y(p.y, p.y_dtype, (int64_t)(t.row0 + m) * p.s.N + n, v);
+            }
+    }
+}
+
+// Row blocks a plan can have at most.
+int64_t max_blocks(int64_t E, int64_t R, int blk) { return (E < R ? E : R) + R / blk; }
+
+int run_simt(const RaggedCall& c) {
+    RaggedPlan* plan = nullptr;
+    const int64_t most = c.w->count < c.R ? c.w->count : c.R;
+    cudaError_t e = cudaMallocAsync((void**)&plan, plan_bytes(most), c.st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (ragged plan)");
+    ragged_plan_kernel<<<1, kMaxExperts, 0, c.st>>>(c.offsets, c.w->count, c.R, kSimtBlk, plan, context_status());
+    e = cudaGetLastError();
+    if (e == cudaSuccess) {
+        SimtParams p{c.w->dev, c.up ? c.up->dev : nullptr, c.w->shape, c.x, c.x_dtype, c.X, c.rows, c.y, c.y_dtype, plan,
+                     context_status()};
+        const int64_t work = max_blocks(c.w->count, c.R, kSimtBlk) * c.w->shape.tiles;
+        const int64_t cap = (int64_t)context_sm_count() * 16;
+        const unsigned grid = (unsigned)(work < cap ? work : cap);
+        if (c.up)
+            ragged_simt_kernel<true><<<grid, TILE_ROWS, 0, c.st>>>(p);
+        else
+            ragged_simt_kernel<false><<<grid, TILE_ROWS, 0, c.st>>>(p);
+        e = cudaGetLastError();
+    }
+    note_launches(2);
+    cudaFreeAsync(plan, c.st);
+    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "ragged product launch");
+}
+
+int run(nxq_experts_t he, nxq_experts_t hu, bool pair, const void* x_dev, int x_dtype, int64_t X, const int32_t* rows_dev,
+        void* y_dev, int y_dtype, int64_t R, const int32_t* offsets_dev, void* stream) {
+    RaggedCall c{};
+    int rc = check_experts(he, &c.w);
+    if (rc || (pair && (rc = check_experts(hu, &c.up)))) return rc;
+    if (pair && (c.w->count != c.up->count || c.w->shape.type != c.up->shape.type || c.w->shape.N != c.up->shape.N ||
+                 c.w->shape.K != c.up->shape.K))
+        return fail(NXQ_ERR_SHAPE, "ragged swiglu: gate (%d x %s [%lld][%lld]) and up (%d x %s [%lld][%lld]) differ",
+                    c.w->count, type_name(c.w->shape.type), (long long)c.w->shape.N, (long long)c.w->shape.K,
+                    c.up->count, type_name(c.up->shape.type), (long long)c.up->shape.N, (long long)c.up->shape.K);
+    if (R < 0 || R > 0x7FFFFFFF || X < 0) return fail(NXQ_ERR_ARG, "ragged: R=%lld X=%lld", (long long)R, (long long)X);
+    if (!dtype_valid(x_dtype) || !dtype_valid(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
+    if (R == 0) return NXQ_OK;
+    if (!x_dev || !y_dev || !offsets_dev) return fail(NXQ_ERR_ARG, "ragged: null activation, output or offsets");
+    if (!rows_dev && X < R)
+        return fail(NXQ_ERR_SHAPE, "ragged: %lld activation rows for %lld slots (and no row indices)", (long long)X, (long long)R);
+    if ((rc = context_ready())) return rc;
+    c.x = x_dev;
+    c.x_dtype = x_dtype;
+    c.X = X;
+    c.rows = rows_dev;
+    c.y = y_dev;
+    c.y_dtype = y_dtype;
+    c.R = R;
+    c.offsets = offsets_dev;
+    c.st = (cudaStream_t)stream;
+    return run_simt(c);
+}
+
+}  // namespace
+
+void experts_shutdown() {
+    std::lock_guard<std::mutex> lk(g_tables_mu);
+    for (ExpertTable* t : g_tables) {
+        cudaFree(t->dev);
+        delete t;
+    }
+    g_tables.clear();
+}
+
+}  // namespace nxq
+
+using namespace nxq;
+
+extern "C" {
+
+NXQ_API int nxq_experts_create(const nxq_weight_t* hs, int count, nxq_experts_t* out) {
+    if (!hs || !out) return fail(NXQ_ERR_ARG, "null argument");
+    if (count < 1 || count > kMaxExperts) return fail(NXQ_ERR_ARG, "%d experts (1 to %d)", count, kMaxExperts);
+    std::vector<const uint8_t*> dev((size_t)count);
+    TiledShape shape{};
+    for (int i = 0; i < count; ++i) {
+        Weight* w = nullptr;
+        if (int rc = check_weight(hs[i], &w)) return rc;
+        if (i == 0) shape = w->shape;
+        if (w->shape.type != shape.type || w->shape.N != shape.N || w->shape.K != shape.K)
+            return fail(NXQ_ERR_SHAPE, "expert %d is %s [%lld][%lld], expert 0 %s [%lld][%lld]", i, type_name(w->shape.type),
+                        (long long)w->shape.N, (long long)w->shape.K, type_name(shape.type), (long long)shape.N,
+                        (long long)shape.K);
+        dev[i] = w->dev;
+    }
+    if (int rc = context_ready()) return rc;
+    ExpertTable* t = new (std::nothrow) ExpertTable();
+    if (!t) return fail(NXQ_ERR_NOMEM, "host allocation failed");
+    t->count = count;
+    t->shape = shape;
+    int held = 0, rc = NXQ_OK;
+    for (; held < count && rc == NXQ_OK; ++held) rc = weight_table_ref(hs[held], 1);
+    if (rc != NXQ_OK) --held;
+    cudaError_t e = cudaSuccess;
+    if (rc == NXQ_OK && (e = cudaMalloc((void**)&t->dev, dev.size() * sizeof(dev[0]))) == cudaSuccess)
+        e = cudaMemcpy(t->dev, dev.data(), dev.size() * sizeof(dev[0]), cudaMemcpyHostToDevice);
+    if (rc != NXQ_OK || e != cudaSuccess) {
+        for (int i = 0; i < held; ++i) weight_table_ref(hs[i], -1);
+        if (t->dev) cudaFree(t->dev);
+        delete t;
+        return rc != NXQ_OK ? rc : cuda_fail(e, "expert table");
+    }
+    t->refs.assign(hs, hs + count);
+    std::lock_guard<std::mutex> lk(g_tables_mu);
+    g_tables.insert(t);
+    *out = reinterpret_cast<nxq_experts_t>(t);
+    return NXQ_OK;
+}
+
+NXQ_API int nxq_experts_release(nxq_experts_t h) {
+    const ExpertTable* t = nullptr;
+    int rc = check_experts(h, &t);
+    if (rc || (rc = context_ready())) return rc;
+    {
+        std::lock_guard<std::mutex> lk(g_tables_mu);
+        if (!g_tables.erase(const_cast<ExpertTable*>(t))) return fail(NXQ_ERR_ARG, "expert table is not live");
+    }
+    // Work queued on any stream may still read the table.
+    cudaDeviceSynchronize();
+    for (nxq_weight_t w : t->refs) weight_table_ref(w, -1);
+    cudaFree(t->dev);
+    delete t;
+    return NXQ_OK;
+}
+
+NXQ_API int nxq_experts_info(nxq_experts_t h, int* count, int* type, int64_t* N, int64_t* K) {
+    const ExpertTable* t = nullptr;
+    if (int rc = check_experts(h, &t)) return rc;
+    if (count) *count = t->count;
+    if (type) *type = t->shape.type;
+    if (N) *N = t->shape.N;
+    if (K) *K = t->shape.K;
+    return NXQ_OK;
+}
+
+NXQ_API int nxq_qmatmul_ragged(nxq_experts_t e, const void* x_dev, int x_dtype, int64_t X, const int32_t* rows_dev,
+                               void* y_dev, int y_dtype, int64_t R, const int32_t* offsets_dev, void* stream) {
+    return run(e, nullptr, false, x_dev, x_dtype, X, rows_dev, y_dev, y_dtype, R, offsets_dev, stream);
+}
+
+NXQ_API int nxq_qmatmul_ragged_swiglu(nxq_experts_t gate, nxq_experts_t up, const void* x_dev, int x_dtype, int64_t X,
+                                      const int32_t* rows_dev, void* h_dev, int h_dtype, int64_t R,
+                                      const int32_t* offsets_dev, void* stream) {
+    return run(gate, up, true, x_dev, x_dtype, X, rows_dev, h_dev, h_dtype, R, offsets_dev, stream);
+}
+
+}  // extern "C"

@@ -22,6 +22,7 @@ __all__ = [
     "kernel_name", "launch_count",
     "TYPES", "GEOMETRY", "F32", "F16", "BF16", "SPLIT_COL", "SPLIT_ROW", "declared_symbols",
     "tp_unique_id", "tp_init", "tp_shutdown", "tp_qmatmul", "tp_allreduce_f32", "GGUF", "NXF", "xxh32", "qmatmul_grouped", "qmatmul_swiglu", "qmatmul_residual", "rmsnorm_qmatmul", "int4_pack", "INT4_ROWS", "INT4_KMAJOR",
+    "embedding", "Experts", "moe_route", "qmatmul_ragged", "qmatmul_ragged_swiglu", "moe_combine",
 ]
 
 LIB_PATH = Path(__file__).with_name("libnxq.so")
@@ -42,7 +43,7 @@ SPLIT_COL, SPLIT_ROW = 0, 1
 
 STATUS = {0: "OK", -1: "ERR_ARG", -2: "ERR_CODEC", -3: "ERR_SHAPE", -4: "ERR_CUDA",
           -5: "ERR_TIMEOUT", -6: "ERR_NOMEM", -7: "ERR_STATE", -8: "ERR_NCCL", -9: "ERR_UNSUPPORTED",
-          -10: "ERR_FORMAT", -11: "ERR_RANGE"}
+          -10: "ERR_FORMAT", -11: "ERR_RANGE", -12: "ERR_INDEX"}
 
 
 class NxqError(RuntimeError):
@@ -90,6 +91,19 @@ _SIGS = {
                             _c.POINTER(_c.c_void_p), _c.c_int, _c.c_int64, _c.c_void_p],
     "nxq_qmatmul_noalloc": [_c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int, _c.c_int64,
                             _c.c_void_p],
+    "nxq_embedding": [_c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float, _c.c_void_p, _c.c_int, _c.c_void_p],
+    "nxq_experts_create": [_c.POINTER(_c.c_void_p), _c.c_int, _c.POINTER(_c.c_void_p)],
+    "nxq_experts_release": [_c.c_void_p],
+    "nxq_experts_info": [_c.c_void_p, _c.POINTER(_c.c_int), _c.POINTER(_c.c_int), _c.POINTER(_c.c_int64),
+                         _c.POINTER(_c.c_int64)],
+    "nxq_moe_route": [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p, _c.c_void_p,
+                      _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p],
+    "nxq_qmatmul_ragged": [_c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int,
+                           _c.c_int64, _c.c_void_p, _c.c_void_p],
+    "nxq_qmatmul_ragged_swiglu": [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_void_p,
+                                  _c.c_int, _c.c_int64, _c.c_void_p, _c.c_void_p],
+    "nxq_moe_combine": [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int,
+                        _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p],
     "nxq_stream_sync": [_c.c_void_p],
     "nxq_set_wait_limit": [_c.c_uint64],
     "nxq_test_hook": [_c.c_int, _c.c_int],
@@ -196,8 +210,13 @@ def _check(rc: int) -> None:
         raise NxqError(rc, last_error())
 
 
+_device: Optional[int] = None
+
+
 def init(device: int = 0) -> None:
+    global _device
     _check(lib().nxq_init(device))
+    _device = device
 
 
 def shutdown() -> None:
@@ -411,6 +430,172 @@ def qmatmul_host(w: Weight, x: np.ndarray, out: Optional[np.ndarray] = None) -> 
     if out is None:
         out = np.empty((M, w.N), dtype=np.float32)
     _check(lib().nxq_qmatmul_host(w.handle, x.ctypes.data, out.ctypes.data, M))
+    return out
+
+
+# ---- embedding and mixture of experts ------------------------------------------
+
+I32, I64 = 0, 1
+
+
+def _arg(ok: bool, message: str) -> None:
+    if not ok:
+        raise NxqError(-1, message)
+
+
+def _tensors(what: str, **tensors) -> None:
+    """Every given tensor is contiguous and on the library's GPU."""
+    for name, t in tensors.items():
+        if t is not None:
+            _arg(t.is_cuda and (_device is None or t.device.index == _device),
+                 f"{what}: {name} is on {t.device}, the library on cuda:{_device}")
+            _arg(t.is_contiguous(), f"{what}: {name} is not contiguous")
+
+
+def _float_code(what: str, name: str, dtype) -> int:
+    import torch
+
+    _arg(dtype in (torch.float32, torch.float16, torch.bfloat16), f"{what}: {name} is {dtype}")
+    return _dtype_code(dtype)
+
+
+def _int32(what: str, **tensors) -> None:
+    import torch
+
+    for name, t in tensors.items():
+        _arg(t is None or t.dtype == torch.int32, f"{what}: {name} must be int32")
+
+
+def _out(what: str, out, shape, dtype, device):
+    """`out` if given (checked), else a new tensor of `shape`."""
+    import torch
+
+    if out is None:
+        return torch.empty(shape, dtype=dtype or torch.float32, device=device)
+    _arg(tuple(out.shape) == tuple(shape), f"{what}: out has shape {tuple(out.shape)}, not {tuple(shape)}")
+    _arg(dtype is None or out.dtype == dtype, f"{what}: out is {out.dtype}, out_dtype {dtype}")
+    return out
+
+
+def _stream_of(stream, tensor) -> ctypes.c_void_p:
+    """The given stream, else the current one of the tensor's device."""
+    if stream is None:
+        import torch
+
+        return ctypes.c_void_p(torch.cuda.current_stream(tensor.device).cuda_stream)
+    return _stream_ptr(stream)
+
+
+def embedding(w: Weight, ids, scale: float = 1.0, out=None, out_dtype=None, stream=None):
+    """scale * decode(W[ids]): rows of a registered table, [*ids.shape, K] (nxq_embedding).
+    ids: int32 or int64; an id outside the table gives zeros and ERR_INDEX at stream_sync."""
+    import torch
+
+    _arg(ids.dtype in (torch.int32, torch.int64), f"embedding: ids are {ids.dtype}, not int32 or int64")
+    _tensors("embedding", ids=ids, out=out)
+    out = _out("embedding", out, (*ids.shape, w.K), out_dtype, ids.device)
+    code = _float_code("embedding", "out", out.dtype)
+    _check(lib().nxq_embedding(w.handle, ids.data_ptr(), I64 if ids.dtype == torch.int64 else I32, ids.numel(), scale,
+                               out.data_ptr(), code, _stream_of(stream, ids)))
+    return out
+
+
+class Experts:
+    """Experts of one projection: registered weights of one block type and shape
+    (nxq_experts_create).  Holds the weights; release it before them."""
+
+    def __init__(self, weights):
+        self.weights = list(weights)
+        n = len(self.weights)
+        _arg(n > 0, "Experts: no weights")
+        h = ctypes.c_void_p()
+        _check(lib().nxq_experts_create((ctypes.c_void_p * n)(*[w.handle.value for w in self.weights]), n, ctypes.byref(h)))
+        self._h = h
+        self.count, self.type, self.N, self.K = n, self.weights[0].type, self.weights[0].N, self.weights[0].K
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        if self._h is None:
+            raise NxqError(-1, "expert table already released")
+        return self._h
+
+    def release(self) -> None:
+        """Releases the table; the weights stay registered."""
+        if self._h is not None:
+            _check(lib().nxq_experts_release(self._h))
+        self._h, self.weights = None, []
+
+
+def moe_route(logits, k: int, normalize: bool = True, stream=None):
+    """Top-k routing of logits [T][E] (nxq_moe_route): (ids [T][k], weights [T][k],
+    offsets [E + 1], rows [T * k], slots [T][k]), on the device."""
+    import torch
+
+    _arg(logits.dim() == 2, f"moe_route: logits have {logits.dim()} dimensions, not 2")
+    code = _float_code("moe_route", "logits", logits.dtype)
+    _tensors("moe_route", logits=logits)
+    T, E = logits.shape
+    _arg(1 <= k <= min(E, 32), f"moe_route: k={k} of {E} experts (at most 32)")
+    i32 = dict(dtype=torch.int32, device=logits.device)
+    ids, slots = torch.empty((T, k), **i32), torch.empty((T, k), **i32)
+    weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+    offsets, rows = torch.empty(E + 1, **i32), torch.empty(T * k, **i32)
+    _check(lib().nxq_moe_route(logits.data_ptr(), code, T, E, k, 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
+                               offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_of(stream, logits)))
+    return ids, weights, offsets, rows, slots
+
+
+def _ragged(what: str, experts, x, offsets, rows, out, out_dtype):
+    """Checks a ragged product's arguments: (X, R, out)."""
+    _arg(x.dim() == 2 and x.shape[1] == experts.K, f"{what}: x is {tuple(x.shape)}, not [rows][{experts.K}]")
+    _int32(what, offsets=offsets, rows=rows)
+    _tensors(what, x=x, offsets=offsets, rows=rows, out=out)
+    _arg(offsets.numel() == experts.count + 1, f"{what}: {offsets.numel()} offsets for {experts.count} experts")
+    _arg(rows is None or rows.dim() == 1, f"{what}: rows must be one-dimensional")
+    R = x.shape[0] if rows is None else rows.numel()
+    return x.shape[0], R, _out(what, out, (R, experts.N), out_dtype, x.device)
+
+
+def qmatmul_ragged(experts: Experts, x, offsets, rows=None, out=None, out_dtype=None, stream=None):
+    """y[s] = x[rows[s]] W_e^T for the slots offsets[e] <= s < offsets[e + 1] of
+    every expert e (nxq_qmatmul_ragged); x[s] without rows.  Rows of `out` that
+    no expert has are left as they are (undefined in a new tensor)."""
+    X, R, out = _ragged("qmatmul_ragged", experts, x, offsets, rows, out, out_dtype)
+    _check(lib().nxq_qmatmul_ragged(experts.handle, x.data_ptr(), _float_code("qmatmul_ragged", "x", x.dtype), X,
+                                    None if rows is None else rows.data_ptr(), out.data_ptr(),
+                                    _float_code("qmatmul_ragged", "out", out.dtype), R, offsets.data_ptr(),
+                                    _stream_of(stream, x)))
+    return out
+
+
+def qmatmul_ragged_swiglu(gate: Experts, up: Experts, x, offsets, rows=None, out=None, out_dtype=None, stream=None):
+    """h[s] = silu(x Wg_e^T) * (x Wu_e^T) with x = x[rows[s]] (nxq_qmatmul_ragged_swiglu)."""
+    X, R, out = _ragged("qmatmul_ragged_swiglu", gate, x, offsets, rows, out, out_dtype)
+    _check(lib().nxq_qmatmul_ragged_swiglu(gate.handle, up.handle, x.data_ptr(),
+                                           _float_code("qmatmul_ragged_swiglu", "x", x.dtype), X,
+                                           None if rows is None else rows.data_ptr(), out.data_ptr(),
+                                           _float_code("qmatmul_ragged_swiglu", "out", out.dtype), R,
+                                           offsets.data_ptr(), _stream_of(stream, x)))
+    return out
+
+
+def moe_combine(h, slots, weights, res=None, out=None, out_dtype=None, stream=None):
+    """y[t] = sum_j weights[t][j] * h[slots[t][j]] (+ res[t]); negative slots are
+    skipped (nxq_moe_combine).  out may be res."""
+    import torch
+
+    what = "moe_combine"
+    _arg(h.dim() == 2 and slots.dim() == 2, f"{what}: h and slots must be two-dimensional")
+    _int32(what, slots=slots)
+    _arg(weights.dtype == torch.float32 and weights.shape == slots.shape, f"{what}: weights must be fp32 of slots' shape")
+    _arg(res is None or (res.dtype == torch.float32 and tuple(res.shape) == (slots.shape[0], h.shape[1])),
+         f"{what}: res must be fp32 [T][N]")
+    _tensors(what, h=h, slots=slots, weights=weights, res=res, out=out)
+    T, k = slots.shape
+    out = _out(what, out, (T, h.shape[1]), out_dtype, h.device)
+    _check(lib().nxq_moe_combine(h.data_ptr(), _float_code(what, "h", h.dtype), h.shape[0], h.shape[1], slots.data_ptr(),
+                                 weights.data_ptr(), T, k, None if res is None else res.data_ptr(), out.data_ptr(),
+                                 _float_code(what, "out", out.dtype), _stream_of(stream, h)))
     return out
 
 
