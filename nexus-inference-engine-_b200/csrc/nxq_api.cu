@@ -23,6 +23,7 @@
 #include "nxq_internal.h"
 #include "qmm_gemm.h"
 #include "qmm_mma.h"
+#include "ragged.h"
 #include "stream_scratch.h"
 
 namespace nxq {
@@ -393,6 +394,7 @@ NXQ_API int nxq_init(int device) {
     int rc = mma_init(device);
     if (rc != NXQ_OK) return rc;
     if ((rc = gemm_init(device)) != NXQ_OK) return rc;
+    if ((rc = ragged_gemm_init()) != NXQ_OK) return rc;
     g_ctx.ready = true;
     return NXQ_OK;
 }

@@ -411,6 +411,20 @@ void gemm_kernel_name(const TiledShape& s, int64_t, char* buf, size_t n) {
     snprintf(buf, n, "tc_gemm<%s,n%d>", type_name(s.type), kNT);
 }
 
+// Activations [rows][K] f16; box 64 (k) x box_rows, 128-byte swizzle; rows and
+// columns beyond the array read as zero.
+int gemm_activation_map(CUtensorMap* tmap, const void* xh, int64_t rows, int64_t K, int box_rows) {
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)K * 2};
+    cuuint32_t box[2] = {(cuuint32_t)kKS, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult cr = g_encode(tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(xh), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) return fail(NXQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    return NXQ_OK;
+}
+
 int gemm_qmatmul(const Weight* w, const void* x, int x_dtype, void* y, int y_dtype, int64_t M, cudaStream_t st) {
     const TiledShape& s = w->shape;
     if (!gemm_supported(s, M)) return NXQ_ERR_UNSUPPORTED;
@@ -424,17 +438,8 @@ int gemm_qmatmul(const Weight* w, const void* x, int x_dtype, void* y, int y_dty
         if (e != cudaSuccess) return cuda_fail(e, "to_half launch");
         xh = sc->xh;
     }
-    // Activations [M][K] f16; box 64 (k) x 256 (tokens), 128-byte swizzle; rows
-    // beyond M and columns beyond K read as zero.
     CUtensorMap tmap;
-    cuuint64_t dims[2] = {(cuuint64_t)s.K, (cuuint64_t)M};
-    cuuint64_t strides[1] = {(cuuint64_t)s.K * 2};
-    cuuint32_t box[2] = {(cuuint32_t)kKS, (cuuint32_t)kNT};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult cr = g_encode(&tmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(xh), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (cr != CUDA_SUCCESS) return fail(NXQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    if (int rc = gemm_activation_map(&tmap, xh, M, s.K, kNT)) return rc;
     switch (s.type) {
         case T_Q4_K: return launch<T_Q4_K>(w, tmap, y, y_dtype, M, st);
         case T_Q4_0: return launch<T_Q4_0>(w, tmap, y, y_dtype, M, st);

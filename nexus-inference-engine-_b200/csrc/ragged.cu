@@ -2,9 +2,11 @@
 // slots s of expert e, with the sizes known on the device only.
 //
 // A call is a plan kernel, which turns the offsets into a list of the experts
-// that have rows (ragged.h), and a product kernel that walks it.  The kernel
-// here is the exact one: fp32 decode (formats.cuh, decode8) and fp32
-// products on the CUDA cores, for every block type and any size.
+// that have rows (ragged.h), where needed a kernel that brings the activations
+// into slot order as f16, and a product kernel that walks the plan: tensor
+// cores (ragged_gemm.cu), or the exact kernel here, with fp32 decode
+// (formats.cuh, decode8) and fp32 products on the CUDA cores, for the block types
+// without a tensor-core decoder.
 #include "ragged.h"
 
 #include <cuda_bf16.h>
@@ -118,8 +120,11 @@ __global__ void __launch_bounds__(TILE_ROWS) ragged_simt_kernel(const SimtParams
     const int r = threadIdx.x;
     const int tiles = (int)p.s.tiles;
     const int64_t total = (int64_t)p.plan->blocks * tiles;
+    if (blockIdx.x >= total) return;
+    RaggedWalk<false> walk;
+    walk.start(p.plan, kSimtBlk, tiles, blockIdx.x);
     for (int64_t g = blockIdx.x; g < total; g += gridDim.x) {
-        const RaggedTile t = ragged_tile(p.plan, kSimtBlk, tiles, g);
+        const RaggedTile t = walk.at(g);
         __syncthreads();
         if (r < kSimtBlk) {
             int64_t row = -1;
@@ -173,31 +178,118 @@ __global__ void __launch_bounds__(TILE_ROWS) ragged_simt_kernel(const SimtParams
     }
 }
 
-// Row blocks a plan can have at most.
-int64_t max_blocks(int64_t E, int64_t R, int blk) { return (E < R ? E : R) + R / blk; }
-
-int run_simt(const RaggedCall& c) {
-    RaggedPlan* plan = nullptr;
-    const int64_t most = c.w->count < c.R ? c.w->count : c.R;
-    cudaError_t e = cudaMallocAsync((void**)&plan, plan_bytes(most), c.st);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (ragged plan)");
-    ragged_plan_kernel<<<1, kMaxExperts, 0, c.st>>>(c.offsets, c.w->count, c.R, kSimtBlk, plan, context_status());
-    e = cudaGetLastError();
-    if (e == cudaSuccess) {
-        SimtParams p{c.w->dev, c.up ? c.up->dev : nullptr, c.w->shape, c.x, c.x_dtype, c.X, c.rows, c.y, c.y_dtype, plan,
-                     context_status()};
-        const int64_t work = max_blocks(c.w->count, c.R, kSimtBlk) * c.w->shape.tiles;
-        const int64_t cap = (int64_t)context_sm_count() * 16;
-        const unsigned grid = (unsigned)(work < cap ? work : cap);
-        if (c.up)
-            ragged_simt_kernel<true><<<grid, TILE_ROWS, 0, c.st>>>(p);
-        else
-            ragged_simt_kernel<false><<<grid, TILE_ROWS, 0, c.st>>>(p);
-        e = cudaGetLastError();
+// The activations of every slot an expert has, as f16 in slot order: xh[s] =
+// f16(x[rows ? rows[s] : s]).  One CTA per slot (walked with a stride), 8 or 1
+// elements per thread (VEC).  fp32 and bf16 values beyond the f16 range and row
+// indices outside [0, X) (zeros) are reported.
+template <int VEC>
+__global__ void __launch_bounds__(256) ragged_rows_kernel(const void* __restrict__ x, int dt, int64_t X, int64_t K,
+                                                          const int32_t* __restrict__ rows,
+                                                          const int32_t* __restrict__ offsets, int E, int64_t R,
+                                                          __half* __restrict__ xh, DeviceStatus* status) {
+    const int64_t lo = offsets[0] > 0 ? offsets[0] : 0, hi = offsets[E] < R ? offsets[E] : R;
+    bool over = false;
+    for (int64_t s = lo + blockIdx.x; s < hi; s += gridDim.x) {
+        int64_t row = rows ? rows[s] : s;
+        if (row < 0 || row >= X) {
+            if (threadIdx.x == 0) raise_index(status, kIndexRow);
+            row = -1;
+        }
+        for (int64_t k = (int64_t)threadIdx.x * VEC; k < K; k += 256 * VEC) {
+            const int64_t i = row * K + k;
+            __half* out = xh + s * K + k;
+            if constexpr (VEC == 1) {
+                const float v = row < 0 ? 0.0f : load_x(x, dt, i);
+                over |= f16_overflows(v);
+                *out = __float2half_rn(v);
+            } else {
+                uint4 h = make_uint4(0u, 0u, 0u, 0u);
+                if (row >= 0 && dt == NXQ_F16) {
+                    h = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(x) + i));
+                } else if (row >= 0) {
+                    float v[8];
+                    if (dt == NXQ_F32) {
+                        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+                        const float4 a = __ldg(q), b = __ldg(q + 1);
+                        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                    } else {
+                        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + i));
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            v[2 * j] = __uint_as_float(w[j] << 16);
+                            v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                        }
+                    }
+                    uint32_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        over |= f16_overflows(v[2 * j]) || f16_overflows(v[2 * j + 1]);
+                        const __half2 p = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                        o[j] = *reinterpret_cast<const uint32_t*>(&p);
+                    }
+                    h = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+                *reinterpret_cast<uint4*>(out) = h;
+            }
+        }
     }
-    note_launches(2);
-    cudaFreeAsync(plan, c.st);
+    if (over) raise_range(status, 1u);
+}
+
+cudaError_t launch_rows(const RaggedCall& c, __half* xh) {
+    const int64_t cap = (int64_t)context_sm_count() * 8;
+    const unsigned grid = (unsigned)(c.R < cap ? c.R : cap);
+    const int64_t K = c.w->shape.K;
+    if (((uintptr_t)c.x % 16) == 0)  // K is a multiple of 32
+        ragged_rows_kernel<8><<<grid, 256, 0, c.st>>>(c.x, c.x_dtype, c.X, K, c.rows, c.offsets, c.w->count, c.R, xh,
+                                                      context_status());
+    else
+        ragged_rows_kernel<1><<<grid, 256, 0, c.st>>>(c.x, c.x_dtype, c.X, K, c.rows, c.offsets, c.w->count, c.R, xh,
+                                                      context_status());
+    note_launches(1);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_plan(const RaggedCall& c, int blk, RaggedPlan* plan) {
+    ragged_plan_kernel<<<1, kMaxExperts, 0, c.st>>>(c.offsets, c.w->count, c.R, blk, plan, context_status());
+    note_launches(1);
+    return cudaGetLastError();
+}
+
+int run_simt(const RaggedCall& c, const RaggedPlan* plan) {
+    SimtParams p{c.w->dev, c.up ? c.up->dev : nullptr, c.w->shape, c.x, c.x_dtype, c.X, c.rows, c.y, c.y_dtype, plan,
+                 context_status()};
+    const int64_t work = ragged_max_blocks(c.w->count, c.R, kSimtBlk) * c.w->shape.tiles;
+    const int64_t cap = (int64_t)context_sm_count() * 16;
+    const unsigned grid = (unsigned)(work < cap ? work : cap);
+    if (c.up)
+        ragged_simt_kernel<true><<<grid, TILE_ROWS, 0, c.st>>>(p);
+    else
+        ragged_simt_kernel<false><<<grid, TILE_ROWS, 0, c.st>>>(p);
+    note_launches(1);
+    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "ragged product launch");
+}
+
+// Plan, activations and product of a call, in one stream-ordered workspace.
+int dispatch(const RaggedCall& c) {
+    const bool gemm = ragged_gemm_supported(c.w->shape);
+    const bool as_is = !gemm || (c.x_dtype == NXQ_F16 && !c.rows && ((uintptr_t)c.x % 16) == 0);
+    const int blk = gemm ? ragged_gemm_blk(c.up != nullptr) : kSimtBlk;
+    const int64_t most = c.w->count < c.R ? c.w->count : c.R;
+    const size_t plan_size = (plan_bytes(most) + 255) & ~(size_t)255;
+    uint8_t* ws = nullptr;
+    cudaError_t e = cudaMallocAsync((void**)&ws, plan_size + (as_is ? 0 : (size_t)c.R * c.w->shape.K * sizeof(__half)), c.st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (ragged workspace)");
+    RaggedPlan* plan = reinterpret_cast<RaggedPlan*>(ws);
+    __half* xh = reinterpret_cast<__half*>(ws + plan_size);
+    int rc = NXQ_OK;
+    if ((e = launch_plan(c, blk, plan)) != cudaSuccess || (!as_is && (e = launch_rows(c, xh)) != cudaSuccess))
+        rc = cuda_fail(e, "ragged plan launch");
+    if (rc == NXQ_OK) rc = gemm ? ragged_gemm(c, as_is ? c.x : xh, as_is ? c.X : c.R, plan) : run_simt(c, plan);
+    cudaFreeAsync(ws, c.st);
+    return rc;
 }
 
 int run(nxq_experts_t he, nxq_experts_t hu, bool pair, const void* x_dev, int x_dtype, int64_t X, const int32_t* rows_dev,
@@ -226,7 +318,7 @@ int run(nxq_experts_t he, nxq_experts_t hu, bool pair, const void* x_dev, int x_
     c.R = R;
     c.offsets = offsets_dev;
     c.st = (cudaStream_t)stream;
-    return run_simt(c);
+    return dispatch(c);
 }
 
 }  // namespace

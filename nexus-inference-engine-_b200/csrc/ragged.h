@@ -50,31 +50,71 @@ struct RaggedCall {
     cudaStream_t st;
 };
 
-// One work tile: weight tile `tile` of entry `i`, rows [row0, row0 + rows).
+// One work tile: weight tile `tile` of expert e, slots [row0, row0 + rows).
 struct RaggedTile {
     int e, tile, row0, rows;
 };
-// Work tile g of a plan whose experts have `tiles` weight tiles each.
-__device__ __forceinline__ RaggedTile ragged_tile(const RaggedPlan* plan, int blk, int tiles, int64_t g) {
-    // The last entry whose first work tile is <= g.
-    int lo = 0, hi = plan->entries - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int64_t)plan->it[mid].blk0 * tiles <= g)
-            lo = mid;
-        else
-            hi = mid - 1;
+
+// Walks a plan's work tiles in ascending order (experts of `tiles` weight tiles,
+// row blocks of at most `blk` slots).  EVEN: an expert's slots are cut into row
+// blocks of nearly equal size, a multiple of 16, instead of full ones and a rest
+// (with more than 8 blocks the rest is small beside them, and the rounding
+// could leave the last block empty).
+template <bool EVEN>
+struct RaggedWalk {
+    const RaggedPlan* plan;
+    int blk, tiles, entries, i;
+    int64_t first, end;  // work tiles of entry i
+    RaggedEntry cur;
+    int nb;
+    __device__ __forceinline__ void load(int j) {
+        i = j;
+        const int4 v = *reinterpret_cast<const int4*>(&plan->it[j]);
+        cur = RaggedEntry{v.x, v.y, v.z, v.w};
+        nb = (cur.rows + blk - 1) / blk;
+        first = (int64_t)cur.blk0 * tiles;
+        end = first + (int64_t)nb * tiles;
     }
-    const RaggedEntry it = plan->it[lo];
-    const int nb = (it.rows + blk - 1) / blk;
-    const int local = (int)(g - (int64_t)it.blk0 * tiles);
-    RaggedTile t;
-    t.e = it.e;
-    t.tile = local / nb;
-    const int b = local - t.tile * nb;
-    t.row0 = it.row0 + b * blk;
-    t.rows = it.rows - b * blk < blk ? it.rows - b * blk : blk;
-    return t;
-}
+    // Starts at work tile g (one that exists).
+    __device__ __forceinline__ void start(const RaggedPlan* p, int blk_, int tiles_, int64_t g) {
+        plan = p;
+        blk = blk_;
+        tiles = tiles_;
+        entries = p->entries;
+        int lo = 0, hi = entries - 1;  // the last entry whose first work tile is <= g
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if ((int64_t)p->it[mid].blk0 * tiles <= g)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        load(lo);
+    }
+    // Work tile g, not before the last one asked for.
+    __device__ __forceinline__ RaggedTile at(int64_t g) {
+        while (g >= end && i + 1 < entries) load(i + 1);
+        const int local = (int)(g - first);
+        RaggedTile t;
+        t.e = cur.e;
+        t.tile = local / nb;
+        const int b = local - t.tile * nb;
+        int rb = blk;
+        if (EVEN && nb <= 8) rb = ((cur.rows + nb - 1) / nb + 15) & ~15;
+        t.row0 = cur.row0 + b * rb;
+        t.rows = cur.rows - b * rb < rb ? cur.rows - b * rb : rb;
+        return t;
+    }
+};
+
+// Row blocks a plan can have at most.
+inline int64_t ragged_max_blocks(int64_t E, int64_t R, int blk) { return (E < R ? E : R) + R / blk; }
+
+// tcgen05 kernel (ragged_gemm.cu): xh [X][K] f16, 16-byte aligned, slot s reads
+// row s.  `plan` is made for row blocks of ragged_gemm_blk(pair) slots.
+int ragged_gemm_init();
+bool ragged_gemm_supported(const TiledShape& s);
+int ragged_gemm_blk(bool pair);
+int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan);
 
 }  // namespace nxq

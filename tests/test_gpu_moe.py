@@ -431,6 +431,26 @@ def test_ragged_infinite_values_stay_in_their_rows(gpu):
             w.release()
 
 
+@pytest.mark.parametrize("n", [2, 200])
+def test_ragged_range_error(gpu, n):
+    ws, _ = make_weights(gpu, 12, 2, 128, 256, 5)
+    E = gpu.Experts(ws)
+    try:
+        x = torch.zeros((n, 256), device="cuda")
+        x[n - 1, 3] = 6.6e4
+        gpu.qmatmul_ragged(E, x, make_offsets([1, n - 1]))
+        with pytest.raises(gpu.NxqError) as e:
+            gpu.stream_sync()
+        assert e.value.name == "ERR_RANGE"
+        x[n - 1, 3] = 65519.0
+        gpu.qmatmul_ragged(E, x, make_offsets([1, n - 1]))
+        gpu.stream_sync()
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
 def test_expert_table_lifetime(gpu):
     ws, _ = make_weights(gpu, 12, 2, 128, 256, 5)
     other = gpu.Weight.register(synth.make_blocks(12, 128, 512, seed=1), 12, 128, 512)
