@@ -10,8 +10,8 @@
 //                as the block has slots for
 //   warps 2-17   four dequant warpgroups: thread r decodes row r's 32-element
 //                group to f16 and writes it to TMEM, the MMA's A operand
-//   warp 1       one thread issues tcgen05.mma kind::f16 M=128, K=16 with N =
-//                the block's slots rounded up to 16 (a short block costs less)
+//   warp 1       one lane issues tcgen05.mma kind::f16 M=128, K=16 with N = the
+//                block's slots rounded up to 16 (a short block costs less)
 //   warps 18-25  epilogue: tcgen05.ld of the accumulator, conversion, store of
 //                the block's slots only
 // Plain form: row blocks of up to 256 slots, one 256-column fp32 accumulator.
@@ -19,6 +19,13 @@
 // accumulators; every k-step feeds the same activations to a gate and an up
 // MMA (warpgroups 0, 1 decode the gate, 2, 3 the up weight), and the
 // epilogue stores silu(gate) * up, so the two products never reach memory.
+//
+// A k-step's activations and its A operand share one ring stage, released by
+// one commit.  There are as many stages as k-steps in a chunk, so every stage
+// index is a constant.  The issuing loop runs warp-wide with only the MMA and
+// the commit in the elected lane: with the loop in one lane and two rings
+// it took 1060 cycles a k-step whatever the block's size (four MMAs
+// at ~92 cycles of issue each, measured), twice the 512 of a 256-slot MMA.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes
 // hold behind a block's slots (the next expert's rows, or zeros) reaches no
@@ -44,7 +51,7 @@ constexpr int kWarpWProducer = kWarpEpi0 + kEpiWarps;
 constexpr int kThreads = 32 * (kWarpWProducer + 1);
 constexpr int kKS = 64;  // reduction elements per k-step (one swizzle atom)
 constexpr int kStepsPerChunk = CHUNK_K / kKS;
-constexpr int kAStages = 4;         // TMEM A buffers of 32 columns
+constexpr int kStages = kStepsPerChunk;  // ring: activations (shared memory) and A operand (TMEM)
 constexpr int kBarBytes = 512;
 constexpr uint32_t kColD = 256;     // accumulators: columns 256..511
 constexpr uint32_t kTmemCols = 512;
@@ -57,12 +64,14 @@ struct Cfg {
     static constexpr int NT = PAIR ? 128 : 256;  // slots per work tile
     static constexpr int XB = NT * kKS * 2;
     static constexpr int kBudget = 227 * 1024 - 1024 - kBarBytes;
-    static constexpr int kX = PAIR ? 6 : 4;
-    static constexpr int kWMax = PAIR ? 6 : 4;
-    static constexpr int fit = (kBudget - kX * XB) / WB;
+    static constexpr int kMats = PAIR ? 2 : 1;
+    static constexpr int kACols = 32 * kMats;    // TMEM columns of a stage's A operand
+    static constexpr int kWMax = 4 * kMats;
+    static constexpr int fit = (kBudget - kStages * XB) / WB;
     static constexpr int kW = fit > kWMax ? kWMax : fit;
     static_assert(kW >= 2, "tile-chunk ring too shallow");
-    static constexpr size_t smem = 1024 + (size_t)kX * XB + (size_t)kW * WB + kBarBytes;
+    static_assert(kStages * kACols <= (int)kColD, "A stages overlap the accumulator");
+    static constexpr size_t smem = 1024 + (size_t)kStages * XB + (size_t)kW * WB + kBarBytes;
 };
 
 struct Params {
@@ -112,23 +121,19 @@ __device__ __forceinline__ void dq_step(const uint8_t* stage, int r, int h, uint
 template <int TYPE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap xmap) {
     using C = Cfg<TYPE, PAIR>;
-    constexpr int WB = C::WB, XB = C::XB, NT = C::NT, kXStages = C::kX, kWStages = C::kW;
-    constexpr int kMats = PAIR ? 2 : 1;
-    static_assert((2 * kXStages + 2 * kWStages + 2 * kAStages + 3) * 8 + 8 <= kBarBytes, "barrier area too small");
-    static_assert(kAStages * 32 <= (int)kColD, "A stages overlap the accumulator");
+    constexpr int WB = C::WB, XB = C::XB, NT = C::NT, kWStages = C::kW, kMats = C::kMats, kACols = C::kACols;
+    static_assert((3 * kStages + 2 * kWStages + 3) * 8 + 8 <= kBarBytes, "barrier area too small");
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
     uint8_t* xs = smem;
-    uint8_t* ws = smem + kXStages * XB;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(ws + kWStages * WB);
-    uint64_t* x_full = bars;
-    uint64_t* x_empty = x_full + kXStages;
-    uint64_t* w_full = x_empty + kXStages;
+    uint8_t* ws = smem + kStages * XB;
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(ws + kWStages * WB);  // activations landed
+    uint64_t* a_full = x_full + kStages;                                 // A operand written
+    uint64_t* empty = a_full + kStages;                                  // the MMA is done with both
+    uint64_t* w_full = empty + kStages;
     uint64_t* w_empty = w_full + kWStages;
-    uint64_t* a_full = w_empty + kWStages;
-    uint64_t* a_empty = a_full + kAStages;
-    uint64_t* d_full = a_empty + kAStages;
+    uint64_t* d_full = w_empty + kWStages;
     uint64_t* d_empty = d_full + 1;
     uint64_t* drain = d_empty + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -141,17 +146,14 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ptx::WaitCtl ctl{abort_flag, p.status};
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kXStages; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             ptx::mbar_init(&x_full[i], 1);
-            ptx::mbar_init(&x_empty[i], 1);
+            ptx::mbar_init(&a_full[i], 8 * kMats);  // the warps that write the A operand
+            ptx::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < kWStages; ++i) {
             ptx::mbar_init(&w_full[i], 1);
             ptx::mbar_init(&w_empty[i], 4 * kDeqGroups / kMats);  // the warps that decode a tile-chunk
-        }
-        for (int i = 0; i < kAStages; ++i) {
-            ptx::mbar_init(&a_full[i], 8);
-            ptx::mbar_init(&a_empty[i], 1);
         }
         ptx::mbar_init(d_full, 1);
         ptx::mbar_init(d_empty, kEpiWarps);
@@ -197,90 +199,93 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             }
         }
     } else if (warp == kWarpProducer) {
-        if (lane == 0) {
-            ptx::prefetch_tmap(&xmap);
-            uint32_t qx = 0;
-            bool ok = true;
-            RaggedWalk<true> walk;
-            walk.start(p.plan, NT, tiles, blockIdx.x);
-            for (int64_t g = blockIdx.x; g < total && ok; g += G) {
-                const RaggedTile t = walk.at(g);
-                const int boxes = (t.rows + kBoxRows - 1) / kBoxRows;
-                for (int c = 0; c < chunks && ok; ++c) {
-                    for (int st = 0; st < kStepsPerChunk; ++st, ++qx) {
-                        const int sx = qx % kXStages;
-                        if (qx >= kXStages && !(ok = ptx::mbar_wait(&x_empty[sx], ((qx / kXStages) & 1) ^ 1u, ctl, 42))) break;
-                        ptx::mbar_arrive_expect_tx(&x_full[sx], boxes * kBoxBytes);
-                        for (int b = 0; b < boxes; ++b)
-                            ptx::tma_load_2d(xs + sx * XB + b * kBoxBytes, &xmap, c * CHUNK_K + st * kKS,
-                                             t.row0 + b * kBoxRows, &x_full[sx]);
-                    }
+        if (lane == 0) ptx::prefetch_tmap(&xmap);
+        uint32_t cc = 0;  // chunks so far: its parity is the stages' phase
+        bool ok = true;
+        RaggedWalk<true> walk;
+        walk.start(p.plan, NT, tiles, blockIdx.x);
+        uint32_t issued = 0;  // k-steps requested
+        for (int64_t g = blockIdx.x; g < total && ok; g += G) {
+            const RaggedTile t = walk.at(g);
+            const int boxes = (t.rows + kBoxRows - 1) / kBoxRows;
+            for (int c = 0; c < chunks && ok; ++c) {
+#pragma unroll
+                for (int st = 0; st < kStages; ++st) {
+                    ok = ok && ptx::mbar_wait(&empty[st], (cc & 1) ^ 1u, ctl, 42);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) continue;
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[st], boxes * kBoxBytes);
+                    __syncwarp();
+                    if (lane < boxes)
+                        ptx::tma_load_2d(xs + st * XB + lane * kBoxBytes, &xmap, c * CHUNK_K + st * kKS,
+                                         t.row0 + lane * kBoxRows, &x_full[st]);
+                    ++issued;
                 }
+                if (ok) ++cc;
             }
-            // Do not leave with copies in flight (bounded, ignoring the abort flag).
-            for (uint32_t k = qx >= kXStages ? qx - kXStages : 0; k < qx; ++k) {
-                const long long t0 = clock64();
-                while (!ptx::mbar_try_wait(&x_full[k % kXStages], (k / kXStages) & 1) && clock64() - t0 < ptx::kWaitCycles) {
-                }
+        }
+        // Do not leave with copies in flight (bounded, ignoring the abort flag).
+        for (uint32_t k = issued >= kStages ? issued - kStages : 0; k < issued; ++k) {
+            const long long t0 = clock64();
+            while (!ptx::mbar_try_wait(&x_full[k % kStages], (k / kStages) & 1) && clock64() - t0 < ptx::kWaitCycles) {
             }
         }
     } else if (warp == kWarpMma) {
-        if (lane == 0) {
-            uint32_t qx = 0, qa = 0, nt = 0;
-            bool ok = true;
-            RaggedWalk<true> walk;
-            walk.start(p.plan, NT, tiles, blockIdx.x);
-            for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
-                const RaggedTile t = walk.at(g);
-                const uint32_t idesc = ptx::idesc_f16_f32(128, (t.rows + 15) & ~15);
-                if (nt > 0 && !(ok = ptx::mbar_wait(d_empty, (nt - 1) & 1, ctl, 43))) break;
-                ptx::tc_fence_after();
-                for (int c = 0; c < chunks && ok; ++c) {
-                    for (int st = 0; st < kStepsPerChunk && ok; ++st, ++qx) {
-                        const int sx = qx % kXStages;
-                        if (!(ok = ptx::mbar_wait(&x_full[sx], (qx / kXStages) & 1, ctl, 44))) break;
-                        const uint32_t xb = ptx::smem_addr(xs + sx * XB);
+        uint32_t cc = 0, nt = 0;
+        bool ok = true;
+        RaggedWalk<true> walk;
+        walk.start(p.plan, NT, tiles, blockIdx.x);
+        const uint64_t desc0 = ptx::desc_sw128_kmajor(ptx::smem_addr(xs));
+        for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
+            const RaggedTile t = walk.at(g);
+            const uint32_t idesc = ptx::idesc_f16_f32(128, (t.rows + 15) & ~15);
+            ok = nt == 0 || ptx::mbar_wait(d_empty, (nt - 1) & 1, ctl, 43);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            ptx::tc_fence_after();
+            for (int c = 0; c < chunks && ok; ++c, ++cc) {
 #pragma unroll
-                        for (int mat = 0; mat < kMats; ++mat, ++qa) {
-                            const int sa = qa % kAStages;
-                            if (!(ok = ptx::mbar_wait(&a_full[sa], (qa / kAStages) & 1, ctl, 45))) break;
-                            ptx::tc_fence_after();
+                for (int st = 0; st < kStages; ++st) {
+                    ok = ok && ptx::mbar_wait(&x_full[st], cc & 1, ctl, 44) && ptx::mbar_wait(&a_full[st], cc & 1, ctl, 45);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) continue;
+                    ptx::tc_fence_after();
+                    if (ptx::elect_one()) {
 #pragma unroll
-                            for (int kk = 0; kk < kKS / 16; ++kk)
-                                ptx::mma_ts_f16(tmem + kColD + mat * NT, tmem + sa * 32 + kk * 8,
-                                                ptx::desc_sw128_kmajor(xb + kk * 32), idesc,
-                                                (c == 0 && st == 0 && kk == 0) ? 0u : 1u);
-                            if (mat == kMats - 1) ptx::mma_commit(&x_empty[sx]);
-                            ptx::mma_commit(&a_empty[sa]);
-                        }
+                        for (int mat = 0; mat < kMats; ++mat)
+                            ptx::mma_ts_f16_k64(tmem + kColD + mat * NT, tmem + st * kACols + mat * 32,
+                                                desc0 + ((st * XB) >> 4), idesc, (c | st) ? 1u : 0u);
+                        ptx::mma_commit(&empty[st]);
+                        if (st == kStages - 1 && c == chunks - 1) ptx::mma_commit(d_full);
                     }
+                    __syncwarp();
                 }
-                if (ok) ptx::mma_commit(d_full);
-            }
-            ptx::mma_commit(drain);
-            const long long t0 = clock64();
-            while (!ptx::mbar_try_wait(drain, 0) && clock64() - t0 < ptx::kWaitCycles) {
             }
         }
+        if (ptx::elect_one()) ptx::mma_commit(drain);
+        __syncwarp();
+        const long long t0 = clock64();
+        while (!ptx::mbar_try_wait(drain, 0) && clock64() - t0 < ptx::kWaitCycles) {
+        }
     } else if (warp < kWarpEpi0) {
-        // A stages are numbered qa = k-step (plain) or 2 k-step + matrix (PAIR).
-        // Warpgroup wg takes the stages of parity wg / 2, k group wg % 2.
+        // Warpgroup wg decodes k group wg % 2 of a k-step: plain, of the k-steps
+        // of parity wg / 2; PAIR, of every k-step of matrix wg / 2.
         const int wg = (warp - kWarpDeq0) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const int h = wg & 1, par = wg >> 1;
-        uint32_t qw = PAIR ? par : 0, qa = PAIR ? par : 0;
+        uint32_t qw = PAIR ? par : 0, cc = 0;
         bool ok = true;
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
-            for (int c = 0; c < chunks && ok; ++c, qw += kMats) {
+            for (int c = 0; c < chunks && ok; ++c, ++cc, qw += kMats) {
                 const int sw = qw % kWStages;
                 if (!(ok = warp_wait(&w_full[sw], (qw / kWStages) & 1, ctl, 46))) break;
                 const uint8_t* stage = ws + sw * WB;
 #pragma unroll
-                for (int st = 0; st < kStepsPerChunk; ++st, qa += kMats) {
+                for (int st = 0; st < kStages; ++st) {
                     if (!PAIR && (st & 1) != par) continue;
-                    const int sa = qa % kAStages;
-                    if (qa >= kAStages && !(ok = warp_wait(&a_empty[sa], ((qa / kAStages) & 1) ^ 1u, ctl, 47))) break;
+                    ok = ok && warp_wait(&empty[st], (cc & 1) ^ 1u, ctl, 47);
+                    if (!ok) continue;
                     ptx::tc_fence_after();
-                    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + sa * 32 + 16 * h;
+                    const uint32_t taddr =
+                        tmem + ((uint32_t)(quad * 32) << 16) + st * kACols + (PAIR ? 32 * par : 0) + 16 * h;
                     if (st == 0) dq_step<TYPE, 0>(stage, r, h, taddr);
                     if (st == 1) dq_step<TYPE, 1>(stage, r, h, taddr);
                     if (st == 2) dq_step<TYPE, 2>(stage, r, h, taddr);
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&a_full[sa]);
+                    if (lane == 0) ptx::mbar_arrive(&a_full[st]);
                 }
                 __syncwarp();
                 if (ok && lane == 0) ptx::mbar_arrive(&w_empty[sw]);
