@@ -276,7 +276,7 @@ int run_simt(const RaggedCall& c, const RaggedPlan* plan) {
 int dispatch(const RaggedCall& c) {
     const bool gemm = ragged_gemm_supported(c.w->shape);
     const bool as_is = !gemm || (c.x_dtype == NXQ_F16 && !c.rows && ((uintptr_t)c.x % 16) == 0);
-    const int blk = gemm ? ragged_gemm_blk(c.up != nullptr) : kSimtBlk;
+    const int blk = gemm ? ragged_gemm_blk() : kSimtBlk;
     const int64_t most = c.w->count < c.R ? c.w->count : c.R;
     const size_t plan_size = (plan_bytes(most) + 255) & ~(size_t)255;
     uint8_t* ws = nullptr;

@@ -111,10 +111,10 @@ struct RaggedWalk {
 inline int64_t ragged_max_blocks(int64_t E, int64_t R, int blk) { return (E < R ? E : R) + R / blk; }
 
 // tcgen05 kernel (ragged_gemm.cu): xh [X][K] f16, 16-byte aligned, slot s reads
-// row s.  `plan` is made for row blocks of ragged_gemm_blk(pair) slots.
+// row s.  `plan` is made for row blocks of ragged_gemm_blk() slots.
 int ragged_gemm_init();
 bool ragged_gemm_supported(const TiledShape& s);
-int ragged_gemm_blk(bool pair);
+int ragged_gemm_blk();
 int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan);
 
 }  // namespace nxq

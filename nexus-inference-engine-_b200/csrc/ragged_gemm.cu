@@ -1,31 +1,32 @@
 // Tensor-core ragged products on tcgen05 / TMEM: y[s] = x[s] W_e^T for the
 // slots of every expert, and the SwiGLU form with a gate and an up product.
 //
-// A persistent grid of one CTA per SM walks the plan's work tiles (ragged.h): 128
-// weight rows x one row block of an expert.  The roles are those of the dense
-// prefill GEMM (qmm_gemm.cu), per 64-element k-step:
+// A persistent grid of one CTA per SM walks the plan's work tiles (ragged.h): two
+// 128-row weight tiles x one row block of up to 128 slots of an expert.  The
+// two tiles are neighbours of one weight (plain), or the gate's and the up
+// weight's (PAIR); both multiply the same activations, so an SM reads 32 bytes of
+// activations and 18 of Q4_K weights per cycle of MMA work, where one tile x
+// 256 slots would read 64 and 9.  Roles, per 64-element k-step:
 //   warp 26      producer: the packed tile-chunks (256 k) by 1-D bulk copies
 //   warp 0       producer: the activations of the row block by TMA, as boxes of
 //                64 k x 64 slots (128-byte swizzle, no multicast), only as many
 //                as the block has slots for
-//   warps 2-17   four dequant warpgroups: thread r decodes row r's 32-element
-//                group to f16 and writes it to TMEM, the MMA's A operand
+//   warps 2-17   four dequant warpgroups, one per tile and k-step parity: thread
+//                r decodes the 64 elements of row r (the lane decoders of the
+//                decode GEMV) and writes them to TMEM, the MMA's A operand
 //   warp 1       one lane issues tcgen05.mma kind::f16 M=128, K=16 with N = the
-//                block's slots rounded up to 16 (a short block costs less)
-//   warps 18-25  epilogue: tcgen05.ld of the accumulator, conversion, store of
-//                the block's slots only
-// Plain form: row blocks of up to 256 slots, one 256-column fp32 accumulator.
-// SwiGLU form (PAIR): row blocks of up to 128 slots and two 128-column
-// accumulators; every k-step feeds the same activations to a gate and an up
-// MMA (warpgroups 0, 1 decode the gate, 2, 3 the up weight), and the
-// epilogue stores silu(gate) * up, so the two products never reach memory.
+//                block's slots rounded up to 16 (a short block costs less), into
+//                one 128-column fp32 accumulator per tile
+//   warps 18-25  epilogue: tcgen05.ld of the accumulators, conversion (PAIR:
+//                silu(gate) * up, so the two products never reach memory), and
+//                16-bit outputs through a staging buffer in shared memory: the
+//                accumulators are handed back as soon as they are read, and
+//                rows leave as 16-byte stores while the next tile's MMAs run
 //
-// A k-step's activations and its A operand share one ring stage, released by
-// one commit.  There are as many stages as k-steps in a chunk, so every stage
-// index is a constant.  The issuing loop runs warp-wide with only the MMA and
-// the commit in the elected lane: with the loop in one lane and two rings
-// it took 1060 cycles a k-step whatever the block's size (four MMAs
-// at ~92 cycles of issue each, measured), twice the 512 of a 256-slot MMA.
+// The A operand's ring has as many stages as a chunk has k-steps, so its indexes
+// are constants; the issuing loop runs warp-wide, half the lanes watching the
+// activations and half the A operand, with only the MMA and the commits in the
+// elected lane.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes
 // hold behind a block's slots (the next expert's rows, or zeros) reaches no
@@ -35,7 +36,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "dq_f16.cuh"
+#include "lane_dq.cuh"
 #include "qmm_gemm.h"
 #include "ragged.h"
 #include "sm100_ptx.cuh"
@@ -45,115 +46,149 @@ namespace nxq {
 namespace {
 
 constexpr int kDeqGroups = 4;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
 constexpr int kWarpProducer = 0, kWarpMma = 1, kWarpDeq0 = 2, kWarpEpi0 = 2 + 4 * kDeqGroups;
 constexpr int kWarpWProducer = kWarpEpi0 + kEpiWarps;
 constexpr int kThreads = 32 * (kWarpWProducer + 1);
-constexpr int kKS = 64;  // reduction elements per k-step (one swizzle atom)
+constexpr int kMats = 2;  // weight tiles of a work tile
+constexpr int kNT = 128;  // slots of a work tile
+constexpr int kKS = 64;   // reduction elements per k-step (one swizzle atom)
 constexpr int kStepsPerChunk = CHUNK_K / kKS;
-constexpr int kStages = kStepsPerChunk;  // ring: activations (shared memory) and A operand (TMEM)
+constexpr int kAStages = kStepsPerChunk;  // TMEM A ring
+constexpr int kACols = 32 * kMats;        // TMEM columns of a stage
 constexpr int kBarBytes = 512;
-constexpr uint32_t kColD = 256;     // accumulators: columns 256..511
+constexpr uint32_t kColD = 256;  // accumulators: columns 256 + 128 mat
 constexpr uint32_t kTmemCols = 512;
 constexpr int kBoxRows = 64;
 constexpr int kBoxBytes = kBoxRows * kKS * 2;
+constexpr int kXB = kNT * kKS * 2;                 // 16 KB of activations per k-step
+constexpr int kStageOut = kNT * TILE_ROWS * 2;     // 32 KB: one tile's 16-bit outputs [slot][row]
+static_assert(kAStages * kACols <= (int)kColD, "A stages overlap the accumulators");
 
-template <int TYPE, bool PAIR>
-struct Cfg {
-    static constexpr int WB = dq::Group<TYPE>::kStage;
-    static constexpr int NT = PAIR ? 128 : 256;  // slots per work tile
-    static constexpr int XB = NT * kKS * 2;
-    static constexpr int kBudget = 227 * 1024 - 1024 - kBarBytes;
-    static constexpr int kMats = PAIR ? 2 : 1;
-    static constexpr int kACols = 32 * kMats;    // TMEM columns of a stage's A operand
-    static constexpr int kWMax = 4 * kMats;
-    static constexpr int fit = (kBudget - kStages * XB) / WB;
-    static constexpr int kW = fit > kWMax ? kWMax : fit;
+// Ring depths: six k-steps of activations where four tile-chunks (two of each
+// tile) still fit beside them, else four, then as many tile-chunks as fit (up to 6).
+template <int TYPE>
+struct Rings {
+    static constexpr int WB = lane::Lane<TYPE>::kStage;
+    static constexpr int kBudget = 227 * 1024 - 1024 - kBarBytes - kStageOut;
+    static constexpr int kX = (kBudget - 6 * kXB) / WB >= 4 ? 6 : 4;
+    static constexpr int fit = (kBudget - kX * kXB) / WB;
+    static constexpr int kW = fit > 6 ? 6 : fit;
     static_assert(kW >= 2, "tile-chunk ring too shallow");
-    static_assert(kStages * kACols <= (int)kColD, "A stages overlap the accumulator");
-    static constexpr size_t smem = 1024 + (size_t)kStages * XB + (size_t)kW * WB + kBarBytes;
+    static_assert((2 * kX + 2 * kW + 2 * kAStages + 3) * 8 + 8 <= kBarBytes, "barrier area too small");
+    static constexpr size_t smem = 1024 + (size_t)kX * kXB + kStageOut + (size_t)kW * WB + kBarBytes;
 };
 
 struct Params {
     const uint8_t* const* w;
     const uint8_t* const* up;
     TiledShape s;
+    int tiles;  // work tiles per row block
     void* y;
     int y_dtype;
+    int vec;  // rows of y are 16-byte aligned
     const RaggedPlan* plan;
     DeviceStatus* status;
 };
 
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// y[m0 + j][n] = v[j] for j < cnt (element offset `off` = m0 * N + n).
-template <typename T>
-__device__ __forceinline__ void store_col(void* y, int64_t off, int64_t N, int cnt, const uint32_t (&v)[32]) {
-    T* q = reinterpret_cast<T*>(y) + off;
-#pragma unroll
-    for (int j = 0; j < 32; ++j, q += N)
-        if (j < cnt) *q = from_f32<T>(__uint_as_float(v[j]));
+__device__ __forceinline__ uint32_t pack16(bool bf16, float a, float b) {
+    if (bf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// silu(g) * u.  The fast division is within 2 ulp; for 1 + exp(-g) above 2^126
+// it gives 0 where the quotient is below 2^-119.
+__device__ __forceinline__ float swiglu1(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const ptx::WaitCtl& c, unsigned where) {
     int ok = 0;
     if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity, c, where) ? 1 : 0;
     return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
 }
+// A barrier of the epilogue warps that tells whether `ok` holds in all of them.
+__device__ __forceinline__ bool epi_all(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "barrier.cta.red.and.pred p, 1, %2, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "n"(kEpiThreads)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
 
-template <int TYPE, int S>
-__device__ __forceinline__ void dq_step(const uint8_t* stage, int r, int h, uint32_t taddr) {
-    uint32_t o[16];
-    if (h == 0)
-        dq::Group<TYPE>::template decode<2 * S>(stage, r, o);
-    else
-        dq::Group<TYPE>::template decode<2 * S + 1>(stage, r, o);
-    ptx::tmem_st16(taddr, o);
+// Ring position: stage index and the phase parity of its current use.
+struct Ring {
+    int i = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++i == n) {
+            i = 0;
+            ph ^= 1u;
+        }
+    }
+};
+
+// Weight tile `mat` of work tile t: the tile's index, and whether it exists (a
+// weight with an odd number of tiles ends with a work tile of one; its second
+// half repeats the first and is not stored).
+template <bool PAIR>
+__device__ __forceinline__ int weight_tile(const RaggedTile& t, int mat, int64_t tiles, bool* exists) {
+    if (PAIR) {
+        *exists = true;
+        return t.tile;
+    }
+    const int i = 2 * t.tile + mat;
+    *exists = i < tiles;
+    return *exists ? i : 2 * t.tile;
 }
 
 template <int TYPE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap xmap) {
-    using C = Cfg<TYPE, PAIR>;
-    constexpr int WB = C::WB, XB = C::XB, NT = C::NT, kWStages = C::kW, kMats = C::kMats, kACols = C::kACols;
-    static_assert((3 * kStages + 2 * kWStages + 3) * 8 + 8 <= kBarBytes, "barrier area too small");
+    using Rg = Rings<TYPE>;
+    constexpr int WB = Rg::WB, kX = Rg::kX, kW = Rg::kW;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
     uint8_t* xs = smem;
-    uint8_t* ws = smem + kStages * XB;
-    uint64_t* x_full = reinterpret_cast<uint64_t*>(ws + kWStages * WB);  // activations landed
-    uint64_t* a_full = x_full + kStages;                                 // A operand written
-    uint64_t* empty = a_full + kStages;                                  // the MMA is done with both
-    uint64_t* w_full = empty + kStages;
-    uint64_t* w_empty = w_full + kWStages;
-    uint64_t* d_full = w_empty + kWStages;
+    uint8_t* stg = xs + kX * kXB;
+    uint8_t* ws = stg + kStageOut;
+    uint64_t* x_full = reinterpret_cast<uint64_t*>(ws + kW * WB);
+    uint64_t* x_empty = x_full + kX;
+    uint64_t* w_full = x_empty + kX;
+    uint64_t* w_empty = w_full + kW;
+    uint64_t* a_full = w_empty + kW;
+    uint64_t* a_empty = a_full + kAStages;
+    uint64_t* d_full = a_empty + kAStages;
     uint64_t* d_empty = d_full + 1;
     uint64_t* drain = d_empty + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int tiles = (int)p.s.tiles;
-    const int64_t total = (int64_t)p.plan->blocks * tiles;
+    const int64_t total = (int64_t)p.plan->blocks * p.tiles;
     if (blockIdx.x >= total) return;  // the whole CTA, before any barrier or TMEM
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ptx::WaitCtl ctl{abort_flag, p.status};
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < kX; ++i) {
             ptx::mbar_init(&x_full[i], 1);
-            ptx::mbar_init(&a_full[i], 8 * kMats);  // the warps that write the A operand
-            ptx::mbar_init(&empty[i], 1);
+            ptx::mbar_init(&x_empty[i], 1);
         }
-        for (int i = 0; i < kWStages; ++i) {
+        for (int i = 0; i < kW; ++i) {
             ptx::mbar_init(&w_full[i], 1);
             ptx::mbar_init(&w_empty[i], 4 * kDeqGroups / kMats);  // the warps that decode a tile-chunk
+        }
+        for (int i = 0; i < kAStages; ++i) {
+            ptx::mbar_init(&a_full[i], 4 * kMats);  // the warps that write a stage
+            ptx::mbar_init(&a_empty[i], 1);
         }
         ptx::mbar_init(d_full, 1);
         ptx::mbar_init(d_empty, kEpiWarps);
@@ -175,66 +210,72 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
 
     if (warp == kWarpWProducer) {
         if (lane == 0) {
-            uint32_t qw = 0;
+            Ring rw;
+            uint32_t issued = 0;
             bool ok = true;
             RaggedWalk<true> walk;
-            walk.start(p.plan, NT, tiles, blockIdx.x);
+            walk.start(p.plan, kNT, p.tiles, blockIdx.x);
             for (int64_t g = blockIdx.x; g < total && ok; g += G) {
                 const RaggedTile t = walk.at(g);
                 const uint8_t* src[kMats];
-                src[0] = p.w[t.e] + p.s.chunk_offset(t.tile, 0);
-                if constexpr (PAIR) src[1] = p.up[t.e] + p.s.chunk_offset(t.tile, 0);
-                for (int c = 0; c < chunks * kMats && ok; ++c, ++qw) {
-                    const int sw = qw % kWStages;
-                    if (qw >= kWStages && !(ok = ptx::mbar_wait(&w_empty[sw], ((qw / kWStages) & 1) ^ 1u, ctl, 41))) break;
-                    ptx::mbar_arrive_expect_tx(&w_full[sw], WB);
-                    ptx::bulk_g2s(ws + sw * WB, src[c % kMats] + (int64_t)(c / kMats) * WB, WB, &w_full[sw]);
+#pragma unroll
+                for (int mat = 0; mat < kMats; ++mat) {
+                    bool exists;
+                    const int wt = weight_tile<PAIR>(t, mat, p.s.tiles, &exists);
+                    src[mat] = (PAIR && mat ? p.up : p.w)[t.e] + p.s.chunk_offset(wt, 0);
                 }
+                for (int c = 0; c < chunks && ok; ++c)
+#pragma unroll
+                    for (int mat = 0; mat < kMats; ++mat) {
+                        ok = ok && ptx::mbar_wait(&w_empty[rw.i], rw.ph ^ 1u, ctl, 41);
+                        if (!ok) continue;
+                        ptx::mbar_arrive_expect_tx(&w_full[rw.i], WB);
+                        ptx::bulk_g2s(ws + rw.i * WB, src[mat] + (int64_t)c * WB, WB, &w_full[rw.i]);
+                        rw.next(kW);
+                        ++issued;
+                    }
             }
             // Do not leave with copies in flight (bounded, ignoring the abort flag).
-            for (uint32_t k = qw >= kWStages ? qw - kWStages : 0; k < qw; ++k) {
+            for (uint32_t k = issued >= kW ? issued - kW : 0; k < issued; ++k) {
                 const long long t0 = clock64();
-                while (!ptx::mbar_try_wait(&w_full[k % kWStages], (k / kWStages) & 1) && clock64() - t0 < ptx::kWaitCycles) {
+                while (!ptx::mbar_try_wait(&w_full[k % kW], (k / kW) & 1) && clock64() - t0 < ptx::kWaitCycles) {
                 }
             }
         }
     } else if (warp == kWarpProducer) {
         if (lane == 0) ptx::prefetch_tmap(&xmap);
-        uint32_t cc = 0;  // chunks so far: its parity is the stages' phase
+        Ring rx;
+        uint32_t issued = 0;
         bool ok = true;
         RaggedWalk<true> walk;
-        walk.start(p.plan, NT, tiles, blockIdx.x);
-        uint32_t issued = 0;  // k-steps requested
+        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
             const RaggedTile t = walk.at(g);
             const int boxes = (t.rows + kBoxRows - 1) / kBoxRows;
-            for (int c = 0; c < chunks && ok; ++c) {
-#pragma unroll
-                for (int st = 0; st < kStages; ++st) {
-                    ok = ok && ptx::mbar_wait(&empty[st], (cc & 1) ^ 1u, ctl, 42);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) continue;
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[st], boxes * kBoxBytes);
-                    __syncwarp();
-                    if (lane < boxes)
-                        ptx::tma_load_2d(xs + st * XB + lane * kBoxBytes, &xmap, c * CHUNK_K + st * kKS,
-                                         t.row0 + lane * kBoxRows, &x_full[st]);
-                    ++issued;
-                }
-                if (ok) ++cc;
+            for (int ks = 0; ks < chunks * kStepsPerChunk && ok; ++ks) {
+                ok = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(&x_empty[rx.i], rx.ph ^ 1u, ctl, 42));
+                if (!ok) break;
+                if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[rx.i], boxes * kBoxBytes);
+                __syncwarp();
+                if (lane < boxes)
+                    ptx::tma_load_2d(xs + rx.i * kXB + lane * kBoxBytes, &xmap, ks * kKS, t.row0 + lane * kBoxRows,
+                                     &x_full[rx.i]);
+                rx.next(kX);
+                ++issued;
             }
         }
         // Do not leave with copies in flight (bounded, ignoring the abort flag).
-        for (uint32_t k = issued >= kStages ? issued - kStages : 0; k < issued; ++k) {
+        for (uint32_t k = issued >= kX ? issued - kX : 0; k < issued; ++k) {
             const long long t0 = clock64();
-            while (!ptx::mbar_try_wait(&x_full[k % kStages], (k / kStages) & 1) && clock64() - t0 < ptx::kWaitCycles) {
+            while (!ptx::mbar_try_wait(&x_full[k % kX], (k / kX) & 1) && clock64() - t0 < ptx::kWaitCycles) {
             }
         }
     } else if (warp == kWarpMma) {
-        uint32_t cc = 0, nt = 0;
+        uint32_t cc = 0, nt = 0;  // chunks and work tiles so far
         bool ok = true;
+        Ring rx;
         RaggedWalk<true> walk;
-        walk.start(p.plan, NT, tiles, blockIdx.x);
+        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
         const uint64_t desc0 = ptx::desc_sw128_kmajor(ptx::smem_addr(xs));
         for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
             const RaggedTile t = walk.at(g);
@@ -244,20 +285,22 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             ptx::tc_fence_after();
             for (int c = 0; c < chunks && ok; ++c, ++cc) {
 #pragma unroll
-                for (int st = 0; st < kStages; ++st) {
-                    ok = ok && ptx::mbar_wait(&x_full[st], cc & 1, ctl, 44) && ptx::mbar_wait(&a_full[st], cc & 1, ctl, 45);
+                for (int st = 0; st < kAStages; ++st) {
+                    ok = ok && ptx::mbar_wait(lane < 16 ? &x_full[rx.i] : &a_full[st], lane < 16 ? rx.ph : (cc & 1), ctl, 44);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) continue;
                     ptx::tc_fence_after();
                     if (ptx::elect_one()) {
 #pragma unroll
                         for (int mat = 0; mat < kMats; ++mat)
-                            ptx::mma_ts_f16_k64(tmem + kColD + mat * NT, tmem + st * kACols + mat * 32,
-                                                desc0 + ((st * XB) >> 4), idesc, (c | st) ? 1u : 0u);
-                        ptx::mma_commit(&empty[st]);
-                        if (st == kStages - 1 && c == chunks - 1) ptx::mma_commit(d_full);
+                            ptx::mma_ts_f16_k64(tmem + kColD + mat * kNT, tmem + st * kACols + mat * 32,
+                                                desc0 + ((uint32_t)(rx.i * kXB) >> 4), idesc, (c | st) ? 1u : 0u);
+                        ptx::mma_commit(&a_empty[st]);
+                        ptx::mma_commit(&x_empty[rx.i]);
+                        if (st == kAStages - 1 && c == chunks - 1) ptx::mma_commit(d_full);
                     }
                     __syncwarp();
+                    rx.next(kX);
                 }
             }
         }
@@ -267,88 +310,167 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         while (!ptx::mbar_try_wait(drain, 0) && clock64() - t0 < ptx::kWaitCycles) {
         }
     } else if (warp < kWarpEpi0) {
-        // Warpgroup wg decodes k group wg % 2 of a k-step: plain, of the k-steps
-        // of parity wg / 2; PAIR, of every k-step of matrix wg / 2.
+        // Warpgroup wg decodes the k-steps of parity wg % 2 of tile wg / 2.
         const int wg = (warp - kWarpDeq0) >> 2, quad = warp & 3, r = quad * 32 + lane;
-        const int h = wg & 1, par = wg >> 1;
-        uint32_t qw = PAIR ? par : 0, cc = 0;
+        const int mat = wg >> 1, par = wg & 1;
+        uint32_t cc = 0;
+        Ring rw;
+        if (mat) rw.next(kW);
         bool ok = true;
+        const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + mat * 32;
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
-            for (int c = 0; c < chunks && ok; ++c, ++cc, qw += kMats) {
-                const int sw = qw % kWStages;
-                if (!(ok = warp_wait(&w_full[sw], (qw / kWStages) & 1, ctl, 46))) break;
-                const uint8_t* stage = ws + sw * WB;
+            for (int c = 0; c < chunks && ok; ++c, ++cc) {
+                if (!(ok = warp_wait(&w_full[rw.i], rw.ph, ctl, 46))) break;
+                const uint8_t* stage = ws + rw.i * WB;
 #pragma unroll
-                for (int st = 0; st < kStages; ++st) {
-                    if (!PAIR && (st & 1) != par) continue;
-                    ok = ok && warp_wait(&empty[st], (cc & 1) ^ 1u, ctl, 47);
+                for (int st = 0; st < kAStages; ++st) {
+                    if ((st & 1) != par) continue;
+                    uint32_t o[32];
+                    {
+                        lane::Lane<TYPE> L;
+                        L.load(stage, r, st);
+#pragma unroll
+                        for (int m = 0; m < 8; ++m) {
+                            uint32_t q[4];
+                            L.pairs(m, q);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[4 * m + i] = q[i];
+                        }
+                    }
+                    ok = ok && warp_wait(&a_empty[st], (cc & 1) ^ 1u, ctl, 47);
                     if (!ok) continue;
                     ptx::tc_fence_after();
-                    const uint32_t taddr =
-                        tmem + ((uint32_t)(quad * 32) << 16) + st * kACols + (PAIR ? 32 * par : 0) + 16 * h;
-                    if (st == 0) dq_step<TYPE, 0>(stage, r, h, taddr);
-                    if (st == 1) dq_step<TYPE, 1>(stage, r, h, taddr);
-                    if (st == 2) dq_step<TYPE, 2>(stage, r, h, taddr);
-                    if (st == 3) dq_step<TYPE, 3>(stage, r, h, taddr);
+                    ptx::tmem_st32(tbase + st * kACols, o);
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(&a_full[st]);
                 }
                 __syncwarp();
-                if (ok && lane == 0) ptx::mbar_arrive(&w_empty[sw]);
+                if (ok && lane == 0) ptx::mbar_arrive(&w_empty[rw.i]);
+                rw.next(kW);
+                rw.next(kW);
             }
         }
     } else {
         // Epilogue: warp (quad, sub) reads TMEM lanes 32 quad .. (its lane
-        // quadrant) = weight row n, and the slots of half `sub` of the tile.
+        // quadrant) = weight row n of each tile, and slots 64 sub .. 64 sub + 63.
         const int ew = warp - kWarpEpi0, quad = warp & 3, r = quad * 32 + lane, sub = ew >> 2;
+        const int tid = threadIdx.x - 32 * kWarpEpi0;
         const int64_t N = p.s.N;
+        const bool bf = p.y_dtype == NXQ_BF16;
+        uint16_t* const out16 = reinterpret_cast<uint16_t*>(stg);  // [slot][row]
         uint32_t nt = 0;
         RaggedWalk<true> walk;
-        walk.start(p.plan, NT, tiles, blockIdx.x);
+        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
+        const uint32_t td = tmem + ((uint32_t)(quad * 32) << 16) + kColD + 64 * sub;
+        // Slots 64 sub + c .. + 15 of a tile's accumulator (PAIR: the outputs).
+        auto read16 = [&](int mat, int c, float (&v)[16]) {
+            uint32_t a[16];
+            ptx::tmem_ld16(td + mat * kNT + c, a);
+            if constexpr (PAIR) {
+                uint32_t u[16];
+                ptx::tmem_ld16(td + kNT + c, u);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = swiglu1(__uint_as_float(a[j]), __uint_as_float(u[j]));
+            } else {
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(a[j]);
+            }
+        };
+        auto put16 = [&](int c, const uint32_t (&q)[8]) {
+            uint16_t* d = out16 + (64 * sub + c) * TILE_ROWS + r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                d[(2 * j) * TILE_ROWS] = (uint16_t)(q[j] & 0xFFFFu);
+                d[(2 * j + 1) * TILE_ROWS] = (uint16_t)(q[j] >> 16);
+            }
+        };
+        // The staged tile wt (16-bit) to y.
+        auto flush = [&](const RaggedTile& t, int wt) {
+            const int64_t n0 = (int64_t)wt * TILE_ROWS;
+            uint16_t* const y = static_cast<uint16_t*>(p.y);
+            for (int i = tid; i < t.rows * 16; i += kEpiThreads) {
+                const int s = i >> 4, c = (i & 15) * 8;
+                const int64_t at = ((int64_t)t.row0 + s) * N + n0 + c;
+                const uint4 q = *reinterpret_cast<const uint4*>(out16 + s * TILE_ROWS + c);
+                if (p.vec && n0 + c + 8 <= N) {
+                    *reinterpret_cast<uint4*>(y + at) = q;
+                } else {
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (n0 + c + j < N) y[at + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+                }
+            }
+        };
         for (int64_t g = blockIdx.x; g < total; g += G, ++nt) {
             const RaggedTile t = walk.at(g);
-            if (!warp_wait(d_full, nt & 1, ctl, 48)) break;
+            bool has1;
+            const int wt0 = PAIR ? t.tile : 2 * t.tile, wt1 = weight_tile<PAIR>(t, 1, p.s.tiles, &has1);
+            // All epilogue warps go on or give up together; nobody still reads
+            // the staging buffer.
+            if (!epi_all(warp_wait(d_full, nt & 1, ctl, 48))) break;
             ptx::tc_fence_after();
-            const int64_t n = (int64_t)t.tile * TILE_ROWS + r;
+            const int left = t.rows - 64 * sub;  // slots of this half
+            if (p.y_dtype == NXQ_F32) {
 #pragma unroll 1
-            for (int cb = 0; cb < NT / 64; ++cb) {
-                const int c0 = sub * (NT / 2) + 32 * cb;  // slot in the tile
-                const int cnt = t.rows - c0;
-                if (cnt <= 0) break;
-                uint32_t v[32];
-                const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16) + kColD + c0;
-                ptx::tmem_ld16(ta, *reinterpret_cast<uint32_t(*)[16]>(&v[0]));
-                ptx::tmem_ld16(ta + 16, *reinterpret_cast<uint32_t(*)[16]>(&v[16]));
-                if constexpr (PAIR) {
+                for (int mat = 0; mat < (PAIR ? 1 : 2); ++mat)
+#pragma unroll 1
+                    for (int c = 0; c < 64 && c < left; c += 16) {
+                        float v[16];
+                        read16(mat, c, v);
+                        const int64_t n = (int64_t)(mat ? wt1 : wt0) * TILE_ROWS + r;
+                        float* q = static_cast<float*>(p.y) + ((int64_t)t.row0 + 64 * sub + c) * N + n;
+                        if (n < N && (mat == 0 || has1))
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        uint32_t u[16];
-                        ptx::tmem_ld16(ta + NT + 16 * hf, u);
-                        ptx::tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float a = __uint_as_float(v[16 * hf + j]);
-                            v[16 * hf + j] = __float_as_uint(a / (1.0f + expf(-a)) * __uint_as_float(u[j]));
-                        }
+                            for (int j = 0; j < 16; ++j, q += N)
+                                if (c + j < left) *q = v[j];
                     }
-                } else {
-                    ptx::tmem_wait_ld();
-                }
-                if (n < N) {
-                    const int64_t off = ((int64_t)t.row0 + c0) * N + n;
-                    if (p.y_dtype == NXQ_BF16)
-                        store_col<__nv_bfloat16>(p.y, off, N, cnt, v);
-                    else if (p.y_dtype == NXQ_F16)
-                        store_col<__half>(p.y, off, N, cnt, v);
-                    else
-                        store_col<float>(p.y, off, N, cnt, v);
-                }
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(d_empty);
+                continue;
+            }
+            // The first tile's (PAIR: the) outputs into the staging buffer, the
+            // second tile's into registers; then the accumulators are free.
+#pragma unroll 1
+            for (int c = 0; c < 64 && c < left; c += 16) {
+                float v[16];
+                uint32_t q[8];
+                read16(0, c, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = pack16(bf, v[2 * j], v[2 * j + 1]);
+                put16(c, q);
+            }
+            uint32_t hold[PAIR ? 1 : 4][8];
+            if constexpr (!PAIR) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (16 * c < left) {
+                        float v[16];
+                        read16(1, 16 * c, v);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) hold[c][j] = pack16(bf, v[2 * j], v[2 * j + 1]);
+                    }
             }
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(d_empty);
+            epi_sync();
+            flush(t, wt0);
+            if constexpr (!PAIR) {
+                if (has1) {
+                    epi_sync();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (16 * c < left) put16(16 * c, hold[c]);
+                    epi_sync();
+                    flush(t, wt1);
+                }
+            }
         }
     }
 
@@ -363,19 +485,19 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
 template <int TYPE>
 int set_attr() {
     cudaError_t e = cudaFuncSetAttribute(ragged_gemm_kernel<TYPE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Cfg<TYPE, false>::smem);
+                                         (int)Rings<TYPE>::smem);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(ragged_gemm_kernel<TYPE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)Cfg<TYPE, true>::smem);
+                                 (int)Rings<TYPE>::smem);
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "cudaFuncSetAttribute (ragged_gemm)");
 }
 
 template <int TYPE>
 int launch(const Params& p, const CUtensorMap& tmap, unsigned grid, cudaStream_t st) {
     if (p.up)
-        ragged_gemm_kernel<TYPE, true><<<grid, kThreads, Cfg<TYPE, true>::smem, st>>>(p, tmap);
+        ragged_gemm_kernel<TYPE, true><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
     else
-        ragged_gemm_kernel<TYPE, false><<<grid, kThreads, Cfg<TYPE, false>::smem, st>>>(p, tmap);
+        ragged_gemm_kernel<TYPE, false><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
     note_launches(1);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "ragged_gemm launch");
@@ -396,14 +518,15 @@ int ragged_gemm_init() {
 // Where the dense prefill GEMM runs (NXQ_PREFILL_KERNEL=simt turns both off).
 bool ragged_gemm_supported(const TiledShape& s) { return gemm_supported(s, 33); }
 
-int ragged_gemm_blk(bool pair) { return pair ? 128 : 256; }
+int ragged_gemm_blk() { return kNT; }
 
 int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan) {
     const TiledShape& s = c.w->shape;
-    Params p{c.w->dev, c.up ? c.up->dev : nullptr, s, c.y, c.y_dtype, plan, context_status()};
+    Params p{c.w->dev, c.up ? c.up->dev : nullptr, s, (int)(c.up ? s.tiles : (s.tiles + 1) / 2), c.y, c.y_dtype,
+             s.N % 8 == 0 && (uintptr_t)c.y % 16 == 0, plan, context_status()};
     CUtensorMap tmap;
     if (int rc = gemm_activation_map(&tmap, xh, X, s.K, kBoxRows)) return rc;
-    const int64_t work = ragged_max_blocks(c.w->count, c.R, ragged_gemm_blk(c.up != nullptr)) * s.tiles;
+    const int64_t work = ragged_max_blocks(c.w->count, c.R, kNT) * p.tiles;
     const unsigned grid = (unsigned)(work < context_sm_count() ? work : context_sm_count());
     switch (s.type) {
         case T_Q4_K: return launch<T_Q4_K>(p, tmap, grid, c.st);
