@@ -14,9 +14,9 @@
 //   warps 2-17   four dequant warpgroups, one per tile and k-step parity: thread
 //                r decodes the 64 elements of row r (the lane decoders of the
 //                decode GEMV) and writes them to TMEM, the MMA's A operand
-//   warp 1       one lane issues tcgen05.mma kind::f16 M=128, K=16 with N = the
-//                block's slots rounded up to 16 (a short block costs less), into
-//                one 128-column fp32 accumulator per tile
+//   warps 1, 27  one for each tile: a lane issues tcgen05.mma kind::f16 M=128,
+//                K=16 with N = the block's slots rounded up to 16 (a short block
+//                costs less), into the tile's 128-column fp32 accumulator
 //   warps 18-25  epilogue: tcgen05.ld of the accumulators, conversion (PAIR:
 //                silu(gate) * up, so the two products never reach memory), and
 //                16-bit outputs through a staging buffer in shared memory: the
@@ -24,9 +24,11 @@
 //                rows leave as 16-byte stores while the next tile's MMAs run
 //
 // The A operand's ring has as many stages as a chunk has k-steps, so its indexes
-// are constants; the issuing loop runs warp-wide, half the lanes watching the
+// are constants; the issuing loops run warp-wide, half the lanes watching the
 // activations and half the A operand, with only the MMA and the commits in the
-// elected lane.
+// elected lane.  Waiting for a stage and handing it back cost an issuing warp
+// about 400 cycles a k-step, against 512 of MMA work for both tiles; with
+// a warp per tile one issues while the other waits.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes
 // hold behind a block's slots (the next expert's rows, or zeros) reaches no
@@ -49,7 +51,8 @@ constexpr int kDeqGroups = 4;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
 constexpr int kWarpProducer = 0, kWarpMma = 1, kWarpDeq0 = 2, kWarpEpi0 = 2 + 4 * kDeqGroups;
 constexpr int kWarpWProducer = kWarpEpi0 + kEpiWarps;
-constexpr int kThreads = 32 * (kWarpWProducer + 1);
+constexpr int kWarpMma1 = kWarpWProducer + 1;
+constexpr int kThreads = 32 * (kWarpMma1 + 1);
 constexpr int kMats = 2;  // weight tiles of a work tile
 constexpr int kNT = 128;  // slots of a work tile
 constexpr int kKS = 64;   // reduction elements per k-step (one swizzle atom)
@@ -75,7 +78,7 @@ struct Rings {
     static constexpr int fit = (kBudget - kX * kXB) / WB;
     static constexpr int kW = fit > 6 ? 6 : fit;
     static_assert(kW >= 2, "tile-chunk ring too shallow");
-    static_assert((2 * kX + 2 * kW + 2 * kAStages + 3) * 8 + 8 <= kBarBytes, "barrier area too small");
+    static_assert((2 * kX + 2 * kW + 2 * kMats * kAStages + 2 + kMats) * 8 + 8 <= kBarBytes, "barrier area too small");
     static constexpr size_t smem = 1024 + (size_t)kX * kXB + kStageOut + (size_t)kW * WB + kBarBytes;
 };
 
@@ -165,11 +168,11 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     uint64_t* w_full = x_empty + kX;
     uint64_t* w_empty = w_full + kW;
     uint64_t* a_full = w_empty + kW;
-    uint64_t* a_empty = a_full + kAStages;
-    uint64_t* d_full = a_empty + kAStages;
+    uint64_t* a_empty = a_full + kMats * kAStages;   // [mat][stage]
+    uint64_t* d_full = a_empty + kMats * kAStages;
     uint64_t* d_empty = d_full + 1;
-    uint64_t* drain = d_empty + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* drain = d_empty + 1;  // [mat]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + kMats);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int64_t total = (int64_t)p.plan->blocks * p.tiles;
@@ -180,19 +183,19 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     if (threadIdx.x == 0) {
         for (int i = 0; i < kX; ++i) {
             ptx::mbar_init(&x_full[i], 1);
-            ptx::mbar_init(&x_empty[i], 1);
+            ptx::mbar_init(&x_empty[i], kMats);  // both tiles' MMAs
         }
         for (int i = 0; i < kW; ++i) {
             ptx::mbar_init(&w_full[i], 1);
             ptx::mbar_init(&w_empty[i], 4 * kDeqGroups / kMats);  // the warps that decode a tile-chunk
         }
-        for (int i = 0; i < kAStages; ++i) {
-            ptx::mbar_init(&a_full[i], 4 * kMats);  // the warps that write a stage
+        for (int i = 0; i < kMats * kAStages; ++i) {
+            ptx::mbar_init(&a_full[i], 4);  // the warps that write a tile's stage
             ptx::mbar_init(&a_empty[i], 1);
         }
-        ptx::mbar_init(d_full, 1);
+        ptx::mbar_init(d_full, kMats);
         ptx::mbar_init(d_empty, kEpiWarps);
-        ptx::mbar_init(drain, 1);
+        for (int i = 0; i < kMats; ++i) ptx::mbar_init(&drain[i], 1);
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
@@ -270,13 +273,18 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             while (!ptx::mbar_try_wait(&x_full[k % kX], (k / kX) & 1) && clock64() - t0 < ptx::kWaitCycles) {
             }
         }
-    } else if (warp == kWarpMma) {
+    } else if (warp == kWarpMma || warp == kWarpMma1) {
+        const int mat = warp == kWarpMma ? 0 : 1;
         uint32_t cc = 0, nt = 0;  // chunks and work tiles so far
         bool ok = true;
         Ring rx;
         RaggedWalk<true> walk;
         walk.start(p.plan, kNT, p.tiles, blockIdx.x);
         const uint64_t desc0 = ptx::desc_sw128_kmajor(ptx::smem_addr(xs));
+        const uint32_t d = tmem + kColD + mat * kNT, a = tmem + mat * 32;
+        uint64_t* const af = a_full + mat * kAStages;
+        uint64_t* const ae = a_empty + mat * kAStages;
+        bool ready = false;
         for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
             const RaggedTile t = walk.at(g);
             const uint32_t idesc = ptx::idesc_f16_f32(128, (t.rows + 15) & ~15);
@@ -286,28 +294,32 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             for (int c = 0; c < chunks && ok; ++c, ++cc) {
 #pragma unroll
                 for (int st = 0; st < kAStages; ++st) {
-                    ok = ok && ptx::mbar_wait(lane < 16 ? &x_full[rx.i] : &a_full[st], lane < 16 ? rx.ph : (cc & 1), ctl, 44);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) continue;
+                    if (!__all_sync(0xFFFFFFFFu, ready)) {
+                        ok = ok && ptx::mbar_wait(lane < 16 ? &x_full[rx.i] : &af[st], lane < 16 ? rx.ph : (cc & 1), ctl, 44);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) continue;
+                    }
+                    const int xi = rx.i;
+                    rx.next(kX);
+                    // The next k-step's barriers, read while this one's MMAs issue.
+                    ready = ptx::mbar_test_wait(lane < 16 ? &x_full[rx.i] : &af[(st + 1) % kAStages],
+                                                lane < 16 ? rx.ph : ((cc + (st + 1 == kAStages)) & 1));
                     ptx::tc_fence_after();
                     if (ptx::elect_one()) {
-#pragma unroll
-                        for (int mat = 0; mat < kMats; ++mat)
-                            ptx::mma_ts_f16_k64(tmem + kColD + mat * kNT, tmem + st * kACols + mat * 32,
-                                                desc0 + ((uint32_t)(rx.i * kXB) >> 4), idesc, (c | st) ? 1u : 0u);
-                        ptx::mma_commit(&a_empty[st]);
-                        ptx::mma_commit(&x_empty[rx.i]);
+                        ptx::mma_ts_f16_k64(d, a + st * kACols, desc0 + ((uint32_t)(xi * kXB) >> 4), idesc,
+                                            (c | st) ? 1u : 0u);
+                        ptx::mma_commit(&ae[st]);
+                        ptx::mma_commit(&x_empty[xi]);
                         if (st == kAStages - 1 && c == chunks - 1) ptx::mma_commit(d_full);
                     }
                     __syncwarp();
-                    rx.next(kX);
                 }
             }
         }
-        if (ptx::elect_one()) ptx::mma_commit(drain);
+        if (ptx::elect_one()) ptx::mma_commit(&drain[mat]);
         __syncwarp();
         const long long t0 = clock64();
-        while (!ptx::mbar_try_wait(drain, 0) && clock64() - t0 < ptx::kWaitCycles) {
+        while (!ptx::mbar_try_wait(&drain[mat], 0) && clock64() - t0 < ptx::kWaitCycles) {
         }
     } else if (warp < kWarpEpi0) {
         // Warpgroup wg decodes the k-steps of parity wg % 2 of tile wg / 2.
@@ -337,14 +349,14 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                             for (int i = 0; i < 4; ++i) o[4 * m + i] = q[i];
                         }
                     }
-                    ok = ok && warp_wait(&a_empty[st], (cc & 1) ^ 1u, ctl, 47);
+                    ok = ok && warp_wait(&a_empty[mat * kAStages + st], (cc & 1) ^ 1u, ctl, 47);
                     if (!ok) continue;
                     ptx::tc_fence_after();
                     ptx::tmem_st32(tbase + st * kACols, o);
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&a_full[st]);
+                    if (lane == 0) ptx::mbar_arrive(&a_full[mat * kAStages + st]);
                 }
                 __syncwarp();
                 if (ok && lane == 0) ptx::mbar_arrive(&w_empty[rw.i]);
