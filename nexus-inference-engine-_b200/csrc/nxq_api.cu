@@ -394,7 +394,7 @@ NXQ_API int nxq_init(int device) {
     int rc = mma_init(device);
     if (rc != NXQ_OK) return rc;
     if ((rc = gemm_init(device)) != NXQ_OK) return rc;
-    if ((rc = ragged_gemm_init()) != NXQ_OK) return rc;
+    if ((rc = ragged_gemm_init()) != NXQ_OK || (rc = ragged_mma_init()) != NXQ_OK) return rc;
     g_ctx.ready = true;
     return NXQ_OK;
 }

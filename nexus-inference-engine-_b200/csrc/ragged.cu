@@ -2,11 +2,12 @@
 // slots s of expert e, with the sizes known on the device only.
 //
 // A call is a plan kernel, which turns the offsets into a list of the experts
-// that have rows (ragged.h), where needed a kernel that brings the activations
-// into slot order as f16, and a product kernel that walks the plan: tensor
-// cores (ragged_gemm.cu), or the exact kernel here, with fp32 decode
-// (formats.cuh, decode8) and fp32 products on the CUDA cores, for the block types
-// without a tensor-core decoder.
+// that have rows (ragged.h) and where needed brings the activations into slot
+// order as f16, and a product kernel that walks the plan: warp-level tensor
+// cores for few slots per expert (ragged_mma.cu), tcgen05 beyond
+// (ragged_gemm.cu), or the exact kernel here, with fp32 decode (formats.cuh,
+// decode8) and fp32 products on the CUDA cores, for the block types without a
+// tensor-core decoder.
 #include "ragged.h"
 
 #include <cuda_bf16.h>
@@ -36,8 +37,8 @@ int check_experts(nxq_experts_t h, const ExpertTable** out) {
 // range is taken only if it lies in [0, R] and starts at or behind every offset
 // before it, so the ranges taken never overlap and hold at most R slots
 // whatever the offsets are; anything else is reported and left out.
-__global__ void __launch_bounds__(kMaxExperts) ragged_plan_kernel(const int32_t* __restrict__ offsets, int E, int64_t R,
-                                                                  int blk, RaggedPlan* plan, DeviceStatus* status) {
+__device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t R, int blk, RaggedPlan* plan,
+                                          DeviceStatus* status) {
     __shared__ int warp_n[32], warp_b[32], warp_m[32];
     const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
     const int o0 = e < E ? offsets[e] : 0, o1 = e < E ? offsets[e + 1] : 0;
@@ -178,42 +179,68 @@ __global__ void __launch_bounds__(TILE_ROWS) ragged_simt_kernel(const SimtParams
     }
 }
 
-// The activations of every slot an expert has, as f16 in slot order: xh[s] =
-// f16(x[rows ? rows[s] : s]).  One CTA per slot (walked with a stride), 8 or 1
-// elements per thread (VEC).  fp32 and bf16 values beyond the f16 range and row
-// indices outside [0, X) (zeros) are reported.
+// What a product kernel needs first, in one launch.  CTA 0 makes the plan and
+// zeroes the counters; the others (none if xh is null) bring the activations of
+// every slot an expert has into slot order as f16, xh[s] = f16(x[rows ? rows[s]
+// : s]), a group of kRowThreads threads per slot and 8 or 1 elements per thread
+// (VEC).  fp32 and bf16 values beyond the f16 range and row indices outside
+// [0, X) (zeros) are reported.
+struct PrepParams {
+    const int32_t* offsets;
+    int E;
+    int64_t R;
+    int blk;
+    RaggedPlan* plan;
+    unsigned* cnt;
+    int n_cnt;
+    const void* x;
+    int x_dtype;
+    int64_t X, K;
+    const int32_t* rows;
+    __half* xh;
+    DeviceStatus* status;
+};
+constexpr int kRowThreads = 256, kRowGroups = kMaxExperts / kRowThreads;
+
 template <int VEC>
-__global__ void __launch_bounds__(256) ragged_rows_kernel(const void* __restrict__ x, int dt, int64_t X, int64_t K,
-                                                          const int32_t* __restrict__ rows,
-                                                          const int32_t* __restrict__ offsets, int E, int64_t R,
-                                                          __half* __restrict__ xh, DeviceStatus* status) {
-    const int64_t lo = offsets[0] > 0 ? offsets[0] : 0, hi = offsets[E] < R ? offsets[E] : R;
+__global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepParams p) {
+    // Programmatic dependent launch: the product kernel may set itself up
+    // meanwhile; this one touches memory only after the kernel before it.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < p.n_cnt; i += kMaxExperts) p.cnt[i] = 0u;
+        make_plan(p.offsets, p.E, p.R, p.blk, p.plan, p.status);
+        return;
+    }
+    const int64_t lo = p.offsets[0] > 0 ? p.offsets[0] : 0, hi = p.offsets[p.E] < p.R ? p.offsets[p.E] : p.R;
+    const int group = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads;
     bool over = false;
-    for (int64_t s = lo + blockIdx.x; s < hi; s += gridDim.x) {
-        int64_t row = rows ? rows[s] : s;
-        if (row < 0 || row >= X) {
-            if (threadIdx.x == 0) raise_index(status, kIndexRow);
+    for (int64_t s = lo + (int64_t)(blockIdx.x - 1) * kRowGroups + group; s < hi; s += (int64_t)(gridDim.x - 1) * kRowGroups) {
+        int64_t row = p.rows ? p.rows[s] : s;
+        if (row < 0 || row >= p.X) {
+            if (lane == 0) raise_index(p.status, kIndexRow);
             row = -1;
         }
-        for (int64_t k = (int64_t)threadIdx.x * VEC; k < K; k += 256 * VEC) {
-            const int64_t i = row * K + k;
-            __half* out = xh + s * K + k;
+        for (int64_t k = (int64_t)lane * VEC; k < p.K; k += kRowThreads * VEC) {
+            const int64_t i = row * p.K + k;
+            __half* out = p.xh + s * p.K + k;
             if constexpr (VEC == 1) {
-                const float v = row < 0 ? 0.0f : load_x(x, dt, i);
+                const float v = row < 0 ? 0.0f : load_x(p.x, p.x_dtype, i);
                 over |= f16_overflows(v);
                 *out = __float2half_rn(v);
             } else {
                 uint4 h = make_uint4(0u, 0u, 0u, 0u);
-                if (row >= 0 && dt == NXQ_F16) {
-                    h = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(x) + i));
+                if (row >= 0 && p.x_dtype == NXQ_F16) {
+                    h = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + i));
                 } else if (row >= 0) {
                     float v[8];
-                    if (dt == NXQ_F32) {
-                        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+                    if (p.x_dtype == NXQ_F32) {
+                        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + i);
                         const float4 a = __ldg(q), b = __ldg(q + 1);
                         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
                     } else {
-                        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + i));
+                        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + i));
                         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -225,8 +252,8 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const void* __restrict
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         over |= f16_overflows(v[2 * j]) || f16_overflows(v[2 * j + 1]);
-                        const __half2 p = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                        o[j] = *reinterpret_cast<const uint32_t*>(&p);
+                        const __half2 q = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                        o[j] = *reinterpret_cast<const uint32_t*>(&q);
                     }
                     h = make_uint4(o[0], o[1], o[2], o[3]);
                 }
@@ -234,27 +261,25 @@ __global__ void __launch_bounds__(256) ragged_rows_kernel(const void* __restrict
             }
         }
     }
-    if (over) raise_range(status, 1u);
+    if (over) raise_range(p.status, 1u);
 }
 
-cudaError_t launch_rows(const RaggedCall& c, __half* xh) {
-    const int64_t cap = (int64_t)context_sm_count() * 8;
-    const unsigned grid = (unsigned)(c.R < cap ? c.R : cap);
-    const int64_t K = c.w->shape.K;
-    if (((uintptr_t)c.x % 16) == 0)  // K is a multiple of 32
-        ragged_rows_kernel<8><<<grid, 256, 0, c.st>>>(c.x, c.x_dtype, c.X, K, c.rows, c.offsets, c.w->count, c.R, xh,
-                                                      context_status());
-    else
-        ragged_rows_kernel<1><<<grid, 256, 0, c.st>>>(c.x, c.x_dtype, c.X, K, c.rows, c.offsets, c.w->count, c.R, xh,
-                                                      context_status());
+cudaError_t launch_prep(const RaggedCall& c, int blk, RaggedPlan* plan, unsigned* cnt, int n_cnt, __half* xh) {
+    const PrepParams p{c.offsets, c.w->count, c.R, blk, plan, cnt, n_cnt, c.x, c.x_dtype, c.X, c.w->shape.K, c.rows, xh,
+                       context_status()};
+    const int64_t most = (int64_t)context_sm_count() * 2, want = (c.R + kRowGroups - 1) / kRowGroups;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1 + (unsigned)(!xh ? 0 : want < most ? want : most));
+    cfg.blockDim = dim3(kMaxExperts);
+    cfg.stream = c.st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool vec = ((uintptr_t)c.x % 16) == 0;  // K is a multiple of 32
     note_launches(1);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_plan(const RaggedCall& c, int blk, RaggedPlan* plan) {
-    ragged_plan_kernel<<<1, kMaxExperts, 0, c.st>>>(c.offsets, c.w->count, c.R, blk, plan, context_status());
-    note_launches(1);
-    return cudaGetLastError();
+    return vec ? cudaLaunchKernelEx(&cfg, ragged_prep_kernel<8>, p) : cudaLaunchKernelEx(&cfg, ragged_prep_kernel<1>, p);
 }
 
 int run_simt(const RaggedCall& c, const RaggedPlan* plan) {
@@ -274,20 +299,34 @@ int run_simt(const RaggedCall& c, const RaggedPlan* plan) {
 
 // Plan, activations and product of a call, in one stream-ordered workspace.
 int dispatch(const RaggedCall& c) {
-    const bool gemm = ragged_gemm_supported(c.w->shape);
-    const bool as_is = !gemm || (c.x_dtype == NXQ_F16 && !c.rows && ((uintptr_t)c.x % 16) == 0);
-    const int blk = gemm ? ragged_gemm_blk() : kSimtBlk;
-    const int64_t most = c.w->count < c.R ? c.w->count : c.R;
-    const size_t plan_size = (plan_bytes(most) + 255) & ~(size_t)255;
+    const int mma = ragged_mma_blk(c);  // few slots per expert
+    const bool gemm = !mma && ragged_gemm_supported(c.w->shape);
+    const int blk = mma ? mma : gemm ? ragged_gemm_blk() : kSimtBlk;
+    // f16 activations are read where they are: by row index (mma), or in slot
+    // order (gemm: TMA boxes).
+    const bool as_is = (!mma && !gemm) || (c.x_dtype == NXQ_F16 && ((uintptr_t)c.x % 16) == 0 && (mma || !c.rows));
+    const int workers = ragged_mma_workers();
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    const size_t plan_size = up(plan_bytes(c.w->count < c.R ? c.w->count : c.R));
+    const size_t cnt_size = mma ? up(workers * sizeof(unsigned)) : 0, part_size = mma ? up(ragged_mma_partials()) : 0;
+    const size_t x_size = as_is ? 0 : (size_t)c.R * c.w->shape.K * sizeof(__half);
     uint8_t* ws = nullptr;
-    cudaError_t e = cudaMallocAsync((void**)&ws, plan_size + (as_is ? 0 : (size_t)c.R * c.w->shape.K * sizeof(__half)), c.st);
+    cudaError_t e = cudaMallocAsync((void**)&ws, plan_size + cnt_size + part_size + x_size, c.st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (ragged workspace)");
     RaggedPlan* plan = reinterpret_cast<RaggedPlan*>(ws);
-    __half* xh = reinterpret_cast<__half*>(ws + plan_size);
+    unsigned* cnt = reinterpret_cast<unsigned*>(ws + plan_size);
+    float* part = reinterpret_cast<float*>(ws + plan_size + cnt_size);
+    __half* xh = as_is ? nullptr : reinterpret_cast<__half*>(ws + plan_size + cnt_size + part_size);
     int rc = NXQ_OK;
-    if ((e = launch_plan(c, blk, plan)) != cudaSuccess || (!as_is && (e = launch_rows(c, xh)) != cudaSuccess))
+    if ((e = launch_prep(c, blk, plan, cnt, mma ? workers : 0, xh)) != cudaSuccess)
         rc = cuda_fail(e, "ragged plan launch");
-    if (rc == NXQ_OK) rc = gemm ? ragged_gemm(c, as_is ? c.x : xh, as_is ? c.X : c.R, plan) : run_simt(c, plan);
+    else if (mma)
+        rc = ragged_mma(c, as_is ? static_cast<const __half*>(c.x) : xh, as_is ? c.X : c.R, as_is ? c.rows : nullptr,
+                        plan, part, cnt);
+    else if (gemm)
+        rc = ragged_gemm(c, as_is ? c.x : xh, as_is ? c.X : c.R, plan);
+    else
+        rc = run_simt(c, plan);
     cudaFreeAsync(ws, c.st);
     return rc;
 }

@@ -117,4 +117,16 @@ bool ragged_gemm_supported(const TiledShape& s);
 int ragged_gemm_blk();
 int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan);
 
+// Warp-level kernel for few slots per expert (ragged_mma.cu): xh [X][K] f16,
+// 16-byte aligned; slot s reads row rows[s] (rows null: s).  `blk` is the slots
+// of a row block (0 from ragged_mma_blk declines); `part` has
+// ragged_mma_partials() bytes, `cnt` ragged_mma_workers() counters, zeroed on
+// the stream.
+int ragged_mma_init();
+int ragged_mma_blk(const RaggedCall& c);
+int ragged_mma_workers();
+size_t ragged_mma_partials();
+int ragged_mma(const RaggedCall& c, const __half* xh, int64_t X, const int32_t* rows, const RaggedPlan* plan, float* part,
+               unsigned* cnt);
+
 }  // namespace nxq
