@@ -416,10 +416,10 @@ __device__ __forceinline__ int q6_tiled_code(const uint8_t* rec, int e) {
     return (int)(lo | (hi << 4));
 }
 
+// Code of element e of a 32-element group of 4-bit codes (4-byte aligned).
 __device__ __forceinline__ int q4_tiled_code(const uint8_t* g, int e) {
-    int byte, shift;
-    q4_code_pos(e, &byte, &shift);
-    return (g[byte] >> shift) & 15;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(g + 4 * (e >> 3));
+    return (int)((w >> q6_lo_bit(e & 31)) & 15u);
 }
 
 // ---------------------------------------------------------------------------
@@ -442,7 +442,8 @@ __device__ __forceinline__ float half_bits_to_float(uint32_t h) {
     return __uint_as_float(sign | ((e + 112u) << 23) | (f << 13));
 }
 
-__device__ __forceinline__ uint32_t rd16(const uint8_t* p) { return (uint32_t)p[0] | ((uint32_t)p[1] << 8); }
+// (Every 16-bit field of the tiled records is 2-byte aligned.)
+__device__ __forceinline__ uint32_t rd16(const uint8_t* p) { return *reinterpret_cast<const uint16_t*>(p); }
 
 // The shared 6-bit scale/min unpack of Q4_K/Q5_K (gguf_importer.cpp:856-861).
 __device__ __forceinline__ void kquant_scale_min(const uint8_t* sc, int g, int* s, int* m) {
@@ -537,10 +538,8 @@ __device__ inline void decode8(int type, const uint8_t* chunk, int r, int e0, fl
         case T_I4G32: case T_I4G64: case T_I4G128: case T_I4G256: {  // quant/gptq.cpp:9-27
             const uint8_t* rec = chunk + (int64_t)r * (i4g_hdr(type) + CHUNK_K / 2);
             const int j = e0 / i4g_gs(type);
-            const float scale = __uint_as_float((uint32_t)rec[8 * j] | ((uint32_t)rec[8 * j + 1] << 8) |
-                                                ((uint32_t)rec[8 * j + 2] << 16) | ((uint32_t)rec[8 * j + 3] << 24));
-            const float zero = __uint_as_float((uint32_t)rec[8 * j + 4] | ((uint32_t)rec[8 * j + 5] << 8) |
-                                               ((uint32_t)rec[8 * j + 6] << 16) | ((uint32_t)rec[8 * j + 7] << 24));
+            const float2 sz = *reinterpret_cast<const float2*>(rec + 8 * j);
+            const float scale = sz.x, zero = sz.y;
             const uint8_t* q = rec + i4g_hdr(type) + 16 * (e0 >> 5);
             for (int i = 0; i < 8; ++i)
                 out[i] = __fmul_rn(__fsub_rn((float)q4_tiled_code(q, (e0 & 31) + i), zero), scale);

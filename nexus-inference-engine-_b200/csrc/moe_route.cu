@@ -4,14 +4,16 @@
 // weights and their order by expert stay on the device.
 //
 // Routing has three steps.  (1) One warp per token: lane l holds the logits of
-// experts l, l + 32, ... as order-preserving integer keys; k rounds of a warp
-// maximum (redux on the key, then on the index among equals, so ties go to
-// the lowest index) pick the choices.  (2) An exclusive scan, over blocks of
-// tokens, of each expert's count.  (3) Every block ranks its own choices: a warp
-// walks a contiguous run of choices in order, equal experts among 32 lanes
-// ranked by their lane (match), so slots are ordered by (expert, token) and do
-// not depend on timing - the counts are integers and no atomic decides a place.
-// Up to kSmallT tokens one CTA does all three.
+// experts l, l + 32, ... as order-preserving integer keys and knows its largest;
+// k rounds of a warp maximum (redux on the key; among lanes with equal keys redux
+// on the index, so ties go to the lowest) pick the choices, and only the lane
+// that held a choice looks for its next largest.  (2) Counts of every expert in
+// every block of tokens, and their exclusive scan over blocks: 32 experts per
+// CTA.  (3) Every block ranks its own choices: a warp walks a contiguous run of
+// choices in order, equal experts among 32 lanes ranked by their lane (match),
+// so slots are ordered by (expert, token) and do not depend on timing - the
+// counts are integers and no atomic decides a place.  Up to kSmallT tokens one
+// CTA does all three.
 #include "nxq_internal.h"
 
 #include <cuda_bf16.h>
@@ -26,6 +28,7 @@ constexpr int kRankWarps = 8;        // contiguous runs a block's choices are ra
 constexpr int kThreads = 32 * kRankWarps;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallT = 128;
+constexpr int kMaxBlocks = 256;      // of tokens
 constexpr float kInf = __builtin_huge_valf();
 
 struct RouteParams {
@@ -40,8 +43,8 @@ struct RouteParams {
     int32_t* offsets;
     int32_t* rows;
     int32_t* slots;
-    int32_t* hist;   // [blocks][E]: counts, then their exclusive scan over blocks
-    int32_t* total;  // [E]
+    int32_t* before;  // [blocks][E]: choices of the expert in the blocks before
+    int32_t* total;   // [E]
 };
 
 __device__ __forceinline__ float load_logit(const void* p, int dt, int64_t i) {
@@ -68,18 +71,27 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The choices of token t by one warp; counts them in hist (shared, [E]).
+// The choices of token t by one warp; lane j < k returns choice j (-1: none).
 template <int V>
-__device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int lane, int32_t* hist) {
+__device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int lane) {
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int e = lane + 32 * i;
         key[i] = e < p.E ? key_of(load_logit(p.logits, p.dtype, t * p.E + e)) : 0u;
     }
-    uint32_t top = 0u;
+    uint32_t top = 0u;  // this lane's largest key, and its expert
+    int at = 0;
+    auto largest = [&] {
+        top = 0u;
 #pragma unroll
-    for (int i = 0; i < V; ++i) top = key[i] > top ? key[i] : top;
+        for (int i = 0; i < V; ++i)
+            if (key[i] > top) {
+                top = key[i];
+                at = lane + 32 * i;
+            }
+    };
+    largest();
     const uint32_t first = __reduce_max_sync(0xFFFFFFFFu, top);
     const float m = value_of(first);
     float all = 0.0f;  // sum over every expert
@@ -91,40 +103,34 @@ __device__ __forceinline__ void choose(const RouteParams& p, int64_t t, int lane
     }
     int my_id = -1;
     float my_p = 0.0f;
-    for (int j = 0; j < p.k; ++j) {
-        const uint32_t best = __reduce_max_sync(0xFFFFFFFFu, top);
-        if (!best) break;
-        int at = 0x7FFFFFFF;
-        if (top == best) {
+    uint32_t best = first;
+    for (int j = 0; j < p.k && best; ++j) {
+        const unsigned who = __ballot_sync(0xFFFFFFFFu, top == best);
+        const int e = __popc(who) == 1 ? __shfl_sync(0xFFFFFFFFu, at, __ffs(who) - 1)
+                                       : __reduce_min_sync(0xFFFFFFFFu, top == best ? at : 0x7FFFFFFF);
+        if (top == best && at == e) {
 #pragma unroll
-            for (int i = V - 1; i >= 0; --i)
-                if (key[i] == best) at = lane + 32 * i;
-        }
-        const int e = __reduce_min_sync(0xFFFFFFFFu, at);
-        if (at == e) {
-            top = 0u;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < V; ++i)
                 if (lane + 32 * i == e) key[i] = 0u;
-                top = key[i] > top ? key[i] : top;
-            }
+            largest();
         }
         if (lane == j) {
             my_id = e;
             my_p = share_of(value_of(best), m);
         }
+        best = __reduce_max_sync(0xFFFFFFFFu, top);
     }
     const float z = p.normalize ? warp_sum(my_p) : all;
     if (lane < p.k) {
         p.ids[t * p.k + lane] = my_id;
         p.weights[t * p.k + lane] = my_id >= 0 ? my_p / z : 0.0f;
-        if (my_id >= 0) atomicAdd(&hist[my_id], 1);
     }
+    return my_id;
 }
 
 // Ranks the choices of tokens [t0, t1): warp w < kRankWarps takes the w-th run
-// of them.  start[w][e] (shared) holds, on entry, nothing; base[e] is the
-// first slot of the block's choices of expert e.
+// of them.  base[e] is the first slot of the block's choices of expert e; start
+// ([kRankWarps][E], shared) is scratch.
 __device__ __forceinline__ void rank_choices(const RouteParams& p, int64_t t0, int64_t t1, int32_t* start,
                                              const int32_t* base, int threads) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -199,41 +205,66 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteP
     int32_t* hist = sm;                // [E]
     int32_t* base = hist + p.E;        // [E + 1]
     int32_t* start = base + p.E + 1;   // [kRankWarps][E]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    for (int e = tid; e < p.E; e += kSmallThreads) hist[e] = 0;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, threads = blockDim.x;
+    for (int e = tid; e < p.E; e += threads) hist[e] = 0;
+    overlap_begin();
     __syncthreads();
-    for (int64_t t = warp; t < p.T; t += kSmallThreads / 32) choose<V>(p, t, lane, hist);
+    int id = -1;
+    for (int64_t t = warp; t < p.T; t += threads / 32) {
+        id = choose<V>(p, t, lane);
+        if (id >= 0) atomicAdd(&hist[id], 1);
+    }
     __syncthreads();
     scan_experts(hist, base, p.E);
-    for (int e = tid; e <= p.E; e += kSmallThreads) p.offsets[e] = base[e];
-    for (int64_t s = base[p.E] + tid; s < p.T * p.k; s += kSmallThreads) p.rows[s] = -1;
-    rank_choices(p, 0, p.T, start, base, kSmallThreads);
+    for (int e = tid; e <= p.E; e += threads) p.offsets[e] = base[e];
+    for (int64_t s = base[p.E] + tid; s < p.T * p.k; s += threads) p.rows[s] = -1;
+    if (p.T == 1) {  // one choice of an expert at most: its slot is the expert's first
+        if (warp == 0 && lane < p.k) {
+            const int slot = id >= 0 ? base[id] : -1;
+            p.slots[lane] = slot;
+            if (slot >= 0) p.rows[slot] = 0;
+        }
+        return;
+    }
+    rank_choices(p, 0, p.T, start, base, threads);
 }
 
+// A warp per token.
 template <int V>
 __global__ void __launch_bounds__(kThreads) route_choose_kernel(const RouteParams p) {
-    extern __shared__ int32_t hist[];  // [E]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    for (int e = tid; e < p.E; e += kThreads) hist[e] = 0;
-    __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
-    for (int64_t t = t0 + warp; t < t1; t += kThreads / 32) choose<V>(p, t, lane, hist);
-    __syncthreads();
-    for (int e = tid; e < p.E; e += kThreads) p.hist[(int64_t)blockIdx.x * p.E + e] = hist[e];
+    overlap_begin();
+    const int64_t t = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (t < p.T) choose<V>(p, t, threadIdx.x & 31);
 }
 
-// 32 experts per CTA, lane = expert; the 32 warps scan a run of blocks each.
+// 32 experts per CTA: counts them in every block of tokens (shared memory), then
+// each warp scans a run of blocks, lane = expert.
 __global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
+    __shared__ int32_t cnt[kMaxBlocks][32];
     __shared__ int32_t part[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int e = blockIdx.x * 32 + lane;
+    const int e0 = blockIdx.x * 32, e = e0 + lane;
+    for (int i = threadIdx.x; i < p.blocks * 32; i += 1024) cnt[i >> 5][i & 31] = 0;
+    overlap_begin();
+    __syncthreads();
+    // Warp w counts the choices of blocks w, w + 32, ...
+    const int64_t n = p.T * p.k, per_block = (int64_t)p.tb * p.k;
+    for (int b = warp; b < p.blocks; b += 32) {
+        const int64_t z = (b + 1) * per_block < n ? (b + 1) * per_block : n;
+#pragma unroll 4
+        for (int64_t c = b * per_block + lane; c < z; c += 32) {
+            const int id = p.ids[c] - e0;
+            if (id >= 0 && id < 32) atomicAdd(&cnt[b][id], 1);
+        }
+    }
+    __syncthreads();
     const int per = (p.blocks + 31) / 32, b0 = warp * per, b1 = b0 + per < p.blocks ? b0 + per : p.blocks;
     int s = 0;
-    if (e < p.E)
-        for (int b = b0; b < b1; ++b) s += p.hist[(int64_t)b * p.E + e];
+    for (int b = b0; b < b1; ++b) s += cnt[b][lane];
     part[warp][lane] = s;
     __syncthreads();
     int at = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < 32; ++w) {
         const int v = part[w][lane];
         if (w < warp) at += v;
@@ -242,9 +273,8 @@ __global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
     if (e >= p.E) return;
     if (warp == 0) p.total[e] = all;
     for (int b = b0; b < b1; ++b) {
-        const int c = p.hist[(int64_t)b * p.E + e];
-        p.hist[(int64_t)b * p.E + e] = at;
-        at += c;
+        p.before[(int64_t)b * p.E + e] = at;
+        at += cnt[b][lane];
     }
 }
 
@@ -254,6 +284,7 @@ __global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams 
     int32_t* base = cnt + p.E;        // [E + 1]
     int32_t* start = base + p.E + 1;  // [kRankWarps][E]
     const int tid = threadIdx.x;
+    overlap_begin();
     for (int e = tid; e < p.E; e += kThreads) cnt[e] = p.total[e];
     __syncthreads();
     scan_experts(cnt, base, p.E);
@@ -262,7 +293,7 @@ __global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams 
         for (int e = tid; e <= p.E; e += kThreads) p.offsets[e] = base[e];
     for (int64_t s = base[p.E] + (int64_t)blockIdx.x * kThreads + tid; s < n; s += (int64_t)gridDim.x * kThreads) p.rows[s] = -1;
     __syncthreads();
-    for (int e = tid; e < p.E; e += kThreads) base[e] += p.hist[(int64_t)blockIdx.x * p.E + e];
+    for (int e = tid; e < p.E; e += kThreads) base[e] += p.before[(int64_t)blockIdx.x * p.E + e];
     __syncthreads();
     const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
     rank_choices(p, t0, t1, start, base, kThreads);
@@ -270,12 +301,13 @@ __global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams 
 
 template <int V>
 cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
-    if (small)
-        route_small_kernel<V><<<1, kSmallThreads, smem, st>>>(p);
-    else
-        route_choose_kernel<V><<<(unsigned)p.blocks, kThreads, p.E * sizeof(int32_t), st>>>(p);
     note_launches(1);
-    return cudaGetLastError();
+    if (small) {
+        const unsigned warps = p.T < 4 ? 4 : p.T < 32 ? (unsigned)p.T : 32;
+        return launch_overlapped(route_small_kernel<V>, 1, 32 * warps, smem, st, p);
+    }
+    const int64_t per = kThreads / 32;
+    return launch_overlapped(route_choose_kernel<V>, (unsigned)((p.T + per - 1) / per), kThreads, 0, st, p);
 }
 
 cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
@@ -290,30 +322,46 @@ cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStr
 
 // ---- combine -------------------------------------------------------------------
 
-constexpr int kCombThreads = 128;
+// One warp sums 32 VEC columns of one token: lane j holds slot and weight j, the
+// rows of up to kBatch experts are loaded before the first is used, and the
+// next item's slots meanwhile.  Bound by reading T k rows of h, so what counts
+// is loads in flight; nothing synchronizes the warps.  (With slots and weights
+// staged once per CTA and two barriers an item: 225 us for 8192 tokens x 8 rows
+// of 4096 bf16.)
+constexpr int kCombThreads = 256;
+constexpr int kBatch = 8;
 
 __device__ __forceinline__ float load_h(const void* p, int dt, int64_t i) { return load_logit(p, dt, i); }
 
-// Eight consecutive values of h at element i (16-byte aligned).
-__device__ __forceinline__ void load_h8(const void* p, int dt, int64_t i, float (&v)[8]) {
-    if (dt == NXQ_F32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 a = __ldg(q), b = __ldg(q + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
-    }
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Eight consecutive values of h as loaded.
+template <bool F32>
+struct Raw8 {
+    uint4 q[F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        const uint4* a = F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i)
+                             : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (dt == NXQ_F16) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        for (int j = 0; j < (F32 ? 2 : 1); ++j) q[j] = __ldcs(a + j);
+    }
+    __device__ __forceinline__ void widen(int dt, float (&v)[8]) const {
+        const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+        if constexpr (F32) {
+            const uint32_t u[4] = {q[1].x, q[1].y, q[1].z, q[1].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]), v[4 + j] = __uint_as_float(u[j]);
         } else {
-            v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (dt == NXQ_F16) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                    v[2 * j] = f.x, v[2 * j + 1] = f.y;
+                } else {
+                    v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                }
+            }
         }
     }
-}
+};
 
 __device__ __forceinline__ void store_as(void* p, int dt, int64_t i, float v) {
     if (dt == NXQ_F32)
@@ -324,41 +372,91 @@ __device__ __forceinline__ void store_as(void* p, int dt, int64_t i, float v) {
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// grid = T * segs CTAs (walked with a stride); a thread sums VEC consecutive
-// columns of one token.  VEC = 8 needs N % 8 == 0 and 16-byte aligned arrays.
-template <int VEC>
+// Items are (token, 32 VEC columns), segs to a token.  VEC = 8 needs N % 8 == 0,
+// h and y 16-byte and an fp32 residual or output 32-byte aligned.  F32: h's type.
+template <int VEC, bool F32>
 __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __restrict__ h, int h_dtype, int64_t R, int64_t N,
                                                                const int32_t* __restrict__ slots,
                                                                const float* __restrict__ weights, int64_t T, int k,
                                                                const float* res, void* y, int y_dtype, int64_t segs,
                                                                DeviceStatus* status) {
-    for (int64_t b = blockIdx.x; b < T * segs; b += gridDim.x) {
-        const int64_t t = b / segs;
-        const int64_t n = ((b - t * segs) * kCombThreads + threadIdx.x) * VEC;
-        if (n >= N) continue;
+    overlap_begin();
+    const int lane = threadIdx.x & 31;
+    const int64_t items = T * segs, step = (int64_t)gridDim.x * (kCombThreads / 32);
+    int64_t it = (int64_t)blockIdx.x * (kCombThreads / 32) + (threadIdx.x >> 5);
+    int next_s = -1;
+    float next_w = 0.0f;
+    auto fetch = [&](int64_t i) {
+        if (i < items && lane < k) {
+            next_s = slots[(i / segs) * k + lane];
+            next_w = weights[(i / segs) * k + lane];
+        }
+    };
+    fetch(it);
+    for (; it < items; it += step) {
+        const int64_t t = it / segs, n = ((it - t * segs) * 32 + lane) * VEC;
+        int my_s = next_s;
+        const float my_w = next_w;
+        if (my_s >= R) {
+            raise_index(status, kIndexSlot);
+            my_s = -1;
+        }
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-        for (int j = 0; j < k; ++j) {
-            const int s = slots[t * k + j];
-            if (s < 0) continue;
-            if (s >= R) {
-                if (n == 0) raise_index(status, kIndexSlot);
-                continue;
+        if constexpr (VEC == 8) {
+            for (int j0 = 0; j0 < k; j0 += kBatch) {
+                Raw8<F32> r[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
+                    if (j0 + j < k && s >= 0 && n < N) r[j].load(h, (int64_t)s * N + n);
+                }
+                if (j0 + kBatch >= k) fetch(it + step);
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
+                    const float w = __shfl_sync(0xFFFFFFFFu, my_w, (j0 + j) & 31);
+                    if (j0 + j < k && s >= 0) {
+                        float v[8];
+                        r[j].widen(h_dtype, v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+                    }
+                }
             }
-            const float w = weights[t * k + j];
-            float v[VEC];
-            if constexpr (VEC == 8)
-                load_h8(h, h_dtype, (int64_t)s * N + n, v);
-            else
-                v[0] = load_h(h, h_dtype, (int64_t)s * N + n);
+            if (n >= N) continue;
+            const int64_t o = t * N + n;
+            if (res) {
+                float v[8];
+                load_f32x8(res + o, v);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, v[i], acc[i]);
-        }
+                for (int i = 0; i < 8; ++i) acc[i] += v[i];
+            }
+            if (y_dtype == NXQ_F32) {
+                store_f32x8(static_cast<float*>(y) + o, acc);
+            } else {
+                uint32_t q[4];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float r = res ? res[t * N + n + i] : 0.0f;
-            store_as(y, y_dtype, t * N + n + i, acc[i] + r);
+                for (int i = 0; i < 4; ++i) {
+                    if (y_dtype == NXQ_F16) {
+                        const __half2 v = __floats2half2_rn(acc[2 * i], acc[2 * i + 1]);
+                        q[i] = *reinterpret_cast<const uint32_t*>(&v);
+                    } else {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
+                        q[i] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                }
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + o) = make_uint4(q[0], q[1], q[2], q[3]);
+            }
+        } else {
+            fetch(it + step);
+            for (int j = 0; j < k; ++j) {
+                const int s = __shfl_sync(0xFFFFFFFFu, my_s, j);
+                const float w = __shfl_sync(0xFFFFFFFFu, my_w, j);
+                if (s >= 0 && n < N) acc[0] = fmaf(w, load_h(h, h_dtype, (int64_t)s * N + n), acc[0]);
+            }
+            if (n < N) store_as(y, y_dtype, t * N + n, acc[0] + (res ? res[t * N + n] : 0.0f));
         }
     }
 }
@@ -393,24 +491,17 @@ NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, i
         cudaError_t e = launch_choose(p, true, smem, st);
         return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "route launch");
     }
-    // At most 1024 blocks of tokens.
-    p.tb = (int)((T + 1023) / 1024);
+    p.tb = (int)((T + kMaxBlocks - 1) / kMaxBlocks);
     if (p.tb < 64) p.tb = 64;
     p.blocks = (int)((T + p.tb - 1) / p.tb);
-    cudaError_t e = cudaMallocAsync((void**)&p.hist, ((size_t)p.blocks + 1) * E * sizeof(int32_t), st);
+    cudaError_t e = cudaMallocAsync((void**)&p.before, ((size_t)p.blocks + 1) * E * sizeof(int32_t), st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (route workspace)");
-    p.total = p.hist + (size_t)p.blocks * E;
+    p.total = p.before + (size_t)p.blocks * E;
     e = launch_choose(p, false, smem, st);
-    if (e == cudaSuccess) {
-        route_scan_kernel<<<(unsigned)((E + 31) / 32), 1024, 0, st>>>(p);
-        e = cudaGetLastError();
-    }
-    if (e == cudaSuccess) {
-        route_rank_kernel<<<(unsigned)p.blocks, kThreads, smem, st>>>(p);
-        e = cudaGetLastError();
-    }
+    if (e == cudaSuccess) e = launch_overlapped(route_scan_kernel, (unsigned)((E + 31) / 32), 1024, 0, st, p);
+    if (e == cudaSuccess) e = launch_overlapped(route_rank_kernel, (unsigned)p.blocks, kThreads, smem, st, p);
     note_launches(2);
-    cudaFreeAsync(p.hist, st);
+    cudaFreeAsync(p.before, st);
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "route launch");
 }
 
@@ -425,18 +516,17 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
     if ((const void*)y_dev == (const void*)res_dev && y_dtype != NXQ_F32)
         return fail(NXQ_ERR_ARG, "combine: y may be the residual only as fp32");
     if (int rc = context_ready()) return rc;
-    const bool vec = N % 8 == 0 && (((uintptr_t)h_dev | (uintptr_t)y_dev | (uintptr_t)res_dev) % 16) == 0;
-    const int64_t segs = (N + (int64_t)kCombThreads * (vec ? 8 : 1) - 1) / ((int64_t)kCombThreads * (vec ? 8 : 1));
+    const bool vec = N % 8 == 0 && (uintptr_t)h_dev % 16 == 0 && (uintptr_t)res_dev % 32 == 0 &&
+                     (uintptr_t)y_dev % (y_dtype == NXQ_F32 ? 32 : 16) == 0;
+    const int64_t per = 32 * (vec ? 8 : 1), segs = (N + per - 1) / per;
     if (T > ((int64_t)1 << 62) / segs) return fail(NXQ_ERR_ARG, "combine: T=%lld N=%lld", (long long)T, (long long)N);
-    const int64_t grid = T * segs < (1 << 30) ? T * segs : (1 << 30);
-    if (vec)
-        combine_kernel<8><<<(unsigned)grid, kCombThreads, 0, (cudaStream_t)stream>>>(
-            h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
-    else
-        combine_kernel<1><<<(unsigned)grid, kCombThreads, 0, (cudaStream_t)stream>>>(
-            h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
+    const int64_t want = (T * segs + kCombThreads / 32 - 1) / (kCombThreads / 32), most = (int64_t)context_sm_count() * 8;
+    const bool f32 = h_dtype == NXQ_F32;
+    const cudaError_t e = launch_overlapped(
+        vec ? (f32 ? combine_kernel<8, true> : combine_kernel<8, false>) : combine_kernel<1, false>,
+        (unsigned)(want < most ? want : most), kCombThreads, 0, (cudaStream_t)stream, h_dev, h_dtype, R, N, slots_dev,
+        weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
     note_launches(1);
-    cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "combine launch");
 }
 

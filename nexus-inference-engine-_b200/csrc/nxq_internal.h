@@ -112,6 +112,44 @@ int weight_table_ref(nxq_weight_t h, int delta);
 // Releases every expert table (nxq_shutdown; the weights go after it).
 void experts_shutdown();
 
+#ifdef __CUDACC__
+// Launch with programmatic stream serialization: the kernel may start while the
+// one before it on the stream drains, and must run griddepcontrol.wait before
+// it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+                              const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+// First thing in such a kernel: lets the next one start, then waits for the one before.
+__device__ __forceinline__ void overlap_begin() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// 32 consecutive bytes (32-byte aligned) in one access.
+__device__ __forceinline__ void store_f32x8(float* p, const float (&v)[8]) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void load_f32x8(const float* p, float (&v)[8]) {
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p)
+                 : "memory");
+}
+#endif
+
 inline bool dtype_valid(int d) { return d == NXQ_F32 || d == NXQ_F16 || d == NXQ_BF16; }
 
 // Process-wide count of kernels launched by the library (nxq_launch_count).

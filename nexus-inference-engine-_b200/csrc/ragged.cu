@@ -204,10 +204,7 @@ constexpr int kRowThreads = 256, kRowGroups = kMaxExperts / kRowThreads;
 
 template <int VEC>
 __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepParams p) {
-    // Programmatic dependent launch: the product kernel may set itself up
-    // meanwhile; this one touches memory only after the kernel before it.
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    overlap_begin();  // the product kernel may set itself up meanwhile
     if (blockIdx.x == 0) {
         for (int i = threadIdx.x; i < p.n_cnt; i += kMaxExperts) p.cnt[i] = 0u;
         make_plan(p.offsets, p.E, p.R, p.blk, p.plan, p.status);
@@ -268,18 +265,10 @@ cudaError_t launch_prep(const RaggedCall& c, int blk, RaggedPlan* plan, unsigned
     const PrepParams p{c.offsets, c.w->count, c.R, blk, plan, cnt, n_cnt, c.x, c.x_dtype, c.X, c.w->shape.K, c.rows, xh,
                        context_status()};
     const int64_t most = (int64_t)context_sm_count() * 2, want = (c.R + kRowGroups - 1) / kRowGroups;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(1 + (unsigned)(!xh ? 0 : want < most ? want : most));
-    cfg.blockDim = dim3(kMaxExperts);
-    cfg.stream = c.st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    const unsigned grid = 1 + (unsigned)(!xh ? 0 : want < most ? want : most);
     const bool vec = ((uintptr_t)c.x % 16) == 0;  // K is a multiple of 32
     note_launches(1);
-    return vec ? cudaLaunchKernelEx(&cfg, ragged_prep_kernel<8>, p) : cudaLaunchKernelEx(&cfg, ragged_prep_kernel<1>, p);
+    return launch_overlapped(vec ? ragged_prep_kernel<8> : ragged_prep_kernel<1>, grid, kMaxExperts, 0, c.st, p);
 }
 
 int run_simt(const RaggedCall& c, const RaggedPlan* plan) {

@@ -141,9 +141,7 @@ __global__ void __launch_bounds__(Cfg<TYPE, PAIR>::kAll, 1) ragged_mma_kernel(co
     }
     __syncthreads();
     const ptx::WaitCtl ctl{&s_abort, p.status};
-    // Programmatic dependent launch: everything above overlaps the plan kernel.
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    overlap_begin();  // everything above overlaps the plan kernel
 
     const int Kc = p.chunks, kun = PAIR ? 2 * Kc : Kc;  // units per tile
     const int U = p.plan->blocks * p.tiles * kun;       // checked on the host to fit
@@ -365,17 +363,7 @@ int set_attr() {
 
 template <int TYPE, bool PAIR>
 int launch(const Params& p, unsigned grid, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(Cfg<TYPE, PAIR>::kAll);
-    cfg.dynamicSmemBytes = Cfg<TYPE, PAIR>::smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, ragged_mma_kernel<TYPE, PAIR>, p);
+    const cudaError_t e = launch_overlapped(ragged_mma_kernel<TYPE, PAIR>, grid, Cfg<TYPE, PAIR>::kAll, Cfg<TYPE, PAIR>::smem, st, p);
     note_launches(1);
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "ragged_mma launch");
 }

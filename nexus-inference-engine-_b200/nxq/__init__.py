@@ -220,7 +220,9 @@ def init(device: int = 0) -> None:
 
 
 def shutdown() -> None:
+    global _device
     _check(lib().nxq_shutdown())
+    _device = None
 
 
 def _stream_ptr(stream) -> ctypes.c_void_p:
@@ -437,66 +439,71 @@ def qmatmul_host(w: Weight, x: np.ndarray, out: Optional[np.ndarray] = None) -> 
 
 I32, I64 = 0, 1
 
+# These calls take a few microseconds on the GPU at decode sizes, as long as a
+# careless Python wrapper: torch is looked up once, messages are built only for
+# an error, and the current stream is read as the bare handle.
+_torch = None
+_FLOATS: dict = {}  # torch dtype -> NXQ_F32 / F16 / BF16
 
-def _arg(ok: bool, message: str) -> None:
-    if not ok:
-        raise NxqError(-1, message)
+
+def _load_torch():
+    global _torch
+    import torch
+
+    _FLOATS.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    _torch = torch
+    return torch
 
 
-def _tensors(what: str, **tensors) -> None:
-    """Every given tensor is contiguous and on the library's GPU."""
-    for name, t in tensors.items():
-        if t is not None:
-            _arg(t.is_cuda and (_device is None or t.device.index == _device),
-                 f"{what}: {name} is on {t.device}, the library on cuda:{_device}")
-            _arg(t.is_contiguous(), f"{what}: {name} is not contiguous")
+def _bad(message: str) -> NxqError:
+    return NxqError(-1, message)
+
+
+def _usable(what: str, name: str, t) -> int:
+    """Device index of a contiguous tensor on the library's GPU."""
+    d = t.get_device()
+    if d < 0 or (d != _device and _device is not None):
+        raise _bad(f"{what}: {name} is on {t.device}, the library on cuda:{_device}")
+    if not t.is_contiguous():
+        raise _bad(f"{what}: {name} is not contiguous")
+    return d
 
 
 def _float_code(what: str, name: str, dtype) -> int:
-    import torch
-
-    _arg(dtype in (torch.float32, torch.float16, torch.bfloat16), f"{what}: {name} is {dtype}")
-    return _dtype_code(dtype)
-
-
-def _int32(what: str, **tensors) -> None:
-    import torch
-
-    for name, t in tensors.items():
-        _arg(t is None or t.dtype == torch.int32, f"{what}: {name} must be int32")
+    code = _FLOATS.get(dtype)
+    if code is None:
+        raise _bad(f"{what}: {name} is {dtype}")
+    return code
 
 
-def _out(what: str, out, shape, dtype, device):
-    """`out` if given (checked), else a new tensor of `shape`."""
-    import torch
-
+def _output(what: str, out, shape: tuple, dtype, like):
+    """`out` if given (checked), else a new tensor of `shape` beside `like`; and its type's code."""
     if out is None:
-        return torch.empty(shape, dtype=dtype or torch.float32, device=device)
-    _arg(tuple(out.shape) == tuple(shape), f"{what}: out has shape {tuple(out.shape)}, not {tuple(shape)}")
-    _arg(dtype is None or out.dtype == dtype, f"{what}: out is {out.dtype}, out_dtype {dtype}")
-    return out
+        out = like.new_empty(shape, dtype=dtype or _torch.float32)
+    else:
+        _usable(what, "out", out)
+        if tuple(out.shape) != shape:
+            raise _bad(f"{what}: out has shape {tuple(out.shape)}, not {shape}")
+        if dtype is not None and out.dtype != dtype:
+            raise _bad(f"{what}: out is {out.dtype}, out_dtype {dtype}")
+    return out, _float_code(what, "out", out.dtype)
 
 
-def _stream_of(stream, tensor) -> ctypes.c_void_p:
-    """The given stream, else the current one of the tensor's device."""
-    if stream is None:
-        import torch
-
-        return ctypes.c_void_p(torch.cuda.current_stream(tensor.device).cuda_stream)
-    return _stream_ptr(stream)
+def _stream_on(stream, device: int):
+    """The given stream, else the current one of the device."""
+    return _torch._C._cuda_getCurrentRawStream(device) if stream is None else _stream_ptr(stream)
 
 
 def embedding(w: Weight, ids, scale: float = 1.0, out=None, out_dtype=None, stream=None):
     """scale * decode(W[ids]): rows of a registered table, [*ids.shape, K] (nxq_embedding).
     ids: int32 or int64; an id outside the table gives zeros and ERR_INDEX at stream_sync."""
-    import torch
-
-    _arg(ids.dtype in (torch.int32, torch.int64), f"embedding: ids are {ids.dtype}, not int32 or int64")
-    _tensors("embedding", ids=ids, out=out)
-    out = _out("embedding", out, (*ids.shape, w.K), out_dtype, ids.device)
-    code = _float_code("embedding", "out", out.dtype)
-    _check(lib().nxq_embedding(w.handle, ids.data_ptr(), I64 if ids.dtype == torch.int64 else I32, ids.numel(), scale,
-                               out.data_ptr(), code, _stream_of(stream, ids)))
+    torch = _torch or _load_torch()
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
+        raise _bad(f"embedding: ids are {ids.dtype}, not int32 or int64")
+    d = _usable("embedding", "ids", ids)
+    out, code = _output("embedding", out, (*ids.shape, w.K), out_dtype, ids)
+    _check(lib().nxq_embedding(w.handle, ids.data_ptr(), I64 if ids.dtype is torch.int64 else I32, ids.numel(), scale,
+                               out.data_ptr(), code, _stream_on(stream, d)))
     return out
 
 
@@ -507,7 +514,8 @@ class Experts:
     def __init__(self, weights):
         self.weights = list(weights)
         n = len(self.weights)
-        _arg(n > 0, "Experts: no weights")
+        if n == 0:
+            raise _bad("Experts: no weights")
         h = ctypes.c_void_p()
         _check(lib().nxq_experts_create((ctypes.c_void_p * n)(*[w.handle.value for w in self.weights]), n, ctypes.byref(h)))
         self._h = h
@@ -529,73 +537,88 @@ class Experts:
 def moe_route(logits, k: int, normalize: bool = True, stream=None):
     """Top-k routing of logits [T][E] (nxq_moe_route): (ids [T][k], weights [T][k],
     offsets [E + 1], rows [T * k], slots [T][k]), on the device."""
-    import torch
-
-    _arg(logits.dim() == 2, f"moe_route: logits have {logits.dim()} dimensions, not 2")
+    torch = _torch or _load_torch()
+    if logits.dim() != 2:
+        raise _bad(f"moe_route: logits have {logits.dim()} dimensions, not 2")
     code = _float_code("moe_route", "logits", logits.dtype)
-    _tensors("moe_route", logits=logits)
+    d = _usable("moe_route", "logits", logits)
     T, E = logits.shape
-    _arg(1 <= k <= min(E, 32), f"moe_route: k={k} of {E} experts (at most 32)")
-    i32 = dict(dtype=torch.int32, device=logits.device)
-    ids, slots = torch.empty((T, k), **i32), torch.empty((T, k), **i32)
-    weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
-    offsets, rows = torch.empty(E + 1, **i32), torch.empty(T * k, **i32)
+    if not 1 <= k <= min(E, 32):
+        raise _bad(f"moe_route: k={k} of {E} experts (at most 32)")
+    i32 = torch.int32
+    ids, slots = logits.new_empty((T, k), dtype=i32), logits.new_empty((T, k), dtype=i32)
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    offsets, rows = logits.new_empty(E + 1, dtype=i32), logits.new_empty(T * k, dtype=i32)
     _check(lib().nxq_moe_route(logits.data_ptr(), code, T, E, k, 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
-                               offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_of(stream, logits)))
+                               offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_on(stream, d)))
     return ids, weights, offsets, rows, slots
 
 
 def _ragged(what: str, experts, x, offsets, rows, out, out_dtype):
-    """Checks a ragged product's arguments: (X, R, out)."""
-    _arg(x.dim() == 2 and x.shape[1] == experts.K, f"{what}: x is {tuple(x.shape)}, not [rows][{experts.K}]")
-    _int32(what, offsets=offsets, rows=rows)
-    _tensors(what, x=x, offsets=offsets, rows=rows, out=out)
-    _arg(offsets.numel() == experts.count + 1, f"{what}: {offsets.numel()} offsets for {experts.count} experts")
-    _arg(rows is None or rows.dim() == 1, f"{what}: rows must be one-dimensional")
-    R = x.shape[0] if rows is None else rows.numel()
-    return x.shape[0], R, _out(what, out, (R, experts.N), out_dtype, x.device)
+    """Checks a ragged product's arguments: (device, x's and out's type codes, X, rows pointer, R, out)."""
+    torch = _torch or _load_torch()
+    if x.dim() != 2 or x.shape[1] != experts.K:
+        raise _bad(f"{what}: x is {tuple(x.shape)}, not [rows][{experts.K}]")
+    code = _float_code(what, "x", x.dtype)
+    if offsets.dtype is not torch.int32 or offsets.numel() != experts.count + 1:
+        raise _bad(f"{what}: offsets are {offsets.numel()} of {offsets.dtype}, not {experts.count + 1} of torch.int32")
+    d = _usable(what, "x", x)
+    _usable(what, "offsets", offsets)
+    X = R = x.shape[0]
+    rp = None
+    if rows is not None:
+        if rows.dtype is not torch.int32 or rows.dim() != 1:
+            raise _bad(f"{what}: rows must be one-dimensional torch.int32")
+        _usable(what, "rows", rows)
+        R, rp = rows.shape[0], rows.data_ptr()
+    out, ycode = _output(what, out, (R, experts.N), out_dtype, x)
+    return d, code, ycode, X, rp, R, out
 
 
 def qmatmul_ragged(experts: Experts, x, offsets, rows=None, out=None, out_dtype=None, stream=None):
     """y[s] = x[rows[s]] W_e^T for the slots offsets[e] <= s < offsets[e + 1] of
     every expert e (nxq_qmatmul_ragged); x[s] without rows.  Rows of `out` that
     no expert has are left as they are (undefined in a new tensor)."""
-    X, R, out = _ragged("qmatmul_ragged", experts, x, offsets, rows, out, out_dtype)
-    _check(lib().nxq_qmatmul_ragged(experts.handle, x.data_ptr(), _float_code("qmatmul_ragged", "x", x.dtype), X,
-                                    None if rows is None else rows.data_ptr(), out.data_ptr(),
-                                    _float_code("qmatmul_ragged", "out", out.dtype), R, offsets.data_ptr(),
-                                    _stream_of(stream, x)))
+    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged", experts, x, offsets, rows, out, out_dtype)
+    _check(lib().nxq_qmatmul_ragged(experts.handle, x.data_ptr(), xc, X, rp, out.data_ptr(), yc, R, offsets.data_ptr(),
+                                    _stream_on(stream, d)))
     return out
 
 
 def qmatmul_ragged_swiglu(gate: Experts, up: Experts, x, offsets, rows=None, out=None, out_dtype=None, stream=None):
     """h[s] = silu(x Wg_e^T) * (x Wu_e^T) with x = x[rows[s]] (nxq_qmatmul_ragged_swiglu)."""
-    X, R, out = _ragged("qmatmul_ragged_swiglu", gate, x, offsets, rows, out, out_dtype)
-    _check(lib().nxq_qmatmul_ragged_swiglu(gate.handle, up.handle, x.data_ptr(),
-                                           _float_code("qmatmul_ragged_swiglu", "x", x.dtype), X,
-                                           None if rows is None else rows.data_ptr(), out.data_ptr(),
-                                           _float_code("qmatmul_ragged_swiglu", "out", out.dtype), R,
-                                           offsets.data_ptr(), _stream_of(stream, x)))
+    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged_swiglu", gate, x, offsets, rows, out, out_dtype)
+    _check(lib().nxq_qmatmul_ragged_swiglu(gate.handle, up.handle, x.data_ptr(), xc, X, rp, out.data_ptr(), yc, R,
+                                           offsets.data_ptr(), _stream_on(stream, d)))
     return out
 
 
 def moe_combine(h, slots, weights, res=None, out=None, out_dtype=None, stream=None):
     """y[t] = sum_j weights[t][j] * h[slots[t][j]] (+ res[t]); negative slots are
     skipped (nxq_moe_combine).  out may be res."""
-    import torch
-
+    torch = _torch or _load_torch()
     what = "moe_combine"
-    _arg(h.dim() == 2 and slots.dim() == 2, f"{what}: h and slots must be two-dimensional")
-    _int32(what, slots=slots)
-    _arg(weights.dtype == torch.float32 and weights.shape == slots.shape, f"{what}: weights must be fp32 of slots' shape")
-    _arg(res is None or (res.dtype == torch.float32 and tuple(res.shape) == (slots.shape[0], h.shape[1])),
-         f"{what}: res must be fp32 [T][N]")
-    _tensors(what, h=h, slots=slots, weights=weights, res=res, out=out)
+    if h.dim() != 2 or slots.dim() != 2:
+        raise _bad(f"{what}: h and slots must be two-dimensional")
+    code = _float_code(what, "h", h.dtype)
+    if slots.dtype is not torch.int32:
+        raise _bad(f"{what}: slots must be torch.int32")
+    if weights.dtype is not torch.float32 or weights.shape != slots.shape:
+        raise _bad(f"{what}: weights must be fp32 of slots' shape")
+    d = _usable(what, "h", h)
+    _usable(what, "slots", slots)
+    _usable(what, "weights", weights)
+    R, N = h.shape
     T, k = slots.shape
-    out = _out(what, out, (T, h.shape[1]), out_dtype, h.device)
-    _check(lib().nxq_moe_combine(h.data_ptr(), _float_code(what, "h", h.dtype), h.shape[0], h.shape[1], slots.data_ptr(),
-                                 weights.data_ptr(), T, k, None if res is None else res.data_ptr(), out.data_ptr(),
-                                 _float_code(what, "out", out.dtype), _stream_of(stream, h)))
+    rp = None
+    if res is not None:
+        if res.dtype is not torch.float32 or tuple(res.shape) != (T, N):
+            raise _bad(f"{what}: res must be fp32 [{T}][{N}]")
+        _usable(what, "res", res)
+        rp = res.data_ptr()
+    out, ycode = _output(what, out, (T, N), out_dtype, h)
+    _check(lib().nxq_moe_combine(h.data_ptr(), code, R, N, slots.data_ptr(), weights.data_ptr(), T, k, rp, out.data_ptr(),
+                                 ycode, _stream_on(stream, d)))
     return out
 
 
