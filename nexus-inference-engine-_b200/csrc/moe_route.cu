@@ -6,15 +6,16 @@
 // Routing has three steps.  (1) One warp per token: lane l holds the logits of
 // experts l, l + 32, ... as order-preserving integer keys and knows its largest;
 // k rounds of a warp maximum (redux on the key; among lanes with equal keys redux
-// on the index, so ties go to the lowest) pick the choices, and only the lane
-// that held a choice looks for its next largest.  (2) Counts of every expert in
-// every block of tokens, and their exclusive scan over blocks: 32 experts per
-// CTA.  (3) Every block ranks its own choices: a warp walks a contiguous run of
+// on the index, so ties go to the lowest) pick the choices; a lane keeps its two
+// largest and looks again only when both are gone.  The block counts its choices
+// of every expert.  (2) An exclusive scan of the counts over blocks, 32 experts
+// per CTA.  (3) Every block ranks its own choices: a warp walks a contiguous run of
 // choices in order, equal experts among 32 lanes ranked by their lane (match),
 // so slots are ordered by (expert, token) and do not depend on timing - the
 // counts are integers and no atomic decides a place.  Up to kSmallT tokens one
 // CTA does all three.
 #include "nxq_internal.h"
+#include "sm100_ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,6 +28,7 @@ constexpr int kMaxE = 1024, kMaxK = 32;
 constexpr int kRankWarps = 8;        // contiguous runs a block's choices are ranked in
 constexpr int kThreads = 32 * kRankWarps;
 constexpr int kSmallThreads = 1024;
+constexpr int kChooseThreads = 512;
 constexpr int kSmallT = 128;
 constexpr int kMaxBlocks = 256;      // of tokens
 constexpr float kInf = __builtin_huge_valf();
@@ -43,7 +45,7 @@ struct RouteParams {
     int32_t* offsets;
     int32_t* rows;
     int32_t* slots;
-    int32_t* before;  // [blocks][E]: choices of the expert in the blocks before
+    int32_t* before;  // [blocks][E]: choices of the expert in the block, then in the blocks before it
     int32_t* total;   // [E]
 };
 
@@ -72,26 +74,51 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // The choices of token t by one warp; lane j < k returns choice j (-1: none).
+// logit: its logits as read_logits left them; they are replaced by token next's
+// (none if < 0), whose loads so overlap the choosing.
 template <int V>
-__device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int lane) {
+__device__ __forceinline__ void read_logits(const RouteParams& p, int64_t t, int lane, float (&logit)[V]) {
+    auto read = [&](const auto* row, auto widen) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) logit[i] = lane + 32 * i < p.E ? widen(row[lane + 32 * i]) : -kInf;
+    };
+    const int64_t at = t * p.E;
+    if (p.dtype == NXQ_F32)
+        read(static_cast<const float*>(p.logits) + at, [](float v) { return v; });
+    else if (p.dtype == NXQ_F16)
+        read(static_cast<const __half*>(p.logits) + at, [](__half v) { return __half2float(v); });
+    else
+        read(static_cast<const __nv_bfloat16*>(p.logits) + at, [](__nv_bfloat16 v) { return __bfloat162float(v); });
+}
+template <int V>
+__device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int64_t next, int lane, float (&logit)[V]) {
     uint32_t key[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = e < p.E ? key_of(load_logit(p.logits, p.dtype, t * p.E + e)) : 0u;
-    }
-    uint32_t top = 0u;  // this lane's largest key, and its expert
-    int at = 0;
-    auto largest = [&] {
-        top = 0u;
+    for (int i = 0; i < V; ++i) key[i] = key_of(logit[i]);
+    if (next >= 0) read_logits<V>(p, next, lane, logit);
+    // This lane's two largest keys behind (last, last_at) in the order of
+    // choice, and their experts: most lanes are asked for no third.
+    uint32_t top, top2;
+    int at = 0, at2 = 0, known;
+    auto look = [&](uint32_t last, int last_at) {
+        top = top2 = 0u;
+        known = 2;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (key[i] > top) {
-                top = key[i];
-                at = lane + 32 * i;
+        for (int i = 0; i < V; ++i) {
+            const int e = lane + 32 * i;
+            const uint32_t k = key[i] < last || (key[i] == last && e > last_at) ? key[i] : 0u;
+            if (k > top) {
+                top2 = top;
+                at2 = at;
+                top = k;
+                at = e;
+            } else if (k > top2) {
+                top2 = k;
+                at2 = e;
             }
+        }
     };
-    largest();
+    look(0xFFFFFFFFu, -1);
     const uint32_t first = __reduce_max_sync(0xFFFFFFFFu, top);
     const float m = value_of(first);
     float all = 0.0f;  // sum over every expert
@@ -102,24 +129,27 @@ __device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int lane)
         all = warp_sum(all);
     }
     int my_id = -1;
-    float my_p = 0.0f;
+    uint32_t my_key = 0u;
     uint32_t best = first;
     for (int j = 0; j < p.k && best; ++j) {
         const unsigned who = __ballot_sync(0xFFFFFFFFu, top == best);
         const int e = __popc(who) == 1 ? __shfl_sync(0xFFFFFFFFu, at, __ffs(who) - 1)
                                        : __reduce_min_sync(0xFFFFFFFFu, top == best ? at : 0x7FFFFFFF);
         if (top == best && at == e) {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (lane + 32 * i == e) key[i] = 0u;
-            largest();
+            if (--known) {
+                top = top2;
+                at = at2;
+            } else {
+                look(best, e);
+            }
         }
         if (lane == j) {
             my_id = e;
-            my_p = share_of(value_of(best), m);
+            my_key = best;
         }
         best = __reduce_max_sync(0xFFFFFFFFu, top);
     }
+    const float my_p = my_id >= 0 ? share_of(value_of(my_key), m) : 0.0f;
     const float z = p.normalize ? warp_sum(my_p) : all;
     if (lane < p.k) {
         p.ids[t * p.k + lane] = my_id;
@@ -210,8 +240,10 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteP
     overlap_begin();
     __syncthreads();
     int id = -1;
+    float logit[V];
+    if (warp < p.T) read_logits<V>(p, warp, lane, logit);
     for (int64_t t = warp; t < p.T; t += threads / 32) {
-        id = choose<V>(p, t, lane);
+        id = choose<V>(p, t, t + threads / 32 < p.T ? t + threads / 32 : -1, lane, logit);
         if (id >= 0) atomicAdd(&hist[id], 1);
     }
     __syncthreads();
@@ -229,38 +261,39 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteP
     rank_choices(p, 0, p.T, start, base, threads);
 }
 
-// A warp per token.
 template <int V>
-__global__ void __launch_bounds__(kThreads) route_choose_kernel(const RouteParams p) {
-    overlap_begin();
-    const int64_t t = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    if (t < p.T) choose<V>(p, t, threadIdx.x & 31);
-}
-
-// 32 experts per CTA: counts them in every block of tokens (shared memory), then
-// each warp scans a run of blocks, lane = expert.
-__global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
-    __shared__ int32_t cnt[kMaxBlocks][32];
-    __shared__ int32_t part[32][33];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int e0 = blockIdx.x * 32, e = e0 + lane;
-    for (int i = threadIdx.x; i < p.blocks * 32; i += 1024) cnt[i >> 5][i & 31] = 0;
+__global__ void __launch_bounds__(kChooseThreads) route_choose_kernel(const RouteParams p) {
+    extern __shared__ int32_t cnt[];  // [E]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int e = tid; e < p.E; e += kChooseThreads) cnt[e] = 0;
     overlap_begin();
     __syncthreads();
-    // Warp w counts the choices of blocks w, w + 32, ...
-    const int64_t n = p.T * p.k, per_block = (int64_t)p.tb * p.k;
-    for (int b = warp; b < p.blocks; b += 32) {
-        const int64_t z = (b + 1) * per_block < n ? (b + 1) * per_block : n;
-#pragma unroll 4
-        for (int64_t c = b * per_block + lane; c < z; c += 32) {
-            const int id = p.ids[c] - e0;
-            if (id >= 0 && id < 32) atomicAdd(&cnt[b][id], 1);
-        }
+    const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
+    constexpr int kStep = kChooseThreads / 32;
+    float logit[V];
+    if (t0 + warp < t1) read_logits<V>(p, t0 + warp, lane, logit);
+    for (int64_t t = t0 + warp; t < t1; t += kStep) {
+        const int id = choose<V>(p, t, t + kStep < t1 ? t + kStep : -1, lane, logit);
+        if (id >= 0) atomicAdd(&cnt[id], 1);
     }
     __syncthreads();
-    const int per = (p.blocks + 31) / 32, b0 = warp * per, b1 = b0 + per < p.blocks ? b0 + per : p.blocks;
-    int s = 0;
-    for (int b = b0; b < b1; ++b) s += cnt[b][lane];
+    for (int e = tid; e < p.E; e += kChooseThreads) p.before[(int64_t)blockIdx.x * p.E + e] = cnt[e];
+}
+
+// 32 experts per CTA, lane = expert; the 32 warps scan a run of blocks each.
+__global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
+    __shared__ int32_t part[32][33];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int e = blockIdx.x * 32 + lane;
+    overlap_begin();
+    constexpr int kPer = kMaxBlocks / 32;  // blocks of a warp, at most
+    const int per = (p.blocks + 31) / 32, b0 = warp * per;
+    int c[kPer], s = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        c[i] = i < per && b0 + i < p.blocks && e < p.E ? p.before[(int64_t)(b0 + i) * p.E + e] : 0;
+        s += c[i];
+    }
     part[warp][lane] = s;
     __syncthreads();
     int at = 0, all = 0;
@@ -272,10 +305,12 @@ __global__ void __launch_bounds__(1024) route_scan_kernel(const RouteParams p) {
     }
     if (e >= p.E) return;
     if (warp == 0) p.total[e] = all;
-    for (int b = b0; b < b1; ++b) {
-        p.before[(int64_t)b * p.E + e] = at;
-        at += cnt[b][lane];
-    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (i < per && b0 + i < p.blocks) {
+            p.before[(int64_t)(b0 + i) * p.E + e] = at;
+            at += c[i];
+        }
 }
 
 __global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams p) {
@@ -306,8 +341,7 @@ cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStr
         const unsigned warps = p.T < 4 ? 4 : p.T < 32 ? (unsigned)p.T : 32;
         return launch_overlapped(route_small_kernel<V>, 1, 32 * warps, smem, st, p);
     }
-    const int64_t per = kThreads / 32;
-    return launch_overlapped(route_choose_kernel<V>, (unsigned)((p.T + per - 1) / per), kThreads, 0, st, p);
+    return launch_overlapped(route_choose_kernel<V>, (unsigned)p.blocks, kChooseThreads, p.E * sizeof(int32_t), st, p);
 }
 
 cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
@@ -372,6 +406,26 @@ __device__ __forceinline__ void store_as(void* p, int dt, int64_t i, float v) {
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// Eight consecutive outputs (fp32: 32-byte, else 16-byte aligned).
+__device__ __forceinline__ void store8(void* y, int dt, int64_t o, const float (&v)[8]) {
+    if (dt == NXQ_F32) {
+        store_f32x8(static_cast<float*>(y) + o, v);
+        return;
+    }
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (dt == NXQ_F16) {
+            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            q[i] = *reinterpret_cast<const uint32_t*>(&p);
+        } else {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            q[i] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + o) = make_uint4(q[0], q[1], q[2], q[3]);
+}
+
 // Items are (token, 32 VEC columns), segs to a token.  VEC = 8 needs N % 8 == 0,
 // h and y 16-byte and an fp32 residual or output 32-byte aligned.  F32: h's type.
 template <int VEC, bool F32>
@@ -383,28 +437,40 @@ __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __res
     overlap_begin();
     const int lane = threadIdx.x & 31;
     const int64_t items = T * segs, step = (int64_t)gridDim.x * (kCombThreads / 32);
-    int64_t it = (int64_t)blockIdx.x * (kCombThreads / 32) + (threadIdx.x >> 5);
+    const int64_t dt = step / segs, dseg = step - dt * segs;  // one step in tokens and segments
+    const int64_t it0 = (int64_t)blockIdx.x * (kCombThreads / 32) + (threadIdx.x >> 5);
+    int64_t t = it0 / segs, seg = it0 - t * segs;
     int next_s = -1;
     float next_w = 0.0f;
-    auto fetch = [&](int64_t i) {
-        if (i < items && lane < k) {
-            next_s = slots[(i / segs) * k + lane];
-            next_w = weights[(i / segs) * k + lane];
+    auto fetch = [&](int64_t tok) {
+        if (tok < T && lane < k) {
+            next_s = slots[tok * k + lane];
+            next_w = weights[tok * k + lane];
         }
     };
-    fetch(it);
-    for (; it < items; it += step) {
-        const int64_t t = it / segs, n = ((it - t * segs) * 32 + lane) * VEC;
+    fetch(t);
+    for (int64_t it = it0; it < items; it += step) {
+        const int64_t n = (seg * 32 + lane) * VEC, o = t * N + n;
         int my_s = next_s;
         const float my_w = next_w;
         if (my_s >= R) {
             raise_index(status, kIndexSlot);
             my_s = -1;
         }
+        t += dt;
+        seg += dseg;
+        if (seg >= segs) {
+            seg -= segs;
+            ++t;
+        }
         float acc[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+        float rv[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) rv[i] = 0.0f;
         if constexpr (VEC == 8) {
+            if (res && n < N) load_f32x8(res + o, rv);
             for (int j0 = 0; j0 < k; j0 += kBatch) {
                 Raw8<F32> r[kBatch];
 #pragma unroll
@@ -412,7 +478,7 @@ __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __res
                     const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
                     if (j0 + j < k && s >= 0 && n < N) r[j].load(h, (int64_t)s * N + n);
                 }
-                if (j0 + kBatch >= k) fetch(it + step);
+                if (j0 + kBatch >= k) fetch(t);
 #pragma unroll
                 for (int j = 0; j < kBatch; ++j) {
                     const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
@@ -426,38 +492,134 @@ __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __res
                 }
             }
             if (n >= N) continue;
-            const int64_t o = t * N + n;
-            if (res) {
-                float v[8];
-                load_f32x8(res + o, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] += v[i];
-            }
-            if (y_dtype == NXQ_F32) {
-                store_f32x8(static_cast<float*>(y) + o, acc);
-            } else {
-                uint32_t q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (y_dtype == NXQ_F16) {
-                        const __half2 v = __floats2half2_rn(acc[2 * i], acc[2 * i + 1]);
-                        q[i] = *reinterpret_cast<const uint32_t*>(&v);
-                    } else {
-                        const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * i], acc[2 * i + 1]);
-                        q[i] = *reinterpret_cast<const uint32_t*>(&v);
-                    }
-                }
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + o) = make_uint4(q[0], q[1], q[2], q[3]);
-            }
+            for (int i = 0; i < 8; ++i) acc[i] += rv[i];
+            store8(y, y_dtype, o, acc);
         } else {
-            fetch(it + step);
+            fetch(t);
             for (int j = 0; j < k; ++j) {
                 const int s = __shfl_sync(0xFFFFFFFFu, my_s, j);
                 const float w = __shfl_sync(0xFFFFFFFFu, my_w, j);
                 if (s >= 0 && n < N) acc[0] = fmaf(w, load_h(h, h_dtype, (int64_t)s * N + n), acc[0]);
             }
-            if (n < N) store_as(y, y_dtype, t * N + n, acc[0] + (res ? res[t * N + n] : 0.0f));
+            if (n < N) store_as(y, y_dtype, o, acc[0] + (res ? res[o] : 0.0f));
         }
+    }
+}
+
+// ---- combine of many tokens ------------------------------------------------------
+// One persistent CTA per SM: a producer warp brings the k rows of a token (or
+// of `seg` columns of it) into a ring of shared memory by one bulk copy each,
+// lane j row j, and 16 warps sum them with a thread per 8 columns; the residual
+// is loaded while the rows are awaited.  Rows of several KB in flight per copy
+// and no registers to hold them.
+constexpr int kBulkWarps = 16, kBulkThreads = 32 * (kBulkWarps + 1);
+constexpr int kBulkStages = 3;
+constexpr int kBulkStage = 72 * 1024;  // bytes of a stage
+constexpr int kCombineBulk = 4;        // tokens per SM from which it is used
+
+template <bool F32>
+__global__ void __launch_bounds__(kBulkThreads, 1) combine_bulk_kernel(const void* __restrict__ h, int h_dtype, int64_t R,
+                                                                       int64_t N, const int32_t* __restrict__ slots,
+                                                                       const float* __restrict__ weights, int64_t T, int k,
+                                                                       const float* res, void* y, int y_dtype, int64_t segs,
+                                                                       int seg, DeviceStatus* status) {
+    constexpr int kSize = F32 ? 4 : 2;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint64_t full[kBulkStages], empty[kBulkStages];
+    __shared__ int s_slot[kBulkStages][kMaxK];  // -1: skipped
+    __shared__ float s_w[kBulkStages][kMaxK];
+    __shared__ int s_abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kBulkStages; ++i) {
+            ptx::mbar_init(&full[i], 1);
+            ptx::mbar_init(&empty[i], kBulkWarps);
+        }
+        s_abort = 0;
+        ptx::fence_mbar_init();
+    }
+    __syncthreads();
+    const ptx::WaitCtl ctl{&s_abort, status};
+    overlap_begin();
+    const int64_t items = T * segs;
+    if (warp == kBulkWarps) {
+        // h was written through the generic proxy; the copies read it through the async one.
+        asm volatile("fence.proxy.async;" ::: "memory");
+        uint32_t u = 0;
+        for (int64_t it = blockIdx.x; it < items; it += gridDim.x, ++u) {
+            const int st = u % kBulkStages;
+            const int64_t t = it / segs, n0 = (it - t * segs) * seg;
+            const uint32_t bytes = (uint32_t)(N - n0 < seg ? N - n0 : seg) * kSize;
+            int s = -1;
+            float w = 0.0f;
+            if (lane < k) {
+                s = slots[t * k + lane];
+                w = weights[t * k + lane];
+                if (s >= R) {
+                    raise_index(status, kIndexSlot);
+                    s = -1;
+                }
+            }
+            int ok = 1;
+            if (u >= kBulkStages) ok = ptx::mbar_wait(&empty[st], (u / kBulkStages - 1) & 1u, ctl, 61) ? 1 : 0;
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (lane < k) {
+                s_slot[st][lane] = s;
+                s_w[st][lane] = w;
+            }
+            const unsigned rows = __ballot_sync(0xFFFFFFFFu, s >= 0);
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_expect_tx(&full[st], __popc(rows) * bytes);
+            __syncwarp();
+            if (s >= 0)
+                ptx::bulk_g2s(ring + (size_t)st * kBulkStage + (size_t)lane * seg * kSize,
+                              static_cast<const uint8_t*>(h) + ((int64_t)s * N + n0) * kSize, bytes, &full[st]);
+        }
+        // Do not leave with copies in flight (bounded, ignoring the abort flag).
+        for (uint32_t i = u >= kBulkStages ? u - kBulkStages : 0; i < u; ++i) {
+            const long long t0 = clock64();
+            while (!ptx::mbar_try_wait(&full[i % kBulkStages], (i / kBulkStages) & 1u) && clock64() - t0 < ptx::kWaitCycles) {
+            }
+        }
+        return;
+    }
+    uint32_t u = 0;
+    for (int64_t it = blockIdx.x; it < items; it += gridDim.x, ++u) {
+        const int st = u % kBulkStages;
+        const int64_t t = it / segs, n0 = (it - t * segs) * seg;
+        const int cols = (int)(N - n0 < seg ? N - n0 : seg);
+        bool landed = false;
+        for (int c = threadIdx.x * 8; c < cols || !landed; c += kBulkWarps * 32 * 8) {
+            const int64_t o = t * N + n0 + c;
+            float acc[8], rv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = rv[i] = 0.0f;
+            if (res && c < cols) load_f32x8(res + o, rv);
+            if (!landed) {
+                if (!ptx::mbar_wait(&full[st], (u / kBulkStages) & 1u, ctl, 62)) return;
+                landed = true;
+            }
+            if (c >= cols) break;
+            const uint8_t* base = ring + (size_t)st * kBulkStage + (size_t)c * kSize;
+            for (int j = 0; j < k; ++j) {
+                if (s_slot[st][j] < 0) continue;
+                const float w = s_w[st][j];
+                Raw8<F32> r;
+                const uint4* q = reinterpret_cast<const uint4*>(base + (size_t)j * seg * kSize);
+#pragma unroll
+                for (int i = 0; i < (F32 ? 2 : 1); ++i) r.q[i] = q[i];
+                float v[8];
+                r.widen(h_dtype, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += rv[i];
+            store8(y, y_dtype, o, acc);
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&empty[st]);
     }
 }
 
@@ -518,10 +680,25 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
     if (int rc = context_ready()) return rc;
     const bool vec = N % 8 == 0 && (uintptr_t)h_dev % 16 == 0 && (uintptr_t)res_dev % 32 == 0 &&
                      (uintptr_t)y_dev % (y_dtype == NXQ_F32 ? 32 : 16) == 0;
+    const bool f32 = h_dtype == NXQ_F32;
+    // Many tokens: bulk copies (kCombineBulk below).
+    if (vec && T >= kCombineBulk * (int64_t)context_sm_count() && T <= ((int64_t)1 << 62) / N) {
+        int64_t seg = kBulkStage / (k * (f32 ? 4 : 2)) / 64 * 64;  // columns of a stage
+        int64_t segs = (N + seg - 1) / seg;
+        seg = ((N + segs - 1) / segs + 63) / 64 * 64;
+        segs = (N + seg - 1) / seg;
+        auto* kernel = f32 ? combine_bulk_kernel<true> : combine_bulk_kernel<false>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBulkStages * kBulkStage);
+        if (e == cudaSuccess)
+            e = launch_overlapped(kernel, (unsigned)context_sm_count(), kBulkThreads, kBulkStages * kBulkStage,
+                                  (cudaStream_t)stream, h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k, res_dev, y_dev,
+                                  y_dtype, segs, (int)seg, context_status());
+        note_launches(1);
+        return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "combine launch");
+    }
     const int64_t per = 32 * (vec ? 8 : 1), segs = (N + per - 1) / per;
     if (T > ((int64_t)1 << 62) / segs) return fail(NXQ_ERR_ARG, "combine: T=%lld N=%lld", (long long)T, (long long)N);
     const int64_t want = (T * segs + kCombThreads / 32 - 1) / (kCombThreads / 32), most = (int64_t)context_sm_count() * 8;
-    const bool f32 = h_dtype == NXQ_F32;
     const cudaError_t e = launch_overlapped(
         vec ? (f32 ? combine_kernel<8, true> : combine_kernel<8, false>) : combine_kernel<1, false>,
         (unsigned)(want < most ? want : most), kCombThreads, 0, (cudaStream_t)stream, h_dev, h_dtype, R, N, slots_dev,

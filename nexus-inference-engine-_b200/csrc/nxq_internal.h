@@ -137,7 +137,7 @@ __device__ __forceinline__ void overlap_begin() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 // 32 consecutive bytes (32-byte aligned) in one access.
-__device__ __forceinline__ void store_f32x8(float* p, const float (&v)[8]) {
+__device__ __forceinline__ void store_f32x8(float* p, const float* v) {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                  "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                  : "memory");

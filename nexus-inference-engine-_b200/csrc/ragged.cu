@@ -33,15 +33,17 @@ int check_experts(nxq_experts_t h, const ExpertTable** out) {
     return NXQ_OK;
 }
 
-// One CTA, thread = expert: writes the experts that have rows.  An expert's
+// One CTA of at least E threads, thread = expert: writes the experts that have rows.  An expert's
 // range is taken only if it lies in [0, R] and starts at or behind every offset
 // before it, so the ranges taken never overlap and hold at most R slots
 // whatever the offsets are; anything else is reported and left out.
 __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t R, int blk, RaggedPlan* plan,
-                                          DeviceStatus* status) {
+                                          const uint8_t* const* w, const uint8_t* const* up, DeviceStatus* status) {
     __shared__ int warp_n[32], warp_b[32], warp_m[32];
     const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
     const int o0 = e < E ? offsets[e] : 0, o1 = e < E ? offsets[e + 1] : 0;
+    const uint8_t* const we = e < E ? w[e] : nullptr;
+    const uint8_t* const ue = e < E && up ? up[e] : nullptr;
     int before = o0;  // the largest offset up to and including o0
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -76,8 +78,8 @@ __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t
         n0 += warp_n[w];
         b0 += warp_b[w];
     }
-    if (has) plan->it[n0 + __popc(act & ((1u << lane) - 1u))] = RaggedEntry{e, a, n, b0 + bs - nb};
-    if (e == kMaxExperts - 1) {
+    if (has) plan->it[n0 + __popc(act & ((1u << lane) - 1u))] = RaggedEntry{e, a, n, b0 + bs - nb, we, ue};
+    if (e == (int)blockDim.x - 1) {
         plan->entries = n0 + __popc(act);
         plan->blocks = b0 + bs;
     }
@@ -100,8 +102,6 @@ __device__ __forceinline__ void store_y(void* y, int dt, int64_t i, float v) {
 constexpr int kSimtBlk = 8;  // rows per work tile
 
 struct SimtParams {
-    const uint8_t* const* w;
-    const uint8_t* const* up;
     TiledShape s;
     const void* x;
     int x_dtype;
@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(TILE_ROWS) ragged_simt_kernel(const SimtParams
                         for (int i = 0; i < 8; ++i) a[m] = fmaf(v[i], xs[m][e0 + i], a[m]);
                 }
             };
-            add(p.w[t.e], acc);
-            if constexpr (PAIR) add(p.up[t.e], accu);
+            add(t.w, acc);
+            if constexpr (PAIR) add(t.up, accu);
         }
         const int64_t n = (int64_t)t.tile * TILE_ROWS + r;
         if (n >= p.s.N) continue;
@@ -191,6 +191,8 @@ struct PrepParams {
     int64_t R;
     int blk;
     RaggedPlan* plan;
+    const uint8_t* const* w;
+    const uint8_t* const* up;
     unsigned* cnt;
     int n_cnt;
     const void* x;
@@ -200,20 +202,20 @@ struct PrepParams {
     __half* xh;
     DeviceStatus* status;
 };
-constexpr int kRowThreads = 256, kRowGroups = kMaxExperts / kRowThreads;
+constexpr int kRowThreads = 256;
 
 template <int VEC>
 __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepParams p) {
     overlap_begin();  // the product kernel may set itself up meanwhile
     if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < p.n_cnt; i += kMaxExperts) p.cnt[i] = 0u;
-        make_plan(p.offsets, p.E, p.R, p.blk, p.plan, p.status);
+        for (int i = threadIdx.x; i < p.n_cnt; i += blockDim.x) p.cnt[i] = 0u;
+        make_plan(p.offsets, p.E, p.R, p.blk, p.plan, p.w, p.up, p.status);
         return;
     }
     const int64_t lo = p.offsets[0] > 0 ? p.offsets[0] : 0, hi = p.offsets[p.E] < p.R ? p.offsets[p.E] : p.R;
-    const int group = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads;
+    const int group = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads, groups = blockDim.x / kRowThreads;
     bool over = false;
-    for (int64_t s = lo + (int64_t)(blockIdx.x - 1) * kRowGroups + group; s < hi; s += (int64_t)(gridDim.x - 1) * kRowGroups) {
+    for (int64_t s = lo + (int64_t)(blockIdx.x - 1) * groups + group; s < hi; s += (int64_t)(gridDim.x - 1) * groups) {
         int64_t row = p.rows ? p.rows[s] : s;
         if (row < 0 || row >= p.X) {
             if (lane == 0) raise_index(p.status, kIndexRow);
@@ -262,17 +264,21 @@ __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepPara
 }
 
 cudaError_t launch_prep(const RaggedCall& c, int blk, RaggedPlan* plan, unsigned* cnt, int n_cnt, __half* xh) {
-    const PrepParams p{c.offsets, c.w->count, c.R, blk, plan, cnt, n_cnt, c.x, c.x_dtype, c.X, c.w->shape.K, c.rows, xh,
+    const PrepParams p{c.offsets, c.w->count, c.R, blk, plan, c.w->dev, c.up ? c.up->dev : nullptr, cnt, n_cnt, c.x, c.x_dtype, c.X, c.w->shape.K, c.rows, xh,
                        context_status()};
-    const int64_t most = (int64_t)context_sm_count() * 2, want = (c.R + kRowGroups - 1) / kRowGroups;
+    // A thread per expert, in whole warps; whole groups of kRowThreads if rows move.
+    const int unit = xh ? kRowThreads : 32;
+    const unsigned threads = (unsigned)((c.w->count + unit - 1) / unit * unit);
+    const int64_t groups = threads / kRowThreads;
+    const int64_t most = (int64_t)context_sm_count() * 8 / (groups ? groups : 1), want = groups ? (c.R + groups - 1) / groups : 0;
     const unsigned grid = 1 + (unsigned)(!xh ? 0 : want < most ? want : most);
     const bool vec = ((uintptr_t)c.x % 16) == 0;  // K is a multiple of 32
     note_launches(1);
-    return launch_overlapped(vec ? ragged_prep_kernel<8> : ragged_prep_kernel<1>, grid, kMaxExperts, 0, c.st, p);
+    return launch_overlapped(vec ? ragged_prep_kernel<8> : ragged_prep_kernel<1>, grid, threads, 0, c.st, p);
 }
 
 int run_simt(const RaggedCall& c, const RaggedPlan* plan) {
-    SimtParams p{c.w->dev, c.up ? c.up->dev : nullptr, c.w->shape, c.x, c.x_dtype, c.X, c.rows, c.y, c.y_dtype, plan,
+    SimtParams p{c.w->shape, c.x, c.x_dtype, c.X, c.rows, c.y, c.y_dtype, plan,
                  context_status()};
     const int64_t work = ragged_max_blocks(c.w->count, c.R, kSimtBlk) * c.w->shape.tiles;
     const int64_t cap = (int64_t)context_sm_count() * 16;

@@ -23,18 +23,23 @@ struct ExpertTable {
 // expert by expert, inside an expert by weight tile and then by row block, so
 // consecutive work tiles read the same weight tile.
 struct RaggedEntry {
-    int e;     // expert
-    int row0;  // first slot
-    int rows;  // slots (> 0)
-    int blk0;  // row blocks of the entries before
+    int e;              // expert
+    int row0;           // first slot
+    int rows;           // slots (> 0)
+    int blk0;           // row blocks of the entries before
+    const uint8_t* w;   // the expert's tiled weight
+    const uint8_t* up;  // its up weight (SwiGLU)
 };
 struct RaggedPlan {
     int entries;
     int blocks;  // row blocks of all entries
-    int pad[2];
+    int pad[6];
     RaggedEntry it[1];
 };
-inline size_t plan_bytes(int64_t max_entries) { return 16 + (size_t)max_entries * sizeof(RaggedEntry); }
+// At least 32 entries, so that a warp may load the first 32 whatever their number.
+inline size_t plan_bytes(int64_t max_entries) {
+    return 32 + (size_t)(max_entries < 32 ? 32 : max_entries) * sizeof(RaggedEntry);
+}
 
 struct RaggedCall {
     const ExpertTable* w;   // (gate) experts
@@ -50,9 +55,11 @@ struct RaggedCall {
     cudaStream_t st;
 };
 
-// One work tile: weight tile `tile` of expert e, slots [row0, row0 + rows).
+// One work tile: weight tile `tile` of the expert's weights, slots [row0, row0 +
+// rows).
 struct RaggedTile {
-    int e, tile, row0, rows;
+    const uint8_t *w, *up;
+    int tile, row0, rows;
 };
 
 // Walks a plan's work tiles in ascending order (experts of `tiles` weight tiles,
@@ -69,25 +76,28 @@ struct RaggedWalk {
     int nb;
     __device__ __forceinline__ void load(int j) {
         i = j;
-        const int4 v = *reinterpret_cast<const int4*>(&plan->it[j]);
-        cur = RaggedEntry{v.x, v.y, v.z, v.w};
+        const int4* q = reinterpret_cast<const int4*>(&plan->it[j]);
+        const int4 v = q[0];
+        const longlong2 a = *reinterpret_cast<const longlong2*>(q + 1);
+        cur = RaggedEntry{v.x, v.y, v.z, v.w, reinterpret_cast<const uint8_t*>(a.x), reinterpret_cast<const uint8_t*>(a.y)};
         nb = (cur.rows + blk - 1) / blk;
         first = (int64_t)cur.blk0 * tiles;
         end = first + (int64_t)nb * tiles;
     }
-    // Starts at work tile g (one that exists).
+    // Starts at work tile g (one that exists).  By a converged warp, which looks
+    // at 32 entries at a time: one round trip to memory for most calls.
     __device__ __forceinline__ void start(const RaggedPlan* p, int blk_, int tiles_, int64_t g) {
         plan = p;
         blk = blk_;
         tiles = tiles_;
         entries = p->entries;
-        int lo = 0, hi = entries - 1;  // the last entry whose first work tile is <= g
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if ((int64_t)p->it[mid].blk0 * tiles <= g)
-                lo = mid;
-            else
-                hi = mid - 1;
+        const int lane = threadIdx.x & 31;
+        int lo = 0;
+        for (int j0 = 0;; j0 += 32) {  // the last entry whose first work tile is <= g
+            const bool in = j0 + lane < entries && (int64_t)p->it[j0 + lane].blk0 * tiles <= g;
+            const unsigned m = __ballot_sync(0xFFFFFFFFu, in);
+            if (m) lo = j0 + 31 - __clz(m);
+            if (m != 0xFFFFFFFFu) break;
         }
         load(lo);
     }
@@ -96,7 +106,8 @@ struct RaggedWalk {
         while (g >= end && i + 1 < entries) load(i + 1);
         const int local = (int)(g - first);
         RaggedTile t;
-        t.e = cur.e;
+        t.w = cur.w;
+        t.up = cur.up;
         t.tile = local / nb;
         const int b = local - t.tile * nb;
         int rb = blk;

@@ -83,8 +83,6 @@ struct Rings {
 };
 
 struct Params {
-    const uint8_t* const* w;
-    const uint8_t* const* up;
     TiledShape s;
     int tiles;  // work tiles per row block
     void* y;
@@ -212,12 +210,12 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     const int64_t G = gridDim.x;
 
     if (warp == kWarpWProducer) {
+        RaggedWalk<true> walk;
+        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
         if (lane == 0) {
             Ring rw;
             uint32_t issued = 0;
             bool ok = true;
-            RaggedWalk<true> walk;
-            walk.start(p.plan, kNT, p.tiles, blockIdx.x);
             for (int64_t g = blockIdx.x; g < total && ok; g += G) {
                 const RaggedTile t = walk.at(g);
                 const uint8_t* src[kMats];
@@ -225,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                 for (int mat = 0; mat < kMats; ++mat) {
                     bool exists;
                     const int wt = weight_tile<PAIR>(t, mat, p.s.tiles, &exists);
-                    src[mat] = (PAIR && mat ? p.up : p.w)[t.e] + p.s.chunk_offset(wt, 0);
+                    src[mat] = (PAIR && mat ? t.up : t.w) + p.s.chunk_offset(wt, 0);
                 }
                 for (int c = 0; c < chunks && ok; ++c)
 #pragma unroll
@@ -353,6 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                     if (!ok) continue;
                     ptx::tc_fence_after();
                     ptx::tmem_st32(tbase + st * kACols, o);
+                    // (Announcing the stage only after the next decode, to hide
+                    // the store's latency, was 5 % slower.)
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
@@ -505,8 +505,8 @@ int set_attr() {
 }
 
 template <int TYPE>
-int launch(const Params& p, const CUtensorMap& tmap, unsigned grid, cudaStream_t st) {
-    if (p.up)
+int launch(const Params& p, const CUtensorMap& tmap, bool pair, unsigned grid, cudaStream_t st) {
+    if (pair)
         ragged_gemm_kernel<TYPE, true><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
     else
         ragged_gemm_kernel<TYPE, false><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
@@ -534,26 +534,26 @@ int ragged_gemm_blk() { return kNT; }
 
 int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan) {
     const TiledShape& s = c.w->shape;
-    Params p{c.w->dev, c.up ? c.up->dev : nullptr, s, (int)(c.up ? s.tiles : (s.tiles + 1) / 2), c.y, c.y_dtype,
+    Params p{s, (int)(c.up ? s.tiles : (s.tiles + 1) / 2), c.y, c.y_dtype,
              s.N % 8 == 0 && (uintptr_t)c.y % 16 == 0, plan, context_status()};
     CUtensorMap tmap;
     if (int rc = gemm_activation_map(&tmap, xh, X, s.K, kBoxRows)) return rc;
     const int64_t work = ragged_max_blocks(c.w->count, c.R, kNT) * p.tiles;
     const unsigned grid = (unsigned)(work < context_sm_count() ? work : context_sm_count());
     switch (s.type) {
-        case T_Q4_K: return launch<T_Q4_K>(p, tmap, grid, c.st);
-        case T_Q4_0: return launch<T_Q4_0>(p, tmap, grid, c.st);
+        case T_Q4_K: return launch<T_Q4_K>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q4_0: return launch<T_Q4_0>(p, tmap, c.up != nullptr, grid, c.st);
         case T_Q8_0:
-        case T_NXF_I8: return launch<T_Q8_0>(p, tmap, grid, c.st);
-        case T_Q3_K: return launch<T_Q3_K>(p, tmap, grid, c.st);
-        case T_I4G128: return launch<T_I4G128>(p, tmap, grid, c.st);
-        case T_Q6_K: return launch<T_Q6_K>(p, tmap, grid, c.st);
-        case T_Q5_K: return launch<T_Q5_K>(p, tmap, grid, c.st);
-        case T_Q4_1: return launch<T_Q4_1>(p, tmap, grid, c.st);
-        case T_Q2_K: return launch<T_Q2_K>(p, tmap, grid, c.st);
-        case T_I4G32: return launch<T_I4G32>(p, tmap, grid, c.st);
-        case T_I4G64: return launch<T_I4G64>(p, tmap, grid, c.st);
-        case T_I4G256: return launch<T_I4G256>(p, tmap, grid, c.st);
+        case T_NXF_I8: return launch<T_Q8_0>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q3_K: return launch<T_Q3_K>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_I4G128: return launch<T_I4G128>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q6_K: return launch<T_Q6_K>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q5_K: return launch<T_Q5_K>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q4_1: return launch<T_Q4_1>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_Q2_K: return launch<T_Q2_K>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_I4G32: return launch<T_I4G32>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_I4G64: return launch<T_I4G64>(p, tmap, c.up != nullptr, grid, c.st);
+        case T_I4G256: return launch<T_I4G256>(p, tmap, c.up != nullptr, grid, c.st);
         default: return NXQ_ERR_UNSUPPORTED;
     }
 }

@@ -76,8 +76,6 @@ struct Cfg {
 };
 
 struct Params {
-    const uint8_t* const* w;
-    const uint8_t* const* up;
     const __half* x;
     int64_t X;
     const int32_t* rows;  // or null: slot s reads row s
@@ -170,8 +168,8 @@ __global__ void __launch_bounds__(Cfg<TYPE, PAIR>::kAll, 1) ragged_mma_kernel(co
         for (int u = 0, t = g0 / kun, c = g0 % kun; u < n; ++u) {
             if (u == 0 || c == 0) {
                 const RaggedTile tl = walk.at(t);
-                wg = p.w[tl.e] + (int64_t)tl.tile * Kc * WB;
-                if constexpr (PAIR) wu = p.up[tl.e] + (int64_t)tl.tile * Kc * WB;
+                wg = tl.w + (int64_t)tl.tile * Kc * WB;
+                if constexpr (PAIR) wu = tl.up + (int64_t)tl.tile * Kc * WB;
                 if (tl.row0 != row0) {
                     row0 = tl.row0;
                     slots = tl.rows;
@@ -369,8 +367,8 @@ int launch(const Params& p, unsigned grid, cudaStream_t st) {
 }
 
 template <int TYPE>
-int launch_type(const Params& p, unsigned grid, cudaStream_t st) {
-    return p.up ? launch<TYPE, true>(p, grid, st) : launch<TYPE, false>(p, grid, st);
+int launch_type(const Params& p, bool pair, unsigned grid, cudaStream_t st) {
+    return pair ? launch<TYPE, true>(p, grid, st) : launch<TYPE, false>(p, grid, st);
 }
 
 }  // namespace
@@ -418,23 +416,23 @@ size_t ragged_mma_partials() { return (size_t)ragged_mma_workers() * 2 * kMT * T
 int ragged_mma(const RaggedCall& c, const __half* xh, int64_t X, const int32_t* rows, const RaggedPlan* plan, float* part,
                unsigned* cnt) {
     const TiledShape& s = c.w->shape;
-    const Params p{c.w->dev, c.up ? c.up->dev : nullptr, xh, X, rows, c.y, c.y_dtype, s.N, s.K, (int)s.chunks,
+    const Params p{xh, X, rows, c.y, c.y_dtype, s.N, s.K, (int)s.chunks,
                    (int)s.tiles, plan, part, cnt, context_status()};
     const unsigned grid = (unsigned)context_sm_count();
     switch (s.type) {
-        case T_Q4_K: return launch_type<T_Q4_K>(p, grid, c.st);
-        case T_Q4_0: return launch_type<T_Q4_0>(p, grid, c.st);
+        case T_Q4_K: return launch_type<T_Q4_K>(p, c.up != nullptr, grid, c.st);
+        case T_Q4_0: return launch_type<T_Q4_0>(p, c.up != nullptr, grid, c.st);
         case T_Q8_0:
-        case T_NXF_I8: return launch_type<T_Q8_0>(p, grid, c.st);
-        case T_Q3_K: return launch_type<T_Q3_K>(p, grid, c.st);
-        case T_I4G128: return launch_type<T_I4G128>(p, grid, c.st);
-        case T_Q6_K: return launch_type<T_Q6_K>(p, grid, c.st);
-        case T_Q5_K: return launch_type<T_Q5_K>(p, grid, c.st);
-        case T_Q4_1: return launch_type<T_Q4_1>(p, grid, c.st);
-        case T_Q2_K: return launch_type<T_Q2_K>(p, grid, c.st);
-        case T_I4G32: return launch_type<T_I4G32>(p, grid, c.st);
-        case T_I4G64: return launch_type<T_I4G64>(p, grid, c.st);
-        case T_I4G256: return launch_type<T_I4G256>(p, grid, c.st);
+        case T_NXF_I8: return launch_type<T_Q8_0>(p, c.up != nullptr, grid, c.st);
+        case T_Q3_K: return launch_type<T_Q3_K>(p, c.up != nullptr, grid, c.st);
+        case T_I4G128: return launch_type<T_I4G128>(p, c.up != nullptr, grid, c.st);
+        case T_Q6_K: return launch_type<T_Q6_K>(p, c.up != nullptr, grid, c.st);
+        case T_Q5_K: return launch_type<T_Q5_K>(p, c.up != nullptr, grid, c.st);
+        case T_Q4_1: return launch_type<T_Q4_1>(p, c.up != nullptr, grid, c.st);
+        case T_Q2_K: return launch_type<T_Q2_K>(p, c.up != nullptr, grid, c.st);
+        case T_I4G32: return launch_type<T_I4G32>(p, c.up != nullptr, grid, c.st);
+        case T_I4G64: return launch_type<T_I4G64>(p, c.up != nullptr, grid, c.st);
+        case T_I4G256: return launch_type<T_I4G256>(p, c.up != nullptr, grid, c.st);
         default: return NXQ_ERR_UNSUPPORTED;
     }
 }

@@ -482,7 +482,7 @@ def test_expert_table_lifetime(gpu):
 # ---- combine ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("N", [1, 8, 33, 1000, 4096])
-@pytest.mark.parametrize("T,k", [(1, 1), (3, 8), (130, 3), (17, 32)])
+@pytest.mark.parametrize("T,k", [(1, 1), (3, 8), (130, 3), (17, 32), (601, 32), (2000, 8)])
 @pytest.mark.parametrize("hdt", DT.keys())
 def test_combine(gpu, N, T, k, hdt):
     g = torch.Generator(device="cuda").manual_seed(N + T)
