@@ -173,9 +173,6 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + kMats);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int64_t total = (int64_t)p.plan->blocks * p.tiles;
-    if (blockIdx.x >= total) return;  // the whole CTA, before any barrier or TMEM
-
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ptx::WaitCtl ctl{abort_flag, p.status};
     if (threadIdx.x == 0) {
@@ -205,7 +202,10 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    overlap_begin();  // everything above overlaps the plan kernel
 
+    // (A CTA without work tiles walks none and leaves.)
+    const int64_t total = (int64_t)p.plan->blocks * p.tiles;
     const int chunks = (int)p.s.chunks;
     const int64_t G = gridDim.x;
 
@@ -245,6 +245,9 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         }
     } else if (warp == kWarpProducer) {
         if (lane == 0) ptx::prefetch_tmap(&xmap);
+        // The activations were written through the generic proxy; TMA reads them
+        // through the async one.
+        asm volatile("fence.proxy.async;" ::: "memory");
         Ring rx;
         uint32_t issued = 0;
         bool ok = true;
@@ -506,12 +509,9 @@ int set_attr() {
 
 template <int TYPE>
 int launch(const Params& p, const CUtensorMap& tmap, bool pair, unsigned grid, cudaStream_t st) {
-    if (pair)
-        ragged_gemm_kernel<TYPE, true><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
-    else
-        ragged_gemm_kernel<TYPE, false><<<grid, kThreads, Rings<TYPE>::smem, st>>>(p, tmap);
+    const cudaError_t e = launch_overlapped(pair ? ragged_gemm_kernel<TYPE, true> : ragged_gemm_kernel<TYPE, false>, grid,
+                                            kThreads, Rings<TYPE>::smem, st, p, tmap);
     note_launches(1);
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "ragged_gemm launch");
 }
 

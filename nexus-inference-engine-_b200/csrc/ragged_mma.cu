@@ -28,9 +28,10 @@
 //
 // Row blocks have up to 8 slots, the columns of one MMA.  Slots behind a block's
 // end hold stale activations of the stage's earlier units: an MMA column
-// depends on its own slot only, and those columns are not stored.  (A variant
-// with blocks of 16, two MMAs for every decoded fragment, was slower up to 6
-// slots per expert and 5 % faster at 8, where the tcgen05 kernel takes over.)
+// depends on its own slot only, and those columns are not stored.  (Variants
+// with blocks of 16 and 32, 2 to 4 MMAs for every decoded fragment, were slower
+// up to 8 slots per expert, where the tcgen05 kernel takes over: their rings are
+// shallower and every warp reads all activation fragments.)
 //
 // What bounds it (64 experts of Q4_K 4096x2048, 256 slots, 290 MB in 82 us = 3.5
 // TB/s): the instructions of the decode, 387 a warp and unit, issue slots 64 %
