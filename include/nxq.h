@@ -298,7 +298,10 @@ NXQ_API int nxq_embedding(nxq_weight_t table, const void* ids_dev, int ids_type,
  * A "slot" is one (token, expert) pair in sorted order.  Calls of one stream
  * run in order; calls on different streams share nothing and may overlap.
  * Their workspaces are stream-ordered allocations (cudaMallocAsync) of each
- * call, so a captured call owns its own inside the graph. */
+ * call, so a captured call owns its own inside the graph (as memory nodes) and
+ * needs no call before the capture; weights and tables that a graph reads must
+ * outlive it.  No counterpart of these declarations runs on the reference's GPU
+ * path. */
 
 /* Experts of one projection: `count` (1 .. 1024) registered weights of one
  * block type and shape, expert e = w[e] (a weight may appear more than once).
@@ -336,7 +339,11 @@ NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, i
  * were), x_dev has X rows (without rows_dev, slot s reads row s and X must be
  * at least R).  Offsets outside [0, R] or descending, and row indices outside
  * [0, X), are skipped (rows of a bad index give zeros) and reported as
- * NXQ_ERR_INDEX.  Weight and activation rounding as in nxq_qmatmul.
+ * NXQ_ERR_INDEX.  Weight and activation rounding as in nxq_qmatmul, and the
+ * same choice by NXQ_DECODE_KERNEL / NXQ_PREFILL_KERNEL: up to 8 slots per
+ * expert on average the warp-level kernel, beyond it the tcgen05 one, with
+ * both set to simt (and for FP16 / FP32 weights) the exact CUDA-core kernel.
+ * The same inputs give the same bits on every call.
  * The _swiglu form takes gate and up tables of the same count, type and shape:
  *   h_dev[s] = silu(x Wg_e^T) * (x Wu_e^T), silu(g) = g / (1 + exp(-g)).
  * R < 2^31. */

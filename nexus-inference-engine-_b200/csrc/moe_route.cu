@@ -5,8 +5,8 @@
 //
 // Routing has three steps.  (1) One warp per token: lane l holds the logits of
 // experts l, l + 32, ... as order-preserving integer keys and knows its largest;
-// k rounds of a warp maximum (redux on the key; among lanes with equal keys redux
-// on the index, so ties go to the lowest) pick the choices; a lane keeps its two
+// k rounds of two warp reductions (the largest key, then the lowest index that has
+// it, so ties go to the lowest) pick the choices; a lane keeps its two
 // largest and looks again only when both are gone.  The block counts its choices
 // of every expert.  (2) An exclusive scan of the counts over blocks, 32 experts
 // per CTA.  (3) Every block ranks its own choices: a warp walks a contiguous run of
@@ -48,12 +48,6 @@ struct RouteParams {
     int32_t* before;  // [blocks][E]: choices of the expert in the block, then in the blocks before it
     int32_t* total;   // [E]
 };
-
-__device__ __forceinline__ float load_logit(const void* p, int dt, int64_t i) {
-    if (dt == NXQ_F32) return static_cast<const float*>(p)[i];
-    if (dt == NXQ_F16) return __half2float(static_cast<const __half*>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
 
 // Larger value, larger key; -0 and +0 equal; 0 for -inf and NaN (never taken).
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -132,9 +126,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int64_t n
     uint32_t my_key = 0u;
     uint32_t best = first;
     for (int j = 0; j < p.k && best; ++j) {
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, top == best);
-        const int e = __popc(who) == 1 ? __shfl_sync(0xFFFFFFFFu, at, __ffs(who) - 1)
-                                       : __reduce_min_sync(0xFFFFFFFFu, top == best ? at : 0x7FFFFFFF);
+        const int e = (int)__reduce_min_sync(0xFFFFFFFFu, top == best ? (unsigned)at : 0x7FFFFFFFu);
         if (top == best && at == e) {
             if (--known) {
                 top = top2;
@@ -365,33 +357,41 @@ cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStr
 constexpr int kCombThreads = 256;
 constexpr int kBatch = 8;
 
-__device__ __forceinline__ float load_h(const void* p, int dt, int64_t i) { return load_logit(p, dt, i); }
-
-// Eight consecutive values of h as loaded.
-template <bool F32>
-struct Raw8 {
-    uint4 q[F32 ? 2 : 1];
+// VEC (8, 2 or 1) consecutive values of h as loaded.
+template <int VEC, bool F32>
+struct Raw {
+    static constexpr int kWords = F32 ? VEC : (VEC + 1) / 2;
+    uint32_t w[kWords];
     __device__ __forceinline__ void load(const void* p, int64_t i) {
-        const uint4* a = F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i)
-                             : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+        if constexpr (VEC == 8) {
+            const uint4* a = F32 ? reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i)
+                                 : reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
-        for (int j = 0; j < (F32 ? 2 : 1); ++j) q[j] = __ldcs(a + j);
-    }
-    __device__ __forceinline__ void widen(int dt, float (&v)[8]) const {
-        const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
-        if constexpr (F32) {
-            const uint32_t u[4] = {q[1].x, q[1].y, q[1].z, q[1].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]), v[4 + j] = __uint_as_float(u[j]);
+            for (int j = 0; j < kWords / 4; ++j) {
+                const uint4 q = __ldcs(a + j);
+                w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
+            }
+        } else if constexpr (F32 && VEC == 2) {
+            const uint2 q = __ldcs(reinterpret_cast<const uint2*>(static_cast<const float*>(p) + i));
+            w[0] = q.x, w[1] = q.y;
+        } else if constexpr (F32 || VEC == 2) {
+            w[0] = __ldcs(F32 ? static_cast<const uint32_t*>(p) + i
+                              : reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i));
         } else {
+            w[0] = __ldcs(static_cast<const uint16_t*>(p) + i);
+        }
+    }
+    __device__ __forceinline__ void widen(int dt, float (&v)[VEC]) const {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (dt == NXQ_F16) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                    v[2 * j] = f.x, v[2 * j + 1] = f.y;
-                } else {
-                    v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-                }
+        for (int j = 0; j < VEC; ++j) {
+            if constexpr (F32) {
+                v[j] = __uint_as_float(w[j]);
+            } else {
+                const uint32_t u = w[j / 2];
+                if (dt == NXQ_F16)
+                    v[j] = __half2float(__ushort_as_half((unsigned short)(j & 1 ? u >> 16 : u & 0xFFFFu)));
+                else
+                    v[j] = __uint_as_float(j & 1 ? u & 0xFFFF0000u : u << 16);
             }
         }
     }
@@ -427,7 +427,8 @@ __device__ __forceinline__ void store8(void* y, int dt, int64_t o, const float (
 }
 
 // Items are (token, 32 VEC columns), segs to a token.  VEC = 8 needs N % 8 == 0,
-// h and y 16-byte and an fp32 residual or output 32-byte aligned.  F32: h's type.
+// h and y 16-byte and an fp32 residual or output 32-byte aligned; VEC = 2 an
+// even N and h aligned to two values.  F32: h's type.
 template <int VEC, bool F32>
 __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __restrict__ h, int h_dtype, int64_t R, int64_t N,
                                                                const int32_t* __restrict__ slots,
@@ -463,46 +464,45 @@ __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __res
             seg -= segs;
             ++t;
         }
-        float acc[VEC];
+        float acc[VEC], rv[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-        float rv[VEC];
+        for (int i = 0; i < VEC; ++i) acc[i] = rv[i] = 0.0f;
+        if (res && n < N) {
+            if constexpr (VEC == 8) {
+                load_f32x8(res + o, rv);
+            } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) rv[i] = 0.0f;
-        if constexpr (VEC == 8) {
-            if (res && n < N) load_f32x8(res + o, rv);
-            for (int j0 = 0; j0 < k; j0 += kBatch) {
-                Raw8<F32> r[kBatch];
+                for (int i = 0; i < VEC; ++i) rv[i] = res[o + i];
+            }
+        }
+        for (int j0 = 0; j0 < k; j0 += kBatch) {
+            Raw<VEC, F32> r[kBatch];
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
-                    if (j0 + j < k && s >= 0 && n < N) r[j].load(h, (int64_t)s * N + n);
-                }
-                if (j0 + kBatch >= k) fetch(t);
+            for (int j = 0; j < kBatch; ++j) {
+                const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
+                if (j0 + j < k && s >= 0 && n < N) r[j].load(h, (int64_t)s * N + n);
+            }
+            if (j0 + kBatch >= k) fetch(t);
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
-                    const float w = __shfl_sync(0xFFFFFFFFu, my_w, (j0 + j) & 31);
-                    if (j0 + j < k && s >= 0) {
-                        float v[8];
-                        r[j].widen(h_dtype, v);
+            for (int j = 0; j < kBatch; ++j) {
+                const int s = __shfl_sync(0xFFFFFFFFu, my_s, (j0 + j) & 31);
+                const float w = __shfl_sync(0xFFFFFFFFu, my_w, (j0 + j) & 31);
+                if (j0 + j < k && s >= 0) {
+                    float v[VEC];
+                    r[j].widen(h_dtype, v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
-                    }
+                    for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, v[i], acc[i]);
                 }
             }
-            if (n >= N) continue;
+        }
+        if (n >= N) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += rv[i];
+        for (int i = 0; i < VEC; ++i) acc[i] += rv[i];
+        if constexpr (VEC == 8) {
             store8(y, y_dtype, o, acc);
         } else {
-            fetch(t);
-            for (int j = 0; j < k; ++j) {
-                const int s = __shfl_sync(0xFFFFFFFFu, my_s, j);
-                const float w = __shfl_sync(0xFFFFFFFFu, my_w, j);
-                if (s >= 0 && n < N) acc[0] = fmaf(w, load_h(h, h_dtype, (int64_t)s * N + n), acc[0]);
-            }
-            if (n < N) store_as(y, y_dtype, o, acc[0] + (res ? res[o] : 0.0f));
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) store_as(y, y_dtype, o + i, acc[i]);
         }
     }
 }
@@ -605,10 +605,13 @@ __global__ void __launch_bounds__(kBulkThreads, 1) combine_bulk_kernel(const voi
             for (int j = 0; j < k; ++j) {
                 if (s_slot[st][j] < 0) continue;
                 const float w = s_w[st][j];
-                Raw8<F32> r;
+                Raw<8, F32> r;
                 const uint4* q = reinterpret_cast<const uint4*>(base + (size_t)j * seg * kSize);
 #pragma unroll
-                for (int i = 0; i < (F32 ? 2 : 1); ++i) r.q[i] = q[i];
+                for (int i = 0; i < (F32 ? 2 : 1); ++i) {
+                    const uint4 x = q[i];
+                    r.w[4 * i] = x.x, r.w[4 * i + 1] = x.y, r.w[4 * i + 2] = x.z, r.w[4 * i + 3] = x.w;
+                }
                 float v[8];
                 r.widen(h_dtype, v);
 #pragma unroll
@@ -696,13 +699,16 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
         note_launches(1);
         return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "combine launch");
     }
-    const int64_t per = 32 * (vec ? 8 : 1), segs = (N + per - 1) / per;
+    const bool pairs = N % 2 == 0 && (uintptr_t)h_dev % (f32 ? 8 : 4) == 0;
+    const int64_t per = 32 * (vec ? 8 : pairs ? 2 : 1), segs = (N + per - 1) / per;
     if (T > ((int64_t)1 << 62) / segs) return fail(NXQ_ERR_ARG, "combine: T=%lld N=%lld", (long long)T, (long long)N);
     const int64_t want = (T * segs + kCombThreads / 32 - 1) / (kCombThreads / 32), most = (int64_t)context_sm_count() * 8;
-    const cudaError_t e = launch_overlapped(
-        vec ? (f32 ? combine_kernel<8, true> : combine_kernel<8, false>) : combine_kernel<1, false>,
-        (unsigned)(want < most ? want : most), kCombThreads, 0, (cudaStream_t)stream, h_dev, h_dtype, R, N, slots_dev,
-        weights_dev, T, k, res_dev, y_dev, y_dtype, segs, context_status());
+    auto* kernel = vec ? (f32 ? combine_kernel<8, true> : combine_kernel<8, false>)
+                   : pairs ? (f32 ? combine_kernel<2, true> : combine_kernel<2, false>)
+                           : (f32 ? combine_kernel<1, true> : combine_kernel<1, false>);
+    const cudaError_t e = launch_overlapped(kernel, (unsigned)(want < most ? want : most), kCombThreads, 0,
+                                            (cudaStream_t)stream, h_dev, h_dtype, R, N, slots_dev, weights_dev, T, k,
+                                            res_dev, y_dev, y_dtype, segs, context_status());
     note_launches(1);
     return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "combine launch");
 }

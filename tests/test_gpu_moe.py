@@ -451,6 +451,69 @@ def test_ragged_range_error(gpu, n):
             w.release()
 
 
+def test_ragged_lost_arrival_times_out(gpu):
+    """A partial sum that is never counted in: the bounded wait of the worker that needs it ends the call
+    with an error, and the next call is right."""
+    ws, W = make_weights(gpu, 12, 2, 1024, 2048, 5)
+    E = gpu.Experts(ws)
+    try:
+        x = torch.randn((6, 2048), device="cuda").half()
+        off = make_offsets([2, 4])
+        y, b = products(W, 12, x, [2, 4], torch.arange(6, device="cuda"))
+        check(gpu.qmatmul_ragged(E, x, off), y, b)
+        gpu.stream_sync()
+        gpu.set_wait_limit(2000)
+        gpu.test_hook(gpu.HOOK_STREAMK_SKIP_COUNT, True)
+        try:
+            gpu.qmatmul_ragged(E, x, off)
+            with pytest.raises(gpu.NxqError) as e:
+                gpu.stream_sync()
+            assert e.value.name == "ERR_TIMEOUT"
+        finally:
+            gpu.test_hook(gpu.HOOK_STREAMK_SKIP_COUNT, False)
+            gpu.set_wait_limit(0)
+        check(gpu.qmatmul_ragged(E, x, off), y, b)
+        gpu.stream_sync()
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
+def test_ragged_crowded_expert(gpu):
+    """Every slot with one expert of many: far from the average that the kernel is chosen by."""
+    ws, W = make_weights(gpu, 2, 40, 130, 256, 5)
+    E = gpu.Experts(ws)
+    try:
+        for n in (200, 300, 4000):
+            counts = [0] * 40
+            counts[17] = n
+            x = torch.randn((n, 256), device="cuda").half()
+            y, b = products(W, 2, x, counts, torch.arange(n, device="cuda"))
+            check(gpu.qmatmul_ragged(E, x, make_offsets(counts)), y, b)
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
+def test_ragged_no_slots(gpu):
+    ws, _ = make_weights(gpu, 12, 2, 128, 256, 5)
+    E = gpu.Experts(ws)
+    try:
+        assert gpu.qmatmul_ragged(E, torch.empty((0, 256), device="cuda"), make_offsets([0, 0])).shape == (0, 128)
+        for R in (5, 60):  # room for slots, none of them used
+            out = torch.full((R, 128), 3.0, device="cuda")
+            gpu.qmatmul_ragged(E, torch.full((R, 256), math.nan, device="cuda"), make_offsets([0, 0]), out=out)
+            gpu.qmatmul_ragged_swiglu(E, E, torch.full((R, 256), math.nan, device="cuda"), make_offsets([0, 0], R), out=out)
+            gpu.stream_sync()
+            assert bool((out == 3).all())
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
 def test_expert_table_lifetime(gpu):
     ws, _ = make_weights(gpu, 12, 2, 128, 256, 5)
     other = gpu.Weight.register(synth.make_blocks(12, 128, 512, seed=1), 12, 128, 512)
@@ -481,7 +544,7 @@ def test_expert_table_lifetime(gpu):
 
 # ---- combine ------------------------------------------------------------------------
 
-@pytest.mark.parametrize("N", [1, 8, 33, 1000, 4096])
+@pytest.mark.parametrize("N", [1, 8, 33, 1000, 1002, 4096])
 @pytest.mark.parametrize("T,k", [(1, 1), (3, 8), (130, 3), (17, 32), (601, 32), (2000, 8)])
 @pytest.mark.parametrize("hdt", DT.keys())
 def test_combine(gpu, N, T, k, hdt):
