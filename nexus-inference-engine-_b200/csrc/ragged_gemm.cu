@@ -23,12 +23,15 @@
 //                accumulators are handed back as soon as they are read, and
 //                rows leave as 16-byte stores while the next tile's MMAs run
 //
-// The A operand's ring has as many stages as a chunk has k-steps, so its indexes
-// are constants; the issuing loops run warp-wide, half the lanes watching the
-// activations and half the A operand, with only the MMA and the commits in the
-// elected lane.  Waiting for a stage and handing it back cost an issuing warp
-// about 400 cycles a k-step, against 512 of MMA work for both tiles; with
-// a warp per tile one issues while the other waits.
+// The issuing loops run warp-wide, half the lanes watching the activations and
+// half the A operand, with only the MMA and the commits in the elected lane.
+// Waiting for a stage and handing it back cost an issuing warp about 400 cycles
+// a k-step, against 512 of MMA work for both tiles; with a warp per tile one
+// issues while the other waits.  The loops are kept short rather than unrolled
+// over the k-steps of a chunk: four copies of the decode and of the issue
+// were 12 % slower for few slots (1024 slots of 64 experts, Q4_K 4096x2048: 117
+// us against 104).  Blocks of 64 slots, which leave TMEM for six A stages, gained
+// 2 to 9 % up to 12 slots per expert and lost from 16 on.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes
 // hold behind a block's slots (the next expert's rows, or zeros) reaches no
@@ -54,31 +57,31 @@ constexpr int kWarpWProducer = kWarpEpi0 + kEpiWarps;
 constexpr int kWarpMma1 = kWarpWProducer + 1;
 constexpr int kThreads = 32 * (kWarpMma1 + 1);
 constexpr int kMats = 2;  // weight tiles of a work tile
-constexpr int kNT = 128;  // slots of a work tile
 constexpr int kKS = 64;   // reduction elements per k-step (one swizzle atom)
 constexpr int kStepsPerChunk = CHUNK_K / kKS;
-constexpr int kAStages = kStepsPerChunk;  // TMEM A ring
 constexpr int kACols = 32 * kMats;        // TMEM columns of a stage
+constexpr int NT = 128;                   // slots of a work tile
 constexpr int kBarBytes = 512;
-constexpr uint32_t kColD = 256;  // accumulators: columns 256 + 128 mat
 constexpr uint32_t kTmemCols = 512;
+constexpr int kColD = (int)kTmemCols - kMats * NT;  // accumulators: columns kColD + NT mat
+constexpr int kA = kColD / kACols;                  // TMEM A ring: the columns left
+static_assert(kA % 2 == 0, "a warpgroup's k-steps keep their parity in the ring");
 constexpr int kBoxRows = 64;
 constexpr int kBoxBytes = kBoxRows * kKS * 2;
-constexpr int kXB = kNT * kKS * 2;                 // 16 KB of activations per k-step
-constexpr int kStageOut = kNT * TILE_ROWS * 2;     // 32 KB: one tile's 16-bit outputs [slot][row]
-static_assert(kAStages * kACols <= (int)kColD, "A stages overlap the accumulators");
+constexpr int kXB = NT * kKS * 2;               // 16 KB of activations per k-step
+constexpr int kStageOut = NT * TILE_ROWS * 2;  // 32 KB: one tile's 16-bit outputs [slot][row]
 
-// Ring depths: six k-steps of activations where four tile-chunks (two of each
-// tile) still fit beside them, else four, then as many tile-chunks as fit (up to 6).
+// Ring depths in shared memory: four k-steps of activations (six, in place of
+// tile-chunks, were no faster), then as many tile-chunks as fit (up to 6).
 template <int TYPE>
 struct Rings {
     static constexpr int WB = lane::Lane<TYPE>::kStage;
     static constexpr int kBudget = 227 * 1024 - 1024 - kBarBytes - kStageOut;
-    static constexpr int kX = (kBudget - 6 * kXB) / WB >= 4 ? 6 : 4;
+    static constexpr int kX = 4;
     static constexpr int fit = (kBudget - kX * kXB) / WB;
     static constexpr int kW = fit > 6 ? 6 : fit;
     static_assert(kW >= 2, "tile-chunk ring too shallow");
-    static_assert((2 * kX + 2 * kW + 2 * kMats * kAStages + 2 + kMats) * 8 + 8 <= kBarBytes, "barrier area too small");
+    static_assert((2 * kX + 2 * kW + 2 * kMats * kA + 2 + kMats) * 8 + 8 <= kBarBytes, "barrier area too small");
     static constexpr size_t smem = 1024 + (size_t)kX * kXB + kStageOut + (size_t)kW * WB + kBarBytes;
 };
 
@@ -105,11 +108,6 @@ __device__ __forceinline__ uint32_t pack16(bool bf16, float a, float b) {
 // it gives 0 where the quotient is below 2^-119.
 __device__ __forceinline__ float swiglu1(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const ptx::WaitCtl& c, unsigned where) {
-    int ok = 0;
-    if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity, c, where) ? 1 : 0;
-    return __shfl_sync(0xFFFFFFFFu, ok, 0) != 0;
-}
 // A barrier of the epilogue warps that tells whether `ok` holds in all of them.
 __device__ __forceinline__ bool epi_all(bool ok) {
     uint32_t r;
@@ -166,8 +164,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     uint64_t* w_full = x_empty + kX;
     uint64_t* w_empty = w_full + kW;
     uint64_t* a_full = w_empty + kW;
-    uint64_t* a_empty = a_full + kMats * kAStages;   // [mat][stage]
-    uint64_t* d_full = a_empty + kMats * kAStages;
+    uint64_t* a_empty = a_full + kMats * kA;   // [mat][stage]
+    uint64_t* d_full = a_empty + kMats * kA;
     uint64_t* d_empty = d_full + 1;
     uint64_t* drain = d_empty + 1;  // [mat]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + kMats);
@@ -184,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             ptx::mbar_init(&w_full[i], 1);
             ptx::mbar_init(&w_empty[i], 4 * kDeqGroups / kMats);  // the warps that decode a tile-chunk
         }
-        for (int i = 0; i < kMats * kAStages; ++i) {
+        for (int i = 0; i < kMats * kA; ++i) {
             ptx::mbar_init(&a_full[i], 4);  // the warps that write a tile's stage
             ptx::mbar_init(&a_empty[i], 1);
         }
@@ -211,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
 
     if (warp == kWarpWProducer) {
         RaggedWalk<true> walk;
-        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
+        walk.start(p.plan, NT, p.tiles, blockIdx.x);
         if (lane == 0) {
             Ring rw;
             uint32_t issued = 0;
@@ -252,12 +250,12 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         uint32_t issued = 0;
         bool ok = true;
         RaggedWalk<true> walk;
-        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
+        walk.start(p.plan, NT, p.tiles, blockIdx.x);
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
             const RaggedTile t = walk.at(g);
             const int boxes = (t.rows + kBoxRows - 1) / kBoxRows;
             for (int ks = 0; ks < chunks * kStepsPerChunk && ok; ++ks) {
-                ok = __all_sync(0xFFFFFFFFu, ptx::mbar_wait(&x_empty[rx.i], rx.ph ^ 1u, ctl, 42));
+                ok = ptx::warp_mbar_wait(&x_empty[rx.i], rx.ph ^ 1u, ctl, 42);
                 if (!ok) break;
                 if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[rx.i], boxes * kBoxBytes);
                 __syncwarp();
@@ -276,45 +274,40 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         }
     } else if (warp == kWarpMma || warp == kWarpMma1) {
         const int mat = warp == kWarpMma ? 0 : 1;
-        uint32_t cc = 0, nt = 0;  // chunks and work tiles so far
+        uint32_t nt = 0;  // work tiles so far
         bool ok = true;
-        Ring rx;
+        Ring rx, ra;
         RaggedWalk<true> walk;
-        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
+        walk.start(p.plan, NT, p.tiles, blockIdx.x);
         const uint64_t desc0 = ptx::desc_sw128_kmajor(ptx::smem_addr(xs));
-        const uint32_t d = tmem + kColD + mat * kNT, a = tmem + mat * 32;
-        uint64_t* const af = a_full + mat * kAStages;
-        uint64_t* const ae = a_empty + mat * kAStages;
+        const uint32_t d = tmem + kColD + mat * NT, a = tmem + mat * 32;
+        uint64_t* const af = a_full + mat * kA;
+        uint64_t* const ae = a_empty + mat * kA;
         bool ready = false;
         for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
             const RaggedTile t = walk.at(g);
             const uint32_t idesc = ptx::idesc_f16_f32(128, (t.rows + 15) & ~15);
-            ok = nt == 0 || ptx::mbar_wait(d_empty, (nt - 1) & 1, ctl, 43);
-            ok = __all_sync(0xFFFFFFFFu, ok);
+            ok = nt == 0 || ptx::warp_mbar_wait(d_empty, (nt - 1) & 1, ctl, 43);
             ptx::tc_fence_after();
-            for (int c = 0; c < chunks && ok; ++c, ++cc) {
-#pragma unroll
-                for (int st = 0; st < kAStages; ++st) {
-                    if (!__all_sync(0xFFFFFFFFu, ready)) {
-                        ok = ok && ptx::mbar_wait(lane < 16 ? &x_full[rx.i] : &af[st], lane < 16 ? rx.ph : (cc & 1), ctl, 44);
-                        ok = __all_sync(0xFFFFFFFFu, ok);
-                        if (!ok) continue;
-                    }
-                    const int xi = rx.i;
-                    rx.next(kX);
-                    // The next k-step's barriers, read while this one's MMAs issue.
-                    ready = ptx::mbar_test_wait(lane < 16 ? &x_full[rx.i] : &af[(st + 1) % kAStages],
-                                                lane < 16 ? rx.ph : ((cc + (st + 1 == kAStages)) & 1));
-                    ptx::tc_fence_after();
-                    if (ptx::elect_one()) {
-                        ptx::mma_ts_f16_k64(d, a + st * kACols, desc0 + ((uint32_t)(xi * kXB) >> 4), idesc,
-                                            (c | st) ? 1u : 0u);
-                        ptx::mma_commit(&ae[st]);
-                        ptx::mma_commit(&x_empty[xi]);
-                        if (st == kAStages - 1 && c == chunks - 1) ptx::mma_commit(d_full);
-                    }
-                    __syncwarp();
+            const int steps = chunks * kStepsPerChunk;
+            for (int ks = 0; ks < steps && ok; ++ks) {
+                if (!__all_sync(0xFFFFFFFFu, ready)) {
+                    ok = ptx::warp_mbar_wait(lane < 16 ? &x_full[rx.i] : &af[ra.i], lane < 16 ? rx.ph : ra.ph, ctl, 44);
+                    if (!ok) break;
                 }
+                const int xi = rx.i, ai = ra.i;
+                rx.next(kX);
+                ra.next(kA);
+                // The next k-step's barriers, read while this one's MMAs issue.
+                ready = ptx::mbar_test_wait(lane < 16 ? &x_full[rx.i] : &af[ra.i], lane < 16 ? rx.ph : ra.ph);
+                ptx::tc_fence_after();
+                if (ptx::elect_one()) {
+                    ptx::mma_ts_f16_k64(d, a + ai * kACols, desc0 + ((uint32_t)(xi * kXB) >> 4), idesc, ks ? 1u : 0u);
+                    ptx::mma_commit(&ae[ai]);
+                    ptx::mma_commit(&x_empty[xi]);
+                    if (ks == steps - 1) ptx::mma_commit(d_full);
+                }
+                __syncwarp();
             }
         }
         if (ptx::elect_one()) ptx::mma_commit(&drain[mat]);
@@ -326,18 +319,17 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         // Warpgroup wg decodes the k-steps of parity wg % 2 of tile wg / 2.
         const int wg = (warp - kWarpDeq0) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const int mat = wg >> 1, par = wg & 1;
-        uint32_t cc = 0;
-        Ring rw;
+        Ring rw, ra;
         if (mat) rw.next(kW);
+        if (par) ra.next(kA);
         bool ok = true;
         const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + mat * 32;
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
-            for (int c = 0; c < chunks && ok; ++c, ++cc) {
-                if (!(ok = warp_wait(&w_full[rw.i], rw.ph, ctl, 46))) break;
+            for (int c = 0; c < chunks && ok; ++c) {
+                if (!(ok = ptx::warp_mbar_wait(&w_full[rw.i], rw.ph, ctl, 46))) break;
                 const uint8_t* stage = ws + rw.i * WB;
-#pragma unroll
-                for (int st = 0; st < kAStages; ++st) {
-                    if ((st & 1) != par) continue;
+#pragma unroll 1
+                for (int st = par; st < kStepsPerChunk; st += 2) {
                     uint32_t o[32];
                     {
                         lane::Lane<TYPE> L;
@@ -350,16 +342,18 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                             for (int i = 0; i < 4; ++i) o[4 * m + i] = q[i];
                         }
                     }
-                    ok = ok && warp_wait(&a_empty[mat * kAStages + st], (cc & 1) ^ 1u, ctl, 47);
-                    if (!ok) continue;
+                    ok = ok && ptx::warp_mbar_wait(&a_empty[mat * kA + ra.i], ra.ph ^ 1u, ctl, 47);
+                    if (!ok) break;
                     ptx::tc_fence_after();
-                    ptx::tmem_st32(tbase + st * kACols, o);
+                    ptx::tmem_st32(tbase + ra.i * kACols, o);
                     // (Announcing the stage only after the next decode, to hide
                     // the store's latency, was 5 % slower.)
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&a_full[mat * kAStages + st]);
+                    if (lane == 0) ptx::mbar_arrive(&a_full[mat * kA + ra.i]);
+                    ra.next(kA);
+                    ra.next(kA);
                 }
                 __syncwarp();
                 if (ok && lane == 0) ptx::mbar_arrive(&w_empty[rw.i]);
@@ -369,23 +363,24 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         }
     } else {
         // Epilogue: warp (quad, sub) reads TMEM lanes 32 quad .. (its lane
-        // quadrant) = weight row n of each tile, and slots 64 sub .. 64 sub + 63.
+        // quadrant) = weight row n of each tile, and half `sub` of the slots.
         const int ew = warp - kWarpEpi0, quad = warp & 3, r = quad * 32 + lane, sub = ew >> 2;
+        constexpr int kHalf = NT / 2;
         const int tid = threadIdx.x - 32 * kWarpEpi0;
         const int64_t N = p.s.N;
         const bool bf = p.y_dtype == NXQ_BF16;
         uint16_t* const out16 = reinterpret_cast<uint16_t*>(stg);  // [slot][row]
         uint32_t nt = 0;
         RaggedWalk<true> walk;
-        walk.start(p.plan, kNT, p.tiles, blockIdx.x);
-        const uint32_t td = tmem + ((uint32_t)(quad * 32) << 16) + kColD + 64 * sub;
-        // Slots 64 sub + c .. + 15 of a tile's accumulator (PAIR: the outputs).
+        walk.start(p.plan, NT, p.tiles, blockIdx.x);
+        const uint32_t td = tmem + ((uint32_t)(quad * 32) << 16) + kColD + kHalf * sub;
+        // Slots kHalf sub + c .. + 15 of a tile's accumulator (PAIR: the outputs).
         auto read16 = [&](int mat, int c, float (&v)[16]) {
             uint32_t a[16];
-            ptx::tmem_ld16(td + mat * kNT + c, a);
+            ptx::tmem_ld16(td + mat * NT + c, a);
             if constexpr (PAIR) {
                 uint32_t u[16];
-                ptx::tmem_ld16(td + kNT + c, u);
+                ptx::tmem_ld16(td + NT + c, u);
                 ptx::tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = swiglu1(__uint_as_float(a[j]), __uint_as_float(u[j]));
@@ -396,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             }
         };
         auto put16 = [&](int c, const uint32_t (&q)[8]) {
-            uint16_t* d = out16 + (64 * sub + c) * TILE_ROWS + r;
+            uint16_t* d = out16 + (kHalf * sub + c) * TILE_ROWS + r;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 d[(2 * j) * TILE_ROWS] = (uint16_t)(q[j] & 0xFFFFu);
@@ -427,18 +422,18 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             const int wt0 = PAIR ? t.tile : 2 * t.tile, wt1 = weight_tile<PAIR>(t, 1, p.s.tiles, &has1);
             // All epilogue warps go on or give up together; nobody still reads
             // the staging buffer.
-            if (!epi_all(warp_wait(d_full, nt & 1, ctl, 48))) break;
+            if (!epi_all(ptx::warp_mbar_wait(d_full, nt & 1, ctl, 48))) break;
             ptx::tc_fence_after();
-            const int left = t.rows - 64 * sub;  // slots of this half
+            const int left = t.rows - kHalf * sub;  // slots of this half
             if (p.y_dtype == NXQ_F32) {
 #pragma unroll 1
                 for (int mat = 0; mat < (PAIR ? 1 : 2); ++mat)
 #pragma unroll 1
-                    for (int c = 0; c < 64 && c < left; c += 16) {
+                    for (int c = 0; c < kHalf && c < left; c += 16) {
                         float v[16];
                         read16(mat, c, v);
                         const int64_t n = (int64_t)(mat ? wt1 : wt0) * TILE_ROWS + r;
-                        float* q = static_cast<float*>(p.y) + ((int64_t)t.row0 + 64 * sub + c) * N + n;
+                        float* q = static_cast<float*>(p.y) + ((int64_t)t.row0 + kHalf * sub + c) * N + n;
                         if (n < N && (mat == 0 || has1))
 #pragma unroll
                             for (int j = 0; j < 16; ++j, q += N)
@@ -452,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             // The first tile's (PAIR: the) outputs into the staging buffer, the
             // second tile's into registers; then the accumulators are free.
 #pragma unroll 1
-            for (int c = 0; c < 64 && c < left; c += 16) {
+            for (int c = 0; c < kHalf && c < left; c += 16) {
                 float v[16];
                 uint32_t q[8];
                 read16(0, c, v);
@@ -460,10 +455,10 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                 for (int j = 0; j < 8; ++j) q[j] = pack16(bf, v[2 * j], v[2 * j + 1]);
                 put16(c, q);
             }
-            uint32_t hold[PAIR ? 1 : 4][8];
+            uint32_t hold[PAIR ? 1 : kHalf / 16][8];
             if constexpr (!PAIR) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < kHalf / 16; ++c)
                     if (16 * c < left) {
                         float v[16];
                         read16(1, 16 * c, v);
@@ -480,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                 if (has1) {
                     epi_sync();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < kHalf / 16; ++c)
                         if (16 * c < left) put16(16 * c, hold[c]);
                     epi_sync();
                     flush(t, wt1);
@@ -530,7 +525,7 @@ int ragged_gemm_init() {
 // Where the dense prefill GEMM runs (NXQ_PREFILL_KERNEL=simt turns both off).
 bool ragged_gemm_supported(const TiledShape& s) { return gemm_supported(s, 33); }
 
-int ragged_gemm_blk() { return kNT; }
+int ragged_gemm_blk() { return NT; }
 
 int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan* plan) {
     const TiledShape& s = c.w->shape;
@@ -538,7 +533,7 @@ int ragged_gemm(const RaggedCall& c, const void* xh, int64_t X, const RaggedPlan
              s.N % 8 == 0 && (uintptr_t)c.y % 16 == 0, plan, context_status()};
     CUtensorMap tmap;
     if (int rc = gemm_activation_map(&tmap, xh, X, s.K, kBoxRows)) return rc;
-    const int64_t work = ragged_max_blocks(c.w->count, c.R, kNT) * p.tiles;
+    const int64_t work = ragged_max_blocks(c.w->count, c.R, NT) * p.tiles;
     const unsigned grid = (unsigned)(work < context_sm_count() ? work : context_sm_count());
     switch (s.type) {
         case T_Q4_K: return launch<T_Q4_K>(p, tmap, c.up != nullptr, grid, c.st);

@@ -186,11 +186,7 @@ __global__ void __launch_bounds__(Cfg<TYPE, PAIR>::kAll, 1) ragged_mma_kernel(co
                 }
             }
             const int stg = u % S;
-            if (u >= S) {
-                int ok = 1;
-                if (lane == 0) ok = ptx::mbar_wait(&empty[stg], (uint32_t)(u / S - 1) & 1u, ctl, 51) ? 1 : 0;
-                if (!__shfl_sync(0xFFFFFFFFu, ok, 0)) break;
-            }
+            if (u >= S && !ptx::warp_mbar_wait(&empty[stg], (uint32_t)(u / S - 1) & 1u, ctl, 51)) break;
             // The activations first: behind a ring full of weight copies they
             // would be what the first units wait for.
             const int cx = PAIR && c >= Kc ? c - Kc : c;
@@ -239,7 +235,7 @@ __global__ void __launch_bounds__(Cfg<TYPE, PAIR>::kAll, 1) ragged_mma_kernel(co
             // Unit c of this tile into the sums A (A2: the second chain).
             auto unit = [&](int c, float(&A)[4], float(&A2)[4]) {
                 const int u = t * kun + c - g0, stg = u % S;
-                if (!dead && !ptx::mbar_wait(&full[stg], (uint32_t)(u / S) & 1u, ctl, 52)) dead = true;
+                if (!dead && !ptx::warp_mbar_wait(&full[stg], (uint32_t)(u / S) & 1u, ctl, 52)) dead = true;
                 if (!dead) {
                     Lane<TYPE> LA, LB;
                     LA.load(wst + stg * WB, 16 * wg + g, tq);
@@ -404,7 +400,7 @@ int ragged_mma_blk(const RaggedCall& c) {
     const TiledShape& s = c.w->shape;
     if (!mma_supported(s, 1)) return 0;
     const int64_t E = c.w->count < c.R ? c.w->count : c.R;
-    if (c.R > 8 * E) return 0;
+    if (c.R > 6 * E) return 0;
     // The kernel numbers units in 32 bits.
     const int64_t units = ragged_max_blocks(c.w->count, c.R, kMT) * s.tiles * s.chunks * 2;
     return units < (int64_t)1 << 31 ? kMT : 0;

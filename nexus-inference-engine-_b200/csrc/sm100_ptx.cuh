@@ -115,6 +115,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
     }
 }
 
+// As mbar_wait, by a converged warp (the lanes may watch different barriers);
+// tells every lane whether all of them saw their phase.  Only the try is
+// inlined: a kernel with many waits stays small, and no lane waits for another
+// to pass its result on.
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, const WaitCtl c, unsigned where) {
+    return mbar_wait(bar, parity, c, where);
+}
+__device__ __forceinline__ bool warp_mbar_wait(uint64_t* bar, uint32_t parity, const WaitCtl& c, unsigned where) {
+    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait_slow(bar, parity, c, where));
+}
+
 // ---- bulk / tensor copies (no multicast) ------------------------------------
 // 1-D bulk copy global -> this CTA's shared memory; completes `bytes` of
 // transaction count on `bar`.  dst/src 16-byte aligned, bytes % 16 == 0.
