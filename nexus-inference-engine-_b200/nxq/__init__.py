@@ -476,10 +476,18 @@ def _float_code(what: str, name: str, dtype) -> int:
     return code
 
 
+def _new(shape: tuple, dtype, device):
+    """An empty contiguous tensor (torch's quickest way to one)."""
+    stride = (shape[1], 1) if len(shape) == 2 else (1,) if len(shape) == 1 else None
+    if stride is None:
+        return _torch.empty(shape, dtype=dtype, device=device)
+    return _torch.empty_strided(shape, stride, dtype=dtype, device=device)
+
+
 def _output(what: str, out, shape: tuple, dtype, like):
     """`out` if given (checked), else a new tensor of `shape` beside `like`; and its type's code."""
     if out is None:
-        out = like.new_empty(shape, dtype=dtype or _torch.float32)
+        out = _new(shape, dtype or _torch.float32, like.device)
     else:
         _usable(what, "out", out)
         if tuple(out.shape) != shape:
@@ -545,10 +553,10 @@ def moe_route(logits, k: int, normalize: bool = True, stream=None):
     T, E = logits.shape
     if not 1 <= k <= min(E, 32):
         raise _bad(f"moe_route: k={k} of {E} experts (at most 32)")
-    i32 = torch.int32
-    ids, slots = logits.new_empty((T, k), dtype=i32), logits.new_empty((T, k), dtype=i32)
-    weights = logits.new_empty((T, k), dtype=torch.float32)
-    offsets, rows = logits.new_empty(E + 1, dtype=i32), logits.new_empty(T * k, dtype=i32)
+    i32, device, choices = torch.int32, logits.device, (T, k)
+    ids, slots = _new(choices, i32, device), _new(choices, i32, device)
+    weights = _new(choices, torch.float32, device)
+    offsets, rows = _new((E + 1,), i32, device), _new((T * k,), i32, device)
     _check(lib().nxq_moe_route(logits.data_ptr(), code, T, E, k, 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
                                offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_on(stream, d)))
     return ids, weights, offsets, rows, slots
