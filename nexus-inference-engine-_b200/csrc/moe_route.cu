@@ -5,9 +5,10 @@
 //
 // Routing has three steps.  (1) One warp per token: lane l holds the logits of
 // experts l, l + 32, ... as order-preserving integer keys and knows its largest;
-// k rounds of two warp reductions (the largest key, then the lowest index that has
-// it, so ties go to the lowest) pick the choices; a lane keeps its two
-// largest and looks again only when both are gone.  The block counts its choices
+// k rounds of warp reductions (the largest key, then the lowest index that has it,
+// so ties go to the lowest; 16-bit logits hold both in one word and need one)
+// pick the choices; a lane keeps its two largest and looks again only when both
+// are gone.  The block counts its choices
 // of every expert.  (2) An exclusive scan of the counts over blocks, 32 experts
 // per CTA.  (3) Every block ranks its own choices: a warp walks a contiguous run of
 // choices in order, equal experts among 32 lanes ranked by their lane (match),
@@ -67,35 +68,21 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The choices of token t by one warp; lane j < k returns choice j (-1: none).
-// logit: its logits as read_logits left them; they are replaced by token next's
-// (none if < 0), whose loads so overlap the choosing.
-template <int V>
-__device__ __forceinline__ void read_logits(const RouteParams& p, int64_t t, int lane, float (&logit)[V]) {
-    auto read = [&](const auto* row, auto widen) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) logit[i] = lane + 32 * i < p.E ? widen(row[lane + 32 * i]) : -kInf;
-    };
-    const int64_t at = t * p.E;
-    if (p.dtype == NXQ_F32)
-        read(static_cast<const float*>(p.logits) + at, [](float v) { return v; });
-    else if (p.dtype == NXQ_F16)
-        read(static_cast<const __half*>(p.logits) + at, [](__half v) { return __half2float(v); });
-    else
-        read(static_cast<const __nv_bfloat16*>(p.logits) + at, [](__nv_bfloat16 v) { return __bfloat162float(v); });
-}
-template <int V>
-__device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int64_t next, int lane, float (&logit)[V]) {
-    uint32_t key[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = key_of(logit[i]);
-    if (next >= 0) read_logits<V>(p, next, lane, logit);
-    // This lane's two largest keys behind (last, last_at) in the order of
-    // choice, and their experts: most lanes are asked for no third.
-    uint32_t top, top2;
-    int at = 0, at2 = 0, known;
-    auto look = [&](uint32_t last, int last_at) {
+// The V logits of type T that a lane holds, as keys of which the warp takes the
+// largest again and again.  A 16-bit logit's key and its index fit into one word, so
+// one reduction finds a choice; fp32 ones keep the two apart.  (bf16 logits
+// that were widened and chosen like fp32 ones: 95 instead of 54 us for 2000
+// tokens, 32 of 1024; 27 instead of 25 us for 16384 tokens, 8 of 256.)
+template <typename T, int V>
+struct Lanes {
+    uint32_t key[V];          // 0: never taken
+    uint32_t top, top2;       // the two largest behind the last choice,
+    int at, at2, known;       // their experts, and how many of the two are left
+    __device__ __forceinline__ void set(int i, int, float v) { key[i] = key_of(v); }
+    // Looks for the two largest behind (last, last_at).
+    __device__ __forceinline__ void look(uint32_t last, int last_at, int lane) {
         top = top2 = 0u;
+        at = at2 = 0;
         known = 2;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -111,37 +98,116 @@ __device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int64_t n
                 at2 = e;
             }
         }
-    };
-    look(0xFFFFFFFFu, -1);
-    const uint32_t first = __reduce_max_sync(0xFFFFFFFFu, top);
-    const float m = value_of(first);
-    float all = 0.0f;  // sum over every expert
-    if (!p.normalize && first) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (key[i]) all += share_of(value_of(key[i]), m);
-        all = warp_sum(all);
     }
-    int my_id = -1;
-    uint32_t my_key = 0u;
-    uint32_t best = first;
-    for (int j = 0; j < p.k && best; ++j) {
-        const int e = (int)__reduce_min_sync(0xFFFFFFFFu, top == best ? (unsigned)at : 0x7FFFFFFFu);
-        if (top == best && at == e) {
+    __device__ __forceinline__ void start(int lane) { look(0xFFFFFFFFu, -1, lane); }
+    __device__ __forceinline__ uint32_t best() const { return __reduce_max_sync(0xFFFFFFFFu, top); }
+    // The expert of the warp's best, which its lane gives up.
+    __device__ __forceinline__ int take(uint32_t b, int lane) {
+        const int e = (int)__reduce_min_sync(0xFFFFFFFFu, top == b ? (unsigned)at : 0x7FFFFFFFu);
+        if (top == b && at == e) {
             if (--known) {
                 top = top2;
                 at = at2;
             } else {
-                look(best, e);
+                look(b, e, lane);
             }
         }
+        return e;
+    }
+    __device__ __forceinline__ static float value(uint32_t b) { return value_of(b); }
+    __device__ __forceinline__ float value_at(int i) const { return value_of(key[i]); }
+};
+
+template <int V>
+struct Lanes16 {
+    uint32_t key[V];  // ordered 16 bits of the logit, then 1023 - expert; 0: never taken
+    uint32_t top, top2;
+    int known;
+    __device__ __forceinline__ void look(uint32_t last) {
+        top = top2 = 0u;
+        known = 2;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const uint32_t k = key[i] < last ? key[i] : 0u;
+            top2 = max(top2, min(top, k));
+            top = max(top, k);
+        }
+    }
+    __device__ __forceinline__ void start(int) { look(0xFFFFFFFFu); }
+    __device__ __forceinline__ uint32_t best() const { return __reduce_max_sync(0xFFFFFFFFu, top); }
+    __device__ __forceinline__ int take(uint32_t b, int) {
+        if (top == b) {
+            if (--known)
+                top = top2;
+            else
+                look(b);
+        }
+        return (int)(kMaxE - 1 - (b & 0xFFFFu));
+    }
+    // -0 counts as +0; -inf and NaN are never taken.
+    __device__ __forceinline__ void set16(int i, int e, uint32_t u, uint32_t inf) {
+        const uint32_t mag = u & 0x7FFFu;
+        if (mag == 0u) u = 0u;
+        const uint32_t ord = (u & 0x8000u) ? 0xFFFFu - u : u + 0x8000u;
+        key[i] = mag > inf || u == (0x8000u | inf) ? 0u : (ord << 16) | (uint32_t)(kMaxE - 1 - e);
+    }
+    __device__ __forceinline__ static uint32_t bits(uint32_t b) {
+        const uint32_t ord = b >> 16;
+        return (ord & 0x8000u) ? ord - 0x8000u : 0xFFFFu - ord;
+    }
+};
+template <int V>
+struct Lanes<__half, V> : Lanes16<V> {
+    __device__ __forceinline__ void set(int i, int e, __half v) { this->set16(i, e, __half_as_ushort(v), 0x7C00u); }
+    __device__ __forceinline__ static float value(uint32_t b) {
+        return __half2float(__ushort_as_half((unsigned short)Lanes16<V>::bits(b)));
+    }
+    __device__ __forceinline__ float value_at(int i) const { return value(this->key[i]); }
+};
+template <int V>
+struct Lanes<__nv_bfloat16, V> : Lanes16<V> {
+    __device__ __forceinline__ void set(int i, int e, __nv_bfloat16 v) { this->set16(i, e, __bfloat16_as_ushort(v), 0x7F80u); }
+    __device__ __forceinline__ static float value(uint32_t b) { return __uint_as_float(Lanes16<V>::bits(b) << 16); }
+    __device__ __forceinline__ float value_at(int i) const { return value(this->key[i]); }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void read_logits(const RouteParams& p, int64_t t, int lane, T (&logit)[V]) {
+    const T* row = static_cast<const T*>(p.logits) + t * p.E;
+#pragma unroll
+    for (int i = 0; i < V; ++i) logit[i] = lane + 32 * i < p.E ? row[lane + 32 * i] : T(-kInf);
+}
+
+// The choices of token t by one warp; lane j < k returns choice j (-1: none).
+// logit: its logits as read_logits left them; they are replaced by token next's
+// (none if < 0), whose loads so overlap the choosing.
+template <typename T, int V>
+__device__ __forceinline__ int choose(const RouteParams& p, int64_t t, int64_t next, int lane, T (&logit)[V]) {
+    Lanes<T, V> l;
+#pragma unroll
+    for (int i = 0; i < V; ++i) l.set(i, lane + 32 * i, logit[i]);
+    if (next >= 0) read_logits<T, V>(p, next, lane, logit);
+    l.start(lane);
+    uint32_t best = l.best();
+    const float m = best ? l.value(best) : 0.0f;
+    float all = 0.0f;  // sum over every expert
+    if (!p.normalize && best) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (l.key[i]) all += share_of(l.value_at(i), m);
+        all = warp_sum(all);
+    }
+    int my_id = -1;
+    uint32_t my_key = 0u;
+    for (int j = 0; j < p.k && best; ++j) {
+        const int e = l.take(best, lane);
         if (lane == j) {
             my_id = e;
             my_key = best;
         }
-        best = __reduce_max_sync(0xFFFFFFFFu, top);
+        best = l.best();
     }
-    const float my_p = my_id >= 0 ? share_of(value_of(my_key), m) : 0.0f;
+    const float my_p = my_id >= 0 ? share_of(l.value(my_key), m) : 0.0f;
     const float z = p.normalize ? warp_sum(my_p) : all;
     if (lane < p.k) {
         p.ids[t * p.k + lane] = my_id;
@@ -221,7 +287,7 @@ __device__ __forceinline__ void scan_experts(const int32_t* cnt, int32_t* out, i
     __syncthreads();
 }
 
-template <int V>
+template <typename T, int V>
 __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteParams p) {
     extern __shared__ int32_t sm[];
     int32_t* hist = sm;                // [E]
@@ -232,10 +298,10 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteP
     overlap_begin();
     __syncthreads();
     int id = -1;
-    float logit[V];
-    if (warp < p.T) read_logits<V>(p, warp, lane, logit);
+    T logit[V];
+    if (warp < p.T) read_logits<T, V>(p, warp, lane, logit);
     for (int64_t t = warp; t < p.T; t += threads / 32) {
-        id = choose<V>(p, t, t + threads / 32 < p.T ? t + threads / 32 : -1, lane, logit);
+        id = choose<T, V>(p, t, t + threads / 32 < p.T ? t + threads / 32 : -1, lane, logit);
         if (id >= 0) atomicAdd(&hist[id], 1);
     }
     __syncthreads();
@@ -253,7 +319,7 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const RouteP
     rank_choices(p, 0, p.T, start, base, threads);
 }
 
-template <int V>
+template <typename T, int V>
 __global__ void __launch_bounds__(kChooseThreads) route_choose_kernel(const RouteParams p) {
     extern __shared__ int32_t cnt[];  // [E]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -262,10 +328,10 @@ __global__ void __launch_bounds__(kChooseThreads) route_choose_kernel(const Rout
     __syncthreads();
     const int64_t t0 = (int64_t)blockIdx.x * p.tb, t1 = t0 + p.tb < p.T ? t0 + p.tb : p.T;
     constexpr int kStep = kChooseThreads / 32;
-    float logit[V];
-    if (t0 + warp < t1) read_logits<V>(p, t0 + warp, lane, logit);
+    T logit[V];
+    if (t0 + warp < t1) read_logits<T, V>(p, t0 + warp, lane, logit);
     for (int64_t t = t0 + warp; t < t1; t += kStep) {
-        const int id = choose<V>(p, t, t + kStep < t1 ? t + kStep : -1, lane, logit);
+        const int id = choose<T, V>(p, t, t + kStep < t1 ? t + kStep : -1, lane, logit);
         if (id >= 0) atomicAdd(&cnt[id], 1);
     }
     __syncthreads();
@@ -326,24 +392,31 @@ __global__ void __launch_bounds__(kThreads) route_rank_kernel(const RouteParams 
     rank_choices(p, t0, t1, start, base, kThreads);
 }
 
-template <int V>
+template <typename T, int V>
 cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
     note_launches(1);
     if (small) {
         const unsigned warps = p.T < 4 ? 4 : p.T < 32 ? (unsigned)p.T : 32;
-        return launch_overlapped(route_small_kernel<V>, 1, 32 * warps, smem, st, p);
+        return launch_overlapped(route_small_kernel<T, V>, 1, 32 * warps, smem, st, p);
     }
-    return launch_overlapped(route_choose_kernel<V>, (unsigned)p.blocks, kChooseThreads, p.E * sizeof(int32_t), st, p);
+    return launch_overlapped(route_choose_kernel<T, V>, (unsigned)p.blocks, kChooseThreads, p.E * sizeof(int32_t), st, p);
+}
+
+template <typename T>
+cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
+    const int v = (p.E + 31) / 32;
+    return v <= 1    ? launch_choose<T, 1>(p, small, smem, st)
+           : v <= 2  ? launch_choose<T, 2>(p, small, smem, st)
+           : v <= 4  ? launch_choose<T, 4>(p, small, smem, st)
+           : v <= 8  ? launch_choose<T, 8>(p, small, smem, st)
+           : v <= 16 ? launch_choose<T, 16>(p, small, smem, st)
+                     : launch_choose<T, 32>(p, small, smem, st);
 }
 
 cudaError_t launch_choose(const RouteParams& p, bool small, size_t smem, cudaStream_t st) {
-    const int v = (p.E + 31) / 32;
-    return v <= 1    ? launch_choose<1>(p, small, smem, st)
-           : v <= 2  ? launch_choose<2>(p, small, smem, st)
-           : v <= 4  ? launch_choose<4>(p, small, smem, st)
-           : v <= 8  ? launch_choose<8>(p, small, smem, st)
-           : v <= 16 ? launch_choose<16>(p, small, smem, st)
-                     : launch_choose<32>(p, small, smem, st);
+    return p.dtype == NXQ_F32   ? launch_choose<float>(p, small, smem, st)
+           : p.dtype == NXQ_F16 ? launch_choose<__half>(p, small, smem, st)
+                                : launch_choose<__nv_bfloat16>(p, small, smem, st);
 }
 
 // ---- combine -------------------------------------------------------------------
