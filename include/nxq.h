@@ -340,7 +340,7 @@ NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, i
  * at least R).  Offsets outside [0, R] or descending, and row indices outside
  * [0, X), are skipped (rows of a bad index give zeros) and reported as
  * NXQ_ERR_INDEX.  Weight and activation rounding as in nxq_qmatmul, and the
- * same choice by NXQ_DECODE_KERNEL / NXQ_PREFILL_KERNEL: up to 8 slots per
+ * same choice by NXQ_DECODE_KERNEL / NXQ_PREFILL_KERNEL: up to 6 slots per
  * expert on average the warp-level kernel, beyond it the tcgen05 one, with
  * both set to simt (and for FP16 / FP32 weights) the exact CUDA-core kernel.
  * The same inputs give the same bits on every call.

@@ -30,7 +30,8 @@
 // issues while the other waits.  The loops are kept short rather than unrolled
 // over the k-steps of a chunk: four copies of the decode and of the issue
 // were 12 % slower for few slots (1024 slots of 64 experts, Q4_K 4096x2048: 117
-// us against 104).  Blocks of 64 slots, which leave TMEM for six A stages, gained
+// us against 104, and 93 with the slow path of the waits out of line; of that,
+// the bytes are worth 48 and the rest is the decode's instructions).  Blocks of 64 slots, which leave TMEM for six A stages, gained
 // 2 to 9 % up to 12 slots per expert and lost from 16 on.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes

@@ -30,8 +30,8 @@
 // end hold stale activations of the stage's earlier units: an MMA column
 // depends on its own slot only, and those columns are not stored.  (Variants
 // with blocks of 16 and 32, 2 to 4 MMAs for every decoded fragment, were slower
-// up to 8 slots per expert, where the tcgen05 kernel takes over: their rings are
-// shallower and every warp reads all activation fragments.)
+// up to 8 slots per expert, and the tcgen05 kernel takes over from 6: their rings
+// are shallower and every warp reads all activation fragments.)
 //
 // What bounds it (64 experts of Q4_K 4096x2048, 256 slots, 290 MB in 82 us = 3.5
 // TB/s): the instructions of the decode, 387 a warp and unit, issue slots 64 %
@@ -390,12 +390,11 @@ int ragged_mma_init() {
     return NXQ_OK;
 }
 
-// Slots of a row block, or 0 to decline: more than 8 slots per expert that can
+// Slots of a row block, or 0 to decline: more than 6 slots per expert that can
 // have any, on average.  Measured (64 experts, routed with a bias, Q4_K
-// 4096x2048, 1 / 2 / 4 / 6 / 8 / 12 slots on average): 49.5 / 67.5 / 82.4 / 97.3 / 115 /
-// 144 us here, 72.5 / 101 / 115 / 115 / 117 / 118 us with the tcgen05 kernel; Q4_0
-// 14336x4096 gate and up, 8 experts: 67 / 97 / 125 / 154 / 183 / 239 against 113 / 141 /
-// 177 / 178 / 180 / 178.
+// 4096x2048, 2 / 4 / 6 / 8 slots on average): 67 / 80 / 94 / 112 us here, 91 to 94 us
+// with the tcgen05 kernel; Q4_0 14336x4096 gate and up, 8 experts, 4 / 8 slots:
+// 120 / 175 against 155 to 161; Q3_K, 4 / 8 slots: 53 / 66 against 62.
 int ragged_mma_blk(const RaggedCall& c) {
     const TiledShape& s = c.w->shape;
     if (!mma_supported(s, 1)) return 0;
