@@ -757,7 +757,7 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
     const bool vec = N % 8 == 0 && (uintptr_t)h_dev % 16 == 0 && (uintptr_t)res_dev % 32 == 0 &&
                      (uintptr_t)y_dev % (y_dtype == NXQ_F32 ? 32 : 16) == 0;
     const bool f32 = h_dtype == NXQ_F32;
-    // Many tokens: bulk copies (kCombineBulk below).
+    // Many tokens: bulk copies (kCombineBulk).
     if (vec && T >= kCombineBulk * (int64_t)context_sm_count() && T <= ((int64_t)1 << 62) / N) {
         int64_t seg = kBulkStage / (k * (f32 ? 4 : 2)) / 64 * 64;  // columns of a stage
         int64_t segs = (N + seg - 1) / seg;

@@ -212,7 +212,15 @@ __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepPara
         make_plan(p.offsets, p.E, p.R, p.blk, p.plan, p.w, p.up, p.status);
         return;
     }
-    const int64_t lo = p.offsets[0] > 0 ? p.offsets[0] : 0, hi = p.offsets[p.E] < p.R ? p.offsets[p.E] : p.R;
+    // Up to the largest offset within [0, R], which is the last one unless an
+    // expert that the plan leaves out comes last.  (A thread per expert.)
+    __shared__ int top[32];
+    const int o1 = (int)threadIdx.x < p.E ? p.offsets[threadIdx.x + 1] : 0;
+    int most = __reduce_max_sync(0xFFFFFFFFu, o1 <= p.R ? o1 : 0);
+    if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = most;
+    __syncthreads();
+    most = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x % 32 < blockDim.x / 32 ? top[threadIdx.x % 32] : 0);
+    const int64_t lo = p.offsets[0] > 0 ? p.offsets[0] : 0, hi = most;
     const int group = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads, groups = blockDim.x / kRowThreads;
     bool over = false;
     for (int64_t s = lo + (int64_t)(blockIdx.x - 1) * groups + group; s < hi; s += (int64_t)(gridDim.x - 1) * groups) {
@@ -375,7 +383,7 @@ extern "C" {
 NXQ_API int nxq_experts_create(const nxq_weight_t* hs, int count, nxq_experts_t* out) {
     if (!hs || !out) return fail(NXQ_ERR_ARG, "null argument");
     if (count < 1 || count > kMaxExperts) return fail(NXQ_ERR_ARG, "%d experts (1 to %d)", count, kMaxExperts);
-    std::vector<const uint8_t*> dev((size_t)count);
+    const uint8_t* dev[kMaxExperts];
     TiledShape shape{};
     for (int i = 0; i < count; ++i) {
         Weight* w = nullptr;
@@ -392,21 +400,33 @@ NXQ_API int nxq_experts_create(const nxq_weight_t* hs, int count, nxq_experts_t*
     if (!t) return fail(NXQ_ERR_NOMEM, "host allocation failed");
     t->count = count;
     t->shape = shape;
+    try {
+        t->refs.assign(hs, hs + count);
+        std::lock_guard<std::mutex> lk(g_tables_mu);
+        g_tables.insert(t);
+    } catch (const std::bad_alloc&) {
+        delete t;
+        return fail(NXQ_ERR_NOMEM, "host allocation failed");
+    }
     int held = 0, rc = NXQ_OK;
     for (; held < count && rc == NXQ_OK; ++held) rc = weight_table_ref(hs[held], 1);
     if (rc != NXQ_OK) --held;
     cudaError_t e = cudaSuccess;
-    if (rc == NXQ_OK && (e = cudaMalloc((void**)&t->dev, dev.size() * sizeof(dev[0]))) == cudaSuccess)
-        e = cudaMemcpy(t->dev, dev.data(), dev.size() * sizeof(dev[0]), cudaMemcpyHostToDevice);
+    const size_t bytes = (size_t)count * sizeof(dev[0]);
+    // The copy is waited for: streams that do not synchronize with the default one read the table.
+    if (rc == NXQ_OK && (e = cudaMalloc((void**)&t->dev, bytes)) == cudaSuccess &&
+        (e = cudaMemcpy(t->dev, dev, bytes, cudaMemcpyHostToDevice)) == cudaSuccess)
+        e = cudaStreamSynchronize(cudaStreamLegacy);
     if (rc != NXQ_OK || e != cudaSuccess) {
         for (int i = 0; i < held; ++i) weight_table_ref(hs[i], -1);
         if (t->dev) cudaFree(t->dev);
+        {
+            std::lock_guard<std::mutex> lk(g_tables_mu);
+            g_tables.erase(t);
+        }
         delete t;
         return rc != NXQ_OK ? rc : cuda_fail(e, "expert table");
     }
-    t->refs.assign(hs, hs + count);
-    std::lock_guard<std::mutex> lk(g_tables_mu);
-    g_tables.insert(t);
     *out = reinterpret_cast<nxq_experts_t>(t);
     return NXQ_OK;
 }

@@ -409,6 +409,30 @@ def test_ragged_bad_indices(gpu, n):
             w.release()
 
 
+@pytest.mark.parametrize("xdt", DT.keys())
+@pytest.mark.parametrize("n", [6, 90])
+def test_ragged_bad_last_offset(gpu, n, xdt):
+    """A last offset that descends leaves out the last expert only: the others' rows are there, whatever x's type."""
+    ws, W = make_weights(gpu, 12, 3, 128, 256, 6)
+    E = gpu.Experts(ws)
+    x = torch.randn((n, 256), device="cuda").to(DT[xdt])
+    h = n // 3
+    try:
+        out = torch.full((n, 128), -7.0, device="cuda")
+        gpu.qmatmul_ragged(E, x, torch.tensor([0, h, 2 * h, 1], dtype=torch.int32, device="cuda"), out=out)
+        with pytest.raises(gpu.NxqError) as e:
+            gpu.stream_sync()
+        assert e.value.name == "ERR_INDEX"
+        for i in range(2):
+            got, want = out[i * h:(i + 1) * h], (x[i * h:(i + 1) * h].double() @ W[i].T).float()
+            assert bool(((got - want).norm() <= 2e-3 * want.norm()).item())
+        assert bool((out[2 * h:] == -7).all())
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
 def test_ragged_infinite_values_stay_in_their_rows(gpu):
     """inf and NaN in a row, or in rows no slot reads, reach no other row."""
     ws, W = make_weights(gpu, 12, 2, 256, 512, 5)
