@@ -6,14 +6,15 @@
 // two tiles are neighbours of one weight (plain), or the gate's and the up
 // weight's (PAIR); both multiply the same activations, so an SM reads 32 bytes of
 // activations and 18 of Q4_K weights per cycle of MMA work, where one tile x
-// 256 slots would read 64 and 9.  Roles, per 64-element k-step:
+// 256 slots would read 64 and 9.  Roles, per k-step of 128 elements:
 //   warp 26      producer: the packed tile-chunks (256 k) by 1-D bulk copies
 //   warp 0       producer: the activations of the row block by TMA, as boxes of
 //                64 k x 64 slots (128-byte swizzle, no multicast), only as many
 //                as the block has slots for
 //   warps 2-17   four dequant warpgroups, one per tile and k-step parity: thread
-//                r decodes the 64 elements of row r (the lane decoders of the
-//                decode GEMV) and writes them to TMEM, the MMA's A operand
+//                r decodes the 128 elements of row r, 64 at a time (the lane
+//                decoders of the decode GEMV), and writes them to TMEM, the MMA's
+//                A operand; a stage belongs to one warpgroup
 //   warps 1, 27  one for each tile: a lane issues tcgen05.mma kind::f16 M=128,
 //                K=16 with N = the block's slots rounded up to 16 (a short block
 //                costs less), into the tile's 128-column fp32 accumulator
@@ -23,16 +24,19 @@
 //                accumulators are handed back as soon as they are read, and
 //                rows leave as 16-byte stores while the next tile's MMAs run
 //
-// The issuing loops run warp-wide, half the lanes watching the activations and
-// half the A operand, with only the MMA and the commits in the elected lane.
-// Waiting for a stage and handing it back cost an issuing warp about 400 cycles
-// a k-step, against 512 of MMA work for both tiles; with a warp per tile one
-// issues while the other waits.  The loops are kept short rather than unrolled
-// over the k-steps of a chunk: four copies of the decode and of the issue
-// were 12 % slower for few slots (1024 slots of 64 experts, Q4_K 4096x2048: 117
-// us against 104, and 93 with the slow path of the waits out of line; of that,
-// the bytes are worth 48 and the rest is the decode's instructions).  Blocks of 64 slots, which leave TMEM for six A stages, gained
-// 2 to 9 % up to 12 slots per expert and lost from 16 on.
+// What bounds it is the latency of handing stages on, not the MMAs (16 to 64
+// cycles each, two issuing warps): an issuing warp needs some 600 cycles from
+// one k-step to the next whatever N is, with its operands there 94 % of the time
+// when a k-step had 64 elements.  So a k-step has 128, with one commit and one
+// handshake for each warpgroup; the issuing loops run warp-wide, half the lanes
+// watching the activations and half the A operand, with only the MMA and the
+// commits in the elected lane.  Loops are kept short rather than unrolled over
+// a chunk: four copies of the decode and of the issue were 12 % slower for few
+// slots (1024 slots of 64 experts, Q4_K 4096x2048: 117 us against 104, and 93
+// with the slow path of the waits out of line).  There the bytes are worth 48 us,
+// and the decode's instructions are what is left.  Blocks of 64 slots, which
+// leave TMEM for more A stages, gained 2 to 9 % up to 12 slots per expert and
+// lost from 16 on.
 //
 // An MMA column depends on its own slot's activations only, so what the boxes
 // hold behind a block's slots (the next expert's rows, or zeros) reaches no
@@ -58,31 +62,38 @@ constexpr int kWarpWProducer = kWarpEpi0 + kEpiWarps;
 constexpr int kWarpMma1 = kWarpWProducer + 1;
 constexpr int kThreads = 32 * (kWarpMma1 + 1);
 constexpr int kMats = 2;  // weight tiles of a work tile
-constexpr int kKS = 64;   // reduction elements per k-step (one swizzle atom)
-constexpr int kStepsPerChunk = CHUNK_K / kKS;
-constexpr int kACols = 32 * kMats;        // TMEM columns of a stage
+constexpr int kKS = 64;   // reduction elements of a swizzle atom
+constexpr int kHalves = 2;                // swizzle atoms of a k-step
+constexpr int kStepsPerChunk = CHUNK_K / (kHalves * kKS);
+constexpr int kACols = 32 * kMats;        // TMEM columns of an atom's A, both tiles
 constexpr int NT = 128;                   // slots of a work tile
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kColD = (int)kTmemCols - kMats * NT;  // accumulators: columns kColD + NT mat
-constexpr int kA = kColD / kACols;                  // TMEM A ring: the columns left
-static_assert(kA % 2 == 0, "a warpgroup's k-steps keep their parity in the ring");
+constexpr int kStages = kColD / (kHalves * kACols);  // of the TMEM A ring: the columns left
 constexpr int kBoxRows = 64;
 constexpr int kBoxBytes = kBoxRows * kKS * 2;
-constexpr int kXB = NT * kKS * 2;               // 16 KB of activations per k-step
+constexpr int kXB = kHalves * NT * kKS * 2;     // 32 KB of activations per k-step
 constexpr int kStageOut = NT * TILE_ROWS * 2;  // 32 KB: one tile's 16-bit outputs [slot][row]
 
-// Ring depths in shared memory: four k-steps of activations (six, in place of
-// tile-chunks, were no faster), then as many tile-chunks as fit (up to 6).
+// Ring depths in shared memory: three k-steps of activations if at least four
+// tile-chunks fit beside them (or no more fit beside two), else two; then as many
+// tile-chunks as fit, up to six.  An even number: the two tiles' chunks alternate
+// in the ring, so each tile keeps its own stages.  With an odd number a stage
+// would change hands, and a warpgroup that waits for a phase of its own could
+// take the phase before the other tile's for it - copies land in any order.
 template <int TYPE>
 struct Rings {
     static constexpr int WB = lane::Lane<TYPE>::kStage;
     static constexpr int kBudget = 227 * 1024 - 1024 - kBarBytes - kStageOut;
-    static constexpr int kX = 4;
-    static constexpr int fit = (kBudget - kX * kXB) / WB;
-    static constexpr int kW = fit > 6 ? 6 : fit;
-    static_assert(kW >= 2, "tile-chunk ring too shallow");
-    static_assert((2 * kX + 2 * kW + 2 * kMats * kA + 2 + kMats) * 8 + 8 <= kBarBytes, "barrier area too small");
+    static constexpr int chunks_beside(int x) {
+        const int n = (kBudget - x * kXB) / WB / kMats * kMats;
+        return n > 6 ? 6 : n;
+    }
+    static constexpr int kX = chunks_beside(3) >= 4 || chunks_beside(3) == chunks_beside(2) ? 3 : 2;
+    static constexpr int kW = chunks_beside(kX);
+    static_assert(kW >= kMats && kW % kMats == 0, "a tile-chunk stage belongs to one tile");
+    static_assert((2 * kX + 2 * kW + 2 * kMats * kStages + 2 + kMats) * 8 + 8 <= kBarBytes, "barrier area too small");
     static constexpr size_t smem = 1024 + (size_t)kX * kXB + kStageOut + (size_t)kW * WB + kBarBytes;
 };
 
@@ -122,7 +133,7 @@ __device__ __forceinline__ bool epi_all(bool ok) {
         : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
+__device__ __forceinline__ void epi_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
 
 // Ring position: stage index and the phase parity of its current use.
 struct Ring {
@@ -153,7 +164,7 @@ __device__ __forceinline__ int weight_tile(const RaggedTile& t, int mat, int64_t
 template <int TYPE, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p, const __grid_constant__ CUtensorMap xmap) {
     using Rg = Rings<TYPE>;
-    constexpr int WB = Rg::WB, kX = Rg::kX, kW = Rg::kW;
+    constexpr int WB = Rg::WB, kW = Rg::kW, kX = Rg::kX;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
@@ -165,8 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     uint64_t* w_full = x_empty + kX;
     uint64_t* w_empty = w_full + kW;
     uint64_t* a_full = w_empty + kW;
-    uint64_t* a_empty = a_full + kMats * kA;   // [mat][stage]
-    uint64_t* d_full = a_empty + kMats * kA;
+    uint64_t* done = a_full + kMats * kStages;  // [mat][stage]: its MMAs are, and no longer read A or x
+    uint64_t* d_full = done + kMats * kStages;
     uint64_t* d_empty = d_full + 1;
     uint64_t* drain = d_empty + 1;  // [mat]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + kMats);
@@ -175,17 +186,14 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ptx::WaitCtl ctl{abort_flag, p.status};
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kX; ++i) {
-            ptx::mbar_init(&x_full[i], 1);
-            ptx::mbar_init(&x_empty[i], kMats);  // both tiles' MMAs
-        }
+        for (int i = 0; i < kX; ++i) { ptx::mbar_init(&x_full[i], 1); ptx::mbar_init(&x_empty[i], kMats); }
         for (int i = 0; i < kW; ++i) {
             ptx::mbar_init(&w_full[i], 1);
             ptx::mbar_init(&w_empty[i], 4 * kDeqGroups / kMats);  // the warps that decode a tile-chunk
         }
-        for (int i = 0; i < kMats * kA; ++i) {
+        for (int i = 0; i < kMats * kStages; ++i) {
             ptx::mbar_init(&a_full[i], 4);  // the warps that write a tile's stage
-            ptx::mbar_init(&a_empty[i], 1);
+            ptx::mbar_init(&done[i], 1);
         }
         ptx::mbar_init(d_full, kMats);
         ptx::mbar_init(d_empty, kEpiWarps);
@@ -193,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         *abort_flag = 0;
         ptx::fence_mbar_init();
     }
+    __syncwarp();
     if (warp == kWarpProducer) {
         ptx::tmem_alloc(tmem_slot, kTmemCols);
         ptx::tmem_relinquish();
@@ -258,11 +267,12 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
             for (int ks = 0; ks < chunks * kStepsPerChunk && ok; ++ks) {
                 ok = ptx::warp_mbar_wait(&x_empty[rx.i], rx.ph ^ 1u, ctl, 42);
                 if (!ok) break;
-                if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[rx.i], boxes * kBoxBytes);
+                if (lane == 0) ptx::mbar_arrive_expect_tx(&x_full[rx.i], kHalves * boxes * kBoxBytes);
                 __syncwarp();
-                if (lane < boxes)
-                    ptx::tma_load_2d(xs + rx.i * kXB + lane * kBoxBytes, &xmap, ks * kKS, t.row0 + lane * kBoxRows,
-                                     &x_full[rx.i]);
+                const int half = lane & 1, box = lane >> 1;
+                if (box < boxes)
+                    ptx::tma_load_2d(xs + rx.i * kXB + half * (kXB / kHalves) + box * kBoxBytes, &xmap,
+                                     (kHalves * ks + half) * kKS, t.row0 + box * kBoxRows, &x_full[rx.i]);
                 rx.next(kX);
                 ++issued;
             }
@@ -282,8 +292,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         walk.start(p.plan, NT, p.tiles, blockIdx.x);
         const uint64_t desc0 = ptx::desc_sw128_kmajor(ptx::smem_addr(xs));
         const uint32_t d = tmem + kColD + mat * NT, a = tmem + mat * 32;
-        uint64_t* const af = a_full + mat * kA;
-        uint64_t* const ae = a_empty + mat * kA;
+        uint64_t* const af = a_full + mat * kStages;
+        uint64_t* const dn = done + mat * kStages;
         bool ready = false;
         for (int64_t g = blockIdx.x; g < total && ok; g += G, ++nt) {
             const RaggedTile t = walk.at(g);
@@ -296,16 +306,19 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                     ok = ptx::warp_mbar_wait(lane < 16 ? &x_full[rx.i] : &af[ra.i], lane < 16 ? rx.ph : ra.ph, ctl, 44);
                     if (!ok) break;
                 }
-                const int xi = rx.i, ai = ra.i;
+                const int i = ra.i, ix = rx.i;
                 rx.next(kX);
-                ra.next(kA);
+                ra.next(kStages);
                 // The next k-step's barriers, read while this one's MMAs issue.
                 ready = ptx::mbar_test_wait(lane < 16 ? &x_full[rx.i] : &af[ra.i], lane < 16 ? rx.ph : ra.ph);
                 ptx::tc_fence_after();
                 if (ptx::elect_one()) {
-                    ptx::mma_ts_f16_k64(d, a + ai * kACols, desc0 + ((uint32_t)(xi * kXB) >> 4), idesc, ks ? 1u : 0u);
-                    ptx::mma_commit(&ae[ai]);
-                    ptx::mma_commit(&x_empty[xi]);
+                    const uint32_t ai = a + i * (kHalves * kACols);
+                    const uint64_t xi = desc0 + ((uint32_t)(ix * kXB) >> 4);
+                    ptx::mma_ts_f16_k64(d, ai, xi, idesc, ks ? 1u : 0u);
+                    ptx::mma_ts_f16_k64(d, ai + kACols, xi + ((uint32_t)(kXB / kHalves) >> 4), idesc, 1u);
+                    ptx::mma_commit(&dn[i]);
+                    ptx::mma_commit(&x_empty[ix]);
                     if (ks == steps - 1) ptx::mma_commit(d_full);
                 }
                 __syncwarp();
@@ -320,21 +333,23 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
         // Warpgroup wg decodes the k-steps of parity wg % 2 of tile wg / 2.
         const int wg = (warp - kWarpDeq0) >> 2, quad = warp & 3, r = quad * 32 + lane;
         const int mat = wg >> 1, par = wg & 1;
-        Ring rw, ra;
+        Ring rw;
         if (mat) rw.next(kW);
-        if (par) ra.next(kA);
         bool ok = true;
-        const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + mat * 32;
+        uint32_t ph = 1u;
+        uint64_t* const mine_done = done + mat * kStages + par;
+        uint64_t* const mine_full = a_full + mat * kStages + par;
+        const uint32_t tbase = tmem + ((uint32_t)(quad * 32) << 16) + mat * 32 + kHalves * par * kACols;
         for (int64_t g = blockIdx.x; g < total && ok; g += G) {
             for (int c = 0; c < chunks && ok; ++c) {
                 if (!(ok = ptx::warp_mbar_wait(&w_full[rw.i], rw.ph, ctl, 46))) break;
                 const uint8_t* stage = ws + rw.i * WB;
 #pragma unroll 1
-                for (int st = par; st < kStepsPerChunk; st += 2) {
+                for (int h = 0; h < kHalves; ++h) {
                     uint32_t o[32];
                     {
                         lane::Lane<TYPE> L;
-                        L.load(stage, r, st);
+                        L.load(stage, r, kHalves * par + h);
 #pragma unroll
                         for (int m = 0; m < 8; ++m) {
                             uint32_t q[4];
@@ -343,21 +358,21 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                             for (int i = 0; i < 4; ++i) o[4 * m + i] = q[i];
                         }
                     }
-                    ok = ok && ptx::warp_mbar_wait(&a_empty[mat * kA + ra.i], ra.ph ^ 1u, ctl, 47);
-                    if (!ok) break;
-                    ptx::tc_fence_after();
-                    ptx::tmem_st32(tbase + ra.i * kACols, o);
-                    // (Announcing the stage only after the next decode, to hide
-                    // the store's latency, was 5 % slower.)
-                    ptx::tmem_wait_st();
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&a_full[mat * kA + ra.i]);
-                    ra.next(kA);
-                    ra.next(kA);
+                    if (h == 0) {
+                        if (!(ok = ptx::warp_mbar_wait(mine_done, ph, ctl, 47))) break;
+                        ptx::tc_fence_after();
+                    }
+                    ptx::tmem_st32(tbase + h * kACols, o);
                 }
+                if (!ok) break;
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before();
                 __syncwarp();
-                if (ok && lane == 0) ptx::mbar_arrive(&w_empty[rw.i]);
+                if (lane == 0) {
+                    ptx::mbar_arrive(mine_full);
+                    ptx::mbar_arrive(&w_empty[rw.i]);
+                }
+                ph ^= 1u;
                 rw.next(kW);
                 rw.next(kW);
             }
@@ -439,6 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
 #pragma unroll
                             for (int j = 0; j < 16; ++j, q += N)
                                 if (c + j < left) *q = v[j];
+                        __syncwarp();
                     }
                 ptx::tc_fence_before();
                 __syncwarp();

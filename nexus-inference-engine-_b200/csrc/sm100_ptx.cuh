@@ -116,15 +116,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
 }
 
 // As mbar_wait, by a converged warp (the lanes may watch different barriers);
-// tells every lane whether all of them saw their phase.  Only the try is
-// inlined: a kernel with many waits stays small, and no lane waits for another
-// to pass its result on.
-static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, const WaitCtl c, unsigned where) {
-    return mbar_wait(bar, parity, c, where);
+// tells every lane whether all of them saw their phase.  Every try ends in a
+// vote, so the warp stays converged throughout, as the aligned tcgen05
+// instructions behind such a wait need it.  A barrier must keep its phase while
+// another lane's is awaited: its next one needs this warp.  Only the first try is
+// inlined: a kernel with many waits stays small.
+static __device__ __noinline__ bool warp_mbar_wait_slow(uint64_t* bar, uint32_t parity, const WaitCtl c, unsigned where) {
+    const long long t0 = clock64();
+    const long long lim = wait_limit(c.status);
+    while (true) {
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait_sleep(bar, parity, 20000u))) return true;
+        const bool late = clock64() - t0 > lim;
+        if (__any_sync(0xFFFFFFFFu, *c.abort)) return false;
+        if (__any_sync(0xFFFFFFFFu, late)) {
+            if ((threadIdx.x & 31) == 0) raise_timeout(c, where);
+            __syncwarp();
+            return false;
+        }
+    }
 }
 __device__ __forceinline__ bool warp_mbar_wait(uint64_t* bar, uint32_t parity, const WaitCtl& c, unsigned where) {
-    if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xFFFFFFFFu, mbar_wait_slow(bar, parity, c, where));
+    return __all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity)) || warp_mbar_wait_slow(bar, parity, c, where);
 }
 
 // ---- bulk / tensor copies (no multicast) ------------------------------------

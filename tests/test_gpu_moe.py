@@ -306,6 +306,29 @@ def test_ragged_rows_left_alone(gpu, N, counts):
     run_ragged(gpu, 2, N, 96, counts, torch.float16, torch.float32, True, False, seed=N, first=3, behind=70)
 
 
+@pytest.mark.parametrize("t", [2, 8, 10, 11, 12, 13, 14, 101],
+                         ids=["Q4_0", "Q8_0", "Q2_K", "Q3_K", "Q4_K", "Q5_K", "Q6_K", "I4G32"])
+def test_ragged_repeats(gpu, t):
+    """Many calls in a row, of every ring depth the block types lead to, give the same bits."""
+    counts = [20, 3, 31, 16, 9, 40, 1, 24]
+    N, K = 1024, 2048
+    ws, W = make_weights(gpu, t, len(counts), N, K, 7)
+    E = gpu.Experts(ws)
+    try:
+        src = torch.arange(sum(counts), device="cuda")
+        x = torch.randn((len(src), K), device="cuda").half()
+        off = make_offsets(counts)
+        first = gpu.qmatmul_ragged(E, x, off)
+        check(first, *products(W, t, x, counts, src))
+        outs = [gpu.qmatmul_ragged(E, x, off) for _ in range(300)]
+        gpu.stream_sync()
+        assert all(torch.equal(o, first) for o in outs)
+    finally:
+        E.release()
+        for w in ws:
+            w.release()
+
+
 def test_ragged_large_shared_tiles(gpu):
     """More work tiles than SMs and tiles cut between CTAs: right, and the same bits on every call."""
     for counts in ([2, 0, 1, 3], [40, 25, 0, 90], [300, 0, 700, 20]):
