@@ -337,9 +337,11 @@ NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, i
  * fp32 accumulation.  offsets_dev: E + 1 ascending int32 values in [0, R]; y_dev
  * has R rows (rows before offsets[0] and from offsets[E] on are left as they
  * were), x_dev has X rows (without rows_dev, slot s reads row s and X must be
- * at least R).  Offsets outside [0, R] or descending, and row indices outside
- * [0, X), are skipped (rows of a bad index give zeros) and reported as
- * NXQ_ERR_INDEX.  Weight and activation rounding as in nxq_qmatmul, and the
+ * at least R).  Bad offsets and row indices are reported as NXQ_ERR_INDEX: an
+ * offset outside [0, R] leaves out the two experts it bounds, one below an
+ * earlier offset the experts that start or end at it (and any other that starts
+ * before the earlier one); a row index outside [0, X) gives a row of zeros.  All
+ * other rows are computed.  Weight and activation rounding as in nxq_qmatmul, and the
  * same choice by NXQ_DECODE_KERNEL / NXQ_PREFILL_KERNEL: up to 6 slots per
  * expert on average the warp-level kernel, beyond it the tcgen05 one, with
  * both set to simt (and for FP16 / FP32 weights) the exact CUDA-core kernel.

@@ -34,9 +34,10 @@ int check_experts(nxq_experts_t h, const ExpertTable** out) {
 }
 
 // One CTA of at least E threads, thread = expert: writes the experts that have rows.  An expert's
-// range is taken only if it lies in [0, R] and starts at or behind every offset
-// before it, so the ranges taken never overlap and hold at most R slots
-// whatever the offsets are; anything else is reported and left out.
+// range is taken only if both its ends lie in [0, R] and it starts at or behind
+// every such offset before it, so the ranges taken never overlap and hold at most
+// R slots whatever the offsets are; anything else is reported and left out.  An
+// offset outside [0, R] so costs the two experts it bounds, and no other.
 __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t R, int blk, RaggedPlan* plan,
                                           const uint8_t* const* w, const uint8_t* const* up, DeviceStatus* status) {
     __shared__ int warp_n[32], warp_b[32], warp_m[32];
@@ -44,7 +45,7 @@ __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t
     const int o0 = e < E ? offsets[e] : 0, o1 = e < E ? offsets[e + 1] : 0;
     const uint8_t* const we = e < E ? w[e] : nullptr;
     const uint8_t* const ue = e < E && up ? up[e] : nullptr;
-    int before = o0;  // the largest offset up to and including o0
+    int before = o0 <= R ? o0 : 0;  // the largest offset within [0, R] (or 0) up to and including o0
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xFFFFFFFFu, before, o);
@@ -55,7 +56,7 @@ __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t
     for (int w = 0; w < warp; ++w) before = warp_m[w] > before ? warp_m[w] : before;
     int a = 0, n = 0;
     if (e < E) {
-        if (o0 < 0 || o0 < before || o1 < o0 || o1 > R)
+        if (o0 < 0 || o0 > R || o0 < before || o1 < o0 || o1 > R)
             raise_index(status, kIndexOffset);
         else
             a = o0, n = o1 - o0;
@@ -220,7 +221,8 @@ __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepPara
     if (threadIdx.x % 32 == 0) top[threadIdx.x / 32] = most;
     __syncthreads();
     most = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x % 32 < blockDim.x / 32 ? top[threadIdx.x % 32] : 0);
-    const int64_t lo = p.offsets[0] > 0 ? p.offsets[0] : 0, hi = most;
+    const int o0 = p.offsets[0];
+    const int64_t lo = o0 > 0 && o0 <= p.R ? o0 : 0, hi = most;  // (a first offset out of range bounds nothing)
     const int group = threadIdx.x / kRowThreads, lane = threadIdx.x % kRowThreads, groups = blockDim.x / kRowThreads;
     bool over = false;
     for (int64_t s = lo + (int64_t)(blockIdx.x - 1) * groups + group; s < hi; s += (int64_t)(gridDim.x - 1) * groups) {
