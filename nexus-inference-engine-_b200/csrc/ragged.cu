@@ -61,7 +61,7 @@ __device__ __forceinline__ void make_plan(const int32_t* offsets, int E, int64_t
         else
             a = o0, n = o1 - o0;
     }
-    const int has = n > 0, nb = (n + blk - 1) / blk;
+    const int has = n > 0, nb = row_blocks(n, blk);
     const unsigned act = __ballot_sync(0xFFFFFFFFu, has);
     int bs = nb;
 #pragma unroll

@@ -55,6 +55,9 @@ struct RaggedCall {
     cudaStream_t st;
 };
 
+// Row blocks of `blk` slots for n >= 0 slots, any int (n + blk - 1 may pass 2^31).
+__host__ __device__ inline int row_blocks(int n, int blk) { return n / blk + (n % blk != 0); }
+
 // One work tile: weight tile `tile` of the expert's weights, slots [row0, row0 +
 // rows).
 struct RaggedTile {
@@ -80,7 +83,7 @@ struct RaggedWalk {
         const int4 v = q[0];
         const longlong2 a = *reinterpret_cast<const longlong2*>(q + 1);
         cur = RaggedEntry{v.x, v.y, v.z, v.w, reinterpret_cast<const uint8_t*>(a.x), reinterpret_cast<const uint8_t*>(a.y)};
-        nb = (cur.rows + blk - 1) / blk;
+        nb = row_blocks(cur.rows, blk);
         first = (int64_t)cur.blk0 * tiles;
         end = first + (int64_t)nb * tiles;
     }

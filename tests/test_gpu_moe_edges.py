@@ -51,3 +51,25 @@ def test_offset_out_of_range_costs_its_neighbours_only(gpu, value, bad, kernel, 
                 assert bool(((out[s].double() - y[s]).abs() <= b[s] + 2.0 ** -24 * y[s].abs() + 2.0 ** -25).all()), e
     finally:
         release([T], ws)
+
+
+def test_most_slots(gpu):
+    """2^31 - 1 slots, all but five of them with one expert."""
+    t, K, R = 122, 32, 2**31 - 1
+    ws, W = make_weights(gpu, t, 2, 1, K, 3)
+    T = gpu.Experts(ws)
+    try:
+        x = torch.randn((2, K), device="cuda")
+        rows = torch.zeros(R, dtype=torch.int32, device="cuda")
+        rows[1::2] = 1
+        out = torch.full((R, 1), -7.0, dtype=torch.bfloat16, device="cuda")
+        gpu.qmatmul_ragged(T, x, torch.tensor([0, 5, R], dtype=torch.int32, device="cuda"), rows=rows, out=out)
+        gpu.stream_sync()
+        for odd in (0, 1):
+            for e, got in enumerate((out[odd:5:2, 0], out[5:][1 - odd::2, 0])):
+                want = (x[odd].double() @ W[e, 0]).item()
+                bound = K * 2.0 ** -24 * (x[odd].double() * W[e, 0]).abs().sum().item()
+                lo, hi = got.min().double().item(), got.max().double().item()
+                assert lo == hi and abs(lo - want) <= bound + 2.0 ** -8 * (abs(want) + bound), (odd, e)
+    finally:
+        release([T], ws)
