@@ -235,6 +235,28 @@ def _stream_ptr(stream) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _empty(shape, dtype, device, stream):
+    """An empty tensor that a call on `stream` (None: the current one) will write.
+    On another stream than the current one it is allocated there, or it could be
+    memory that work queued on the current stream still reads; and it is not
+    reused before the work that the current stream has queued when it is freed."""
+    import torch
+
+    if stream is not None:
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device(device.type, torch.cuda.current_device())
+        here = torch.cuda.current_stream(device)
+        ptr = _stream_ptr(stream).value or 0
+        if ptr != here.cuda_stream:
+            there = torch.cuda.ExternalStream(ptr, device=device) if ptr else torch.cuda.default_stream(device)
+            with torch.cuda.stream(there):
+                t = torch.empty(shape, dtype=dtype, device=device)
+            t.record_stream(here)
+            return t
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _dtype_code(t) -> int:
     import torch
 
@@ -317,7 +339,7 @@ class Weight:
         import torch
 
         if out is None:
-            out = torch.empty((self.N, self.K), dtype=torch.float32, device="cuda")
+            out = _empty((self.N, self.K), torch.float32, "cuda", stream)
         _check(lib().nxq_dequant(self.handle, out.data_ptr(), _stream_ptr(stream)))
         return out
 
@@ -334,7 +356,7 @@ def qmatmul(w: Weight, x, out=None, out_dtype=None, stream=None):
     assert x.is_cuda and x.is_contiguous() and x.shape[-1] == w.K
     M = x.numel() // w.K
     if out is None:
-        out = torch.empty((M, w.N), dtype=out_dtype or torch.float32, device=x.device)
+        out = _empty((M, w.N), out_dtype or torch.float32, x.device, stream)
     _check(lib().nxq_qmatmul(w.handle, x.data_ptr(), _dtype_code(x.dtype), out.data_ptr(),
                              _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -361,8 +383,7 @@ def qmatmul_grouped(ws, xs, outs=None, out_dtype=None, stream=None):
     ws, xs = list(ws), list(xs)
     assert len(ws) == len(xs)
     if outs is None:
-        outs = [torch.empty((x.numel() // w.K, w.N), dtype=out_dtype or torch.float32, device=x.device)
-                for w, x in zip(ws, xs)]
+        outs = [_empty((x.numel() // w.K, w.N), out_dtype or torch.float32, x.device, stream) for w, x in zip(ws, xs)]
     n = len(ws)
     Ms = []
     for w, x, y in zip(ws, xs, outs):
@@ -385,7 +406,7 @@ def qmatmul_swiglu(w_gate: Weight, w_up: Weight, x, out=None, out_dtype=None, st
     assert x.is_cuda and x.is_contiguous() and x.shape[-1] == w_gate.K
     M = x.numel() // w_gate.K
     if out is None:
-        out = torch.empty((M, w_gate.N), dtype=out_dtype or torch.float32, device=x.device)
+        out = _empty((M, w_gate.N), out_dtype or torch.float32, x.device, stream)
     _check(lib().nxq_qmatmul_swiglu(w_gate.handle, w_up.handle, x.data_ptr(), _dtype_code(x.dtype), out.data_ptr(),
                                     _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -399,7 +420,7 @@ def qmatmul_residual(w: Weight, x, res, out=None, out_dtype=None, stream=None):
     M = x.numel() // w.K
     assert res.dtype == torch.float32 and res.is_contiguous() and res.numel() == M * w.N
     if out is None:
-        out = torch.empty((M, w.N), dtype=out_dtype or torch.float32, device=x.device)
+        out = _empty((M, w.N), out_dtype or torch.float32, x.device, stream)
     _check(lib().nxq_qmatmul_residual(w.handle, x.data_ptr(), _dtype_code(x.dtype), res.data_ptr(), out.data_ptr(),
                                       _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -416,7 +437,7 @@ def rmsnorm_qmatmul(ws, x, norm, eps: float, outs=None, out_dtype=None, stream=N
     assert norm.dtype == torch.float32 and norm.is_contiguous() and norm.numel() == K
     M = x.numel() // K
     if outs is None:
-        outs = [torch.empty((M, w.N), dtype=out_dtype or torch.float32, device=x.device) for w in ws]
+        outs = [_empty((M, w.N), out_dtype or torch.float32, x.device, stream) for w in ws]
     n = len(ws)
     arr = ctypes.c_void_p * n
     _check(lib().nxq_rmsnorm_qmatmul(arr(*[w.handle.value for w in ws]), n, x.data_ptr(), _dtype_code(x.dtype),
@@ -476,18 +497,20 @@ def _float_code(what: str, name: str, dtype) -> int:
     return code
 
 
-def _new(shape: tuple, dtype, device):
-    """An empty contiguous tensor (torch's quickest way to one)."""
+def _new(shape: tuple, dtype, device, stream):
+    """As _empty; on the current stream by torch's quickest way to one."""
+    if stream is not None:
+        return _empty(shape, dtype, device, stream)
     stride = (shape[1], 1) if len(shape) == 2 else (1,) if len(shape) == 1 else None
     if stride is None:
         return _torch.empty(shape, dtype=dtype, device=device)
     return _torch.empty_strided(shape, stride, dtype=dtype, device=device)
 
 
-def _output(what: str, out, shape: tuple, dtype, like):
+def _output(what: str, out, shape: tuple, dtype, like, stream):
     """`out` if given (checked), else a new tensor of `shape` beside `like`; and its type's code."""
     if out is None:
-        out = _new(shape, dtype or _torch.float32, like.device)
+        out = _new(shape, dtype or _torch.float32, like.device, stream)
     else:
         _usable(what, "out", out)
         if tuple(out.shape) != shape:
@@ -509,7 +532,7 @@ def embedding(w: Weight, ids, scale: float = 1.0, out=None, out_dtype=None, stre
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise _bad(f"embedding: ids are {ids.dtype}, not int32 or int64")
     d = _usable("embedding", "ids", ids)
-    out, code = _output("embedding", out, (*ids.shape, w.K), out_dtype, ids)
+    out, code = _output("embedding", out, (*ids.shape, w.K), out_dtype, ids, stream)
     _check(lib().nxq_embedding(w.handle, ids.data_ptr(), I64 if ids.dtype is torch.int64 else I32, ids.numel(), scale,
                                out.data_ptr(), code, _stream_on(stream, d)))
     return out
@@ -554,15 +577,15 @@ def moe_route(logits, k: int, normalize: bool = True, stream=None):
     if not 1 <= k <= min(E, 32):
         raise _bad(f"moe_route: k={k} of {E} experts (at most 32)")
     i32, device, choices = torch.int32, logits.device, (T, k)
-    ids, slots = _new(choices, i32, device), _new(choices, i32, device)
-    weights = _new(choices, torch.float32, device)
-    offsets, rows = _new((E + 1,), i32, device), _new((T * k,), i32, device)
+    ids, slots = _new(choices, i32, device, stream), _new(choices, i32, device, stream)
+    weights = _new(choices, torch.float32, device, stream)
+    offsets, rows = _new((E + 1,), i32, device, stream), _new((T * k,), i32, device, stream)
     _check(lib().nxq_moe_route(logits.data_ptr(), code, T, E, k, 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
                                offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_on(stream, d)))
     return ids, weights, offsets, rows, slots
 
 
-def _ragged(what: str, experts, x, offsets, rows, out, out_dtype):
+def _ragged(what: str, experts, x, offsets, rows, out, out_dtype, stream):
     """Checks a ragged product's arguments: (device, x's and out's type codes, X, rows pointer, R, out)."""
     torch = _torch or _load_torch()
     if x.dim() != 2 or x.shape[1] != experts.K:
@@ -579,7 +602,7 @@ def _ragged(what: str, experts, x, offsets, rows, out, out_dtype):
             raise _bad(f"{what}: rows must be one-dimensional torch.int32")
         _usable(what, "rows", rows)
         R, rp = rows.shape[0], rows.data_ptr()
-    out, ycode = _output(what, out, (R, experts.N), out_dtype, x)
+    out, ycode = _output(what, out, (R, experts.N), out_dtype, x, stream)
     return d, code, ycode, X, rp, R, out
 
 
@@ -587,7 +610,7 @@ def qmatmul_ragged(experts: Experts, x, offsets, rows=None, out=None, out_dtype=
     """y[s] = x[rows[s]] W_e^T for the slots offsets[e] <= s < offsets[e + 1] of
     every expert e (nxq_qmatmul_ragged); x[s] without rows.  Rows of `out` that
     no expert has are left as they are (undefined in a new tensor)."""
-    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged", experts, x, offsets, rows, out, out_dtype)
+    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged", experts, x, offsets, rows, out, out_dtype, stream)
     _check(lib().nxq_qmatmul_ragged(experts.handle, x.data_ptr(), xc, X, rp, out.data_ptr(), yc, R, offsets.data_ptr(),
                                     _stream_on(stream, d)))
     return out
@@ -595,7 +618,7 @@ def qmatmul_ragged(experts: Experts, x, offsets, rows=None, out=None, out_dtype=
 
 def qmatmul_ragged_swiglu(gate: Experts, up: Experts, x, offsets, rows=None, out=None, out_dtype=None, stream=None):
     """h[s] = silu(x Wg_e^T) * (x Wu_e^T) with x = x[rows[s]] (nxq_qmatmul_ragged_swiglu)."""
-    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged_swiglu", gate, x, offsets, rows, out, out_dtype)
+    d, xc, yc, X, rp, R, out = _ragged("qmatmul_ragged_swiglu", gate, x, offsets, rows, out, out_dtype, stream)
     _check(lib().nxq_qmatmul_ragged_swiglu(gate.handle, up.handle, x.data_ptr(), xc, X, rp, out.data_ptr(), yc, R,
                                            offsets.data_ptr(), _stream_on(stream, d)))
     return out
@@ -624,7 +647,7 @@ def moe_combine(h, slots, weights, res=None, out=None, out_dtype=None, stream=No
             raise _bad(f"{what}: res must be fp32 [{T}][{N}]")
         _usable(what, "res", res)
         rp = res.data_ptr()
-    out, ycode = _output(what, out, (T, N), out_dtype, h)
+    out, ycode = _output(what, out, (T, N), out_dtype, h, stream)
     _check(lib().nxq_moe_combine(h.data_ptr(), code, R, N, slots.data_ptr(), weights.data_ptr(), T, k, rp, out.data_ptr(),
                                  ycode, _stream_on(stream, d)))
     return out

@@ -7,7 +7,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_moe import DT, make_weights, products
+from nxq import synth
+from test_gpu_moe import DT, make_offsets, make_weights, products
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,75 @@ def test_most_slots(gpu):
                 assert lo == hi and abs(lo - want) <= bound + 2.0 ** -8 * (abs(want) + bound), (odd, e)
     finally:
         release([T], ws)
+
+
+def stream_calls(gpu):
+    """name -> call(stream) -> its new outputs; each large enough to take a freed tensor's place."""
+    N, K, T, E, k = 1024, 256, 640, 4, 2
+    w = gpu.Weight.register(synth.make_blocks(12, N, K, seed=1), 12, N, K)
+    ws, _ = make_weights(gpu, 12, E, N, K, 6)
+    X = gpu.Experts(ws)
+    x = torch.randn((T, K), device="cuda").half()
+    off = make_offsets([T // E] * E)
+    res = torch.randn((T, N), device="cuda")
+    h = torch.randn((T, N), device="cuda")
+    logits = torch.randn((70000, 64), device="cuda")
+    ids = torch.randint(0, N, (4096,), device="cuda")
+    slots = torch.zeros((T, k), dtype=torch.int32, device="cuda")
+    share = torch.ones((T, k), device="cuda")
+    norm = torch.ones(K, device="cuda")
+    calls = {
+        "embedding": lambda s: [gpu.embedding(w, ids, stream=s)],
+        "moe_route": lambda s: list(gpu.moe_route(logits, 8, stream=s)),
+        "qmatmul_ragged": lambda s: [gpu.qmatmul_ragged(X, x, off, stream=s)],
+        "qmatmul_ragged_swiglu": lambda s: [gpu.qmatmul_ragged_swiglu(X, X, x, off, stream=s)],
+        "moe_combine": lambda s: [gpu.moe_combine(h, slots, share, res=res, stream=s)],
+        "dequant": lambda s: [w.dequant(stream=s)],
+        "qmatmul": lambda s: [gpu.qmatmul(w, x, stream=s)],
+        "qmatmul_grouped": lambda s: gpu.qmatmul_grouped([w, w], [x, x], stream=s),
+        "qmatmul_swiglu": lambda s: [gpu.qmatmul_swiglu(w, w, x, stream=s)],
+        "qmatmul_residual": lambda s: [gpu.qmatmul_residual(w, x, res, stream=s)],
+        "rmsnorm_qmatmul": lambda s: gpu.rmsnorm_qmatmul([w, w], x, norm, 1e-5, stream=s),
+    }
+    return calls, [X], [w, *ws]
+
+
+@pytest.mark.parametrize("handle", [False, True], ids=["stream", "handle"])
+def test_outputs_on_another_stream(gpu, handle):
+    """A call on another stream writes no memory that the current stream still reads, and its outputs
+    outlive the work that the current stream does on them."""
+    calls, tables, weights = stream_calls(gpu)
+    side = torch.cuda.Stream()
+    s = side.cuda_stream if handle else side
+    try:
+        for name, call in calls.items():
+            want = call(None)
+            for _ in range(2):  # sizes the stream's scratch
+                call(s)
+            torch.cuda.synchronize()
+            old = [torch.full_like(o, 3) for o in want]
+            kept = [torch.empty_like(o) for o in want]
+            torch.cuda.synchronize()
+            torch.cuda._sleep(40_000_000)  # some 20 ms before the current stream reads them
+            for a, b in zip(kept, old):
+                a.copy_(b)
+            del old, b
+            got = call(s)
+            torch.cuda.current_stream().wait_stream(side)
+            copies = [torch.empty_like(o) for o in got]
+            torch.cuda._sleep(40_000_000)
+            for a, b in zip(copies, got):
+                a.copy_(b)
+            shapes = [(o.shape, o.dtype) for o in got]
+            del got, b
+            with torch.cuda.stream(side):
+                junk = [torch.full(shape, 5, dtype=dtype, device="cuda") for shape, dtype in shapes]
+            torch.cuda.synchronize()
+            for a, c, o in zip(kept, copies, want):
+                assert bool((a == 3).all()), f"{name}: wrote a tensor that was still read"
+                assert torch.equal(c, o), f"{name}: its outputs were reused while they were read"
+            del junk
+        gpu.stream_sync()
+    finally:
+        torch.cuda.synchronize()
+        release(tables, weights)
