@@ -107,8 +107,8 @@ __device__ __forceinline__ void decode16(const uint8_t* chunk, int r, int e0, fl
 // Items are (token, kEmbElems elements); every block holds a multiple of 32 elements.
 template <int TYPE>
 __global__ void __launch_bounds__(kEmbThreads) embedding_kernel(const uint8_t* __restrict__ tiled, TiledShape s,
-                                                                const void* __restrict__ ids, int ids_type, int64_t T,
-                                                                float scale, void* __restrict__ y, int y_dtype, int wide,
+                                                                const void* ids, int ids_type, int64_t T,
+                                                                float scale, void* y, int y_dtype, int wide,
                                                                 DeviceStatus* status) {
     overlap_begin();
     constexpr int kPerChunk = CHUNK_K / kEmbElems;

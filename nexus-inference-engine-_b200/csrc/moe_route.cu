@@ -503,9 +503,9 @@ __device__ __forceinline__ void store8(void* y, int dt, int64_t o, const float (
 // h and y 16-byte and an fp32 residual or output 32-byte aligned; VEC = 2 an
 // even N and h aligned to two values.  F32: h's type.
 template <int VEC, bool F32>
-__global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* __restrict__ h, int h_dtype, int64_t R, int64_t N,
-                                                               const int32_t* __restrict__ slots,
-                                                               const float* __restrict__ weights, int64_t T, int k,
+__global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* h, int h_dtype, int64_t R, int64_t N,
+                                                               const int32_t* slots,
+                                                               const float* weights, int64_t T, int k,
                                                                const float* res, void* y, int y_dtype, int64_t segs,
                                                                DeviceStatus* status) {
     overlap_begin();
@@ -592,9 +592,9 @@ constexpr int kBulkStage = 72 * 1024;  // bytes of a stage
 constexpr int kCombineBulk = 4;        // tokens per SM from which it is used
 
 template <bool F32>
-__global__ void __launch_bounds__(kBulkThreads, 1) combine_bulk_kernel(const void* __restrict__ h, int h_dtype, int64_t R,
-                                                                       int64_t N, const int32_t* __restrict__ slots,
-                                                                       const float* __restrict__ weights, int64_t T, int k,
+__global__ void __launch_bounds__(kBulkThreads, 1) combine_bulk_kernel(const void* h, int h_dtype, int64_t R,
+                                                                       int64_t N, const int32_t* slots,
+                                                                       const float* weights, int64_t T, int k,
                                                                        const float* res, void* y, int y_dtype, int64_t segs,
                                                                        int seg, DeviceStatus* status) {
     constexpr int kSize = F32 ? 4 : 2;

@@ -115,7 +115,10 @@ void experts_shutdown();
 #ifdef __CUDACC__
 // Launch with programmatic stream serialization: the kernel may start while the
 // one before it on the stream drains, and must run griddepcontrol.wait before
-// it touches memory.
+// it touches memory.  What that one may still be writing is not read-only for
+// the life of this kernel: no __ldg on it and no const __restrict__ pointer to it
+// (which allow loads by the non-coherent path, ahead of the wait).  Registered
+// weights are complete before any call can name them and may have both.
 template <typename... Params, typename... Args>
 cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
                               const Args&... args) {

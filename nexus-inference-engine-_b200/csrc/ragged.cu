@@ -241,15 +241,15 @@ __global__ void __launch_bounds__(kMaxExperts) ragged_prep_kernel(const PrepPara
             } else {
                 uint4 h = make_uint4(0u, 0u, 0u, 0u);
                 if (row >= 0 && p.x_dtype == NXQ_F16) {
-                    h = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + i));
+                    h = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.x) + i);
                 } else if (row >= 0) {
                     float v[8];
                     if (p.x_dtype == NXQ_F32) {
                         const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + i);
-                        const float4 a = __ldg(q), b = __ldg(q + 1);
+                        const float4 a = q[0], b = q[1];
                         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
                     } else {
-                        const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + i));
+                        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x) + i);
                         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
