@@ -295,6 +295,7 @@ NXQ_API int nxq_embedding(nxq_weight_t table, const void* ids_dev, int ids_type,
  *   nxq_qmatmul_ragged_swiglu  gate and up projections of the sorted rows
  *   nxq_qmatmul_ragged      down projection
  *   nxq_moe_combine         weighted sum per token, plus the residual
+ * Arrays must be aligned to their element type (NXQ_ERR_ARG otherwise).
  * A "slot" is one (token, expert) pair in sorted order.  Calls of one stream
  * run in order; calls on different streams share nothing and may overlap.
  * Their workspaces are stream-ordered allocations (cudaMallocAsync) of each

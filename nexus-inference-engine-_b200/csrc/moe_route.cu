@@ -717,6 +717,9 @@ NXQ_API int nxq_moe_route(const void* logits_dev, int dtype, int64_t T, int E, i
     if (!offsets_dev) return fail(NXQ_ERR_ARG, "route: null offsets");
     if (T > 0 && (!logits_dev || !ids_dev || !weights_dev || !rows_dev || !slots_dev))
         return fail(NXQ_ERR_ARG, "route: null array");
+    if (!aligned_as(logits_dev, dtype) || !aligned_4(ids_dev) || !aligned_4(weights_dev) || !aligned_4(offsets_dev) ||
+        !aligned_4(rows_dev) || !aligned_4(slots_dev))
+        return fail(NXQ_ERR_ARG, "route: an array is not aligned to its type");
     if (int rc = context_ready()) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     if (T == 0) {
@@ -751,6 +754,9 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
     if (!dtype_valid(h_dtype) || !dtype_valid(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
     if (T == 0 || N == 0) return NXQ_OK;
     if (!slots_dev || !weights_dev || !y_dev || (R > 0 && !h_dev)) return fail(NXQ_ERR_ARG, "combine: null array");
+    if (!aligned_as(h_dev, h_dtype) || !aligned_as(y_dev, y_dtype) || !aligned_4(slots_dev) || !aligned_4(weights_dev) ||
+        !aligned_4(res_dev))
+        return fail(NXQ_ERR_ARG, "combine: an array is not aligned to its type");
     if ((const void*)y_dev == (const void*)res_dev && y_dtype != NXQ_F32)
         return fail(NXQ_ERR_ARG, "combine: y may be the residual only as fp32");
     if (int rc = context_ready()) return rc;

@@ -154,6 +154,10 @@ __device__ __forceinline__ void load_f32x8(const float* p, float (&v)[8]) {
 #endif
 
 inline bool dtype_valid(int d) { return d == NXQ_F32 || d == NXQ_F16 || d == NXQ_BF16; }
+// Whether a device pointer (or null) lies on a multiple of its type's size: kernels
+// access elements whole, and an access across that boundary is a fault.
+inline bool aligned_as(const void* p, int dtype) { return (uintptr_t)p % (dtype == NXQ_F32 ? 4 : 2) == 0; }
+inline bool aligned_4(const void* p) { return (uintptr_t)p % 4 == 0; }
 
 // Process-wide count of kernels launched by the library (nxq_launch_count).
 void note_launches(unsigned n);

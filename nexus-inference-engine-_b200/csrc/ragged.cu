@@ -350,6 +350,8 @@ int run(nxq_experts_t he, nxq_experts_t hu, bool pair, const void* x_dev, int x_
     if (!dtype_valid(x_dtype) || !dtype_valid(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
     if (R == 0) return NXQ_OK;
     if (!x_dev || !y_dev || !offsets_dev) return fail(NXQ_ERR_ARG, "ragged: null activation, output or offsets");
+    if (!aligned_as(x_dev, x_dtype) || !aligned_as(y_dev, y_dtype) || !aligned_4(offsets_dev) || !aligned_4(rows_dev))
+        return fail(NXQ_ERR_ARG, "ragged: an array is not aligned to its type");
     if (!rows_dev && X < R)
         return fail(NXQ_ERR_SHAPE, "ragged: %lld activation rows for %lld slots (and no row indices)", (long long)X, (long long)R);
     if ((rc = context_ready())) return rc;

@@ -146,3 +146,27 @@ def test_outputs_on_another_stream(gpu, handle):
     finally:
         torch.cuda.synchronize()
         release(tables, weights)
+
+
+@pytest.mark.parametrize("pair", [False, True], ids=["plain", "swiglu"])
+def test_unaligned_arrays_are_refused(gpu, pair):
+    """Arrays off their element type's boundary never reach a kernel."""
+    ws, _ = make_weights(gpu, 12, 2, 128, 256, 5)
+    T = gpu.Experts(ws)
+    L, buf = gpu.lib(), torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    size = {gpu.F32: 4, gpu.F16: 2, gpu.BF16: 2}
+    try:
+        for xd in size:
+            for yd in size:
+                for bad, n in enumerate((size[xd], 4, size[yd], 4)):  # x, rows, y, offsets
+                    for by in range(1, n):
+                        x, rows, y, off = (buf.data_ptr() + 16384 * i + (by if i == bad else 0) for i in range(4))
+                        before = gpu.launch_count()
+                        if pair:
+                            rc = L.nxq_qmatmul_ragged_swiglu(T.handle, T.handle, x, xd, 4, rows, y, yd, 4, off, None)
+                        else:
+                            rc = L.nxq_qmatmul_ragged(T.handle, x, xd, 4, rows, y, yd, 4, off, None)
+                        assert rc == -1 and "aligned" in gpu.last_error() and gpu.launch_count() == before
+        gpu.stream_sync()
+    finally:
+        release([T], ws)
