@@ -250,12 +250,14 @@ int check_weight(nxq_weight_t h, Weight** out) {
     return NXQ_OK;
 }
 
-int weight_table_ref(nxq_weight_t h, int delta) {
+int weight_table_ref(nxq_weight_t h, int delta, Weight** out) {
     Weight* w = reinterpret_cast<Weight*>(h);
+    if (!w) return fail(NXQ_ERR_ARG, "null weight handle");
     std::lock_guard<std::mutex> lk(g_ctx.mu);
     if (!g_ctx.live.count(w) || w->magic != kWeightMagic)
         return fail(NXQ_ERR_ARG, "weight handle is not live (released or foreign)");
     w->tables += delta;
+    if (out) *out = w;
     return NXQ_OK;
 }
 

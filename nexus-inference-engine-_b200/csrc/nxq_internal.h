@@ -107,8 +107,9 @@ int context_sm_count();
 
 // NXQ_OK and the weight behind a live handle, else the status the C ABI returns.
 int check_weight(nxq_weight_t h, Weight** out);
-// Adds `delta` references of expert tables to the weight behind a live handle.
-int weight_table_ref(nxq_weight_t h, int delta);
+// Adds `delta` references of expert tables to the weight behind a live handle and
+// gives the weight: with a reference held, nxq_weight_release refuses it.
+int weight_table_ref(nxq_weight_t h, int delta, Weight** out = nullptr);
 // Releases every expert table (nxq_shutdown; the weights go after it).
 void experts_shutdown();
 

@@ -387,49 +387,49 @@ extern "C" {
 NXQ_API int nxq_experts_create(const nxq_weight_t* hs, int count, nxq_experts_t* out) {
     if (!hs || !out) return fail(NXQ_ERR_ARG, "null argument");
     if (count < 1 || count > kMaxExperts) return fail(NXQ_ERR_ARG, "%d experts (1 to %d)", count, kMaxExperts);
+    // The references come first: another thread may release a weight until it has one.
     const uint8_t* dev[kMaxExperts];
     TiledShape shape{};
+    int held = 0;
+    auto give_back = [&](int status) {
+        for (int i = 0; i < held; ++i) weight_table_ref(hs[i], -1);
+        return status;
+    };
     for (int i = 0; i < count; ++i) {
         Weight* w = nullptr;
-        if (int rc = check_weight(hs[i], &w)) return rc;
+        if (int rc = weight_table_ref(hs[i], 1, &w)) return give_back(rc);
+        ++held;
         if (i == 0) shape = w->shape;
         if (w->shape.type != shape.type || w->shape.N != shape.N || w->shape.K != shape.K)
-            return fail(NXQ_ERR_SHAPE, "expert %d is %s [%lld][%lld], expert 0 %s [%lld][%lld]", i, type_name(w->shape.type),
-                        (long long)w->shape.N, (long long)w->shape.K, type_name(shape.type), (long long)shape.N,
-                        (long long)shape.K);
+            return give_back(fail(NXQ_ERR_SHAPE, "expert %d is %s [%lld][%lld], expert 0 %s [%lld][%lld]", i,
+                                  type_name(w->shape.type), (long long)w->shape.N, (long long)w->shape.K,
+                                  type_name(shape.type), (long long)shape.N, (long long)shape.K));
         dev[i] = w->dev;
     }
-    if (int rc = context_ready()) return rc;
+    if (int rc = context_ready()) return give_back(rc);
     ExpertTable* t = new (std::nothrow) ExpertTable();
-    if (!t) return fail(NXQ_ERR_NOMEM, "host allocation failed");
+    if (!t) return give_back(fail(NXQ_ERR_NOMEM, "host allocation failed"));
     t->count = count;
     t->shape = shape;
-    try {
-        t->refs.assign(hs, hs + count);
-        std::lock_guard<std::mutex> lk(g_tables_mu);
-        g_tables.insert(t);
-    } catch (const std::bad_alloc&) {
-        delete t;
-        return fail(NXQ_ERR_NOMEM, "host allocation failed");
-    }
-    int held = 0, rc = NXQ_OK;
-    for (; held < count && rc == NXQ_OK; ++held) rc = weight_table_ref(hs[held], 1);
-    if (rc != NXQ_OK) --held;
-    cudaError_t e = cudaSuccess;
     const size_t bytes = (size_t)count * sizeof(dev[0]);
     // The copy is waited for: streams that do not synchronize with the default one read the table.
-    if (rc == NXQ_OK && (e = cudaMalloc((void**)&t->dev, bytes)) == cudaSuccess &&
-        (e = cudaMemcpy(t->dev, dev, bytes, cudaMemcpyHostToDevice)) == cudaSuccess)
+    cudaError_t e = cudaMalloc((void**)&t->dev, bytes);
+    if (e == cudaSuccess && (e = cudaMemcpy(t->dev, dev, bytes, cudaMemcpyHostToDevice)) == cudaSuccess)
         e = cudaStreamSynchronize(cudaStreamLegacy);
-    if (rc != NXQ_OK || e != cudaSuccess) {
-        for (int i = 0; i < held; ++i) weight_table_ref(hs[i], -1);
-        if (t->dev) cudaFree(t->dev);
-        {
+    int rc = e == cudaSuccess ? NXQ_OK : cuda_fail(e, "expert table");
+    if (rc == NXQ_OK) {
+        try {
+            t->refs.assign(hs, hs + count);
             std::lock_guard<std::mutex> lk(g_tables_mu);
-            g_tables.erase(t);
+            g_tables.insert(t);
+        } catch (const std::bad_alloc&) {
+            rc = fail(NXQ_ERR_NOMEM, "host allocation failed");
         }
+    }
+    if (rc != NXQ_OK) {
+        if (t->dev) cudaFree(t->dev);
         delete t;
-        return rc != NXQ_OK ? rc : cuda_fail(e, "expert table");
+        return give_back(rc);
     }
     *out = reinterpret_cast<nxq_experts_t>(t);
     return NXQ_OK;

@@ -170,3 +170,64 @@ def test_unaligned_arrays_are_refused(gpu, pair):
         gpu.stream_sync()
     finally:
         release([T], ws)
+
+
+def test_tables_while_weights_are_released(gpu):
+    """A table holds the weights it was made from, whatever another thread releases meanwhile."""
+    import threading
+    import time
+
+    t, N, K, E = 12, 128, 256, 64
+    blocks = synth.make_blocks(t, N, K, seed=1)
+    ws = [gpu.Weight.register(blocks, t, N, K) for _ in range(E)]
+    x = torch.randn((E, K), device="cuda").half()
+    off = make_offsets([1] * E)
+    W = ws[0].dequant().double()
+    want = (x.double() @ W.T).float()
+    rng = synth.rng(8)
+    bad, counts = [], {"made": 0, "gone": 0, "kept": 0}
+    stop = threading.Event()
+
+    def renew():
+        try:
+            while not stop.is_set():
+                for i in (E - 1, E // 2):
+                    try:
+                        ws[i].release()
+                    except gpu.NxqError as e:
+                        if e.name != "ERR_STATE":
+                            bad.append(repr(e))
+                        counts["kept"] += 1
+                        time.sleep(1e-4)
+                        continue
+                    ws[i] = gpu.Weight.register(blocks, t, N, K)
+                    time.sleep(2e-3 * rng.random())  # a while in which tables can be made
+        except Exception as e:  # noqa: BLE001
+            bad.append(repr(e))
+
+    thread = threading.Thread(target=renew)
+    thread.start()
+    try:
+        end = time.time() + 3
+        while time.time() < end and not bad:
+            try:
+                T = gpu.Experts(ws)
+            except gpu.NxqError as e:  # a weight was gone
+                if e.code != -1:
+                    bad.append(repr(e))
+                counts["gone"] += 1
+                time.sleep(1e-4)
+                continue
+            counts["made"] += 1
+            y = gpu.qmatmul_ragged(T, x, off)
+            if not ((y - want).norm() <= 2e-3 * want.norm()).item():
+                bad.append("wrong product")
+            T.release()
+        gpu.stream_sync()
+    finally:
+        stop.set()
+        thread.join()
+    assert not bad, bad[:3]
+    assert counts["made"] > 0, counts
+    for w in ws:
+        w.release()  # no reference was left behind
