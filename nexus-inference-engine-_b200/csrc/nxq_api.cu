@@ -547,6 +547,8 @@ NXQ_API int nxq_weight_release(nxq_weight_t h) {
     rc = check_ready();
     if (rc) return rc;
     std::lock_guard<std::mutex> lk(g_ctx.mu);
+    // Another thread may have released it since.
+    if (!g_ctx.live.count(w)) return fail(NXQ_ERR_ARG, "weight handle is not live (released or foreign)");
     if (w->tables)
         return fail(NXQ_ERR_STATE, "the weight belongs to %d live expert table(s): release them first", w->tables);
     g_ctx.live.erase(w);

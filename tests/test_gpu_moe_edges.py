@@ -231,3 +231,25 @@ def test_tables_while_weights_are_released(gpu):
     assert counts["made"] > 0, counts
     for w in ws:
         w.release()  # no reference was left behind
+
+
+def test_weight_released_from_two_threads(gpu):
+    """Of several threads that release a weight at once, one does and the others are told."""
+    import threading
+
+    blocks = synth.make_blocks(12, 128, 256, seed=1)
+    threads = 4
+    barrier = threading.Barrier(threads)
+    for _ in range(100):
+        w = gpu.Weight.register(blocks, 12, 128, 256)
+        rcs = []
+
+        def release_it(h=w.handle):
+            barrier.wait()
+            rcs.append(gpu.lib().nxq_weight_release(h))
+
+        ts = [threading.Thread(target=release_it) for _ in range(threads)]
+        [t.start() for t in ts]
+        [t.join() for t in ts]
+        assert sorted(rcs) == [-1] * (threads - 1) + [0]
+        w._h = None
