@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from nxq import synth
-from test_gpu_moe import DT, make_offsets, make_weights, products
+from test_gpu_moe import DT, EXACT, TYPE_NAMES, check, make_offsets, make_weights, products, swiglu
 
 pytestmark = pytest.mark.gpu
 
@@ -253,3 +253,54 @@ def test_weight_released_from_two_threads(gpu):
         [t.join() for t in ts]
         assert sorted(rcs) == [-1] * (threads - 1) + [0]
         w._h = None
+
+
+MANY = {"tcgen05": [16, 3, 131, 0, 40, 17, 1, 64] * 4, "warp": [3, 0, 5, 1, 8, 9, 2, 4] * 4}
+TENSOR_TYPES = {n: t for n, t in TYPE_NAMES.items() if t not in EXACT}
+
+
+@pytest.mark.parametrize("ydt", ["f32", "bf16"])
+@pytest.mark.parametrize("pair", [False, True], ids=["plain", "swiglu"])
+@pytest.mark.parametrize("kernel", MANY.keys())
+@pytest.mark.parametrize("t", TENSOR_TYPES.values(), ids=TENSOR_TYPES.keys())
+def test_many_work_tiles(gpu, t, kernel, pair, ydt):
+    """Every CTA walks several work tiles: what its rings, accumulators and staging carry from one to the
+    next (an odd number of chunks and of weight tiles, row blocks of every size) gives the right product, and
+    the same bits on every call."""
+    counts, N, K, distinct = MANY[kernel], 3900, 1280, 4
+    E, n = len(counts), sum(counts)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    weight_tiles = -(-N // 128)
+    per_block, blk = ((weight_tiles if pair else -(-weight_tiles // 2)), 128) if kernel == "tcgen05" else (weight_tiles, 8)
+    assert (n > 6 * E) == (kernel == "tcgen05")  # the kernel that such a call takes
+    assert sum(-(-c // blk) for c in counts) * per_block >= 3 * sms
+    tables, weights, W = [], [], []
+    try:
+        for seed in ((10, 50) if pair else (10,)):
+            ws, dec = make_weights(gpu, t, distinct, N, K, seed)
+            weights += ws
+            W.append(dec[torch.arange(E) % distinct])
+            tables.append(gpu.Experts([ws[e % distinct] for e in range(E)]))
+        g = torch.Generator(device="cuda").manual_seed(t)
+        off = make_offsets(counts)
+        if pair:  # gathered rows; small ones keep the gate's sigmoid away from 0 and 1
+            x = (0.05 * torch.randn((n // 2, K), device="cuda", generator=g)).bfloat16()
+            rows = torch.randint(0, n // 2, (n,), device="cuda", generator=g, dtype=torch.int32)
+            src = rows.long()
+        else:
+            x, rows, src = torch.randn((n, K), device="cuda", generator=g).half(), None, torch.arange(n, device="cuda")
+
+        def call():
+            f = gpu.qmatmul_ragged_swiglu if pair else gpu.qmatmul_ragged
+            return f(*tables, x, off, rows=rows, out_dtype=DT[ydt])
+
+        first = call()
+        y, b = products(W[0], t, x, counts, src)
+        if pair:
+            y, b = swiglu(y, b, *products(W[1], t, x, counts, src))
+        check(first, y, b)
+        again = [call() for _ in range(12)]
+        gpu.stream_sync()
+        assert all(torch.equal(a, first) for a in again)
+    finally:
+        release(tables, weights)
