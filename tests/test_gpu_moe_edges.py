@@ -4,6 +4,7 @@ Bounds as in test_gpu_moe.py, whose helpers are used here.
 """
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -304,3 +305,49 @@ def test_many_work_tiles(gpu, t, kernel, pair, ydt):
         assert all(torch.equal(a, first) for a in again)
     finally:
         release(tables, weights)
+
+
+GATES = [0.0, -0.0, 1e-3, -1e-3, 1.0, -1.0, 60.0, -60.0, 88.0, -86.5, -87.25, -87.5, -88.0, -88.5, -88.6875, -89.0,
+         -100.0, -120.0, 1000.0, -1000.0]
+
+
+@pytest.mark.parametrize("u", [1.0, -3.0, 96.0])
+@pytest.mark.parametrize("kernel", KERNELS.keys())
+def test_swiglu_of_far_gates(gpu, kernel, u):
+    """silu over the whole range of its exponential, in every product kernel.
+
+    Weights are 0 and 1, so the gate and up values are the activations, exactly.  In half steps of fp32
+    (2^-24): expf is within 2 units in the last place (4), the sum within half of one (1), the quotient within 2
+    in the tcgen05 kernel's fast division (4), the product within half of one (1).  Where exp(-g) passes the
+    fp32 range the quotient is 0: off by at most |g| 2^-128.
+    """
+    N, K = 128, 32
+    def blocks(k):  # w[n][k] = 1, all else 0
+        if kernel == "exact":
+            b = np.zeros((N, 1, K), np.float16)
+            b[:, :, k] = 1
+            return b.view(np.uint8)
+        b = np.zeros((N, 1, 18), np.uint8)  # Q4_0: a half scale, then 16 bytes of codes, (code - 8) * scale
+        b[:, :, :2] = np.array([1], np.float16).view(np.uint8)
+        b[:, :, 2:] = 0x88
+        b[:, :, 2 + k] = 0x89
+        return b
+
+    t = 121 if kernel == "exact" else 2
+    per = 4 if kernel == "warp" else len(GATES)  # slots per expert
+    E = len(GATES) // per
+    gate, up = (gpu.Weight.register(blocks(k), t, N, K) for k in (0, 1))
+    G, Up = gpu.Experts([gate] * E), gpu.Experts([up] * E)
+    try:
+        x = torch.zeros((len(GATES), K), device="cuda", dtype=torch.float16)
+        x[:, 0], x[:, 1] = torch.tensor(GATES), u
+        got = gpu.qmatmul_ragged_swiglu(G, Up, x, make_offsets([per] * E)).double()
+        gpu.stream_sync()
+        g = x[:, :1].double()
+        want = g / (1 + torch.exp(-g)) * u
+        lost = torch.where(g < -88.7, g.abs() * abs(u) * 2.0 ** -128, 0.0)
+        err = (got - want).abs()
+        bad = (err > 10 * 2.0 ** -24 * want.abs() + lost).any(1)
+        assert not bool(bad.any()), [(a.item(), b[0].item()) for a, b in zip(g[bad][:, 0], got[bad])]
+    finally:
+        release([G, Up], [gate, up])
