@@ -589,7 +589,20 @@ __global__ void __launch_bounds__(kCombThreads) combine_kernel(const void* h, in
 constexpr int kBulkWarps = 16, kBulkThreads = 32 * (kBulkWarps + 1);
 constexpr int kBulkStages = 3;
 constexpr int kBulkStage = 72 * 1024;  // bytes of a stage
-constexpr int kCombineBulk = 4;        // tokens per SM from which it is used
+
+// A CTA needs 0.9 us and 0.06 us a row for a token however short the rows are,
+// where combine_kernel's time goes by the bytes.  So: from 4 tokens per SM, and
+// from 6 KB + 2.25 KB a row of h per token.  Measured, combine_kernel / this one
+// in us, fp32 residual and output:
+//   4000 tokens, bf16:  k = 2, N = 2048 (8 KB): 39 / 29;    k = 8, N = 1024 (16 KB): 27 / 36
+//     k = 8, N = 1536 (24 KB): 38 / 38;  N = 2048 (32 KB): 49 / 40;  N = 4096: 90 / 61
+//     k = 16, N = 1024 (32 KB): 42 / 53;  N = 1536 (48 KB): 61 / 56
+//     k = 32, N = 512 (32 KB): 38 / 88;  N = 1024 (64 KB): 71 / 88
+//   8192 tokens, bf16, k = 8:  N = 64: 10.5 / 66;  N = 1024: 50 / 70;  N = 2048: 92 / 79;  N = 4096: 176 / 121
+//   600 tokens, bf16, k = 8:  N = 512: 3.1 / 7.5;  N = 2048: 9.3 / 8.7;  N = 4096: 15.7 / 12.6
+inline bool combine_by_bulk(int64_t T, int k, int64_t row_bytes, int sms) {
+    return T >= 4 * (int64_t)sms && row_bytes >= 2304 + 6144 / k;
+}
 
 template <bool F32>
 __global__ void __launch_bounds__(kBulkThreads, 1) combine_bulk_kernel(const void* h, int h_dtype, int64_t R,
@@ -763,8 +776,7 @@ NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N
     const bool vec = N % 8 == 0 && (uintptr_t)h_dev % 16 == 0 && (uintptr_t)res_dev % 32 == 0 &&
                      (uintptr_t)y_dev % (y_dtype == NXQ_F32 ? 32 : 16) == 0;
     const bool f32 = h_dtype == NXQ_F32;
-    // Many tokens: bulk copies (kCombineBulk).
-    if (vec && T >= kCombineBulk * (int64_t)context_sm_count() && T <= ((int64_t)1 << 62) / N) {
+    if (vec && combine_by_bulk(T, k, N * (f32 ? 4 : 2), context_sm_count()) && T <= ((int64_t)1 << 62) / N) {
         int64_t seg = kBulkStage / (k * (f32 ? 4 : 2)) / 64 * 64;  // columns of a stage
         int64_t segs = (N + seg - 1) / seg;
         seg = ((N + segs - 1) / segs + 63) / 64 * 64;

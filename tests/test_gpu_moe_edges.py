@@ -351,3 +351,22 @@ def test_swiglu_of_far_gates(gpu, kernel, u):
         assert not bool(bad.any()), [(a.item(), b[0].item()) for a, b in zip(g[bad][:, 0], got[bad])]
     finally:
         release([G, Up], [gate, up])
+
+
+@pytest.mark.parametrize("hdt", DT.keys())
+@pytest.mark.parametrize("k,N", [(1, 64), (1, 4096), (2, 1536), (2, 2560), (8, 64), (8, 1024), (8, 1536), (8, 1544),
+                                 (8, 2048), (16, 1344), (16, 1352), (32, 128), (32, 1248)])
+def test_combine_of_many_tokens(gpu, k, N, hdt):
+    """Rows on both sides of the size from which many tokens are combined by bulk copies."""
+    T = 5 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    g = torch.Generator(device="cuda").manual_seed(N + k)
+    h = torch.randn((T * k, N), device="cuda", generator=g).to(DT[hdt])
+    slots = torch.randperm(T * k, device="cuda", generator=g).to(torch.int32).view(T, k)
+    w = torch.rand((T, k), device="cuda", generator=g)
+    slots[torch.rand((T, k), device="cuda", generator=g) < 0.2] = -1
+    res = torch.randn((T, N), device="cuda", generator=g)
+    parts = h[slots.clamp(min=0).long()].double() * (w * (slots >= 0)).double()[:, :, None]
+    bound = (k + 2) * 2.0 ** -24 * (parts.abs().sum(1) + res.double().abs())
+    for dt in DT.values():
+        check(gpu.moe_combine(h, slots, w, res=res, out_dtype=dt), parts.sum(1) + res.double(), bound)
+    gpu.stream_sync()
