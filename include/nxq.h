@@ -68,7 +68,12 @@ typedef enum {
  * keeps them in fp32).  A finite activation of magnitude >= 65520 has no f16
  * value; the kernel that rounds it records NXQ_ERR_RANGE in the context's
  * status word, which the next nxq_stream_sync (or the synchronous
- * nxq_qmatmul_host) returns, and that call's outputs are not finite.  The
+ * nxq_qmatmul_host) returns, and that call's outputs are not finite.  Small
+ * values are not reported: a rounding is within 2^-11 of the value down to
+ * 2^-14 in magnitude and within 2^-25 absolutely below it, so that values up to
+ * 2^-25 become zero.  Decoded weights are rounded to f16 too (once, from fp32
+ * scales and offsets rounded to f16).  All of this holds for the ragged expert
+ * products as well.  The
  * CUDA-core kernel (NXQ_DECODE_KERNEL=simt / NXQ_PREFILL_KERNEL=simt, and
  * nxq_qmatmul_noalloc) computes in fp32 and has no such limit. */
 

@@ -370,3 +370,27 @@ def test_combine_of_many_tokens(gpu, k, N, hdt):
     for dt in DT.values():
         check(gpu.moe_combine(h, slots, w, res=res, out_dtype=dt), parts.sum(1) + res.double(), bound)
     gpu.stream_sync()
+
+
+@pytest.mark.parametrize("power", [-12, -16, -20, -24])
+@pytest.mark.parametrize("xdt", DT.keys())
+@pytest.mark.parametrize("kernel", KERNELS.keys())
+def test_small_activations(gpu, kernel, xdt, power):
+    """fp32 and bf16 activations below 2^-14 are rounded to multiples of 2^-24 where products run in f16: each
+    is off by at most 2^-25 (and by 2^-11 of itself above), which the weights carry into the sum.  f16
+    activations, and the exact kernel, lose nothing."""
+    t, m = KERNELS[kernel]
+    E, N, K = 3, 128, 256
+    ws, W = make_weights(gpu, t, E, N, K, 6)
+    T = gpu.Experts(ws)
+    try:
+        x = (2.0 ** power * torch.randn((E * m, K), device="cuda")).to(DT[xdt])
+        y, b = products(W, t, x, [m] * E, torch.arange(E * m, device="cuda"))
+        if xdt != "f16" and t not in EXACT:
+            b = b + 2.0 ** -25 * 1.01 * W.abs().sum(2).repeat_interleave(m, 0)
+        got = gpu.qmatmul_ragged(T, x, make_offsets([m] * E)).double()
+        gpu.stream_sync()
+        # Sums of f16 products are multiples of 2^-48, far above the smallest fp32.
+        assert bool(((got - y).abs() <= b + 2.0 ** -24 * (y.abs() + b)).all())
+    finally:
+        release([T], ws)
