@@ -8,7 +8,8 @@
 // One thread decodes 16 consecutive elements, which share one scale in every
 // format, from whole code words (decode16), and stores them in accesses of 32
 // or 16 bytes.  (Two decode8 calls instead, with their byte-wise addressing,
-// took 430 instructions and 39 us for 8192 rows of 4096; now 30.5 us for 153 MB.)
+// took 430 instructions and 39 us for 8192 rows of 4096; now 30.5 us for 153 MB.
+// Q2_K, Q3_K and the NXF chunk types still take decode8.)
 // A resident grid walks all (token, 16 elements) items; the id of the item after
 // next and the record of the next are on their way to the L2 cache meanwhile,
 // since a row's records lie 256 elements x 128 rows apart and each is a short

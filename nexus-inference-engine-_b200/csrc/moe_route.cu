@@ -30,6 +30,8 @@ constexpr int kRankWarps = 8;        // contiguous runs a block's choices are ra
 constexpr int kThreads = 32 * kRankWarps;
 constexpr int kSmallThreads = 1024;
 constexpr int kChooseThreads = 512;
+// One CTA up to here: 2.6 us for 1 token, 6.2 for 32, 14.9 for 128 (256 experts, k = 8,
+// in a graph), where the three kernels take 14.7.
 constexpr int kSmallT = 128;
 constexpr int kMaxBlocks = 256;      // of tokens
 constexpr float kInf = __builtin_huge_valf();

@@ -28,14 +28,15 @@
 // cycles each, two issuing warps): an issuing warp needs some 600 cycles from
 // one k-step to the next whatever N is, with its operands there 94 % of the time
 // when a k-step had 64 elements.  So a k-step has 128, with one handshake for
-// each warpgroup (32768 slots of 64 experts: 567 to 553 us; gate and up of
-// 2048x4096: 1165 to 1120); the issuing loops run warp-wide, half the lanes
+// each warpgroup (1 to 4 % in one run; 32768 slots of 64 experts, Q4_K 4096x2048,
+// now take 545 to 585 us under the power cap); the issuing loops run warp-wide, half the lanes
 // watching the activations and half the A operand, with only the MMA and the
 // commits in the elected lane.  Loops are kept short rather than unrolled over
 // a chunk: four copies of the decode and of the issue were 12 % slower for few
 // slots (1024 slots of 64 experts, Q4_K 4096x2048: 117 us against 104, and 93
-// with the slow path of the waits out of line).  There the bytes are worth 48 us,
-// and the decode's instructions are what is left.  Blocks of 64 slots, which
+// with the slow path of the waits out of line; 91 today, with f16 activations
+// and three input sets in turn).  There the bytes are worth 48 us, and neither
+// DRAM nor a pipe is full: 2.6 instructions per cycle, the ALU pipe at 55 %.  Blocks of 64 slots, which
 // leave TMEM for more A stages, gained 2 to 9 % up to 12 slots per expert and
 // lost from 16 on.
 //
@@ -84,6 +85,10 @@ constexpr int kStageOut = NT * TILE_ROWS * 2;  // 32 KB: one tile's 16-bit outpu
 // in the ring, so each tile keeps its own stages.  With an odd number a stage
 // would change hands, and a warpgroup that waits for a phase of its own could
 // take the phase before the other tile's for it - copies land in any order.
+// Every type has two or three stages per tile but Q8_0 (and NXF INT8), whose
+// chunks of 34 KB leave room for one: the next copy starts when the chunk before
+// is decoded (64 experts x 16 slots, 4096x2048: 132 us, 67 % of the copy rate; Q4_K
+// 91 us, 53 %).
 template <int TYPE>
 struct Rings {
     static constexpr int WB = lane::Lane<TYPE>::kStage;
@@ -483,6 +488,8 @@ __global__ void __launch_bounds__(kThreads, 1) ragged_gemm_kernel(const Params p
                 for (int j = 0; j < 8; ++j) q[j] = pack16(bf, v[2 * j], v[2 * j + 1]);
                 put16(c, q);
             }
+            // (`hold` is what the plain kernels spill 116 to 128 bytes for, at the 72
+            // registers that 896 threads leave; the SwiGLU ones spill none.)
             uint32_t hold[PAIR ? 1 : kHalf / 16][8];
             if constexpr (!PAIR) {
 #pragma unroll

@@ -23,8 +23,10 @@
 // .. b1, which reach it at the start of theirs, store their fp32 partials in the
 // call's workspace and count themselves in on b0's counter; b0 waits (bounded)
 // and adds the partials in worker order, so the sum does not depend on timing.
-// Every CTA of the launch is resident and a worker publishes without waiting, so
-// the waits end.
+// A worker publishes before any wait of its own and waits for later workers only,
+// so the waits end in whatever order the CTAs get their SMs.  The bound (2 s by
+// default) does count the time in which a later CTA has no SM: beside a kernel of
+// another stream that holds SMs for longer, the call ends with NXQ_ERR_TIMEOUT.
 //
 // Row blocks have up to 8 slots, the columns of one MMA.  Slots behind a block's
 // end hold stale activations of the stage's earlier units: an MMA column
@@ -394,7 +396,11 @@ int ragged_mma_init() {
 // have any, on average.  Measured (64 experts, routed with a bias, Q4_K
 // 4096x2048, 2 / 4 / 6 / 8 slots on average): 67 / 80 / 94 / 112 us here, 91 to 94 us
 // with the tcgen05 kernel; Q4_0 14336x4096 gate and up, 8 experts, 4 / 8 slots:
-// 120 / 175 against 155 to 161; Q3_K, 4 / 8 slots: 53 / 66 against 62.
+// 120 / 175 against 155 to 161; Q3_K, 4 / 8 slots: 53 / 66 against 62.  Other types
+// at 4096x2048, 64 experts, 2 / 4 / 6 / 8 slots, here and there: Q8_0 86 / 112 / 132 /
+// 157 and 101 / 123 / 130 / 130; Q6_K 72 / 90 / 102 / 123 and 90 / 104 / 105 / 106; Q5_K
+// 77 / 95 / 116 / 134 and 83 / 101 / 102 / 102.  One limit for all costs 14 % at worst
+// (Q5_K at 6 slots).
 int ragged_mma_blk(const RaggedCall& c) {
     const TiledShape& s = c.w->shape;
     if (!mma_supported(s, 1)) return 0;
