@@ -4,9 +4,15 @@ Bounds as in test_gpu_moe.py, whose helpers are used here.
 """
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
+
+from conftest import PKG, ROOT
 
 from nxq import synth
 from test_gpu_moe import DT, EXACT, TYPE_NAMES, check, make_offsets, make_weights, products, swiglu
@@ -394,3 +400,42 @@ def test_small_activations(gpu, kernel, xdt, power):
         assert bool(((got - y).abs() <= b + 2.0 ** -24 * (y.abs() + b)).all())
     finally:
         release([T], ws)
+
+
+CHOICE = """
+import sys, torch
+sys.path[:0] = [{tests!r}, {pkg!r}, {root!r}]
+import nxq
+from test_gpu_moe import make_offsets, make_weights, products, swiglu
+nxq.init(0)
+decode, prefill = {decode}, {prefill}  # whether each is the exact kernel
+for counts in ([2, 0, 3, 1], [40, 3, 0, 130]):
+    n = sum(counts)
+    exact = decode and prefill
+    ws, W = make_weights(nxq, 12, 4, 200, 512, 6)
+    T = nxq.Experts(ws)
+    x = 0.05 * torch.randn((n, 512), device="cuda")
+    x[0, 0] = 1e-9  # zero in f16
+    x[n - 1, 1] = 1e5 if exact else 1.0  # beyond f16
+    off = make_offsets(counts)
+    got, pair = nxq.qmatmul_ragged(T, x, off), nxq.qmatmul_ragged_swiglu(T, T, x, off)
+    nxq.stream_sync()
+    y, b = products(W, 121 if exact else 12, x, counts, torch.arange(n, device="cuda"))
+    if not exact:
+        b = b + 2.0 ** -25 * 1.01 * W.abs().sum(2).max()
+    assert bool(((got.double() - y).abs() <= b + 2.0 ** -24 * y.abs()).all()), counts
+    h, hb = swiglu(y, b, y, b)
+    assert bool(((pair.double() - h).abs() <= hb + 2.0 ** -24 * h.abs()).all()), counts
+"""
+
+
+@pytest.mark.parametrize("decode", [False, True], ids=["", "decode-simt"])
+@pytest.mark.parametrize("prefill", [False, True], ids=["", "prefill-simt"])
+def test_kernel_choice_by_environment(gpu, decode, prefill):
+    """NXQ_DECODE_KERNEL / NXQ_PREFILL_KERNEL = simt: with both, the exact kernel takes every call and f16's
+    range does not apply; with one, the other tensor-core kernel takes the calls or the exact one does."""
+    env = {k: v for k, v in os.environ.items() if k not in ("NXQ_DECODE_KERNEL", "NXQ_PREFILL_KERNEL")}
+    env.update({"NXQ_DECODE_KERNEL": "simt"} if decode else {}, **({"NXQ_PREFILL_KERNEL": "simt"} if prefill else {}))
+    code = CHOICE.format(tests=str(ROOT / "tests"), pkg=str(PKG), root=str(ROOT), decode=decode, prefill=prefill)
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
