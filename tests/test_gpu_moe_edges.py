@@ -81,6 +81,28 @@ def test_most_slots(gpu):
                 assert lo == hi and abs(lo - want) <= bound + 2.0 ** -8 * (abs(want) + bound), (odd, e)
     finally:
         release([T], ws)
+        del rows, out, got
+        torch.cuda.empty_cache()
+
+
+def test_most_tokens(gpu):
+    """2^31 - 1 choices: token t takes expert t % 2."""
+    T, step = 2**31 - 1, 2**28
+    logits = torch.zeros((T, 2), dtype=torch.bfloat16, device="cuda")
+    logits[1::2, 1] = 1
+    ids, w, offsets, rows, slots = gpu.moe_route(logits, 1)
+    gpu.stream_sync()
+    del logits
+    even = (T + 1) // 2
+    assert offsets.tolist() == [0, even, T]
+    for a in range(0, T, step):
+        z = min(a + step, T)
+        t = torch.arange(a, z, device="cuda")  # as a token, then as a slot
+        assert torch.equal(ids[a:z, 0], (t % 2).int()) and bool((w[a:z] == 1).all())
+        assert torch.equal(slots[a:z, 0], (t // 2 + (t % 2) * even).int())
+        assert torch.equal(rows[a:z], torch.where(t < even, 2 * t, 2 * (t - even) + 1).int())
+    del ids, w, rows, slots, t
+    torch.cuda.empty_cache()
 
 
 def stream_calls(gpu):
