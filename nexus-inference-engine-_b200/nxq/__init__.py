@@ -235,26 +235,34 @@ def _stream_ptr(stream) -> ctypes.c_void_p:
     return ctypes.c_void_p(stream.cuda_stream)
 
 
-def _empty(shape, dtype, device, stream):
-    """An empty tensor that a call on `stream` (None: the current one) will write.
-    On another stream than the current one it is allocated there, or it could be
-    memory that work queued on the current stream still reads; and it is not
-    reused before the work that the current stream has queued when it is freed."""
-    import torch
-
-    if stream is not None:
-        device = torch.device(device)
-        if device.index is None:
-            device = torch.device(device.type, torch.cuda.current_device())
+def _empty(specs, device, stream) -> list:
+    """Empty tensors, a (shape, dtype) each, that a call on `stream` (None: the
+    current one) will write.  On another stream than the current one they are
+    allocated there, or they could be memory that work queued on the current stream
+    still reads; and they are not reused before the work that the current stream has
+    queued when they are freed."""
+    torch = _torch or _load_torch()
+    if stream is not None and not _is_current(stream, device):
         here = torch.cuda.current_stream(device)
-        ptr = _stream_ptr(stream).value or 0
-        if ptr != here.cuda_stream:
+        there = stream
+        if not isinstance(stream, torch.cuda.Stream):
+            ptr = stream if isinstance(stream, int) else stream.cuda_stream
             there = torch.cuda.ExternalStream(ptr, device=device) if ptr else torch.cuda.default_stream(device)
-            with torch.cuda.stream(there):
-                t = torch.empty(shape, dtype=dtype, device=device)
+        with torch.cuda.stream(there):
+            new = [torch.empty(shape, dtype=dtype, device=device) for shape, dtype in specs]
+        for t in new:
             t.record_stream(here)
-            return t
-    return torch.empty(shape, dtype=dtype, device=device)
+        return new
+    return [torch.empty(shape, dtype=dtype, device=device) for shape, dtype in specs]
+
+
+def _is_current(stream, device) -> bool:
+    """Whether `stream` is the device's current stream."""
+    index = device.index
+    if index is None:
+        index = _torch.cuda.current_device()
+    ptr = stream if isinstance(stream, int) else stream.cuda_stream
+    return ptr == _torch._C._cuda_getCurrentRawStream(index)
 
 
 def _dtype_code(t) -> int:
@@ -339,7 +347,7 @@ class Weight:
         import torch
 
         if out is None:
-            out = _empty((self.N, self.K), torch.float32, "cuda", stream)
+            out, = _empty([((self.N, self.K), torch.float32)], torch.device("cuda"), stream)
         _check(lib().nxq_dequant(self.handle, out.data_ptr(), _stream_ptr(stream)))
         return out
 
@@ -356,7 +364,7 @@ def qmatmul(w: Weight, x, out=None, out_dtype=None, stream=None):
     assert x.is_cuda and x.is_contiguous() and x.shape[-1] == w.K
     M = x.numel() // w.K
     if out is None:
-        out = _empty((M, w.N), out_dtype or torch.float32, x.device, stream)
+        out, = _empty([((M, w.N), out_dtype or torch.float32)], x.device, stream)
     _check(lib().nxq_qmatmul(w.handle, x.data_ptr(), _dtype_code(x.dtype), out.data_ptr(),
                              _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -383,7 +391,8 @@ def qmatmul_grouped(ws, xs, outs=None, out_dtype=None, stream=None):
     ws, xs = list(ws), list(xs)
     assert len(ws) == len(xs)
     if outs is None:
-        outs = [_empty((x.numel() // w.K, w.N), out_dtype or torch.float32, x.device, stream) for w, x in zip(ws, xs)]
+        outs = _empty([((x.numel() // w.K, w.N), out_dtype or torch.float32) for w, x in zip(ws, xs)],
+                      xs[0].device if xs else None, stream if xs else None)
     n = len(ws)
     Ms = []
     for w, x, y in zip(ws, xs, outs):
@@ -406,7 +415,7 @@ def qmatmul_swiglu(w_gate: Weight, w_up: Weight, x, out=None, out_dtype=None, st
     assert x.is_cuda and x.is_contiguous() and x.shape[-1] == w_gate.K
     M = x.numel() // w_gate.K
     if out is None:
-        out = _empty((M, w_gate.N), out_dtype or torch.float32, x.device, stream)
+        out, = _empty([((M, w_gate.N), out_dtype or torch.float32)], x.device, stream)
     _check(lib().nxq_qmatmul_swiglu(w_gate.handle, w_up.handle, x.data_ptr(), _dtype_code(x.dtype), out.data_ptr(),
                                     _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -420,7 +429,7 @@ def qmatmul_residual(w: Weight, x, res, out=None, out_dtype=None, stream=None):
     M = x.numel() // w.K
     assert res.dtype == torch.float32 and res.is_contiguous() and res.numel() == M * w.N
     if out is None:
-        out = _empty((M, w.N), out_dtype or torch.float32, x.device, stream)
+        out, = _empty([((M, w.N), out_dtype or torch.float32)], x.device, stream)
     _check(lib().nxq_qmatmul_residual(w.handle, x.data_ptr(), _dtype_code(x.dtype), res.data_ptr(), out.data_ptr(),
                                       _dtype_code(out.dtype), M, _stream_ptr(stream)))
     return out
@@ -437,7 +446,7 @@ def rmsnorm_qmatmul(ws, x, norm, eps: float, outs=None, out_dtype=None, stream=N
     assert norm.dtype == torch.float32 and norm.is_contiguous() and norm.numel() == K
     M = x.numel() // K
     if outs is None:
-        outs = [_empty((M, w.N), out_dtype or torch.float32, x.device, stream) for w in ws]
+        outs = _empty([((M, w.N), out_dtype or torch.float32) for w in ws], x.device, stream)
     n = len(ws)
     arr = ctypes.c_void_p * n
     _check(lib().nxq_rmsnorm_qmatmul(arr(*[w.handle.value for w in ws]), n, x.data_ptr(), _dtype_code(x.dtype),
@@ -497,10 +506,8 @@ def _float_code(what: str, name: str, dtype) -> int:
     return code
 
 
-def _new(shape: tuple, dtype, device, stream):
-    """As _empty; on the current stream by torch's quickest way to one."""
-    if stream is not None:
-        return _empty(shape, dtype, device, stream)
+def _new(shape: tuple, dtype, device):
+    """An empty contiguous tensor (torch's quickest way to one)."""
     stride = (shape[1], 1) if len(shape) == 2 else (1,) if len(shape) == 1 else None
     if stride is None:
         return _torch.empty(shape, dtype=dtype, device=device)
@@ -510,7 +517,11 @@ def _new(shape: tuple, dtype, device, stream):
 def _output(what: str, out, shape: tuple, dtype, like, stream):
     """`out` if given (checked), else a new tensor of `shape` beside `like`; and its type's code."""
     if out is None:
-        out = _new(shape, dtype or _torch.float32, like.device, stream)
+        dtype = dtype or _torch.float32
+        if stream is None or _is_current(stream, like.device):
+            out = _new(shape, dtype, like.device)
+        else:
+            out, = _empty([(shape, dtype)], like.device, stream)
     else:
         _usable(what, "out", out)
         if tuple(out.shape) != shape:
@@ -577,9 +588,11 @@ def moe_route(logits, k: int, normalize: bool = True, stream=None):
     if not 1 <= k <= min(E, 32):
         raise _bad(f"moe_route: k={k} of {E} experts (at most 32)")
     i32, device, choices = torch.int32, logits.device, (T, k)
-    ids, slots = _new(choices, i32, device, stream), _new(choices, i32, device, stream)
-    weights = _new(choices, torch.float32, device, stream)
-    offsets, rows = _new((E + 1,), i32, device, stream), _new((T * k,), i32, device, stream)
+    specs = ((choices, i32), (choices, torch.float32), ((E + 1,), i32), ((T * k,), i32), (choices, i32))
+    if stream is None or _is_current(stream, device):
+        ids, weights, offsets, rows, slots = [_new(shape, dtype, device) for shape, dtype in specs]
+    else:
+        ids, weights, offsets, rows, slots = _empty(specs, device, stream)
     _check(lib().nxq_moe_route(logits.data_ptr(), code, T, E, k, 1 if normalize else 0, ids.data_ptr(), weights.data_ptr(),
                                offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(), _stream_on(stream, d)))
     return ids, weights, offsets, rows, slots
