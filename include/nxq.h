@@ -58,7 +58,8 @@ typedef enum {
     NXQ_ERR_FORMAT = -10,     /* a GGUF / NXF file that is malformed or truncated */
     NXQ_ERR_RANGE = -11,      /* an activation outside the f16 range (see below) */
     NXQ_ERR_INDEX = -12       /* an index in device memory outside its range: a token
-                               * id, an expert offset, a row or slot index (reported by
+                               * id, an expert offset, a row or slot index, a sequence's
+                               * offset or length, a page (reported by
                                * nxq_stream_sync; that access was skipped) */
 } nxq_status;
 
@@ -369,6 +370,125 @@ NXQ_API int nxq_qmatmul_ragged_swiglu(nxq_experts_t gate, nxq_experts_t up, cons
 NXQ_API int nxq_moe_combine(const void* h_dev, int h_dtype, int64_t R, int64_t N, const int32_t* slots_dev,
                             const float* weights_dev, int64_t T, int k, const float* res_dev, void* y_dev,
                             int y_dtype, void* stream);
+
+/* ---- attention over a paged cache --------------------------------------------
+ * What lies between a layer's q/k/v projections and its output projection, with
+ * all lengths on the device, so a step needs no host round trip and can be
+ * captured into a CUDA graph (the reference runs attention on the host per head,
+ * or by attention_gpu.metal:40-66 over a flat cache of 256 tokens):
+ *   nxq_rope             norm and position rotation of queries and keys
+ *   nxq_kv_append        the same on the way into the cache, with the values
+ *   nxq_paged_attention  new tokens over their sequence's cached keys and values
+ * Arrays must be aligned to their element type (NXQ_ERR_ARG otherwise).  Forward
+ * only, as all of the library.  Calls of one stream run in order; calls on
+ * different streams share nothing and may overlap (workspaces as for the
+ * mixture-of-experts calls). */
+
+/* Heads of T tokens: element d of head h of token t is
+ * dev[t * token_stride + h * head_stride + d] (strides in elements, not negative). */
+typedef struct {
+    void* dev;
+    int heads;
+    int64_t token_stride, head_stride;
+} nxq_heads;
+
+/* The cache of one layer: slot i of page p of head h holds head_dim consecutive
+ * elements of type dtype (NXQ_F16 or NXQ_BF16) at
+ * k_dev (v_dev) + p * page_stride + h * head_stride + i * slot_stride (in elements).
+ * k_dev and v_dev 16-byte aligned, strides positive multiples of 8, head_dim a multiple
+ * of 8 up to 256. */
+typedef struct {
+    void *k_dev, *v_dev;
+    int dtype;
+    int64_t pages;
+    int page_size, heads, head_dim;
+    int64_t page_stride, head_stride, slot_stride;
+} nxq_kv_cache;
+
+/* The sequences of a step (1 <= sequences <= 65536).  Sequence s has the new tokens
+ * q_offsets[s] .. q_offsets[s + 1] - 1 of T <= 2^30 (ascending; rows before the first and
+ * behind the last sequence's are left as they were) and kv_lens[s] tokens in the cache with them: new
+ * token i of n is at position kv_lens[s] - n + i.  Position j is slot j % page_size
+ * of page block_table[s * table_stride + j / page_size]; table_pages entries of a
+ * row may be used.  Only entries that a call needs are read: those of new tokens
+ * (append), of visible keys (attention).
+ * A sequence whose offsets lie outside [0, T] or descend, or whose length is
+ * negative or beyond table_pages * page_size (or 2^30), is left out and reported as NXQ_ERR_INDEX; a
+ * page outside [0, pages) is reported too: a token is not appended there, and its
+ * keys and values count as zeros.  Rows that descending offsets give to two sequences hold
+ * what either of them writes. */
+typedef struct {
+    int sequences;
+    const int32_t *q_offsets_dev, *kv_lens_dev, *block_table_dev;
+    int64_t table_stride, table_pages;
+} nxq_kv_batch;
+
+/* Frequencies of the position rotation, in radians per position, of dims / 2 pairs
+ * (host only, in 64 bits):
+ *   NXQ_ROPE_PLAIN   f_i = base^(-2 i / dims)
+ *   NXQ_ROPE_LINEAR  f_i / factor
+ *   NXQ_ROPE_NTK     with base factor^(dims / (dims - 2)) times as large
+ *   NXQ_ROPE_YARN    f_i / factor for slow pairs, f_i for fast ones, a ramp over i
+ *                    between the pairs that turn `high` (default 32) and `low` (1) times in
+ *                    `trained` positions; *scale = 0.1 ln(factor) + 1
+ *   NXQ_ROPE_BLEND   the same by the turns t_i = trained f_i / 2 pi themselves: f_i /
+ *                    factor below `low` (1), f_i above `high` (4), linear in t_i between
+ * *scale (may be NULL) is 1 unless said.  low = high = 0 take the defaults. */
+typedef enum {
+    NXQ_ROPE_PLAIN = 0, NXQ_ROPE_LINEAR = 1, NXQ_ROPE_NTK = 2, NXQ_ROPE_YARN = 3, NXQ_ROPE_BLEND = 4
+} nxq_rope_scaling;
+NXQ_API int nxq_rope_frequencies(int dims, double base, int scaling, double factor, double trained, double low,
+                                 double high, double* inv_freq, float* scale);
+
+/* A position rotation: pair i < dims / 2 of a head, (x_a, x_b), becomes
+ *   scale (x_a cos - x_b sin), scale (x_a sin + x_b cos),   angle = position * inv_freq[i],
+ * with (a, b) = (i, i + dims / 2) (NXQ_ROPE_HALF) or (2 i, 2 i + 1)
+ * (NXQ_ROPE_INTERLEAVED); elements from dims on stay.  dims even, 2 .. 512.  Angles are
+ * exact at any position (fixed point, 2^-64 of a turn per position), sines and cosines
+ * within a few units of fp32.  nxq_rope_release waits for the device. */
+typedef enum { NXQ_ROPE_HALF = 0, NXQ_ROPE_INTERLEAVED = 1 } nxq_rope_layout;
+typedef struct nxq_rope_s* nxq_rope_t;
+NXQ_API int nxq_rope_create(const double* inv_freq, int dims, int layout, float scale, nxq_rope_t* out);
+NXQ_API int nxq_rope_release(nxq_rope_t r);
+
+/* q_out = R(positions[t]) norm(q), k_out likewise, for T tokens of heads of head_dim (1 .. 512)
+ * elements; k and k_out may be NULL (queries only).  norm(x) = x r w with r = 1 /
+ * sqrt(sum(x^2) / head_dim + eps), w = q_norm / k_norm ([head_dim] fp32) where given, else
+ * norm(x) = x.  fp32, one rounding to y_dtype (a finite value beyond f16 is reported as NXQ_ERR_RANGE).
+ * positions: int32 or int64 (nxq_index_type).  q_out may be q (same strides
+ * and type).  rope may be NULL (norms only; positions are then not read). */
+NXQ_API int nxq_rope(nxq_rope_t rope, const void* positions_dev, int positions_type, int64_t T, int head_dim,
+                     const nxq_heads* q, const float* q_norm, const nxq_heads* k, const float* k_norm, float eps,
+                     int x_dtype, const nxq_heads* q_out, const nxq_heads* k_out, int y_dtype, void* stream);
+
+/* Appends the keys and values of the batch's new tokens (T rows; k and v have the cache's
+ * heads and head_dim) at their positions: keys normed and rotated as by nxq_rope, values
+ * as they are, both rounded once to the cache's type.  Their queries are normed
+ * and rotated on the way if q is given (q NULL: none).  rope NULL: no rotation.  q_out may be q.
+ * Two sequences must not append to the same slot.  A new token whose position is
+ * negative (more new tokens than kv_lens) is reported and left out. */
+NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, int64_t T, const nxq_heads* k,
+                          const nxq_heads* v, const float* k_norm, nxq_rope_t rope, const nxq_heads* q,
+                          const float* q_norm, float eps, int x_dtype, const nxq_heads* q_out, int y_dtype,
+                          void* stream);
+
+/* Attention of the batch's new tokens (T rows of q, of the cache's type; q->heads a
+ * multiple g of the cache's heads, query head h reading key head h / g):
+ *   out = sum_j p_j v_j,  p = softmax over the visible j of scale * q k_j.
+ * The query at position p sees j <= p; with window > 0 only j > p - window and the
+ * first `sinks` tokens j < sinks.  window 0: all.  A query that sees no key (its position is
+ * negative) gives zeros.  lse_dev (or NULL): [T][heads] fp32, the natural logarithm
+ * of sum_j exp(scale * q k_j), -inf where no key is seen.  Keys and values that no
+ * query of the batch sees are not read, so freed pages may have any table entry and
+ * unused slots any content; a value that only some queries see reaches no other
+ * query, be it infinite or NaN.
+ * max_new: the most new tokens that any sequence has, where the host knows it (0: T); a
+ * sequence with more is left out and reported.  Scores, statistics and sums are fp32;
+ * probabilities are rounded to the cache's type for the product with the values.  The
+ * same inputs give the same bits on every call. */
+NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads* q, int64_t T,
+                                float scale, int64_t window, int64_t sinks, int64_t max_new, const nxq_heads* out,
+                                int y_dtype, float* lse_dev, void* stream);
 
 /* Host-buffer form, synchronous: the drop-in for ComputeDispatch::gemm_int4
  * (compute_dispatch.h:59-61, .cpp:142-176) - fp32 activations [M][K] in, fp32

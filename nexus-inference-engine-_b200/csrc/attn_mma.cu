@@ -1,0 +1,579 @@
+// Attention over the paged cache for few rows per sequence and key head: single
+// new tokens, drafted ones (and every shape that the tcgen05 kernel does not take).
+//
+// Bound by memory: a key and its value are read once per key head and meet up to 16
+// MT rows.  So the kernel is built around loads: two CTAs per SM, each with an equal
+// share of the call's 64-key units (attn_plan.cuh), each of its four warps streaming
+// its own 16 keys of a unit through a ring of its own by cp.async (16 bytes a lane, the
+// page of every key looked up a unit ahead), with no barrier between units.  Rows of
+// a key that no query of the item sees are filled with zeros instead of read.
+//
+// A warp multiplies on mma.sync.m16n8k16: scores of 16 MT rows x 16 keys, then weights
+// times values, with the maximum, the sum of weights and the output of its own keys
+// in registers (fp32).  At 64 keys per unit that is 128 instructions per 32 KB, 256
+// of the 1390 cycles in which an SM gets 32 KB.  An item ends with the four warps'
+// states joined in shared memory.
+//
+// Weights are relative to a maximum that is raised only when a score passes it by
+// 2^8, so most units need no rescaling; an f16 cache's weights get a factor 2^7 on top,
+// which keeps small ones out of f16's subnormals (2^15 at most).
+#include "attn_plan.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace nxq {
+
+namespace {
+
+using namespace attn;
+
+constexpr int kThreads = 128, kWarps = 4, kSlice = 16, kKeys = kWarps * kSlice;
+constexpr float kSlack = 8.0f;
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes global -> shared, or 16 zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ float value_of(uint32_t bits) {
+    if constexpr (BF16) return __uint_as_float(bits << 16);
+    return __half2float(__ushort_as_half((unsigned short)bits));
+}
+// Whether a 16-bit value is infinite or NaN.
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint32_t bits) {
+    constexpr uint32_t m = BF16 ? 0x7F80u : 0x7C00u;
+    return (bits & m) == m;
+}
+
+template <int DP, int MT>
+struct Shape {
+    static constexpr int kStages = DP == 64 ? 6 : DP == 128 ? (MT == 1 ? 3 : 2) : 2;
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kSliceBytes = kSlice * DP * 2;                 // a warp's keys (or values) of a unit
+    static constexpr int kRing = kWarps * kStages * 2 * kSliceBytes;
+    static constexpr bool kQInRegs = MT == 1 && DP <= 128;
+    static constexpr int kQBytes = kRows * DP * 2;
+    static constexpr int kJoin = 2 * 16 * DP * 4 + kWarps * kRows * 8;  // two warps' outputs of 16 rows, all statistics
+    // The plan, the queries (if they go on to registers) and the join share one region.
+    static constexpr int kShared0 = kJoin > (int)sizeof(PlanSmem) ? kJoin : (int)sizeof(PlanSmem);
+    static constexpr int kShared = kShared0 > kQBytes ? kShared0 : kQBytes;
+    static constexpr int kSmem = kRing + kShared + (kQInRegs ? 0 : kQBytes);
+    static constexpr int kCtas = 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
+};
+
+// Swizzled offset of 16-byte chunk c of row r in a block of rows of DP 16-bit elements.
+template <int DP>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return (uint32_t)(r * DP * 2 + ((c ^ (r & 7)) << 4));
+}
+
+template <bool BF16, int DP, int MT>
+__global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
+    using Sh = Shape<DP, MT>;
+    constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kChunks = DP / 8, kSteps = DP / 16, kTiles = DP / 8;
+    constexpr float kShift = BF16 ? 0.0f : 7.0f;
+    using W = Walk<kRows, kKeys>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* const shared = smem + Sh::kRing;
+    PlanSmem& plan = *reinterpret_cast<PlanSmem*>(shared);
+    float* const join = reinterpret_cast<float*>(shared);
+    float* const join_ml = join + 2 * 16 * DP;  // [warp][kRows] maximum, then sum
+    uint8_t* const qs = Sh::kQInRegs ? shared : shared + Sh::kShared;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // The join kernel may start its set-up when all before this kernel is complete.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    plan_total<kRows, kKeys, kThreads>(p, plan);
+    const long long total = plan.total, first = run_start(total, blockIdx.x, gridDim.x);
+    const long long units = run_start(total, blockIdx.x + 1, gridDim.x) - first;
+    if (units == 0) return;
+    plan_locate<kRows, kKeys, kThreads>(p, plan, first);
+
+    W ahead, w;  // the piece being loaded, and the one being computed
+    w.start(p, plan, units);
+    ahead = w;
+    __syncthreads();  // the plan has been read: its memory is the join's
+    int au = 0;       // unit of `ahead` whose pages are looked up next
+    bool more = true;
+
+    // The page entry of this lane's key (lanes 16 .. 31 repeat 0 .. 15) of the unit after
+    // the one being copied, and what is needed to turn it into an address.
+    int entry = 0, slot = 0, entry_head = 0;
+    bool want = false;
+    auto look_up = [&]() {
+        want = false;
+        if (!more) return;
+        const int j = ahead.key0(au) + warp * kSlice + (lane & 15);
+        want = any_sees(p, ahead.it, j);
+        entry_head = ahead.head;
+        if (want) {
+            const int page = p.page_shift >= 0 ? j >> p.page_shift : j / p.b.page;
+            slot = j - page * p.b.page;
+            entry = p.b.table[ahead.s * p.b.table_stride + page];
+        }
+        if (++au == ahead.count) {
+            au = 0;
+            more = ahead.next(p);
+        }
+    };
+    const uint32_t ring = smem_of(smem) + warp * kStages * 2 * Sh::kSliceBytes;
+    auto copy_unit = [&](int stage) {
+        int64_t at = -1;
+        if (want) {
+            if (entry < 0 || entry >= p.b.pages)
+                raise_index(p.status, kIndexPage);
+            else
+                at = entry * p.page_stride + slot * p.slot_stride + entry_head * p.head_stride;
+        }
+        const uint32_t dst = ring + stage * 2 * Sh::kSliceBytes;
+#pragma unroll
+        for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+            const int e = i * 32 + lane, r = e / kChunks, c = e % kChunks;
+            const int64_t row = __shfl_sync(0xFFFFFFFFu, at, r);
+            const bool read = row >= 0 && c * 8 < p.D;
+            const int64_t o = read ? row + c * 8 : 0;
+            copy16(dst + chunk_at<DP>(r, c), static_cast<const uint16_t*>(p.k) + o, read);
+            copy16(dst + Sh::kSliceBytes + chunk_at<DP>(r, c), static_cast<const uint16_t*>(p.v) + o, read);
+        }
+    };
+    look_up();
+    for (int i = 0; i < kStages - 1; ++i) {
+        copy_unit(i);
+        copies_commit();
+        look_up();
+    }
+
+    int stage = 0;
+    bool go = true;
+    while (go) {
+        // Queries of the piece: rows of DP, zeros behind D and behind the item's rows.
+        const int64_t row0 = (int64_t)w.item * kRows;
+        auto query_at = [&](int r) {  // token and query head of row r, as an element offset in q
+            const int64_t t = (row0 + r) / p.G;
+            const int g = (int)((row0 + r) - t * p.G);
+            return (w.q.q0 + t) * p.q_token + ((int64_t)w.head * p.G + g) * p.q_head;
+        };
+        for (int e = threadIdx.x; e < kRows * kChunks; e += kThreads) {
+            const int r = e / kChunks, c = e % kChunks;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (r < w.it.rows && c * 8 < p.D) {
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + query_at(r) + c * 8;
+                if (p.q_vec) {
+                    v = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[i] = (uint32_t)src[2 * i] | (uint32_t)src[2 * i + 1] << 16;
+                    v = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+            *reinterpret_cast<uint4*>(qs + chunk_at<DP>(r, c)) = v;
+        }
+        __syncthreads();
+        const uint32_t qa = smem_of(qs);
+        // A fragment of 16 rows x 16 elements: lanes 0-15 rows, low 8 elements; 16-31 the same rows, high 8.
+        auto query = [&](int mt, int ks, uint32_t (&a)[4]) {
+            ldsm4(qa + chunk_at<DP>(16 * mt + (lane & 15), 2 * ks + (lane >> 4)), a);
+        };
+        uint32_t qf[Sh::kQInRegs ? kSteps : 1][4];
+        if constexpr (Sh::kQInRegs) {
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) query(0, ks, qf[ks]);
+        }
+        int pos[MT][2];  // positions of this lane's rows (-1: none)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * mt + 8 * h + (lane >> 2);
+                pos[mt][h] = r < w.it.rows ? w.q.len - w.q.n + (int)((row0 + r) / p.G) : -1;
+            }
+        float o[MT][kTiles][4], m[MT][2], l[MT][2];  // m: maximum in use, in units of c q k
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[mt][t][i] = 0.0f;
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.0f;
+        }
+
+        for (int u = 0; u < w.count; ++u) {
+            copies_wait<kStages - 2>();
+            __syncwarp();  // the unit is there, and the one before has been read by all lanes: its stage takes the unit kStages - 1 ahead
+            copy_unit(stage == 0 ? kStages - 1 : stage - 1);
+            copies_commit();
+            look_up();
+            const uint32_t ks0 = ring + stage * 2 * Sh::kSliceBytes, vs0 = ks0 + Sh::kSliceBytes;
+            const int j0 = w.key0(u) + warp * kSlice;
+            float s[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][nt][i] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+                uint32_t b[4];  // keys 0-7 low, high; keys 8-15 low, high
+                ldsm4(ks0 + chunk_at<DP>((lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), b);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t a[4];
+                    if constexpr (Sh::kQInRegs) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) a[i] = qf[ks][i];
+                    } else {
+                        query(mt, ks, a);
+                    }
+                    mma<BF16>(s[mt][0], a, b[0], b[1]);
+                    mma<BF16>(s[mt][1], a, b[2], b[3]);
+                }
+            }
+            const bool masked = !all_see(p, w.it, j0, kSlice);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float& x = s[mt][nt][i];
+                        x *= p.c;
+                        if (masked && !sees(p, pos[mt][i >> 1], j0 + 8 * nt + 2 * (lane & 3) + (i & 1))) x = -INFINITY;
+                    }
+            // Maxima of the rows; lanes of a quad share a row.
+            bool raise = false;
+            float top[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
+                    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
+                    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+                    top[mt][h] = v;
+                    raise |= v > m[mt][h] + kSlack || (m[mt][h] == -INFINITY && v > -INFINITY);
+                }
+            if (__any_sync(0xFFFFFFFFu, raise)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float now = fmaxf(m[mt][h], top[mt][h]);
+                        // (From -inf: nothing has been added yet.)
+                        const float f = m[mt][h] == -INFINITY ? 0.0f : exp2_fast(m[mt][h] - now);
+                        m[mt][h] = now;
+                        l[mt][h] *= f;
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            o[mt][t][2 * h] *= f;
+                            o[mt][t][2 * h + 1] *= f;
+                        }
+                    }
+            }
+            uint32_t pa[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float base = m[mt][h] == -INFINITY ? 0.0f : m[mt][h] - kShift;
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        float& x = s[mt][nt][2 * h];
+                        float& y = s[mt][nt][2 * h + 1];
+                        x = exp2_fast(x - base);
+                        y = exp2_fast(y - base);
+                        l[mt][h] += x + y;
+                        pa[mt][2 * nt + h] = pack2<BF16>(x, y);
+                    }
+                }
+            }
+            // A value that not all rows see may be infinite or NaN, and its weight of zero
+            // must not meet it: such elements are added to the rows that see them one by
+            // one, and are zeros to the product below.
+            if (masked && w.it.p_lo != w.it.p_hi) {
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+                    uint32_t v[4];
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                                 : "r"(vs0 + (i * 32 + lane) * 16)
+                                 : "memory");
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bad |= not_finite<BF16>(v[k] & 0xFFFFu) || not_finite<BF16>(v[k] >> 16);
+                }
+                if (__any_sync(0xFFFFFFFFu, bad)) {
+                    uint8_t* const vs = smem + (vs0 - smem_of(smem));
+#pragma unroll 1
+                    for (int k = 0; k < kSlice; ++k) {
+                        float wt[MT][2];
+                        bool see[MT][2];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                // Key k's weight is in lane (k % 8) / 2 of the quad, element k % 2 of tile k / 8.
+                                const float e0 = k < 8 ? s[mt][0][2 * h] : s[mt][1][2 * h];
+                                const float e1 = k < 8 ? s[mt][0][2 * h + 1] : s[mt][1][2 * h + 1];
+                                wt[mt][h] = __shfl_sync(0xFFFFFFFFu, (k & 1) ? e1 : e0, (lane & ~3) | ((k & 7) >> 1));
+                                see[mt][h] = sees(p, pos[mt][h], j0 + k);
+                            }
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            const uint32_t two = *reinterpret_cast<const uint32_t*>(vs + chunk_at<DP>(k, t) + 4 * (lane & 3));
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t bits = e ? two >> 16 : two & 0xFFFFu;
+                                if (not_finite<BF16>(bits)) {
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                        for (int h = 0; h < 2; ++h)
+                                            if (see[mt][h]) o[mt][t][2 * h + e] += wt[mt][h] * value_of<BF16>(bits);
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    for (int i = lane; i < kSlice * DP; i += 32) {
+                        uint16_t* e = reinterpret_cast<uint16_t*>(vs) + i;
+                        if (not_finite<BF16>(*e)) *e = 0;
+                    }
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < kTiles; t += 2) {
+                uint32_t b[4];  // tile t: keys 0-7, 8-15; tile t + 1: the same
+                ldsm4t(vs0 + chunk_at<DP>(lane & 15, t + (lane >> 4)), b);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma<BF16>(o[mt][t], pa[mt], b[0], b[1]);
+                    mma<BF16>(o[mt][t + 1], pa[mt], b[2], b[3]);
+                }
+            }
+            if (++stage == kStages) stage = 0;
+        }
+
+        // Join the warps: everybody's factor against the largest maximum, then outputs
+        // of warps 2, 3 onto 0, 1, and of 1 onto 0, 16 rows at a time.
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
+            }
+        __syncthreads();  // (queries are read from here on no more)
+        if ((lane & 3) == 0)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 16 * mt + 8 * h + (lane >> 2);
+                    join_ml[warp * kRows + r] = m[mt][h];
+                    join_ml[(kWarps + warp) * kRows + r] = l[mt][h];
+                }
+        __syncthreads();
+        float big[MT][2], sum[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * mt + 8 * h + (lane >> 2);
+                float x = -INFINITY, y = 0.0f;
+                for (int k = 0; k < kWarps; ++k) x = fmaxf(x, join_ml[k * kRows + r]);
+                for (int k = 0; k < kWarps; ++k) {  // (without a maximum the sum is 0, or NaN)
+                    const float mk = join_ml[k * kRows + r], lk = join_ml[(kWarps + k) * kRows + r];
+                    y += mk > -INFINITY ? lk * exp2_fast(mk - x) : lk;
+                }
+                big[mt][h] = x;
+                sum[mt][h] = y;
+                const float f = m[mt][h] == -INFINITY ? 1.0f : exp2_fast(m[mt][h] - x);  // (1: zeros, or NaN)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    o[mt][t][2 * h] *= f;
+                    o[mt][t][2 * h + 1] *= f;
+                }
+            }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int step = 2; step; step >>= 1) {
+                if (mt || step == 1) __syncthreads();
+                if (warp >= step && warp < 2 * step) {
+                    float4* d = reinterpret_cast<float4*>(join + (warp - step) * 16 * DP) + lane;
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) d[t * 32] = make_float4(o[mt][t][0], o[mt][t][1], o[mt][t][2], o[mt][t][3]);
+                }
+                __syncthreads();
+                if (warp < step) {
+                    const float4* d = reinterpret_cast<const float4*>(join + warp * 16 * DP) + lane;
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        const float4 x = d[t * 32];
+                        o[mt][t][0] += x.x, o[mt][t][1] += x.y, o[mt][t][2] += x.z, o[mt][t][3] += x.w;
+                    }
+                }
+            }
+        }
+        if (warp == 0) {
+            const bool whole = w.whole();
+            float* const part = whole ? nullptr : p.part + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 16 * mt + 8 * h + (lane >> 2);
+                    if (r >= w.it.rows) continue;
+                    const int64_t t = (row0 + r) / p.G;
+                    const int head = w.head * p.G + (int)(row0 + r - t * p.G);
+                    const int64_t row = w.q.q0 + t;
+                    if (whole) {
+                        const float f = sum[mt][h] == 0.0f ? 0.0f : 1.0f / sum[mt][h];
+                        const int64_t at = row * p.o_token + head * p.o_head;
+#pragma unroll
+                        for (int tt = 0; tt < kTiles; ++tt) {
+                            const int d = 8 * tt + 2 * (lane & 3);
+                            if (d >= p.D) break;
+                            const float x = o[mt][tt][2 * h] * f, y = o[mt][tt][2 * h + 1] * f;
+                            if (p.y_dtype == NXQ_F32) {
+                                float* e = static_cast<float*>(p.out) + at + d;
+                                e[0] = x, e[1] = y;
+                            } else {
+                                const uint32_t two = p.y_dtype == NXQ_BF16 ? pack2<true>(x, y) : pack2<false>(x, y);
+                                uint16_t* e = static_cast<uint16_t*>(p.out) + at + d;
+                                if (p.o_vec) {
+                                    *reinterpret_cast<uint32_t*>(e) = two;
+                                } else {
+                                    e[0] = (uint16_t)two, e[1] = (uint16_t)(two >> 16);
+                                }
+                            }
+                        }
+                        if (p.lse && (lane & 3) == 0)
+                            p.lse[row * ((int64_t)p.Hk * p.G) + head] =
+                                sum[mt][h] == 0.0f ? -INFINITY : (big[mt][h] - kShift + log2f(sum[mt][h])) * 0.6931471805599453f;
+                    } else {
+#pragma unroll
+                        for (int tt = 0; tt < kTiles; ++tt) {
+                            const int d = 8 * tt + 2 * (lane & 3);
+                            if (d >= p.D) break;
+                            *reinterpret_cast<float2*>(part + (int64_t)r * p.D + d) = make_float2(o[mt][tt][2 * h], o[mt][tt][2 * h + 1]);
+                        }
+                        if ((lane & 3) == 0) {
+                            part[(int64_t)kRows * p.D + r] = big[mt][h] - kShift;
+                            part[(int64_t)kRows * p.D + kRows + r] = sum[mt][h];
+                        }
+                    }
+                }
+        }
+        __syncthreads();  // the join's memory is the next piece's queries'
+        go = w.next(p);
+    }
+    copies_wait<0>();
+}
+
+template <int DP, int MT>
+int set_attr() {
+    cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<false, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         Shape<DP, MT>::kSmem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(attn_mma_kernel<true, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 Shape<DP, MT>::kSmem);
+    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
+}
+
+template <int DP>
+unsigned grid_of() {
+    static_assert(DP == 256 || Shape<DP, 1>::kCtas == Shape<DP, 2>::kCtas, "one grid for both");
+    return (unsigned)context_sm_count() * Shape<DP, 1>::kCtas;
+}
+
+template <int DP>
+cudaError_t launch(const AttnParams& p, int dtype, int rows, cudaStream_t st) {
+    const unsigned grid = grid_of<DP>();
+    if constexpr (DP <= 128)
+        if (rows == 32)
+            return launch_overlapped(dtype == NXQ_BF16 ? attn_mma_kernel<true, DP, 2> : attn_mma_kernel<false, DP, 2>, grid,
+                                     kThreads, Shape<DP, 2>::kSmem, st, p);
+    return launch_overlapped(dtype == NXQ_BF16 ? attn_mma_kernel<true, DP, 1> : attn_mma_kernel<false, DP, 1>, grid, kThreads,
+                             Shape<DP, 1>::kSmem, st, p);
+}
+
+}  // namespace
+
+int attn_mma_init() {
+    int rc;
+    if ((rc = set_attr<64, 1>()) || (rc = set_attr<64, 2>()) || (rc = set_attr<128, 1>()) || (rc = set_attr<128, 2>()) ||
+        (rc = set_attr<256, 1>()))
+        return rc;
+    return NXQ_OK;
+}
+
+// (Heads beyond 128 elements: 32 rows of outputs do not fit the registers.)
+int attn_mma_rows(int D, int64_t rows) { return rows <= 16 || D > 128 ? 16 : 32; }
+
+unsigned attn_mma_grid(int D) { return D <= 64 ? grid_of<64>() : D <= 128 ? grid_of<128>() : grid_of<256>(); }
+
+int attn_mma(const AttnParams& p, int dtype, int rows, cudaStream_t st) {
+    note_launches(1);
+    const cudaError_t e = p.D <= 64    ? launch<64>(p, dtype, rows, st)
+                          : p.D <= 128 ? launch<128>(p, dtype, rows, st)
+                                       : launch<256>(p, dtype, rows, st);
+    if (e != cudaSuccess) return cuda_fail(e, "attention launch");
+    const cudaError_t j = launch_attn_join(p, rows, kKeys, attn_mma_grid(p.D), st);
+    return j == cudaSuccess ? NXQ_OK : cuda_fail(j, "attention join launch");
+}
+
+}  // namespace nxq

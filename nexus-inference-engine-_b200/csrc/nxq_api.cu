@@ -20,6 +20,7 @@
 #include <vector>
 #include <unordered_set>
 
+#include "attention.h"
 #include "nxq_internal.h"
 #include "qmm_gemm.h"
 #include "qmm_mma.h"
@@ -140,17 +141,19 @@ int report_status(const DeviceStatus& st) {
     cudaMemset(g_ctx.status, 0, 2 * sizeof(unsigned));
     if (st.code == kStatusRange) {
         static const char* const what[] = {"?", "the f16 conversion of fp32/bf16 activations",
-                                           "the RMSNorm prologue", "the decode GEMV's activation staging"};
+                                           "the RMSNorm prologue", "the decode GEMV's activation staging",
+                                           "an f16 output of a rotation or an f16 cache"};
         return fail(NXQ_ERR_RANGE,
                     "an activation of magnitude >= 65520 reached %s: it is outside the f16 range the "
                     "tensor-core kernels compute in (results of that call are not finite)",
-                    what[st.where < 4 ? st.where : 0]);
+                    what[st.where < 5 ? st.where : 0]);
     }
     if (st.code == kStatusIndex) {
         static const char* const what[] = {"an index", "a token id of an embedding lookup",
                                            "an expert offset of a ragged product", "a row index of a ragged product",
-                                           "a slot index of a combine"};
-        return fail(NXQ_ERR_INDEX, "%s was outside its range (that access was skipped)", what[st.where < 5 ? st.where : 0]);
+                                           "a slot index of a combine", "the offsets or length of a sequence",
+                                           "a page of a sequence", "the position of a new token"};
+        return fail(NXQ_ERR_INDEX, "%s was outside its range (that access was skipped)", what[st.where < 8 ? st.where : 0]);
     }
     scratch_reset_counters();
     return fail(NXQ_ERR_TIMEOUT, "device-side bounded wait expired (code %u at %u)", st.code, st.where);
@@ -397,6 +400,7 @@ NXQ_API int nxq_init(int device) {
     if (rc != NXQ_OK) return rc;
     if ((rc = gemm_init(device)) != NXQ_OK) return rc;
     if ((rc = ragged_gemm_init()) != NXQ_OK || (rc = ragged_mma_init()) != NXQ_OK) return rc;
+    if ((rc = attn_mma_init()) != NXQ_OK) return rc;
     g_ctx.ready = true;
     return NXQ_OK;
 }
@@ -407,6 +411,7 @@ NXQ_API int nxq_shutdown(void) {
     cudaSetDevice(g_ctx.device);
     cudaDeviceSynchronize();
     experts_shutdown();
+    ropes_shutdown();
     {
         std::lock_guard<std::mutex> lk2(g_ctx.mu);
         for (Weight* w : g_ctx.live) {

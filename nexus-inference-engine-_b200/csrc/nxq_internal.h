@@ -90,7 +90,8 @@ __device__ __forceinline__ void raise_range(DeviceStatus* st, unsigned where) {
 }
 
 // Records an index error (first error wins; `where`: kIndex*).
-constexpr unsigned kIndexToken = 1u, kIndexOffset = 2u, kIndexRow = 3u, kIndexSlot = 4u;
+constexpr unsigned kIndexToken = 1u, kIndexOffset = 2u, kIndexRow = 3u, kIndexSlot = 4u, kIndexSeq = 5u, kIndexPage = 6u,
+                   kIndexPosition = 7u;
 __device__ __forceinline__ void raise_index(DeviceStatus* st, unsigned where) {
     if (st && atomicCAS(&st->code, 0u, kStatusIndex) == 0u) {
         st->where = where;

@@ -23,6 +23,7 @@ __all__ = [
     "TYPES", "GEOMETRY", "F32", "F16", "BF16", "SPLIT_COL", "SPLIT_ROW", "declared_symbols",
     "tp_unique_id", "tp_init", "tp_shutdown", "tp_qmatmul", "tp_allreduce_f32", "GGUF", "NXF", "xxh32", "qmatmul_grouped", "qmatmul_swiglu", "qmatmul_residual", "rmsnorm_qmatmul", "int4_pack", "INT4_ROWS", "INT4_KMAJOR",
     "embedding", "Experts", "moe_route", "qmatmul_ragged", "qmatmul_ragged_swiglu", "moe_combine",
+    "Rope", "rope_frequencies", "rope", "KVCache", "kv_append", "paged_attention",
 ]
 
 LIB_PATH = Path(__file__).with_name("libnxq.so")
@@ -104,6 +105,16 @@ _SIGS = {
                                   _c.c_int, _c.c_int64, _c.c_void_p, _c.c_void_p],
     "nxq_moe_combine": [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int,
                         _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p],
+    "nxq_rope_frequencies": [_c.c_int, _c.c_double, _c.c_int, _c.c_double, _c.c_double, _c.c_double, _c.c_double,
+                             _c.c_void_p, _c.c_void_p],
+    "nxq_rope_create": [_c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.POINTER(_c.c_void_p)],
+    "nxq_rope_release": [_c.c_void_p],
+    "nxq_rope": [_c.c_void_p, _c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+                 _c.c_void_p, _c.c_float, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p],
+    "nxq_kv_append": [_c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+                      _c.c_void_p, _c.c_void_p, _c.c_float, _c.c_int, _c.c_void_p, _c.c_int, _c.c_void_p],
+    "nxq_paged_attention": [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_float, _c.c_int64, _c.c_int64,
+                            _c.c_int64, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p],
     "nxq_stream_sync": [_c.c_void_p],
     "nxq_set_wait_limit": [_c.c_uint64],
     "nxq_test_hook": [_c.c_int, _c.c_int],
@@ -664,6 +675,257 @@ def moe_combine(h, slots, weights, res=None, out=None, out_dtype=None, stream=No
     _check(lib().nxq_moe_combine(h.data_ptr(), code, R, N, slots.data_ptr(), weights.data_ptr(), T, k, rp, out.data_ptr(),
                                  ycode, _stream_on(stream, d)))
     return out
+
+
+# ---- attention over a paged cache ------------------------------------------------
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+_LAYOUTS = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
+_SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "blend": 4}
+
+
+class _Heads(ctypes.Structure):
+    """nxq_heads"""
+
+    _fields_ = [("dev", _c.c_void_p), ("heads", _c.c_int), ("token_stride", _c.c_int64), ("head_stride", _c.c_int64)]
+
+
+class _Cache(ctypes.Structure):
+    """nxq_kv_cache"""
+
+    _fields_ = [("k_dev", _c.c_void_p), ("v_dev", _c.c_void_p), ("dtype", _c.c_int), ("pages", _c.c_int64),
+                ("page_size", _c.c_int), ("heads", _c.c_int), ("head_dim", _c.c_int), ("page_stride", _c.c_int64),
+                ("head_stride", _c.c_int64), ("slot_stride", _c.c_int64)]
+
+
+class _Batch(ctypes.Structure):
+    """nxq_kv_batch"""
+
+    _fields_ = [("sequences", _c.c_int), ("q_offsets_dev", _c.c_void_p), ("kv_lens_dev", _c.c_void_p),
+                ("block_table_dev", _c.c_void_p), ("table_stride", _c.c_int64), ("table_pages", _c.c_int64)]
+
+
+def rope_frequencies(dims: int, base: float = 10000.0, scaling: str = "plain", factor: float = 1.0,
+                     trained: float = 0.0, low: float = 0.0, high: float = 0.0):
+    """(frequencies, scale) for Rope: radians per position of dims / 2 pairs
+    (nxq_rope_frequencies; "plain", "linear", "ntk", "yarn" or "blend").  Host only."""
+    if scaling not in _SCALINGS:
+        raise _bad(f"rope_frequencies: scaling {scaling!r}, not one of {', '.join(_SCALINGS)}")
+    inv = np.zeros(max(dims // 2, 1), dtype=np.float64)
+    scale = ctypes.c_float()
+    _check(lib().nxq_rope_frequencies(dims, base, _SCALINGS[scaling], factor, trained, low, high, inv.ctypes.data,
+                                      ctypes.byref(scale)))
+    return inv, scale.value
+
+
+class Rope:
+    """A position rotation (nxq_rope_create): pair i of a head turns by position *
+    inv_freq[i], pairs (i, i + dims / 2) for layout "half", (2 i, 2 i + 1) for "interleaved";
+    sines and cosines times `scale`.  Stays on the GPU until release()."""
+
+    def __init__(self, inv_freq, layout: str = "half", scale: float = 1.0):
+        if layout not in _LAYOUTS:
+            raise _bad(f"Rope: layout {layout!r}, not half or interleaved")
+        f = np.ascontiguousarray(inv_freq, dtype=np.float64)
+        if f.ndim != 1:
+            raise _bad(f"Rope: frequencies of shape {f.shape}")
+        h = ctypes.c_void_p()
+        _check(lib().nxq_rope_create(f.ctypes.data, 2 * f.size, _LAYOUTS[layout], scale, ctypes.byref(h)))
+        self._h = h
+        self.dims, self.layout, self.scale = 2 * f.size, layout, scale
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        if self._h is None:
+            raise NxqError(-1, "rotation already released")
+        return self._h
+
+    def release(self) -> None:
+        if self._h is not None:
+            _check(lib().nxq_rope_release(self._h))
+        self._h = None
+
+
+def _on_device(what: str, name: str, t) -> int:
+    """Device index of a tensor on the library's GPU, whatever its strides."""
+    d = t.get_device()
+    if d < 0 or (d != _device and _device is not None):
+        raise _bad(f"{what}: {name} is on {t.device}, the library on cuda:{_device}")
+    return d
+
+
+def _rows(what: str, name: str, t, heads=None, head_dim=None, tokens=None):
+    """nxq_heads of a tensor [T][heads][D] whose last dimension is contiguous."""
+    if t.dim() != 3:
+        raise _bad(f"{what}: {name} has {t.dim()} dimensions, not tokens, heads, elements")
+    T, H, D = t.shape
+    if (heads is not None and H != heads) or (head_dim is not None and D != head_dim) or (tokens is not None and T != tokens):
+        want = " ".join(f"[{'any' if x is None else x}]" for x in (tokens, heads, head_dim))
+        raise _bad(f"{what}: {name} is {tuple(t.shape)}, not {want}")
+    _on_device(what, name, t)
+    ts, hs, ds = t.stride()
+    if ds != 1 and D > 1:
+        raise _bad(f"{what}: the elements of {name}'s heads are not contiguous")
+    return _Heads(t.data_ptr(), H, ts, hs)
+
+
+def _norm(what: str, name: str, w, head_dim: int):
+    if w is None:
+        return None
+    if w.dtype is not _torch.float32 or tuple(w.shape) != (head_dim,):
+        raise _bad(f"{what}: {name} must be fp32 [{head_dim}]")
+    _usable(what, name, w)
+    return w.data_ptr()
+
+
+def _rows_out(what: str, out, like, dtype, stream):
+    """`out` if given (any strides of tokens and heads), else a new tensor of `like`'s shape; and its type's code."""
+    if out is None:
+        return _output(what, None, tuple(like.shape), dtype, like, stream)
+    if tuple(out.shape) != tuple(like.shape):
+        raise _bad(f"{what}: out has shape {tuple(out.shape)}, not {tuple(like.shape)}")
+    if dtype is not None and out.dtype != dtype:
+        raise _bad(f"{what}: out is {out.dtype}, out_dtype {dtype}")
+    return out, _float_code(what, "out", out.dtype)
+
+
+def rope(r: Optional[Rope], positions, q, k=None, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, k_out=None,
+         out_dtype=None, stream=None):
+    """Norm over each head (where a weight is given) and position rotation (where
+    `r` is) of queries [T][Hq][D] and keys [T][Hk][D] (nxq_rope): q_out, or (q_out,
+    k_out) with keys.  positions: int32 or int64 [T]; None without `r`.  Tokens and
+    heads may have any strides; q_out may be q."""
+    torch = _torch or _load_torch()
+    what = "rope"
+    qr = _rows(what, "q", q)
+    T, _, D = q.shape
+    code = _float_code(what, "q", q.dtype)
+    kr = ko = None
+    if k is not None:
+        kr = _rows(what, "k", k, head_dim=D, tokens=T)
+        if k.dtype != q.dtype:
+            raise _bad(f"{what}: q is {q.dtype}, k {k.dtype}")
+    pp, pt = None, I32
+    if r is not None:
+        if positions is None or (positions.dtype is not torch.int64 and positions.dtype is not torch.int32) or tuple(positions.shape) != (T,):
+            raise _bad(f"{what}: positions must be int32 or int64 [{T}]")
+        _usable(what, "positions", positions)
+        pp, pt = positions.data_ptr(), I64 if positions.dtype is torch.int64 else I32
+    qn, kn = _norm(what, "q_norm", q_norm, D), _norm(what, "k_norm", k_norm, D)
+    q_out, ycode = _rows_out(what, q_out, q, out_dtype, stream)
+    qo = _rows(what, "q_out", q_out)
+    if k is not None:
+        k_out, kcode = _rows_out(what, k_out, k, q_out.dtype, stream)
+        ko = _rows(what, "k_out", k_out)
+    elif k_out is not None:
+        raise _bad(f"{what}: k_out without k")
+    b = ctypes.byref
+    _check(lib().nxq_rope(r.handle if r is not None else None, pp, pt, T, D, b(qr), qn, b(kr) if kr else None, kn, eps, code,
+                          b(qo), b(ko) if ko else None, ycode, _stream_on(stream, q.get_device())))
+    return q_out if k is None else (q_out, k_out)
+
+
+class KVCache:
+    """The paged cache of one layer over two tensors of f16 or bf16: keys and values
+    [pages][heads][slots][D] (order "heads") or [pages][slots][heads][D] ("tokens"), of
+    the same strides, which must be positive multiples of 8 (the elements' 1)."""
+
+    def __init__(self, keys, values, order: str = "heads"):
+        _torch or _load_torch()
+        what = "KVCache"
+        if order not in ("heads", "tokens"):
+            raise _bad(f"{what}: order {order!r}, not heads or tokens")
+        if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.stride() != values.stride():
+            raise _bad(f"{what}: keys and values must be alike, with four dimensions")
+        if keys.dtype not in (_torch.float16, _torch.bfloat16):
+            raise _bad(f"{what}: a cache of {keys.dtype} (float16 or bfloat16)")
+        _on_device(what, "keys", keys)
+        _on_device(what, "values", values)
+        if keys.stride(3) != 1:
+            raise _bad(f"{what}: the elements of a head are not contiguous")
+        h, t = (1, 2) if order == "heads" else (2, 1)
+        self.keys, self.values, self.order = keys, values, order
+        self.pages, self.heads, self.page_size, self.head_dim = keys.shape[0], keys.shape[h], keys.shape[t], keys.shape[3]
+        self.dtype, self.device = keys.dtype, keys.device
+        self._c = _Cache(keys.data_ptr(), values.data_ptr(), _FLOATS[keys.dtype], self.pages, self.page_size, self.heads,
+                         self.head_dim, keys.stride(0), keys.stride(h), keys.stride(t))
+        self._ref = ctypes.byref(self._c)
+
+
+def _batch(what: str, q_offsets, kv_lens, block_table):
+    """nxq_kv_batch of int32 tensors [S + 1], [S] and [S][pages]."""
+    i32 = _torch.int32
+    if kv_lens.dim() != 1 or kv_lens.dtype is not i32 or kv_lens.shape[0] < 1:
+        raise _bad(f"{what}: kv_lens must be int32, one for each sequence")
+    S = kv_lens.shape[0]
+    if q_offsets.dtype is not i32 or tuple(q_offsets.shape) != (S + 1,):
+        raise _bad(f"{what}: q_offsets must be int32 [{S + 1}]")
+    if block_table.dtype is not i32 or block_table.dim() != 2 or block_table.shape[0] != S:
+        raise _bad(f"{what}: block_table must be int32 [{S}][pages]")
+    _usable(what, "kv_lens", kv_lens)
+    _usable(what, "q_offsets", q_offsets)
+    _on_device(what, "block_table", block_table)
+    pages = block_table.shape[1]
+    if pages > 1 and block_table.stride(1) != 1:
+        raise _bad(f"{what}: the rows of block_table are not contiguous")
+    return _Batch(S, q_offsets.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), pages)
+
+
+def kv_append(cache: KVCache, k, v, q_offsets, kv_lens, block_table, rope: Optional[Rope] = None, q=None, q_norm=None,
+              k_norm=None, eps: float = 1e-6, q_out=None, out_dtype=None, stream=None):
+    """Appends keys (normed and rotated) and values [T][heads][D] of new tokens to
+    the cache at their positions (nxq_kv_append): sequence s has rows q_offsets[s] ..
+    q_offsets[s + 1] - 1 and kv_lens[s] tokens with them.  With queries q [T][Hq][D]
+    returns them normed and rotated."""
+    _torch or _load_torch()
+    what = "kv_append"
+    kr = _rows(what, "k", k, heads=cache.heads, head_dim=cache.head_dim)
+    T, D = k.shape[0], cache.head_dim
+    vr = _rows(what, "v", v, heads=cache.heads, head_dim=D, tokens=T)
+    code = _float_code(what, "k", k.dtype)
+    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise _bad(f"{what}: q, k and v are of different types")
+    batch = _batch(what, q_offsets, kv_lens, block_table)
+    qn, kn = _norm(what, "q_norm", q_norm, D), _norm(what, "k_norm", k_norm, D)
+    qr = qo = None
+    ycode = F32
+    if q is not None:
+        qr = _rows(what, "q", q, head_dim=D, tokens=T)
+        q_out, ycode = _rows_out(what, q_out, q, out_dtype, stream)
+        qo = _rows(what, "q_out", q_out)
+    elif q_out is not None:
+        raise _bad(f"{what}: q_out without q")
+    b = ctypes.byref
+    _check(lib().nxq_kv_append(cache._ref, b(batch), T, b(kr), b(vr), kn, rope.handle if rope is not None else None,
+                               b(qr) if qr else None, qn, eps, code, b(qo) if qo else None, ycode,
+                               _stream_on(stream, k.get_device())))
+    return q_out
+
+
+def paged_attention(q, cache: KVCache, q_offsets, kv_lens, block_table, scale: Optional[float] = None, window: int = 0,
+                    sinks: int = 0, max_new: int = 0, out=None, out_dtype=None, return_lse: bool = False, stream=None):
+    """Attention of new tokens q [T][Hq][D] over their sequences' cached keys and
+    values, causal (nxq_paged_attention): sequence s has rows q_offsets[s] ..
+    q_offsets[s + 1] - 1, the last of its kv_lens[s] tokens.  scale: 1 / sqrt(D) unless given.
+    window: keys that a query sees, itself among them (0: all), besides the first
+    `sinks`.  max_new: the most new tokens of any sequence, if known.  Rows of `out` that no sequence has
+    are left as they are (undefined in a new tensor).  return_lse: (out, lse [T][Hq])."""
+    torch = _torch or _load_torch()
+    what = "paged_attention"
+    qr = _rows(what, "q", q, head_dim=cache.head_dim)
+    if q.dtype != cache.dtype:
+        raise _bad(f"{what}: q is {q.dtype}, the cache {cache.dtype}")
+    batch = _batch(what, q_offsets, kv_lens, block_table)
+    out, ycode = _rows_out(what, out, q, out_dtype, stream)
+    oh = _rows(what, "out", out)
+    lse = None
+    if return_lse:
+        lse, _ = _output(what, None, tuple(q.shape[:2]), torch.float32, q, stream)
+    b = ctypes.byref
+    _check(lib().nxq_paged_attention(cache._ref, b(batch), b(qr), q.shape[0], cache.head_dim ** -0.5 if scale is None else scale,
+                                     window, sinks, max_new, b(oh), ycode, lse.data_ptr() if return_lse else None,
+                                     _stream_on(stream, q.get_device())))
+    return (out, lse) if return_lse else out
 
 
 def stream_sync(stream=None) -> None:
