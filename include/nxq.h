@@ -481,11 +481,13 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
  * of sum_j exp(scale * q k_j), -inf where no key is seen.  Keys and values that no
  * query of the batch sees are not read, so freed pages may have any table entry and
  * unused slots any content; a value that only some queries see reaches no other
- * query, be it infinite or NaN.
+ * query, be it infinite or NaN (what an infinite value gives to those that see it is
+ * infinite, or NaN with an fp32 output).
  * max_new: the most new tokens that any sequence has, where the host knows it (0: T); a
  * sequence with more is left out and reported.  Scores, statistics and sums are fp32;
- * probabilities are rounded to the cache's type for the product with the values.  The
- * same inputs give the same bits on every call. */
+ * probabilities are rounded to the cache's type for the product with the values (where
+ * y_dtype is NXQ_F32, to two numbers of that type, with twice its digits).  The same
+ * inputs give the same bits on every call. */
 NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads* q, int64_t T,
                                 float scale, int64_t window, int64_t sinks, int64_t max_new, const nxq_heads* out,
                                 int y_dtype, float* lse_dev, void* stream);

@@ -12,6 +12,7 @@ namespace {
 
 using namespace attn;
 
+constexpr int kFewRows = 32;
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
 // Joins the pieces of items cut between runs.  CTA (c, g) takes the item that begins in run
@@ -145,12 +146,29 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     p.rows_lo = 0;
     p.rows_hi = INT64_MAX;
     p.first = 1;
+    // Sequences of up to kFewRows rows per key head go to the kernel that streams the cache, those
+    // with more to the tcgen05 kernel, each by a launch that leaves the others out; only
+    // one launch where the host can tell (a sequence alone has T rows in all but odd cases, and
+    // the tcgen05 kernel takes any number).
     const int64_t most = (int64_t)p.max_new * p.G;
-    const int rows = attn_mma_rows(p.D, most);
+    const bool tc = most > kFewRows && attn_tc_supported(cache);
+    const bool few = !tc || p.b.S > 1;
+    const int rows = attn_mma_rows(p.D, tc ? kFewRows : most);
     const unsigned runs = attn_mma_grid(p.D);
-    cudaError_t e = cudaMallocAsync((void**)&p.part, 2 * runs * part_floats(rows, p.D) * sizeof(float), st);
+    size_t floats = few ? 2 * runs * part_floats(rows, p.D) : 0;
+    if (tc && 2 * attn_tc_grid() * part_floats(attn_tc_rows(), p.D) > floats)
+        floats = 2 * attn_tc_grid() * part_floats(attn_tc_rows(), p.D);
+    cudaError_t e = cudaMallocAsync((void**)&p.part, floats * sizeof(float), st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (attention workspace)");
-    const int rc = attn_mma(p, cache->dtype, rows, st);
+    int rc = NXQ_OK;
+    if (few) {
+        if (tc) p.rows_hi = kFewRows;
+        rc = attn_mma(p, cache->dtype, rows, st);
+        p.rows_lo = tc ? kFewRows : 0;
+        p.rows_hi = INT64_MAX;
+        p.first = 0;
+    }
+    if (tc && rc == NXQ_OK) rc = attn_tc(p, cache, st);
     cudaFreeAsync(p.part, st);
     return rc;
 }
@@ -160,6 +178,7 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
 cudaError_t launch_attn_join(const AttnParams& p, int rows, int keys, unsigned runs, cudaStream_t st) {
     if (rows == 16 && keys == 64) return join<16, 64>(p, runs, st);
     if (rows == 32 && keys == 64) return join<32, 64>(p, runs, st);
+    if (rows == 256 && keys == 128) return join<256, 128>(p, runs, st);
     return cudaErrorInvalidValue;
 }
 

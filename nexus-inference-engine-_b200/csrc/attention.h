@@ -77,6 +77,14 @@ int attn_mma_rows(int D, int64_t rows);           // rows of an item where a seq
 unsigned attn_mma_grid(int D);
 int attn_mma(const AttnParams& p, int dtype, int rows, cudaStream_t st);
 
+// Kernel of many rows (attn_tc.cu), for caches that it can read: a grid of
+// attn_tc_grid() runs, items of attn_tc_rows() rows.
+int attn_tc_init();
+bool attn_tc_supported(const nxq_kv_cache* c);
+int attn_tc_rows();
+unsigned attn_tc_grid();
+int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st);
+
 // Joins the partial results of a launch of `runs` runs with items of `rows` rows and
 // `keys` keys per unit (attention.cu).
 cudaError_t launch_attn_join(const AttnParams& p, int rows, int keys, unsigned runs, cudaStream_t st);

@@ -16,7 +16,9 @@
 //
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8, so most units need no rescaling; an f16 cache's weights get a factor 2^7 on top,
-// which keeps small ones out of f16's subnormals (2^15 at most).
+// which keeps small ones out of f16's subnormals (2^15 at most).  They are rounded to the
+// cache's type for the product with the values; where the output is fp32 (SPLIT) what
+// the rounding leaves goes through a second product, so that they keep twice its digits.
 #include "attn_plan.cuh"
 
 #include <cuda_bf16.h>
@@ -115,7 +117,7 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
     return (uint32_t)(r * DP * 2 + ((c ^ (r & 7)) << 4));
 }
 
-template <bool BF16, int DP, int MT>
+template <bool BF16, bool SPLIT, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using Sh = Shape<DP, MT>;
     constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kChunks = DP / 8, kSteps = DP / 16, kTiles = DP / 8;
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                         }
                     }
             }
-            uint32_t pa[MT][4];
+            uint32_t pa[MT][4], pb[SPLIT ? MT : 1][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -334,7 +336,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                         x = exp2_fast(x - base);
                         y = exp2_fast(y - base);
                         l[mt][h] += x + y;
-                        pa[mt][2 * nt + h] = pack2<BF16>(x, y);
+                        const uint32_t two = pack2<BF16>(x, y);
+                        pa[mt][2 * nt + h] = two;
+                        if constexpr (SPLIT)
+                            pb[mt][2 * nt + h] = pack2<BF16>(x - value_of<BF16>(two & 0xFFFFu), y - value_of<BF16>(two >> 16));
                     }
                 }
             }
@@ -401,6 +406,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                 for (int mt = 0; mt < MT; ++mt) {
                     mma<BF16>(o[mt][t], pa[mt], b[0], b[1]);
                     mma<BF16>(o[mt][t + 1], pa[mt], b[2], b[3]);
+                    if constexpr (SPLIT) {
+                        mma<BF16>(o[mt][t], pb[mt], b[0], b[1]);
+                        mma<BF16>(o[mt][t + 1], pb[mt], b[2], b[3]);
+                    }
                 }
             }
             if (++stage == kStages) stage = 0;
@@ -525,13 +534,19 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
 }
 
 template <int DP, int MT>
+auto* kernel_of(bool bf16, bool split) {
+    return bf16 ? (split ? attn_mma_kernel<true, true, DP, MT> : attn_mma_kernel<true, false, DP, MT>)
+                : (split ? attn_mma_kernel<false, true, DP, MT> : attn_mma_kernel<false, false, DP, MT>);
+}
+
+template <int DP, int MT>
 int set_attr() {
-    cudaError_t e = cudaFuncSetAttribute(attn_mma_kernel<false, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         Shape<DP, MT>::kSmem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(attn_mma_kernel<true, DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 Shape<DP, MT>::kSmem);
-    return e == cudaSuccess ? NXQ_OK : cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
+    for (int i = 0; i < 4; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   Shape<DP, MT>::kSmem);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
+    }
+    return NXQ_OK;
 }
 
 template <int DP>
@@ -540,15 +555,9 @@ unsigned grid_of() {
     return (unsigned)context_sm_count() * Shape<DP, 1>::kCtas;
 }
 
-template <int DP>
-cudaError_t launch(const AttnParams& p, int dtype, int rows, cudaStream_t st) {
-    const unsigned grid = grid_of<DP>();
-    if constexpr (DP <= 128)
-        if (rows == 32)
-            return launch_overlapped(dtype == NXQ_BF16 ? attn_mma_kernel<true, DP, 2> : attn_mma_kernel<false, DP, 2>, grid,
-                                     kThreads, Shape<DP, 2>::kSmem, st, p);
-    return launch_overlapped(dtype == NXQ_BF16 ? attn_mma_kernel<true, DP, 1> : attn_mma_kernel<false, DP, 1>, grid, kThreads,
-                             Shape<DP, 1>::kSmem, st, p);
+template <int DP, int MT>
+cudaError_t launch(const AttnParams& p, bool bf16, cudaStream_t st) {
+    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32), grid_of<DP>(), kThreads, Shape<DP, MT>::kSmem, st, p);
 }
 
 }  // namespace
@@ -568,9 +577,10 @@ unsigned attn_mma_grid(int D) { return D <= 64 ? grid_of<64>() : D <= 128 ? grid
 
 int attn_mma(const AttnParams& p, int dtype, int rows, cudaStream_t st) {
     note_launches(1);
-    const cudaError_t e = p.D <= 64    ? launch<64>(p, dtype, rows, st)
-                          : p.D <= 128 ? launch<128>(p, dtype, rows, st)
-                                       : launch<256>(p, dtype, rows, st);
+    const bool bf = dtype == NXQ_BF16, two = rows == 32;
+    const cudaError_t e = p.D <= 64    ? (two ? launch<64, 2>(p, bf, st) : launch<64, 1>(p, bf, st))
+                          : p.D <= 128 ? (two ? launch<128, 2>(p, bf, st) : launch<128, 1>(p, bf, st))
+                                       : launch<256, 1>(p, bf, st);
     if (e != cudaSuccess) return cuda_fail(e, "attention launch");
     const cudaError_t j = launch_attn_join(p, rows, kKeys, attn_mma_grid(p.D), st);
     return j == cudaSuccess ? NXQ_OK : cuda_fail(j, "attention join launch");

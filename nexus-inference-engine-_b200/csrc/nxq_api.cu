@@ -400,7 +400,7 @@ NXQ_API int nxq_init(int device) {
     if (rc != NXQ_OK) return rc;
     if ((rc = gemm_init(device)) != NXQ_OK) return rc;
     if ((rc = ragged_gemm_init()) != NXQ_OK || (rc = ragged_mma_init()) != NXQ_OK) return rc;
-    if ((rc = attn_mma_init()) != NXQ_OK) return rc;
+    if ((rc = attn_mma_init()) != NXQ_OK || (rc = attn_tc_init()) != NXQ_OK) return rc;
     g_ctx.ready = true;
     return NXQ_OK;
 }

@@ -425,6 +425,21 @@ int gemm_activation_map(CUtensorMap* tmap, const void* xh, int64_t rows, int64_t
     return NXQ_OK;
 }
 
+bool tensor_maps() { return g_encode != nullptr; }
+
+int tensor_map_16(CUtensorMap* tmap, bool bf16, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                  const uint32_t* box) {
+    cuuint64_t d[5], s[5];
+    cuuint32_t b[5], one[5];
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i], b[i] = box[i], one[i] = 1;
+        if (i) s[i - 1] = strides[i - 1];
+    }
+    return (int)g_encode(tmap, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                         const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 int gemm_qmatmul(const Weight* w, const void* x, int x_dtype, void* y, int y_dtype, int64_t M, cudaStream_t st) {
     const TiledShape& s = w->shape;
     if (!gemm_supported(s, M)) return NXQ_ERR_UNSUPPORTED;

@@ -21,4 +21,11 @@ int gemm_qmatmul(const Weight* w, const void* x, int x_dtype, void* y, int y_dty
 // box_rows rows, 128-byte swizzle; needs gemm_init with the kernel enabled.
 int gemm_activation_map(CUtensorMap* tmap, const void* xh, int64_t rows, int64_t K, int box_rows);
 
+// Whether tensor maps can be made (not with NXQ_PREFILL_KERNEL=simt), and one of 16-bit
+// elements for boxes with a 128-byte swizzle: 0, or the driver's error.  `rank`
+// dimensions, the first contiguous; `strides` of the others in bytes.
+bool tensor_maps();
+int tensor_map_16(CUtensorMap* tmap, bool bf16, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                  const uint32_t* box);
+
 }  // namespace nxq

@@ -56,7 +56,7 @@ class Paged:
     def attend(self, nxq, **kw):
         return nxq.paged_attention(self.q, self.cache, self.q_offsets, self.kv_lens, self.table, **kw)
 
-    def expected(self, scale=None, window=0, sinks=0, rows=None):
+    def expected(self, scale=None, window=0, sinks=0, y=None):
         """(out, bound, lse) of every new token in 64 bits, and a bound on |error| but for the output's rounding."""
         scale = self.D ** -0.5 if scale is None else scale
         G, dev = self.Hq // self.Hk, self.q.device
@@ -64,6 +64,8 @@ class Paged:
         bound = torch.zeros_like(out)
         lse = torch.full((self.T, self.Hq), -math.inf, dtype=torch.float64, device=dev)
         u = HALF_STEP[self.q.dtype]
+        if y is torch.float32:  # weights as two numbers of the cache's type
+            u = u * u
         at = 0
         for i, (n, t) in enumerate(zip(self.new, self.total)):
             k = self.k[i].double().repeat_interleave(G, dim=1).transpose(0, 1)  # [Hq][t][D]
@@ -101,7 +103,7 @@ class Paged:
         return out, bound, lse
 
     def check(self, got, lse=None, **kw):
-        want, bound, want_lse = self.expected(**kw)
+        want, bound, want_lse = self.expected(y=got.dtype, **kw)
         half = HALF_STEP[got.dtype]
         err = (got.double() - want).abs()
         tol = bound * (1 + half) + half * want.abs() + 2.0 ** -24

@@ -78,6 +78,16 @@ def test_split_histories(gpu, S, total, dt):
     run(gpu, p, y=dt)
 
 
+@pytest.mark.parametrize("dt,D,y", [("bf16", 128, "bf16"), ("f16", 64, "f32"), ("f16", 80, "f16")])
+@pytest.mark.parametrize("window", [0, 300])
+def test_long_runs(gpu, dt, D, y, window):
+    # Many items and key blocks for each run: rings go round many times, items of one and two tiles alternate.
+    new, ctx = [2200, 31, 700, 100, 17, 900], [500, 4000, 0, 1000, 300, 0]
+    p = Paged(gpu, new, [n + c for n, c in zip(new, ctx)], 32, 8, D, 32, DT[dt], seed=D)
+    for max_new in (0, 2200):
+        run(gpu, p, y=y, window=window, sinks=4, max_new=max_new)
+
+
 def test_many_sequences(gpu):
     # More than one chunk of the plan (256), with some that have nothing to do.
     rng = random.Random(1)
@@ -107,22 +117,23 @@ def test_values_that_only_some_queries_see(gpu, new, bad):
     D, ctx = 64, 70
     for dt in (torch.float16, torch.bfloat16):
         p = Paged(gpu, new, [n + ctx for n in new], 4, 2, D, 16, dt, seed=2)
-        clean, _ = p.attend(gpu, return_lse=True, window=50)
+        clean = {y: p.attend(gpu, window=50, out_dtype=y) for y in (dt, torch.float32)}
         at = [ctx + new[0] - 1, 30]  # the last token of sequence 0; one that leaves the window in sequence 1
         p.v[0][at[0], 1, 5] = bad
         p.v[1][at[1], 0, 7] = bad
         p.store()
-        got = p.attend(gpu, window=50)
-        gpu.stream_sync()
-        hit = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+        hit = torch.zeros((p.T, 4, D), dtype=torch.bool, device="cuda")
         hit[new[0] - 1, 2:, 5] = True  # query heads 2, 3 read key head 1
         for i in range(new[1]):
             if at[1] > ctx + i - 50:
                 hit[new[0] + i, :2, 7] = True
-        assert torch.equal(got[~hit], clean[~hit])
-        assert not torch.isfinite(got[hit]).any()
-        if not math.isnan(bad):
-            assert bool((got[hit] == bad).all())
+        for y in (dt, torch.float32):
+            got = p.attend(gpu, window=50, out_dtype=y)
+            gpu.stream_sync()
+            assert torch.equal(got[~hit], clean[y][~hit])
+            assert not torch.isfinite(got[hit]).any()
+            if y is dt and not math.isnan(bad):  # (an fp32 output may be NaN there)
+                assert bool((got[hit] == bad).all())
 
 
 def test_keys_that_only_some_queries_see(gpu):
