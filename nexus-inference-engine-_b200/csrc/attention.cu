@@ -16,73 +16,57 @@ constexpr int kFewRows = 32;
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
 // Joins the pieces of items cut between runs.  CTA (c, g) takes the item that begins in run
-// c and ends behind it, if there is one, and of that rows kRowsPer g ...: a warp per row,
-// first the largest maximum and the sum of weights over the pieces, then the sum of their
-// outputs, in order of the runs whatever order they were written in.
-constexpr int kRowsPer = 4 * kJoinWarps;
-
-template <int ROWS, int KEYS>
+// c and ends behind it, if there is one, and of that the rows PER g kJoinWarps ...: a warp per
+// row, first the largest maximum over the pieces, then the sums of weights and outputs, in
+// order of the runs whatever order they were written in.  Nothing but latency counts:
+// a row of 128 elements is one load of a warp per piece, eight of them in flight, and a
+// CTA has few rows (one item of 16 rows in 37 pieces: 88 us with 16 rows per CTA,
+// 4.0 with 4).
+template <int ROWS, int PER>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p, const int runs) {
-    __shared__ PlanSmem plan;
-    // The lengths are complete before the kernel that writes the pieces begins (it waits for
-    // them before it lets this one start); the pieces when it has ended.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    plan_total<ROWS, KEYS, kJoinThreads>(p, plan);
-    const long long total = plan.total, r = blockIdx.x;
-    const long long here = run_start(total, r, runs), end = run_start(total, r + 1, runs);
-    long long first = 0, last = 0;
-    bool cut = here < end && end < total;
-    if (cut) {
-        plan_locate<ROWS, KEYS, kJoinThreads>(p, plan, end);
-        cut = plan.off > 0 && end - plan.off >= here;
-    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!cut) return;
-    bool bad;
-    const Seq q = launch_seq(p, plan.s, &bad);
-    const Item it = make_item<ROWS, KEYS>(p, q, plan.item);
-    first = end - plan.off;
-    last = first + it.units;
-    // Piece i: with a unit or more in every run, run r + i; else the run that unit first + i is.
-    auto run_of = [&](long long x) { return ((x + 1) * runs - 1) / total; };
-    const int pieces = (int)(total >= runs ? run_of(last - 1) - r + 1 : it.units);
+    const int r = blockIdx.x;
+    const int4* const note = reinterpret_cast<const int4*>(static_cast<const Cut*>(p.work) + r);
+    const int4 n0 = note[0], n1 = note[1];
+    const Cut cut{n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, {0, 0}};
+    if (cut.pieces == 0) return;
     const size_t floats = part_floats(ROWS, p.D);
-    auto part_of = [&](int i) {
-        const long long run = total >= runs ? r + i : run_of(first + i);
-        return p.part + (2 * run + (i == 0 ? 1 : 0)) * floats;
-    };
+    const float* const slots = reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.work) + cuts_bytes(runs));
+    // Piece 0 is in run r's slot 1, piece i in run r + i's slot 0.
+    auto part_of = [&](int i) { return slots + (2 * (size_t)(r + i) + (i == 0 ? 1 : 0)) * floats; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int k = 0; k < kRowsPer / kJoinWarps; ++k) {
-        const int row = (int)blockIdx.y * kRowsPer + k * kJoinWarps + warp;
-        if (row >= it.rows) continue;
+#pragma unroll 1
+    for (int k = 0; k < PER; ++k) {
+        const int row = ((int)blockIdx.y * PER + k) * kJoinWarps + warp;
+        if (row >= cut.rows) break;
         float top = -INFINITY;
-        for (int i = lane; i < pieces; i += 32) top = fmaxf(top, part_of(i)[(size_t)ROWS * p.D + row]);
+        for (int i = lane; i < cut.pieces; i += 32) top = fmaxf(top, part_of(i)[(size_t)ROWS * p.D + row]);
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         float sum = 0.0f;
         float acc[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < pieces; ++i) {
+#pragma unroll 8
+        for (int i = 0; i < cut.pieces; ++i) {
             const float* part = part_of(i);
             const float m = part[(size_t)ROWS * p.D + row], l = part[(size_t)ROWS * p.D + ROWS + row];
+            float4 v[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (4 * lane + 128 * h < p.D) v[h] = *reinterpret_cast<const float4*>(part + (size_t)row * p.D + 4 * lane + 128 * h);
             const float f = m > -INFINITY ? exp2f(m - top) : 1.0f;  // (1: zeros, or NaN)
             sum = fmaf(l, f, sum);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int d = 4 * lane + 128 * h;
-                if (d < p.D) {
-                    const float4 v = *reinterpret_cast<const float4*>(part + (size_t)row * p.D + d);
-                    acc[4 * h] = fmaf(v.x, f, acc[4 * h]);
-                    acc[4 * h + 1] = fmaf(v.y, f, acc[4 * h + 1]);
-                    acc[4 * h + 2] = fmaf(v.z, f, acc[4 * h + 2]);
-                    acc[4 * h + 3] = fmaf(v.w, f, acc[4 * h + 3]);
-                }
+                acc[4 * h] = fmaf(v[h].x, f, acc[4 * h]);
+                acc[4 * h + 1] = fmaf(v[h].y, f, acc[4 * h + 1]);
+                acc[4 * h + 2] = fmaf(v[h].z, f, acc[4 * h + 2]);
+                acc[4 * h + 3] = fmaf(v[h].w, f, acc[4 * h + 3]);
             }
         }
-        const int64_t flat = (int64_t)plan.item * ROWS + row, t = flat / p.G;
-        const int head = plan.head * p.G + (int)(flat - t * p.G);
-        const int64_t at = (q.q0 + t) * p.o_token + head * p.o_head;
+        const int g = cut.r0 + row, t = (int)((unsigned)g / (unsigned)p.G), head = cut.head * p.G + (g - t * p.G);
+        const int64_t token = (int64_t)cut.q0 + cut.t0 + t, at = token * p.o_token + head * p.o_head;
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -99,14 +83,14 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
                     static_cast<__half*>(p.out)[at + d] = __float2half_rn(v);
             }
         if (p.lse && lane == 0)
-            p.lse[(q.q0 + t) * ((int64_t)p.Hk * p.G) + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            p.lse[token * ((int64_t)p.Hk * p.G) + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     }
 }
 
-template <int ROWS, int KEYS>
+template <int ROWS, int PER>
 cudaError_t join(const AttnParams& p, unsigned runs, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(runs, (ROWS + kRowsPer - 1) / kRowsPer);
+    cfg.gridDim = dim3(runs, ROWS / (PER * kJoinWarps));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -115,8 +99,10 @@ cudaError_t join(const AttnParams& p, unsigned runs, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     note_launches(1);
-    return cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, KEYS>, p, (int)runs);
+    return cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, PER>, p, (int)runs);
 }
+
+size_t work_bytes(unsigned runs, int rows, int D) { return cuts_bytes(runs) + 2 * runs * part_floats(rows, D) * sizeof(float); }
 
 int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads* q, int64_t T, float scale, int64_t window,
            int64_t sinks, int64_t max_new, const nxq_heads* out, int y_dtype, float* lse, cudaStream_t st) {
@@ -133,10 +119,13 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     p.Hk = cache->heads, p.G = q->heads / cache->heads, p.D = cache->head_dim;
     p.y_dtype = y_dtype;
     p.q_vec = (uintptr_t)q->dev % 16 == 0 && q->token_stride % 8 == 0 && q->head_stride % 8 == 0;
-    p.o_vec = (uintptr_t)out->dev % 16 == 0 && out->token_stride % 8 == 0 && out->head_stride % 8 == 0;
+    const uintptr_t o_bits = (uintptr_t)out->dev |
+                             (uintptr_t)(out->token_stride | out->head_stride) * (y_dtype == NXQ_F32 ? 4 : 2);
+    p.o_vec = o_bits % 32 == 0 ? 2 : o_bits % 16 == 0 ? 1 : 0;
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i)
         if (cache->page_size == 1 << i) p.page_shift = i;
+    p.page_align = cache->page_size & -cache->page_size;
     p.c = scale * 1.4426950408889634f;
     // No position reaches kMaxTokens, so a window of that size hides nothing.
     p.window = window < kMaxTokens ? (int)window : 0;
@@ -147,18 +136,18 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     p.rows_hi = INT64_MAX;
     p.first = 1;
     // Sequences of up to kFewRows rows per key head go to the kernel that streams the cache, those
-    // with more to the tcgen05 kernel, each by a launch that leaves the others out; only
-    // one launch where the host can tell (a sequence alone has T rows in all but odd cases, and
-    // the tcgen05 kernel takes any number).
+    // with more to the tcgen05 kernel, each by a launch that leaves the others out.  Where the
+    // average is above kFewRows the tcgen05 kernel takes them all: beside chunks of that
+    // size, single tokens cost it no more than their bytes, and the second pair of
+    // launches would cost some 5 us.
     const int64_t most = (int64_t)p.max_new * p.G;
     const bool tc = most > kFewRows && attn_tc_supported(cache);
-    const bool few = !tc || p.b.S > 1;
+    const bool few = !tc || T * p.G <= (int64_t)kFewRows * p.b.S;
     const int rows = attn_mma_rows(p.D, tc ? kFewRows : most);
     const unsigned runs = attn_mma_grid(p.D);
-    size_t floats = few ? 2 * runs * part_floats(rows, p.D) : 0;
-    if (tc && 2 * attn_tc_grid() * part_floats(attn_tc_rows(), p.D) > floats)
-        floats = 2 * attn_tc_grid() * part_floats(attn_tc_rows(), p.D);
-    cudaError_t e = cudaMallocAsync((void**)&p.part, floats * sizeof(float), st);
+    size_t bytes = few ? work_bytes(runs, rows, p.D) : 0;
+    if (tc && work_bytes(attn_tc_grid(), attn_tc_rows(), p.D) > bytes) bytes = work_bytes(attn_tc_grid(), attn_tc_rows(), p.D);
+    cudaError_t e = cudaMallocAsync(&p.work, bytes, st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (attention workspace)");
     int rc = NXQ_OK;
     if (few) {
@@ -169,16 +158,16 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
         p.first = 0;
     }
     if (tc && rc == NXQ_OK) rc = attn_tc(p, cache, st);
-    cudaFreeAsync(p.part, st);
+    cudaFreeAsync(p.work, st);
     return rc;
 }
 
 }  // namespace
 
-cudaError_t launch_attn_join(const AttnParams& p, int rows, int keys, unsigned runs, cudaStream_t st) {
-    if (rows == 16 && keys == 64) return join<16, 64>(p, runs, st);
-    if (rows == 32 && keys == 64) return join<32, 64>(p, runs, st);
-    if (rows == 256 && keys == 128) return join<256, 128>(p, runs, st);
+cudaError_t launch_attn_join(const AttnParams& p, int rows, unsigned runs, cudaStream_t st) {
+    if (rows == 16) return join<16, 1>(p, runs, st);
+    if (rows == 32) return join<32, 1>(p, runs, st);
+    if (rows == 256) return join<256, 2>(p, runs, st);
     return cudaErrorInvalidValue;
 }
 
@@ -201,7 +190,7 @@ NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* b
     if ((rc = check_heads("queries", q, cache->dtype)) || (rc = check_heads("output", out, y_dtype))) return rc;
     if (q->heads % cache->heads || q->heads != out->heads)
         return fail(NXQ_ERR_SHAPE, "%d query heads and %d output heads for %d key heads", q->heads, out->heads, cache->heads);
-    if (T * (q->heads / cache->heads) > (int64_t)1 << 34)
+    if (T * (q->heads / cache->heads) > 0x7FFFFFFF)
         return fail(NXQ_ERR_SHAPE, "%lld rows of %d query heads per key head", (long long)T, q->heads / cache->heads);
     if (!aligned_4(lse_dev)) return fail(NXQ_ERR_ARG, "lse is not aligned to its type");
     if ((rc = context_ready())) return rc;

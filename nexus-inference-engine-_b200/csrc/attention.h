@@ -59,14 +59,15 @@ struct AttnParams {
     int64_t page_stride, head_stride, slot_stride;
     int Hk, G, D;      // key heads, query heads per key head, elements of a head
     int y_dtype;
-    int q_vec, o_vec;  // rows of q (of the output) are multiples of 16 bytes, at such an address
+    int q_vec, o_vec;  // rows of q (of the output) are multiples of 16 bytes, at such an address (o_vec 2: of 32)
     int page_shift;    // log2 of the page size, or -1
+    int page_align;    // the largest power of two that divides the page size
     float c;           // scale * log2(e): weights are exp2(c q k)
     int window, sinks; // window 0: none
     int max_new;
     int64_t rows_lo, rows_hi;  // sequences of rows_lo < n G <= rows_hi rows are this launch's
     int first;             // reports what is wrong with the batch
-    float* part;           // partial results of runs (attn_plan.cuh)
+    void* work;            // partial results of runs (attn_plan.cuh)
     DeviceStatus* status;
 };
 
@@ -85,8 +86,7 @@ int attn_tc_rows();
 unsigned attn_tc_grid();
 int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st);
 
-// Joins the partial results of a launch of `runs` runs with items of `rows` rows and
-// `keys` keys per unit (attention.cu).
-cudaError_t launch_attn_join(const AttnParams& p, int rows, int keys, unsigned runs, cudaStream_t st);
+// Joins the partial results of a launch of `runs` runs with items of `rows` rows (attention.cu).
+cudaError_t launch_attn_join(const AttnParams& p, int rows, unsigned runs, cudaStream_t st);
 
 }  // namespace nxq

@@ -3,9 +3,9 @@
 //
 // Bound by memory: a key and its value are read once per key head and meet up to 16
 // MT rows.  So the kernel is built around loads: two CTAs per SM, each with an equal
-// share of the call's 64-key units (attn_plan.cuh), each of its four warps streaming
-// its own 16 keys of a unit through a ring of its own by cp.async (16 bytes a lane, the
-// page of every key looked up a unit ahead), with no barrier between units.  Rows of
+// share of the call's units of 64 keys (128 for short heads; attn_plan.cuh), each of its
+// four warps streaming its own quarter of a unit through a ring of its own by cp.async
+// (16 bytes a lane, pages looked up a unit ahead), with no barrier between units.  Rows of
 // a key that no query of the item sees are filled with zeros instead of read.
 //
 // A warp multiplies on mma.sync.m16n8k16: scores of 16 MT rows x 16 keys, then weights
@@ -30,7 +30,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kThreads = 128, kWarps = 4, kSlice = 16, kKeys = kWarps * kSlice;
+constexpr int kThreads = 128, kWarps = 4;
 constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -97,7 +97,9 @@ __device__ __forceinline__ bool not_finite(uint32_t bits) {
 
 template <int DP, int MT>
 struct Shape {
-    static constexpr int kStages = DP == 64 ? 6 : DP == 128 ? (MT == 1 ? 3 : 2) : 2;
+    static constexpr int kSlice = DP == 64 ? 32 : 16;  // keys of a unit per warp: 4 KB or more of each
+    static constexpr int kKeys = kWarps * kSlice;
+    static constexpr int kStages = DP <= 128 && MT == 1 ? 3 : 2;
     static constexpr int kRows = 16 * MT;
     static constexpr int kSliceBytes = kSlice * DP * 2;                 // a warp's keys (or values) of a unit
     static constexpr int kRing = kWarps * kStages * 2 * kSliceBytes;
@@ -120,7 +122,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 template <bool BF16, bool SPLIT, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using Sh = Shape<DP, MT>;
-    constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kChunks = DP / 8, kSteps = DP / 16, kTiles = DP / 8;
+    constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kSlice = Sh::kSlice, kKeys = Sh::kKeys;
+    constexpr int kChunks = DP / 8, kSteps = DP / 16, kTiles = DP / 8, kNT = kSlice / 8;
     constexpr float kShift = BF16 ? 0.0f : 7.0f;
     using W = Walk<kRows, kKeys>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -131,14 +134,17 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     uint8_t* const qs = Sh::kQInRegs ? shared : shared + Sh::kShared;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // The join kernel may start its set-up when all before this kernel is complete.
+    // The join kernel may start when all before this kernel is complete.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    Cut* const note = static_cast<Cut*>(p.work) + blockIdx.x;
+    float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(p.work) + cuts_bytes(gridDim.x));
+    if (threadIdx.x == 0) note->pieces = 0;
     plan_total<kRows, kKeys, kThreads>(p, plan);
-    const long long total = plan.total, first = run_start(total, blockIdx.x, gridDim.x);
-    const long long units = run_start(total, blockIdx.x + 1, gridDim.x) - first;
+    const Runs runs(plan.total, gridDim.x);
+    const long long units = runs.units(blockIdx.x);
     if (units == 0) return;
-    plan_locate<kRows, kKeys, kThreads>(p, plan, first);
+    plan_locate<kRows, kKeys, kThreads>(p, plan, runs.start(blockIdx.x));
 
     W ahead, w;  // the piece being loaded, and the one being computed
     w.start(p, plan, units);
@@ -147,18 +153,34 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     int au = 0;       // unit of `ahead` whose pages are looked up next
     bool more = true;
 
-    // The page entry of this lane's key (lanes 16 .. 31 repeat 0 .. 15) of the unit after
-    // the one being copied, and what is needed to turn it into an address.
-    int entry = 0, slot = 0, entry_head = 0;
+    // The unit after the one being copied: the page entry and slot of its keys, and which
+    // of them are wanted.  Where pages hold whole slices a warp's keys share one entry, its
+    // first key's slot and a range (rows below `upto`, but not gap0 .. gap1 - 1); else
+    // lane i has key i's (lanes from kSlice on repeat).
+    const bool paged = p.page_align >= kSlice;
+    int entry = 0, slot = 0, entry_head = 0, upto = 0, gap0 = 0, gap1 = 0;
     bool want = false;
     auto look_up = [&]() {
         want = false;
         if (!more) return;
-        const int j = ahead.key0(au) + warp * kSlice + (lane & 15);
-        want = any_sees(p, ahead.it, j);
+        int j = ahead.key0(au) + warp * kSlice;
         entry_head = ahead.head;
+        if (paged) {
+            upto = ahead.it.p_hi + 1 - j;
+            want = upto > 0;
+            upto = upto < kSlice ? upto : kSlice;
+            gap0 = gap1 = 0;
+            if (p.window > 0) {
+                gap0 = p.sinks > j ? p.sinks - j : 0;
+                gap1 = ahead.it.p_lo - p.window + 1 - j;
+                want = want && !(gap0 == 0 && gap1 >= upto);
+            }
+        } else {
+            j += lane & (kSlice - 1);
+            want = any_sees(p, ahead.it, j);
+        }
         if (want) {
-            const int page = p.page_shift >= 0 ? j >> p.page_shift : j / p.b.page;
+            const int page = p.page_shift >= 0 ? j >> p.page_shift : (int)((unsigned)j / (unsigned)p.b.page);
             slot = j - page * p.b.page;
             entry = p.b.table[ahead.s * p.b.table_stride + page];
         }
@@ -168,6 +190,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
         }
     };
     const uint32_t ring = smem_of(smem) + warp * kStages * 2 * Sh::kSliceBytes;
+    // A lane copies 16-byte pieces of rows kStep apart.
+    constexpr int kPieces = kSlice * kChunks / 32, kStep = kChunks >= 32 ? 1 : 32 / kChunks;
+    const int lane_row = lane / kChunks, lane_chunk = lane % kChunks;
+    const bool in_head = lane_chunk * 8 < p.D;
     auto copy_unit = [&](int stage) {
         int64_t at = -1;
         if (want) {
@@ -176,15 +202,38 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
             else
                 at = entry * p.page_stride + slot * p.slot_stride + entry_head * p.head_stride;
         }
-        const uint32_t dst = ring + stage * 2 * Sh::kSliceBytes;
+        const uint32_t dst = ring + stage * 2 * Sh::kSliceBytes + lane_row * DP * 2;
+        auto piece = [&](int i, const uint16_t* k, const uint16_t* v, bool read) {
+            const uint32_t d = dst + i * kStep * DP * 2 + ((lane_chunk ^ lane_row ^ ((i * kStep) & 7)) << 4);
+            copy16(d, k, read);
+            copy16(d + Sh::kSliceBytes, v, read);
+        };
+        static_assert(kChunks <= 32, "a lane has one place in its rows");
+        if (paged) {
+            const bool some = at >= 0 && in_head;
+            const int64_t o = some ? at + lane_row * p.slot_stride + lane_chunk * 8 : 0, step = some ? kStep * p.slot_stride : 0;
+            const uint16_t* k = static_cast<const uint16_t*>(p.k) + o;
+            const uint16_t* v = static_cast<const uint16_t*>(p.v) + o;
+            if (upto == kSlice && gap1 <= gap0) {
 #pragma unroll
-        for (int i = 0; i < kSlice * kChunks / 32; ++i) {
-            const int e = i * 32 + lane, r = e / kChunks, c = e % kChunks;
-            const int64_t row = __shfl_sync(0xFFFFFFFFu, at, r);
-            const bool read = row >= 0 && c * 8 < p.D;
-            const int64_t o = read ? row + c * 8 : 0;
-            copy16(dst + chunk_at<DP>(r, c), static_cast<const uint16_t*>(p.k) + o, read);
-            copy16(dst + Sh::kSliceBytes + chunk_at<DP>(r, c), static_cast<const uint16_t*>(p.v) + o, read);
+                for (int i = 0; i < kPieces; ++i, k += step, v += step) piece(i, k, v, some);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int r = lane_row + i * kStep;
+                    const bool read = some && r < upto && (r < gap0 || r >= gap1);
+                    piece(i, read ? k + i * step : static_cast<const uint16_t*>(p.k),
+                          read ? v + i * step : static_cast<const uint16_t*>(p.v), read);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int64_t row = __shfl_sync(0xFFFFFFFFu, at, lane_row + i * kStep);
+                const bool read = row >= 0 && in_head;
+                const int64_t o = read ? row + lane_chunk * 8 : 0;
+                piece(i, static_cast<const uint16_t*>(p.k) + o, static_cast<const uint16_t*>(p.v) + o, read);
+            }
         }
     };
     look_up();
@@ -198,11 +247,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     bool go = true;
     while (go) {
         // Queries of the piece: rows of DP, zeros behind D and behind the item's rows.
-        const int64_t row0 = (int64_t)w.item * kRows;
-        auto query_at = [&](int r) {  // token and query head of row r, as an element offset in q
-            const int64_t t = (row0 + r) / p.G;
-            const int g = (int)((row0 + r) - t * p.G);
-            return (w.q.q0 + t) * p.q_token + ((int64_t)w.head * p.G + g) * p.q_head;
+        if (threadIdx.x == 0) w.cut(runs, blockIdx.x, note);
+        auto token_of = [&](int r) { return (int)((unsigned)(w.it.r0 + r) / (unsigned)p.G); };  // from the item's first on
+        auto query_at = [&](int r) {  // row r's place in q
+            const int t = token_of(r), g = w.it.r0 + r - t * p.G;
+            return ((int64_t)w.q.q0 + w.it.t0 + t) * p.q_token + ((int64_t)w.head * p.G + g) * p.q_head;
         };
         for (int e = threadIdx.x; e < kRows * kChunks; e += kThreads) {
             const int r = e / kChunks, c = e % kChunks;
@@ -237,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = 16 * mt + 8 * h + (lane >> 2);
-                pos[mt][h] = r < w.it.rows ? w.q.len - w.q.n + (int)((row0 + r) / p.G) : -1;
+                pos[mt][h] = r < w.it.rows ? w.it.p_lo + token_of(r) : -1;
             }
         float o[MT][kTiles][4], m[MT][2], l[MT][2];  // m: maximum in use, in units of c q k
 #pragma unroll
@@ -258,17 +307,19 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
             look_up();
             const uint32_t ks0 = ring + stage * 2 * Sh::kSliceBytes, vs0 = ks0 + Sh::kSliceBytes;
             const int j0 = w.key0(u) + warp * kSlice;
-            float s[MT][2][4];
+            float s[MT][kNT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[mt][nt][i] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) {
-                uint32_t b[4];  // keys 0-7 low, high; keys 8-15 low, high
-                ldsm4(ks0 + chunk_at<DP>((lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), b);
+                uint32_t b[kNT / 2][4];  // of 16 keys: 0-7 low, high elements; 8-15 low, high
+#pragma unroll
+                for (int n = 0; n < kNT / 2; ++n)
+                    ldsm4(ks0 + chunk_at<DP>(16 * n + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)), b[n]);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     uint32_t a[4];
@@ -278,21 +329,22 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                     } else {
                         query(mt, ks, a);
                     }
-                    mma<BF16>(s[mt][0], a, b[0], b[1]);
-                    mma<BF16>(s[mt][1], a, b[2], b[3]);
+#pragma unroll
+                    for (int n = 0; n < kNT / 2; ++n) {
+                        mma<BF16>(s[mt][2 * n], a, b[n][0], b[n][1]);
+                        mma<BF16>(s[mt][2 * n + 1], a, b[n][2], b[n][3]);
+                    }
                 }
             }
             const bool masked = !all_see(p, w.it, j0, kSlice);
+            if (masked)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float& x = s[mt][nt][i];
-                        x *= p.c;
-                        if (masked && !sees(p, pos[mt][i >> 1], j0 + 8 * nt + 2 * (lane & 3) + (i & 1))) x = -INFINITY;
-                    }
+                        for (int i = 0; i < 4; ++i)
+                            if (!sees(p, pos[mt][i >> 1], j0 + 8 * nt + 2 * (lane & 3) + (i & 1))) s[mt][nt][i] = -INFINITY;
             // Maxima of the rows; lanes of a quad share a row.
             bool raise = false;
             float top[MT][2];
@@ -300,9 +352,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float v = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
+                    float v = fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]);
+#pragma unroll
+                    for (int nt = 1; nt < kNT; ++nt) v = fmaxf(v, fmaxf(s[mt][nt][2 * h], s[mt][nt][2 * h + 1]));
                     v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-                    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+                    v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2)) * p.c;
                     top[mt][h] = v;
                     raise |= v > m[mt][h] + kSlack || (m[mt][h] == -INFINITY && v > -INFINITY);
                 }
@@ -323,23 +377,23 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                         }
                     }
             }
-            uint32_t pa[MT][4], pb[SPLIT ? MT : 1][4];
+            uint32_t pa[MT][kNT / 2][4], pb[SPLIT ? MT : 1][kNT / 2][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float base = m[mt][h] == -INFINITY ? 0.0f : m[mt][h] - kShift;
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
+                    for (int nt = 0; nt < kNT; ++nt) {
                         float& x = s[mt][nt][2 * h];
                         float& y = s[mt][nt][2 * h + 1];
-                        x = exp2_fast(x - base);
-                        y = exp2_fast(y - base);
+                        x = exp2_fast(fmaf(x, p.c, -base));
+                        y = exp2_fast(fmaf(y, p.c, -base));
                         l[mt][h] += x + y;
                         const uint32_t two = pack2<BF16>(x, y);
-                        pa[mt][2 * nt + h] = two;
+                        pa[mt][nt >> 1][2 * (nt & 1) + h] = two;
                         if constexpr (SPLIT)
-                            pb[mt][2 * nt + h] = pack2<BF16>(x - value_of<BF16>(two & 0xFFFFu), y - value_of<BF16>(two >> 16));
+                            pb[mt][nt >> 1][2 * (nt & 1) + h] = pack2<BF16>(x - value_of<BF16>(two & 0xFFFFu), y - value_of<BF16>(two >> 16));
                     }
                 }
             }
@@ -349,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
             if (masked && w.it.p_lo != w.it.p_hi) {
                 bool bad = false;
 #pragma unroll
-                for (int i = 0; i < kSlice * kChunks / 32; ++i) {
+                for (int i = 0; i < kPieces; ++i) {
                     uint32_t v[4];
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
@@ -369,9 +423,11 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 // Key k's weight is in lane (k % 8) / 2 of the quad, element k % 2 of tile k / 8.
-                                const float e0 = k < 8 ? s[mt][0][2 * h] : s[mt][1][2 * h];
-                                const float e1 = k < 8 ? s[mt][0][2 * h + 1] : s[mt][1][2 * h + 1];
-                                wt[mt][h] = __shfl_sync(0xFFFFFFFFu, (k & 1) ? e1 : e0, (lane & ~3) | ((k & 7) >> 1));
+                                float e = 0.0f;
+#pragma unroll
+                                for (int nt = 0; nt < kNT; ++nt)
+                                    if (k >> 3 == nt) e = (k & 1) ? s[mt][nt][2 * h + 1] : s[mt][nt][2 * h];
+                                wt[mt][h] = __shfl_sync(0xFFFFFFFFu, e, (lane & ~3) | ((k & 7) >> 1));
                                 see[mt][h] = sees(p, pos[mt][h], j0 + k);
                             }
 #pragma unroll
@@ -399,19 +455,21 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                 }
             }
 #pragma unroll
-            for (int t = 0; t < kTiles; t += 2) {
-                uint32_t b[4];  // tile t: keys 0-7, 8-15; tile t + 1: the same
-                ldsm4t(vs0 + chunk_at<DP>(lane & 15, t + (lane >> 4)), b);
+            for (int n = 0; n < kNT / 2; ++n)
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    mma<BF16>(o[mt][t], pa[mt], b[0], b[1]);
-                    mma<BF16>(o[mt][t + 1], pa[mt], b[2], b[3]);
-                    if constexpr (SPLIT) {
-                        mma<BF16>(o[mt][t], pb[mt], b[0], b[1]);
-                        mma<BF16>(o[mt][t + 1], pb[mt], b[2], b[3]);
+                for (int t = 0; t < kTiles; t += 2) {
+                    uint32_t b[4];  // tile t: keys 0-7, 8-15; tile t + 1: the same
+                    ldsm4t(vs0 + chunk_at<DP>(16 * n + (lane & 15), t + (lane >> 4)), b);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        mma<BF16>(o[mt][t], pa[mt][n], b[0], b[1]);
+                        mma<BF16>(o[mt][t + 1], pa[mt][n], b[2], b[3]);
+                        if constexpr (SPLIT) {
+                            mma<BF16>(o[mt][t], pb[mt][n], b[0], b[1]);
+                            mma<BF16>(o[mt][t + 1], pb[mt][n], b[2], b[3]);
+                        }
                     }
                 }
-            }
             if (++stage == kStages) stage = 0;
         }
 
@@ -479,16 +537,15 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
         }
         if (warp == 0) {
             const bool whole = w.whole();
-            float* const part = whole ? nullptr : p.part + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
+            float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int r = 16 * mt + 8 * h + (lane >> 2);
                     if (r >= w.it.rows) continue;
-                    const int64_t t = (row0 + r) / p.G;
-                    const int head = w.head * p.G + (int)(row0 + r - t * p.G);
-                    const int64_t row = w.q.q0 + t;
+                    const int t = token_of(r), head = w.head * p.G + (w.it.r0 + r - t * p.G);
+                    const int64_t row = (int64_t)w.q.q0 + w.it.t0 + t;
                     if (whole) {
                         const float f = sum[mt][h] == 0.0f ? 0.0f : 1.0f / sum[mt][h];
                         const int64_t at = row * p.o_token + head * p.o_head;
@@ -582,7 +639,7 @@ int attn_mma(const AttnParams& p, int dtype, int rows, cudaStream_t st) {
                           : p.D <= 128 ? (two ? launch<128, 2>(p, bf, st) : launch<128, 1>(p, bf, st))
                                        : launch<256, 1>(p, bf, st);
     if (e != cudaSuccess) return cuda_fail(e, "attention launch");
-    const cudaError_t j = launch_attn_join(p, rows, kKeys, attn_mma_grid(p.D), st);
+    const cudaError_t j = launch_attn_join(p, rows, attn_mma_grid(p.D), st);
     return j == cudaSuccess ? NXQ_OK : cuda_fail(j, "attention join launch");
 }
 

@@ -9,7 +9,8 @@
 // share of consecutive units, whatever the lengths are.  A run that holds an item
 // whole writes its output; pieces of an item cut between runs go to the workspace,
 // two slots a run (0: a piece that starts inside an item, 1: one that starts an item
-// and does not end it), and the join kernel adds them up in order of the runs.
+// and does not end it), the run in which the item starts leaves a note of it, and the
+// join kernel adds the pieces up in order of the runs.
 #pragma once
 #include "attention.h"
 
@@ -18,9 +19,15 @@ namespace attn {
 
 constexpr int kPlanChunk = 256;  // sequences looked at together
 
-// Rows [row0, row0 + rows) of a sequence's n G, and their units.
+__device__ __forceinline__ long long divide(long long n, int d) {
+    return (unsigned long long)n >> 32 ? n / d : (long long)((unsigned)n / (unsigned)d);
+}
+
+// An item's rows: row r is token t0 + (r0 + r) / G of its sequence's new ones, query head
+// (r0 + r) % G.
 struct Item {
     int rows;
+    int t0, r0;
     int p_lo, p_hi;        // positions of the first and the last row
     int head_blocks;       // units that hold the sinks (blocks 0 ..)
     int skip;              // unit u >= head_blocks is block u + skip
@@ -30,10 +37,12 @@ struct Item {
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Item make_item(const AttnParams& p, const Seq& q, int j) {
     Item it;
-    const int64_t total = (int64_t)q.n * p.G, row0 = (int64_t)j * ROWS;
-    it.rows = (int)(total - row0 < ROWS ? total - row0 : ROWS);
-    it.p_lo = q.len - q.n + (int)(row0 / p.G);
-    it.p_hi = q.len - q.n + (int)((row0 + it.rows - 1) / p.G);
+    const int total = q.n * p.G, row0 = j * ROWS;  // below 2^31 (nxq_paged_attention)
+    it.rows = total - row0 < ROWS ? total - row0 : ROWS;
+    it.t0 = (int)((unsigned)row0 / (unsigned)p.G);
+    it.r0 = row0 - it.t0 * p.G;
+    it.p_lo = q.len - q.n + it.t0;
+    it.p_hi = it.p_lo + (int)((unsigned)(it.r0 + it.rows - 1) / (unsigned)p.G);
     const int end = it.p_hi < 0 ? 0 : it.p_hi / KEYS + 1;  // blocks up to the last visible key
     int lo = 0, heads = 0;
     if (p.window > 0 && it.p_lo >= p.window) {
@@ -53,7 +62,7 @@ __device__ __forceinline__ Item make_item(const AttnParams& p, const Seq& q, int
 // Items of a sequence and key head.
 template <int ROWS>
 __device__ __forceinline__ int items_of(const AttnParams& p, const Seq& q) {
-    return (int)(((int64_t)q.n * p.G + ROWS - 1) / ROWS);
+    return (int)(((unsigned)(q.n * p.G) + ROWS - 1) / ROWS);
 }
 // Sequence s if it is this launch's, else one without rows.
 __device__ __forceinline__ Seq launch_seq(const AttnParams& p, int s, bool* bad) {
@@ -159,7 +168,7 @@ __device__ __forceinline__ void plan_locate(const AttnParams& p, PlanSmem& sm, l
     if (threadIdx.x < 32) {
         const int i = warp_locate([&](int i) { return sm.units[i] * p.Hk; }, kPlanChunk, x);
         const long long per = sm.units[i];
-        const int head = (int)(x / per);
+        const int head = (int)(((unsigned long long)x | per) >> 32 ? x / per : (unsigned)x / (unsigned)per);
         x -= head * per;
         bool bad;
         const Seq q = launch_seq(p, c * kPlanChunk + i, &bad);
@@ -176,8 +185,33 @@ __device__ __forceinline__ void plan_locate(const AttnParams& p, PlanSmem& sm, l
     __syncthreads();
 }
 
-// First unit of run r of `runs`.
-__device__ __forceinline__ long long run_start(long long total, unsigned r, unsigned runs) { return total * r / runs; }
+// The units of a launch's runs: run r < live has units each, or one more if r < more;
+// the other runs (fewer units than runs) have none.
+struct Runs {
+    long long each;
+    int more, live;
+    __device__ __forceinline__ Runs(long long total, int grid) {
+        live = total < grid ? (int)total : grid;
+        each = live ? divide(total, live) : 0;
+        more = (int)(total - each * live);
+    }
+    __device__ __forceinline__ long long start(int r) const { return r < live ? each * r + (r < more ? r : more) : each * live + more; }
+    __device__ __forceinline__ long long units(int r) const { return r < live ? each + (r < more) : 0; }
+    // Runs that `left` units behind run r, directly after it, reach into.
+    __device__ __forceinline__ int behind(int r, int left) const {
+        if (each >= left) return 1;
+        const unsigned e = (unsigned)each, big = more > r + 1 ? more - r - 1 : 0;  // of them with a unit more
+        return (unsigned long long)big * (e + 1) >= (unsigned)left ? (left + e) / (e + 1) : big + (left - big * (e + 1) + e - 1) / e;
+    }
+};
+
+// What the join kernel has to do for a run: the item that begins in it and ends behind it.
+struct Cut {
+    int pieces;  // 0: there is none
+    int rows, r0, t0;
+    int q0, head, pad[2];
+};
+__host__ __device__ inline size_t cuts_bytes(unsigned runs) { return runs * sizeof(Cut); }
 
 // Walks a run's pieces.  Every lane of a warp holds the same values.
 template <int ROWS, int KEYS>
@@ -222,6 +256,11 @@ struct Walk {
     }
     __device__ __forceinline__ bool whole() const { return count == it.units; }
     __device__ __forceinline__ int slot() const { return off ? 0 : 1; }  // of a piece that is not whole
+    // The cut of run r, if this piece is its first.
+    __device__ __forceinline__ void cut(const Runs& runs, int r, Cut* to) const {
+        if (off || whole()) return;
+        *to = Cut{1 + runs.behind(r, it.units - count), it.rows, it.r0, it.t0, q.q0, head, {0, 0}};
+    }
     // First key of the piece's unit u.
     __device__ __forceinline__ int key0(int u) const {
         u += off;
@@ -242,7 +281,8 @@ __device__ __forceinline__ bool any_sees(const AttnParams& p, const Item& it, in
     return j <= it.p_hi && (p.window <= 0 || j > it.p_lo - p.window || j < p.sinks);
 }
 
-// A partial result in the workspace: [ROWS][D] fp32 sums of weights times values, then
+// The workspace: Cut [runs], then slots [runs][2] of partial results.
+// A partial result: [ROWS][D] fp32 sums of weights times values, then
 // [ROWS] maxima (in units of c q k) and [ROWS] sums of weights, all relative to the maximum.
 __host__ __device__ inline size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }
 

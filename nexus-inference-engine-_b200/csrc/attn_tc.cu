@@ -3,25 +3,28 @@
 //
 // A persistent grid of one CTA per SM, each with an equal share of the call's units
 // (attn_plan.cuh): an item is 256 rows of one (sequence, key head) as two tiles of 128, a
-// unit one block of 128 keys with its values, which both tiles share.  Roles:
+// unit one block of 64 keys with its values, which both tiles share.  Roles:
 //   warp 0      producer: keys and values by TMA, one box per page (or part of one) and 64
 //               elements, straight from the scattered pages into 128-byte-swizzled
-//               blocks [64 elements][128 keys]; five of them in a ring
-//   warp 1      issues tcgen05.mma: S_t = Q_t K^T (fp32 in TMEM), O_t += P_t V with P_t
-//               from TMEM and V as it lies (its head elements contiguous)
+//               blocks [64 elements][64 keys]; ten of them in a ring
+//   warps 1, 12 issue tcgen05.mma, one for each tile: S_t = Q_t K^T (fp32 in TMEM), O_t +=
+//               P_t V with P_t from TMEM and V as it lies (its head elements contiguous)
 //   warps 2, 3  bring an item's queries into shared memory, and look through the values of
 //               units that not all rows see for any that is infinite or NaN (they take
 //               part in handing every block back: a wait by phase parity must see every phase)
 //   warps 4-7   softmax of tile 0, 8-11 of tile 1: a thread per row, so a row's maximum
 //               and sum need no shuffles; reads S_t, writes P_t over it, corrects O_t
 //               when the maximum in use is raised, and stores the outputs
-// While one tile's weights are computed, the other's products run: S_t of a unit is
-// issued right after O_t of the one before.  tcgen05.mma of one thread run in order, so
-// S_t being there tells that O_t is up to date, and the next S_t may be issued over a
-// P_t that is still to be read.
+// S_t has two buffers and is issued two units ahead of the O_t += P_t V that needs it,
+// across items as well, so the softmax warps find the next scores there, and the
+// tiles, which nothing but the blocks ties together, take turns at the exponential unit.  (One buffer of 128 keys, each tile's
+// softmax beside the other's products: 4000 cycles for 128 keys, of which 1660 waiting for
+// the tile's own products.)  tcgen05.mma of one thread run in order, so S_t may be issued
+// over a P_t that is still to be read.
 //
-// Bound by the exponentials and the products alike: a unit is 4 x 512 cycles of MMA (D =
-// 128) and 2 x 128 x 128 exponentials, 16 a cycle, 2048 cycles.
+// Bound by the exponentials and the products alike: 128 keys are 2 x 128 x 128 exponentials,
+// 16 a cycle, 2048 cycles, and, at D = 128, about 2500 cycles of MMA (scores of 64 keys
+// take 128 + 64 rows from shared memory, 48 cycles for 32 of arithmetic).
 //
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8 (so O_t is seldom read back), f16 ones times 2^7; rounding and SPLIT as in
@@ -41,18 +44,19 @@ namespace {
 using namespace attn;
 
 constexpr int kThreads = 384, kTile = 128, kRows = 2 * kTile, kKeys = 128;
-constexpr int kWarpProducer = 0, kWarpMma = 1, kWarpHelper0 = 2, kHelpers = 64, kWarpSoft0 = 4;
-constexpr int kSlots = 5;
+constexpr int kWarpProducer = 0, kWarpMma = 1, kWarpHelper = 2, kWarpSoft0 = 4;
+constexpr int kSlots = 5, kAhead = 1;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kColS = 0, kColO = 2 * kKeys;  // S_t at kColS + 128 t, O_t at kColO + 128 t
+constexpr int kColO = 2 * kKeys;  // S_t at kKeys t, O_t at kColO + 128 t
 constexpr float kSlack = 8.0f;
-constexpr int kChunkBytes = kKeys * 128;  // 64 elements of 128 keys (or rows)
+constexpr int kChunkBytes = kKeys * 128, kQChunkBytes = kTile * 128;  // 64 elements of a block's keys, of a tile's rows
 
 template <int DP>
 struct Shape {
     static constexpr int kChunks = DP / 64;
-    static constexpr int kBlock = kChunks * kChunkBytes;  // 128 keys, values, or rows of queries
-    static constexpr int kSmem = 1024 + 2 * kBlock + kSlots * kBlock + 512;
+    static constexpr int kBlock = kChunks * kChunkBytes;    // keys, or values, of a unit
+    static constexpr int kQTile = kChunks * kQChunkBytes;  // queries of a tile
+    static constexpr int kSmem = 1024 + 2 * kQTile + kSlots * kBlock + 512;
     static_assert(sizeof(PlanSmem) <= kSlots * kBlock, "the plan is made where the ring will be");
     static_assert(kSmem <= 227 * 1024, "");
 };
@@ -103,13 +107,26 @@ __device__ __forceinline__ bool not_finite(uint32_t bits) {
     return (bits & m) == m;
 }
 
+// The larger of a and |b| in both halves; NaN if either is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    b &= 0x7FFF7FFFu;
+    if constexpr (BF16)
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // A and B of the same 16-bit type, fp32 accumulation; b_mn: B's N elements are contiguous.
 __host__ __device__ constexpr uint32_t idesc16(bool bf16, int n, bool b_mn) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 
-// Position in the ring of key and value blocks, and the parity of its current use.
+// The blocks of a run's units: keys of unit 0, then values of unit g and keys of unit g + 1
+// (while there are), g = 0, 1, ...  Position in the ring, and the parity of its current use.
 struct Ring {
     int i = 0;
     uint32_t ph = 0;
@@ -128,14 +145,15 @@ __device__ __forceinline__ bool mixed(const AttnParams& p, const Item& it, int j
 template <bool BF16, bool SPLIT, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
-                   const __grid_constant__ CUtensorMap vmap, const int box) {
+                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap, const int box,
+                   const int q_boxes) {
     using Sh = Shape<DP>;
     using W = Walk<kRows, kKeys>;
     constexpr float kShift = BF16 ? 0.0f : 7.0f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
     uint8_t* const qs = smem;
-    uint8_t* const ring = qs + 2 * Sh::kBlock;
+    uint8_t* const ring = qs + 2 * Sh::kQTile;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(ring + kSlots * Sh::kBlock);
     uint64_t* const kv_full = bars;
     uint64_t* const kv_empty = kv_full + kSlots;
@@ -143,14 +161,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* const q_full = looked + kSlots;
     uint64_t* const q_empty = q_full + 1;
     uint64_t* const s_full = q_empty + 1;  // [tile]
-    uint64_t* const p_full = s_full + 2;
-    uint64_t* const o_full = p_full + 2;
-    uint64_t* const meet = o_full + 2;  // the softmax warps: of tile 0 alone, of both
+    uint64_t* const p_full = s_full + 2;   // [tile]
+    uint64_t* const o_full = p_full + 2;   // [tile] the item's products are in O_t
+    uint64_t* const meet = o_full + 2;     // the softmax warps: of tile 0 alone, of both
     uint64_t* const drain = meet + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* const found = abort_flag + 1;     // [slot] its values are not all finite
     volatile int* const started = found + kSlots;   // [tile] O_t was set before its first product
+    static_assert((3 * kSlots + 2 + 6 + 2 + 1) * 8 + (2 + kSlots + 2) * 4 <= 512, "barrier area too small");
 
     PlanSmem& plan = *reinterpret_cast<PlanSmem*>(ring);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -158,11 +177,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             ptx::mbar_init(&kv_full[i], 1);
-            ptx::mbar_init(&kv_empty[i], 1 + kHelpers / 32);  // the products, and both helpers
-            ptx::mbar_init(&looked[i], kHelpers / 32);
+            ptx::mbar_init(&kv_empty[i], 2);  // the products, and the helper
+            ptx::mbar_init(&looked[i], 1);
             found[i] = 0;
         }
-        ptx::mbar_init(q_full, kHelpers / 32);
+        ptx::mbar_init(q_full, 1);
         ptx::mbar_init(q_empty, 1);
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(&s_full[t], 1);
@@ -189,20 +208,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     plan_total<kRows, kKeys, kThreads>(p, plan);
-    const long long total = plan.total, first = run_start(total, blockIdx.x, gridDim.x);
-    const long long units = run_start(total, blockIdx.x + 1, gridDim.x) - first;
+    const Runs runs(plan.total, gridDim.x);
+    const int units = (int)runs.units(blockIdx.x);  // (a run of 2^31 units would take an hour)
     W w;
     bool go = units > 0;
     if (go) {
-        plan_locate<kRows, kKeys, kThreads>(p, plan, first);
+        plan_locate<kRows, kKeys, kThreads>(p, plan, runs.start(blockIdx.x));
         w.start(p, plan, units);
     }
+    Cut* const note = static_cast<Cut*>(p.work) + blockIdx.x;
+    float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(p.work) + cuts_bytes(gridDim.x));
     __syncthreads();  // the plan has been read: its memory is the ring's
 
     if (warp == kWarpProducer) {
         if (lane == 0) {
             ptx::prefetch_tmap(&kmap);
             ptx::prefetch_tmap(&vmap);
+            note->pieces = 0;
         }
         // The plan, and the cache, were written through the generic proxy; TMA works through the async one.
         asm volatile("fence.proxy.async;" ::: "memory");
@@ -211,37 +233,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         const int boxes = kKeys / box, b = lane % boxes, chunk = lane / boxes;
         const bool mine = chunk < Sh::kChunks;
-        while (go && ok) {
-            const int32_t* const table = p.b.table + w.s * p.b.table_stride;
-            for (int u = 0; u < w.count && ok; ++u) {
-                const int j = w.key0(u) + b * box;
-                // Boxes without a key that a row sees read nothing: a page of -1 gives zeros.
-                const bool want = mine && j <= w.it.p_hi &&
-                                  (p.window <= 0 || j + box - 1 > w.it.p_lo - p.window || j < p.sinks);
-                int page = -1, slot = 0;
-                if (want) {
-                    const int n = p.page_shift >= 0 ? j >> p.page_shift : j / p.b.page;
-                    slot = j - n * p.b.page;
-                    page = table[n];
-                    if (page < 0 || page >= p.b.pages) {
-                        raise_index(p.status, kIndexPage);
-                        page = -1;
-                    }
-                }
+        // Where a unit's box of this lane lies.  The page entries of keys are asked for a unit
+        // ahead (a load of some 700 cycles, twice a unit, was what the ring waited for: 2235
+        // cycles for 64 keys), and values take the places of their keys two units before.
+        struct Place {
+            int page, slot, head;
+        };
+        Place places[kAhead + 1];  // of the keys copied last, the oldest first; then the next ones'
+        bool asked = false;        // a page is wanted for the last of them
+        int u = 0;                 // of w, whose unit is looked up next
+        auto look_up = [&]() {
+            const int j = w.key0(u) + b * box;
+            // Boxes without a key that a row sees read nothing: a page of -1 gives zeros.
+            Place& x = places[kAhead];
+            x = Place{-1, 0, w.head};
+            asked = mine && j <= w.it.p_hi && (p.window <= 0 || j + box - 1 > w.it.p_lo - p.window || j < p.sinks);
+            if (asked) {
+                const int n = p.page_shift >= 0 ? j >> p.page_shift : (int)((unsigned)j / (unsigned)p.b.page);
+                x.slot = j - n * p.b.page;
+                x.page = p.b.table[w.s * p.b.table_stride + n];
+            }
+            if (u == 0 && lane == 0) w.cut(runs, blockIdx.x, note);
+            if (++u == w.count) {
+                u = 0;
+                w.next(p);
+            }
+        };
+        auto copy = [&](const Place& x, const CUtensorMap* map) {
+            if (!(ok = ptx::warp_mbar_wait(&kv_empty[r.i], r.ph ^ 1u, ctl, 61))) return;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(&kv_full[r.i], Sh::kBlock);
+            __syncwarp();
+            if (mine)
+                ptx::tma_load_4d(ring + r.i * Sh::kBlock + chunk * kChunkBytes + b * box * 128, map, 64 * chunk, x.slot, x.head, x.page,
+                                 &kv_full[r.i]);
+            r.next();
+            ++issued;
+        };
+        if (go) {
+            look_up();
+            for (int g = -kAhead; g < units && ok; ++g) {
+                if (g >= 0) copy(places[0], &vmap);
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    ok = ok && ptx::warp_mbar_wait(&kv_empty[r.i], r.ph ^ 1u, ctl, 61);
-                    if (!ok) continue;
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&kv_full[r.i], Sh::kBlock);
-                    __syncwarp();
-                    if (mine)
-                        ptx::tma_load_4d(ring + r.i * Sh::kBlock + chunk * kChunkBytes + b * box * 128, kv ? &vmap : &kmap,
-                                         64 * chunk, slot, w.head, page, &kv_full[r.i]);
-                    r.next();
-                    ++issued;
+                for (int i = 0; i < kAhead; ++i) places[i] = places[i + 1];
+                if (ok && g + kAhead < units) {
+                    Place& x = places[kAhead - 1];
+                    if (asked && (x.page < 0 || x.page >= p.b.pages)) {
+                        raise_index(p.status, kIndexPage);
+                        x.page = -1;
+                    }
+                    if (g + kAhead + 1 < units) look_up();
+                    copy(x, &kmap);
                 }
             }
-            go = w.next(p);
         }
         // Do not leave with copies in flight (bounded, ignoring the abort flag).
         for (uint32_t k = issued >= kSlots ? issued - kSlots : 0; k < issued; ++k) {
@@ -253,180 +296,181 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t qd = ptx::desc_sw128_kmajor(ptx::smem_addr(qs)), kd = ptx::desc_sw128_kmajor(ptx::smem_addr(ring));
         const uint64_t vd = ptx::desc_sw128_mnmajor(ptx::smem_addr(ring), kChunkBytes);
         constexpr uint32_t kIdS = idesc16(BF16, kKeys, false), kIdO = idesc16(BF16, DP, true);
-        // S_t = Q_t K^T, from the block in slot i.
         const bool lead = ptx::elect_one();  // one lane issues, and commits what it issued
+        // S_t = Q_t K^T, the keys in slot i.
         auto scores = [&](int t, int i) {
-            if (!lead) return;
-            const uint64_t a = qd + ((uint32_t)(t * Sh::kBlock) >> 4), b = kd + ((uint32_t)(i * Sh::kBlock) >> 4);
+            const uint64_t a = qd + ((uint32_t)(t * Sh::kQTile) >> 4), b = kd + ((uint32_t)(i * Sh::kBlock) >> 4);
 #pragma unroll
             for (int c = 0; c < Sh::kChunks; ++c)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    ptx::mma_ss_f16(tmem + kColS + kKeys * t, a + c * (kChunkBytes >> 4) + 2 * k, b + c * (kChunkBytes >> 4) + 2 * k,
-                                    kIdS, c || k ? 1u : 0u);
+                for (int e = 0; e < 4; ++e)
+                    ptx::mma_ss_f16(tmem + kKeys * t, a + c * (kQChunkBytes >> 4) + 2 * e, b + c * (kChunkBytes >> 4) + 2 * e, kIdS,
+                                    c || e ? 1u : 0u);
+            ptx::mma_commit(&s_full[t]);
         };
-        // O_t (+)= P_t V, from the block in slot i.
-        auto outputs = [&](int t, int i, uint32_t accumulate) {
-            if (!lead) return;
+        // O_t (+)= P_t V, the values in slot i.
+        auto outputs = [&](int t, int i, bool fresh, bool last) {
             const uint64_t b = vd + ((uint32_t)(i * Sh::kBlock) >> 4);
+            const uint32_t accumulate = !fresh || started[t] ? 1u : 0u;
 #pragma unroll
             for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    ptx::mma_ts_f16(tmem + kColO + 128 * t, tmem + kColS + kKeys * t + 64 * h + 8 * k, b + k * (2048 >> 4), kIdO,
-                                    h || k ? 1u : accumulate);
+                for (int e = 0; e < kKeys / 16; ++e)
+                    ptx::mma_ts_f16(tmem + kColO + 128 * t, tmem + kKeys * t + 64 * h + 8 * e, b + e * (2048 >> 4), kIdO,
+                                    h || e ? 1u : accumulate);
+            if (last) ptx::mma_commit(&o_full[t]);
         };
-        auto commit = [&](uint64_t* bar) {
-            if (lead) ptx::mma_commit(bar);
-            __syncwarp();
-        };
-        Ring kr, vr;   // the next block of keys, and of values
-        vr.next();
-        uint32_t q_ph = 0, p_ph[2] = {0, 0};
+        Ring r;
+        uint32_t q_ph = 0, p_ph0 = 0, p_ph1 = 0;
         bool ok = true;
-        auto two = [](const W& x) { return x.it.rows > kTile; };
-        auto queries = [&]() {  // of the next piece
-            ok = ok && ptx::warp_mbar_wait(q_full, q_ph, ctl, 62);
-            q_ph ^= 1u;
-        };
-        int tiles = 0;
         if (go) {
-            queries();
-            ok = ok && ptx::warp_mbar_wait(&kv_full[kr.i], kr.ph, ctl, 63);
-            ptx::tc_fence_after();
-            tiles = two(w) ? 2 : 1;
-            if (ok)
-                for (int t = 0; t < tiles; ++t) {
-                    scores(t, kr.i);
-                    __syncwarp();
-                    commit(&s_full[t]);
+            int left = w.count;  // units of the piece from unit g on
+            bool two = w.it.rows > kTile, fresh = true;
+            // Step g: outputs of unit g and scores of unit g + 1, tile 0's and then tile 1's: a wait for all
+            // that a tile's need (different lanes for each barrier) and one go of the issuing lane.
+            for (int g = -1; g < units; ++g) {
+                const bool has_o = g >= 0, has_s = g + 1 < units, last = has_o && left == 1, had = two && has_o;
+                const bool s_fresh = has_s && (last || !has_o);
+                if (last && has_s) {
+                    w.next(p);
+                    left = w.count + 1;
+                    two = w.it.rows > kTile;
                 }
-            if (ok) {
-                commit(&kv_empty[kr.i]);
-                if (w.count == 1) commit(q_empty);
-            }
-            kr.next();
-            kr.next();
-        }
-        while (go && ok) {
-            for (int u = 0; u < w.count && ok; ++u) {
-                const bool last = u + 1 == w.count;
-                W after = w;
-                const bool more = !last || after.next(p);
-                const int next_tiles = !more ? 0 : last ? (two(after) ? 2 : 1) : tiles;
-                if (!(ok = ptx::warp_mbar_wait(&kv_full[vr.i], vr.ph, ctl, 64))) break;
-                bool keys = false;  // the next unit's keys (and queries) are there
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (t < tiles) {
-                        if (!(ok = ptx::warp_mbar_wait(&p_full[t], p_ph[t], ctl, 65))) break;
-                        p_ph[t] ^= 1u;
-                        ptx::tc_fence_after();
-                        outputs(t, vr.i, u > 0 || started[t] ? 1u : 0u);
-                        __syncwarp();
-                        if (last) commit(&o_full[t]);
-                    }
-                    if (t == tiles - 1) commit(&kv_empty[vr.i]);
-                    if (t < next_tiles) {
-                        if (!keys) {
-                            if (last) queries();
-                            ok = ok && ptx::warp_mbar_wait(&kv_full[kr.i], kr.ph, ctl, 66);
-                            if (!ok) break;
-                            ptx::tc_fence_after();
-                            keys = true;
-                        }
-                        scores(t, kr.i);
-                        __syncwarp();
-                        commit(&s_full[t]);
-                        if (t == next_tiles - 1) {
-                            commit(&kv_empty[kr.i]);
-                            if ((last ? after.count : w.count - u - 1) == 1) commit(q_empty);
-                        }
-                    }
+                const bool s_last = has_s && left == (has_o ? 2 : 1);
+                const Ring v = r;
+                if (has_o) r.next();
+                const Ring k = r;
+                if (has_s) r.next();
+                uint64_t* bar = has_o ? &kv_full[v.i] : &kv_full[k.i];
+                uint32_t ph = has_o ? v.ph : k.ph;
+                const int part = lane & 3;
+                if (part == 1 && has_o) bar = &p_full[0], ph = p_ph0;
+                if (part == 2 && has_s) bar = &kv_full[k.i], ph = k.ph;
+                if (part == 3 && s_fresh) bar = q_full, ph = q_ph;
+                if (!(ok = ptx::warp_mbar_wait(bar, ph, ctl, 64))) break;
+                ptx::tc_fence_after();
+                if (lead) {
+                    if (has_o) outputs(0, v.i, fresh, last);
+                    if (has_s) scores(0, k.i);
                 }
-                if (more) {
-                    kr.next();
-                    kr.next();
+                __syncwarp();
+                if (had) {
+                    if (!(ok = ptx::warp_mbar_wait(&p_full[1], p_ph1, ctl, 65))) break;
+                    ptx::tc_fence_after();
                 }
-                vr.next();
-                vr.next();
-                if (last) {
-                    go = more;
-                    w = after;
-                    tiles = next_tiles;
-                    break;
+                if (lead) {
+                    if (had) outputs(1, v.i, fresh, last);
+                    if (has_o) ptx::mma_commit(&kv_empty[v.i]);
+                    if (has_s && two) scores(1, k.i);
+                    if (has_s) ptx::mma_commit(&kv_empty[k.i]);
+                    if (s_last) ptx::mma_commit(q_empty);
                 }
+                __syncwarp();
+                p_ph0 ^= has_o;
+                p_ph1 ^= had;
+                q_ph ^= s_fresh;
+                left -= has_o;
+                fresh = s_fresh;
             }
         }
-        commit(drain);
+        if (lead) ptx::mma_commit(drain);
+        __syncwarp();
         const long long t0 = clock64();
         while (!ptx::mbar_try_wait(drain, 0) && clock64() - t0 < ptx::kWaitCycles) {
         }
-    } else if (warp < kWarpSoft0) {
-        // Helpers: warp h brings tile h's queries.
-        const int tile = warp - kWarpHelper0, tid = threadIdx.x - 32 * kWarpHelper0;
+    } else if (warp == kWarpHelper) {
         bool ok = true;
-        uint32_t q_ph = 0;
+        if (lane == 0 && q_boxes) ptx::prefetch_tmap(&qmap);
+        asm volatile("fence.proxy.async;" ::: "memory");  // (queries, as the cache above)
+        uint32_t q_ph = 0, q_loads = 0;
         bool first_piece = true;
-        Ring r;
-        while (go && ok) {
+        auto queries = [&](const W& x) {
             if (!first_piece) {
                 ok = ptx::warp_mbar_wait(q_empty, q_ph, ctl, 67);
                 q_ph ^= 1u;
-                if (!ok) break;
+                if (!ok) return;
             }
             first_piece = false;
-            const int64_t row0 = (int64_t)w.item * kRows + tile * kTile;
-            const int rows = w.it.rows - tile * kTile;
-            if (rows > 0) {
-                int64_t at[4];  // of rows lane, lane + 32, ...: their offset in q, -1 behind the last
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t f = row0 + 32 * i + lane, t = f / p.G;
-                    at[i] = 32 * i + lane < rows ? (w.q.q0 + t) * p.q_token + ((int64_t)w.head * p.G + (f - t * p.G)) * p.q_head : -1;
+            const int tiles = x.it.rows > kTile ? 2 : 1;
+            if (q_boxes) {
+                // Whole tokens in every tile: a box of their group's heads for each 64 elements.  (Rows
+                // behind the item's are other rows of q, or zeros, and are not stored.)
+                if (lane == 0) ptx::mbar_arrive_expect_tx(q_full, tiles * Sh::kQTile);
+                __syncwarp();
+                if (lane < tiles * Sh::kChunks) {
+                    const int tile = lane / Sh::kChunks, c = lane % Sh::kChunks;
+                    ptx::tma_load_3d(qs + tile * Sh::kQTile + c * kQChunkBytes, &qmap, 64 * c, x.head * p.G,
+                                     x.q.q0 + x.it.t0 + tile * (kTile / p.G), q_full);
                 }
-                uint8_t* const dst = qs + tile * Sh::kBlock;
-                const uint32_t dst32 = ptx::smem_addr(dst);
-                constexpr int kPer = DP / 8;  // 16-byte pieces of a row
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll 4
-                    for (int e = lane; e < 32 * kPer; e += 32) {
-                        const int r0 = e / kPer, c = e % kPer;
-                        const int64_t a = __shfl_sync(0xFFFFFFFFu, at[i], r0);
-                        const int row = 32 * i + r0;
-                        const uint32_t o = (c >> 3) * kChunkBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                        const bool read = a >= 0 && c * 8 < p.D;
-                        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (read ? a + c * 8 : 0);
-                        if (p.q_vec) {
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst32 + o), "l"(src), "r"(read ? 16 : 0)
-                                         : "memory");
-                        } else {
-                            uint32_t h[4] = {0u, 0u, 0u, 0u};
-                            if (read)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) h[k] = (uint32_t)src[2 * k] | (uint32_t)src[2 * k + 1] << 16;
-                            *reinterpret_cast<uint4*>(dst + o) = make_uint4(h[0], h[1], h[2], h[3]);
-                        }
-                    }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                ++q_loads;
+                return;
             }
+            // A lane has one 16-byte piece of rows kStep apart.
+            constexpr int kPer = DP / 8, kStep = 32 / kPer;
+            const int piece = lane % kPer, first = lane / kPer;
+            const int f = x.it.r0 + first, t = (int)((unsigned)f / (unsigned)p.G);
+            int g = f - t * p.G;
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + ((int64_t)x.q.q0 + x.it.t0 + t) * p.q_token +
+                                  ((int64_t)x.head * p.G + g) * p.q_head + piece * 8;
+            const int64_t to_token = p.q_token - p.G * p.q_head;
+            uint8_t* const dst = qs + (piece >> 3) * kQChunkBytes + first * 128;
+            const bool in_head = piece * 8 < p.D;
+#pragma unroll 8
+            for (int row = first, i = 0; i < tiles * kTile; row += kStep, i += kStep) {
+                uint8_t* const to = dst + (i / kTile) * (Sh::kQTile - kQChunkBytes) + i * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                const bool read = row < x.it.rows && in_head;
+                if (p.q_vec) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_addr(to)), "l"(read ? src : p.q),
+                                 "r"(read ? 16 : 0)
+                                 : "memory");
+                } else {
+                    uint32_t h[4] = {0u, 0u, 0u, 0u};
+                    if (read)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) h[k] = (uint32_t)src[2 * k] | (uint32_t)src[2 * k + 1] << 16;
+                    *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+                src += kStep * p.q_head;
+                for (g += kStep; g >= p.G; g -= p.G) src += to_token;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(q_full);
-            for (int u = 0; u < w.count && ok; ++u) {
-                const bool look = mixed(p, w.it, w.key0(u));
-                for (int kv = 0; kv < 2 && ok; ++kv, r.next()) {
+        };
+        if (go) {
+            Ring r;
+            W wk = w, wv = w;
+            int uk = 0, uv = 0;
+            for (int g = -kAhead; g < units && ok; ++g) {
+                if (g >= 0) {
+                    const int j0 = wv.key0(uv);
+                    const Item it = wv.it;
+                    if (++uv == wv.count) {
+                        uv = 0;
+                        wv.next(p);
+                    }
                     if (!(ok = ptx::warp_mbar_wait(&kv_full[r.i], r.ph, ctl, 68))) break;
-                    if (kv && look) {
-                        bool bad = false;
+                    if (mixed(p, it, j0)) {
+                        // The largest magnitude, NaN above all, among the keys that not all rows see: behind
+                        // the first row's position, or up to where the last row's window begins.
+                        const int behind = it.p_lo + 1 - j0, before = p.window > 0 ? it.p_hi - p.window + 1 - j0 : 0;
+                        const uint8_t* const block = ring + r.i * Sh::kBlock;
+                        uint32_t big = 0;
+                        auto look = [&](int from, int to) {
+                            from = from > 0 ? from : 0, to = to < kKeys ? to : kKeys;
 #pragma unroll 4
-                        for (int i = tid; i < Sh::kBlock / 16; i += kHelpers) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(ring + r.i * Sh::kBlock + 16 * i);
-                            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                            for (int i = 8 * from + lane; i < 8 * to; i += 32)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) bad |= not_finite<BF16>(x[k] & 0xFFFFu) || not_finite<BF16>(x[k] >> 16);
-                        }
-                        bad = __any_sync(0xFFFFFFFFu, bad);
+                                for (int c = 0; c < Sh::kChunks; ++c) {
+                                    const uint4 v = *reinterpret_cast<const uint4*>(block + c * kChunkBytes + 16 * i);
+                                    big = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(big, v.x), v.y), v.z), v.w);
+                                }
+                        };
+                        look(0, before);
+                        look(behind > before ? behind : before, kKeys);
+                        const bool bad = __any_sync(0xFFFFFFFFu, not_finite<BF16>(big & 0xFFFFu) || not_finite<BF16>(big >> 16));
                         if (lane == 0) {
                             if (bad) found[r.i] = 1;
                             ptx::mbar_arrive(&looked[r.i]);
@@ -434,91 +478,102 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(&kv_empty[r.i]);
+                    r.next();
+                }
+                if (g + kAhead < units) {
+                    if (uk == 0) {
+                        queries(wk);
+                        if (!ok) break;
+                    }
+                    if (++uk == wk.count) {
+                        uk = 0;
+                        wk.next(p);
+                    }
+                    if (!(ok = ptx::warp_mbar_wait(&kv_full[r.i], r.ph, ctl, 68))) break;
+                    if (lane == 0) ptx::mbar_arrive(&kv_empty[r.i]);
+                    __syncwarp();
+                    r.next();
                 }
             }
-            go = w.next(p);
         }
-    } else {
+        // Do not leave with copies in flight (as the producer).
+        if (q_loads) {
+            const long long t0 = clock64();
+            while (!ptx::mbar_try_wait(q_full, (q_loads - 1) & 1) && clock64() - t0 < ptx::kWaitCycles) {
+            }
+        }
+    } else if (warp >= kWarpSoft0) {
         // Softmax of tile t: a thread per row.
         const int t = (warp - kWarpSoft0) >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const uint32_t ts = tmem + lanes + kColS + kKeys * t, to = tmem + lanes + kColO + 128 * t;
-        uint32_t s_ph = 0, o_ph = 0, meet_ph[2] = {0, 0}, looked_ph = 0;  // looked_ph: a bit per slot
-        Ring r;
-        r.next();  // values
+        const uint32_t ts = tmem + lanes + kKeys * t, to = tmem + lanes + kColO + 128 * t;
+        uint32_t s_ph = 0, o_ph = 0;
+        uint32_t meet_ph[2] = {0, 0}, looked_ph = 0;  // looked_ph: a bit per slot
+        int left = units;        // of the run, from the piece's unit on
+        Ring r;                  // the unit's values
+        for (int i = 0; i < (units < kAhead ? units : kAhead); ++i) r.next();
+        auto step = [&]() {
+            r.next();
+            if (left > kAhead) r.next();
+            --left;
+        };
         bool ok = true;
         while (go && ok) {
             const int tiles = w.it.rows > kTile ? 2 : 1;
             if (t >= tiles) {  // (the ring moves on, and so do the units looked through)
-                for (int u = 0; u < w.count; ++u, r.next(), r.next())
+                for (int u = 0; u < w.count; ++u, step())
                     if (mixed(p, w.it, w.key0(u))) looked_ph ^= 1u << r.i;
                 go = w.next(p);
                 continue;
             }
-            const int64_t flat = (int64_t)w.item * kRows + t * kTile + row, tok = flat / p.G;
-            const int head = w.head * p.G + (int)(flat - tok * p.G);
+            const int flat = w.it.r0 + t * kTile + row, tok = (int)((unsigned)flat / (unsigned)p.G);
+            const int head = w.head * p.G + (flat - tok * p.G);
             const bool mine = t * kTile + row < w.it.rows;
-            const int pos = mine ? w.q.len - w.q.n + (int)tok : -1;
+            const int pos = mine ? w.it.p_lo + tok : -1;
             float m = -INFINITY, l = 0.0f;
-            for (int u = 0; u < w.count; ++u, r.next(), r.next()) {
+            // Raises the maximum in use of rows whose new one is too far above, and corrects what
+            // has been summed in unit u - 1 and before.
+            auto raise_to = [&](float now, int u) {
+                if (!__any_sync(0xFFFFFFFFu, now > m + kSlack || (m == -INFINITY && now > -INFINITY))) return;
+                const float to_m = fmaxf(m, now), f = m == -INFINITY ? 0.0f : exp2_fast(m - to_m);
+                m = to_m;
+                l *= f;
+                if (u == 0) return;
+#pragma unroll 1
+                for (int d = 0; d < DP; d += 16) {
+                    uint32_t o[16];
+                    ptx::tmem_ld16(to + d, o);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                    ptx::tmem_st16(to + d, o);
+                }
+                ptx::tmem_wait_st();
+            };
+            for (int u = 0; u < w.count; ++u, step()) {
                 const int j0 = w.key0(u);
+                // (With S_t of a unit O_t has the unit before.)
                 if (!(ok = ptx::warp_mbar_wait(&s_full[t], s_ph, ctl, 69))) break;
                 s_ph ^= 1u;
                 ptx::tc_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ptx::tmem_ld32(ts + 32 * i, s[i]);
-                ptx::tmem_wait_ld();
                 const bool hidden = mixed(p, w.it, j0);
-                if (hidden) {
-                    const int hi = pos - j0, lo = p.window > 0 ? pos - p.window - j0 : -1, sk = p.sinks - j0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int j = 32 * i + k;
-                            if (j > hi || (j <= lo && j >= sk)) s[i][k] = 0xFF800000u;
-                        }
-                }
-                float top[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    top[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-                    for (int k = 1; k < 32; k += 1) top[i] = fmaxf(top[i], __uint_as_float(s[i][k]));
-                }
-                const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c;
-                const bool raise = now > m + kSlack || (m == -INFINITY && now > -INFINITY);
-                if (__any_sync(0xFFFFFFFFu, raise)) {
-                    const float to_m = fmaxf(m, now), f = m == -INFINITY ? 0.0f : exp2_fast(m - to_m);
-                    m = to_m;
-                    l *= f;
-                    if (u > 0) {
-#pragma unroll 1
-                        for (int d = 0; d < DP; d += 16) {
-                            uint32_t o[16];
-                            ptx::tmem_ld16(to + d, o);
-                            ptx::tmem_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            ptx::tmem_st16(to + d, o);
-                        }
-                        ptx::tmem_wait_st();
-                    }
-                }
-                const float base = m == -INFINITY ? 0.0f : m - kShift;
-                // A value that not all rows see may be infinite or NaN, and a weight of zero must
-                // not meet it: such elements are added to the rows that see them here, and are zeros
-                // to the product.
                 if (hidden) {
                     if (!(ok = ptx::warp_mbar_wait(&looked[r.i], (looked_ph >> r.i) & 1u, ctl, 70))) break;
                     looked_ph ^= 1u << r.i;
+                    // A value that not all rows see may be infinite or NaN, and a weight of zero must
+                    // not meet it: such elements are added to the rows that see them here, and are
+                    // zeros to the product.
                     if (found[r.i]) {
+                        float now = -INFINITY;
+#pragma unroll 1
+                        for (int k = 0; k < kKeys; ++k) {
+                            const float x = __uint_as_float(ptx::tmem_ld1(ts + k));
+                            ptx::tmem_wait_ld();
+                            if (sees(p, pos, j0 + k)) now = fmaxf(now, x * p.c);
+                        }
+                        raise_to(now, u);
+                        const float base = m == -INFINITY ? 0.0f : m - kShift;
                         uint8_t* const vs = ring + r.i * Sh::kBlock;
-                        auto value = [&](int k, int d) {
-                            return reinterpret_cast<uint16_t*>(vs + (d >> 6) * kChunkBytes + k * 128 +
-                                                               ((((d >> 3) & 7) ^ (k & 7)) << 4)) + (d & 7);
-                        };
                         if (u == 0) {
 #pragma unroll 1
                             for (int d = 0; d < DP; ++d) ptx::tmem_st1(to + d, 0u);
@@ -529,7 +584,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int k = 0; k < kKeys; ++k)
 #pragma unroll 1
                             for (int d = 0; d < DP; ++d) {
-                                const uint32_t bits = *value(k, d);
+                                const uint32_t bits = *(reinterpret_cast<const uint16_t*>(
+                                                            vs + (d >> 6) * kChunkBytes + k * 128 +
+                                                            ((((d >> 3) & 7) ^ (k & 7)) << 4)) + (d & 7));
                                 if (!not_finite<BF16>(bits)) continue;  // (the same in all lanes)
                                 float x = __uint_as_float(ptx::tmem_ld1(ts + k)), o = __uint_as_float(ptx::tmem_ld1(to + d));
                                 ptx::tmem_wait_ld();
@@ -538,12 +595,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 ptx::tmem_wait_st();
                             }
                         // Everybody has read them; then everybody has cleared them.
-                        for (int step = 0; step < 2 && ok; ++step) {
+                        for (int both = 0; both < 2 && ok; ++both) {
                             __syncwarp();
                             if (lane == 0) ptx::mbar_arrive(&meet[tiles - 1]);
                             ok = ptx::warp_mbar_wait(&meet[tiles - 1], meet_ph[tiles - 1], ctl, 71);
                             meet_ph[tiles - 1] ^= 1u;
-                            if (step == 0 && ok) {
+                            if (both == 0 && ok) {
                                 for (int i = threadIdx.x - 32 * kWarpSoft0; i < Sh::kBlock / 2; i += tiles * kTile) {
                                     uint16_t* e = reinterpret_cast<uint16_t*>(vs) + i;
                                     if (not_finite<BF16>(*e)) *e = 0;
@@ -555,24 +612,77 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (warp == kWarpSoft0 && lane == 0) found[r.i] = 0;
                     }
                 }
-                const uint64_t c2 = pair(p.c, p.c), b2 = pair(-base, -base);
+                // The scores do not fit the registers beside everything else: 64 keys are read, then the other
+                // 64 and made weights, then the first 64 again.
+                const int hi = pos - j0, lo = p.window > 0 ? pos - p.window - j0 : -1, sk = p.sinks - j0;
+                auto read = [&](int half, uint32_t (&s)[2][32]) {
+                    ptx::tmem_ld32(ts + 64 * half, s[0]);
+                    ptx::tmem_ld32(ts + 64 * half + 32, s[1]);
+                };
+                auto mask = [&](int half, uint32_t (&s)[2][32]) {
+                    if (!hidden) return;
+                    // 32 keys at a time, against the positions of the warp's rows: most are seen by all.
+                    const int low = __reduce_min_sync(0xFFFFFFFFu, hi), high = __reduce_max_sync(0xFFFFFFFFu, lo);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 64 * half + 32 * i;
+                        if (j + 31 > low)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (j + k > hi) s[i][k] = 0xFF800000u;
+                        if (j <= high && j + 31 >= sk)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k)
+                                if (j + k <= lo && j + k >= sk) s[i][k] = 0xFF800000u;
+                    }
+                };
+                auto largest = [&](const uint32_t (&s)[2][32]) {
+                    float top[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t* x = s[i >> 1] + 16 * (i & 1);
+                        top[i] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+#pragma unroll
+                        for (int k = 2; k < 16; k += 2) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[k])), __uint_as_float(x[k + 1]));
+                    }
+                    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                };
                 uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+                // Weights of 64 keys, packed (and what the packing leaves, SPLIT).
+                auto weights = [&](const uint32_t (&s)[2][32], uint64_t c2, uint64_t b2, uint32_t (&y)[32], uint32_t (&z)[SPLIT ? 32 : 1]) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t hi[16], lo[SPLIT ? 16 : 1];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        float2 x = unpair(fma2(pair(__uint_as_float(s[i][2 * k]), __uint_as_float(s[i][2 * k + 1])), c2, b2));
+                    for (int k = 0; k < 32; ++k) {
+                        const uint32_t* q = s[k >> 4] + 2 * (k & 15);
+                        float2 x = unpair(fma2(pair(__uint_as_float(q[0]), __uint_as_float(q[1])), c2, b2));
                         x.x = exp2_fast(x.x);
                         x.y = exp2_fast(x.y);
                         sum[k & 3] = add2(sum[k & 3], pair(x.x, x.y));
-                        hi[k] = pack2<BF16>(x.x, x.y);
-                        if constexpr (SPLIT)
-                            lo[k] = pack2<BF16>(x.x - value_of<BF16>(hi[k] & 0xFFFFu), x.y - value_of<BF16>(hi[k] >> 16));
+                        y[k] = pack2<BF16>(x.x, x.y);
+                        if constexpr (SPLIT) z[k] = pack2<BF16>(x.x - value_of<BF16>(y[k] & 0xFFFFu), x.y - value_of<BF16>(y[k] >> 16));
                     }
-                    ptx::tmem_st16(ts + 16 * i, hi);
-                    if constexpr (SPLIT) ptx::tmem_st16(ts + 64 + 16 * i, lo);
-                }
+                };
+                uint32_t s[2][32];
+                read(0, s);
+                ptx::tmem_wait_ld();
+                mask(0, s);
+                float now = largest(s);
+                read(1, s);
+                ptx::tmem_wait_ld();
+                mask(1, s);
+                now = fmaxf(now, largest(s));
+                raise_to(now * p.c, u);
+                const float base = m == -INFINITY ? 0.0f : m - kShift;
+                const uint64_t c2 = pair(p.c, p.c), b2 = pair(-base, -base);
+                uint32_t y1[32], z1[SPLIT ? 32 : 1], y0[32], z0[SPLIT ? 32 : 1], s0[2][32];
+                weights(s, c2, b2, y1, z1);
+                read(0, s0);
+                ptx::tmem_wait_ld();
+                ptx::tmem_st32(ts + 32, y1);
+                if constexpr (SPLIT) ptx::tmem_st32(ts + 96, z1);
+                mask(0, s0);
+                weights(s0, c2, b2, y0, z0);
+                ptx::tmem_st32(ts, y0);
+                if constexpr (SPLIT) ptx::tmem_st32(ts + 64, z0);
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
                 __syncwarp();
@@ -581,48 +691,60 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l += a.x + a.y;
             }
             if (!ok) break;
-            if (!(ok = ptx::warp_mbar_wait(&o_full[t], o_ph, ctl, 72))) break;
+            if (!(ok = ptx::warp_mbar_wait(&o_full[t], o_ph, ctl, 73))) break;
             o_ph ^= 1u;
             ptx::tc_fence_after();
             if (row == 0) started[t] = 0;
             const bool whole = w.whole();
-            float* const part = whole ? nullptr : p.part + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
+            float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
             const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t token = w.q.q0 + tok, at = token * p.o_token + head * p.o_head;
+            const int64_t token = (int64_t)w.q.q0 + w.it.t0 + tok, at = token * p.o_token + head * p.o_head;
+            const bool wide = p.o_vec > 1;
 #pragma unroll 1
-            for (int d = 0; d < DP && d < p.D; d += 16) {
-                uint32_t o[16];
-                ptx::tmem_ld16(to + d, o);
+            for (int d = 0; d < DP && d < p.D; d += 32) {
+                uint32_t o[32];
+                ptx::tmem_ld32(to + d, o);
                 ptx::tmem_wait_ld();
                 if (!mine) continue;
-                float v[16];
+                float v[32];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
+                for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]) * f;
+                if (!whole || p.y_dtype == NXQ_F32) {
+                    float* const q = whole ? static_cast<float*>(p.out) + at + d : part + (int64_t)(t * kTile + row) * p.D + d;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int e = d + 8 * h;
-                    if (e >= p.D) continue;
-                    const float* x = v + 8 * h;
-                    if (!whole || p.y_dtype == NXQ_F32) {
-                        float* q = whole ? static_cast<float*>(p.out) + at + e : part + (int64_t)(t * kTile + row) * p.D + e;
-                        if (!whole || p.o_vec) {
-                            *reinterpret_cast<float4*>(q) = make_float4(x[0], x[1], x[2], x[3]);
-                            *reinterpret_cast<float4*>(q + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                    for (int h = 0; h < 4; ++h) {
+                        if (d + 8 * h >= p.D) break;
+                        if (!whole || wide) {
+                            store_f32x8(q + 8 * h, v + 8 * h);
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) q[k] = x[k];
+                            for (int k = 0; k < 8; ++k) q[8 * h + k] = v[8 * h + k];
                         }
-                    } else {
-                        uint32_t y[4];
+                    }
+                } else {
+                    uint16_t* const q = static_cast<uint16_t*>(p.out) + at + d;
+                    uint32_t y[16];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            y[k] = p.y_dtype == NXQ_BF16 ? pack2<true>(x[2 * k], x[2 * k + 1]) : pack2<false>(x[2 * k], x[2 * k + 1]);
-                        uint16_t* q = static_cast<uint16_t*>(p.out) + at + e;
-                        if (p.o_vec) {
-                            *reinterpret_cast<uint4*>(q) = make_uint4(y[0], y[1], y[2], y[3]);
+                    for (int k = 0; k < 16; ++k)
+                        y[k] = p.y_dtype == NXQ_BF16 ? pack2<true>(v[2 * k], v[2 * k + 1]) : pack2<false>(v[2 * k], v[2 * k + 1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (d + 16 * h >= p.D) break;
+                        if (wide && d + 16 * h + 16 <= p.D) {
+                            store_f32x8(reinterpret_cast<float*>(q + 16 * h), reinterpret_cast<const float*>(y + 8 * h));
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) q[k] = (uint16_t)(y[k >> 1] >> (16 * (k & 1)));
+                            for (int e = 0; e < 2; ++e) {
+                                if (d + 16 * h + 8 * e >= p.D) break;
+                                const uint32_t* z = y + 8 * h + 4 * e;
+                                uint16_t* const to_y = q + 16 * h + 8 * e;
+                                if (p.o_vec) {
+                                    *reinterpret_cast<uint4*>(to_y) = make_uint4(z[0], z[1], z[2], z[3]);
+                                } else {
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) to_y[k] = (uint16_t)(z[k >> 1] >> (16 * (k & 1)));
+                                }
+                            }
                         }
                     }
                 }
@@ -670,6 +792,16 @@ int box_rows(int page) {
     return b;
 }
 
+// Queries [tokens][heads][D] in boxes of a group's heads and as many tokens as a tile has.
+int query_map(CUtensorMap* map, const AttnParams& p, bool bf16) {
+    const uint64_t dims[3] = {(uint64_t)p.D, (uint64_t)p.Hk * p.G, (uint64_t)p.b.T};
+    const uint64_t strides[2] = {2 * (uint64_t)p.q_head, 2 * (uint64_t)p.q_token};
+    const uint32_t boxes[3] = {64, (uint32_t)p.G, (uint32_t)(kTile / p.G)};
+    if (const int e = tensor_map_16(map, bf16, p.q, 3, dims, strides, boxes))
+        return fail(NXQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", e);
+    return NXQ_OK;
+}
+
 int cache_map(CUtensorMap* map, const nxq_kv_cache* c, const void* base, int box) {
     const uint64_t dims[4] = {(uint64_t)c->head_dim, (uint64_t)c->page_size, (uint64_t)c->heads, (uint64_t)c->pages};
     const uint64_t strides[3] = {2 * (uint64_t)c->slot_stride, 2 * (uint64_t)c->head_stride, 2 * (uint64_t)c->page_stride};
@@ -700,16 +832,22 @@ unsigned attn_tc_grid() { return (unsigned)context_sm_count(); }
 
 int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st) {
     const int box = box_rows(cache->page_size);
-    CUtensorMap k, v;
+    const bool bf = cache->dtype == NXQ_BF16, split = p.y_dtype == NXQ_F32;
+    CUtensorMap k, v, q{};
     int rc;
     if ((rc = cache_map(&k, cache, cache->k_dev, box)) || (rc = cache_map(&v, cache, cache->v_dev, box))) return rc;
-    const bool bf = cache->dtype == NXQ_BF16, split = p.y_dtype == NXQ_F32;
+    // Queries by TMA where tiles hold whole tokens and rows are such that a tensor map takes them; by
+    // 16-byte copies of two warps otherwise (10000 cycles for an item, against 2000).
+    const int64_t far = (int64_t)1 << 38;
+    const int q_boxes = kTile % p.G == 0 && p.q_vec && p.q_head > 0 && p.q_token > 0 && p.q_head < far && p.q_token < far;
+    if (q_boxes && (rc = query_map(&q, p, bf))) return rc;
     note_launches(1);
-    const cudaError_t e =
-        p.D <= 64 ? launch_overlapped(kernel_of<64>(bf, split), attn_tc_grid(), kThreads, Shape<64>::kSmem, st, p, k, v, box)
-                  : launch_overlapped(kernel_of<128>(bf, split), attn_tc_grid(), kThreads, Shape<128>::kSmem, st, p, k, v, box);
+    const cudaError_t e = p.D <= 64 ? launch_overlapped(kernel_of<64>(bf, split), attn_tc_grid(), kThreads, Shape<64>::kSmem, st,
+                                                        p, k, v, q, box, q_boxes)
+                                    : launch_overlapped(kernel_of<128>(bf, split), attn_tc_grid(), kThreads, Shape<128>::kSmem,
+                                                        st, p, k, v, q, box, q_boxes);
     if (e != cudaSuccess) return cuda_fail(e, "attention launch (tcgen05)");
-    const cudaError_t j = launch_attn_join(p, kRows, kKeys, attn_tc_grid(), st);
+    const cudaError_t j = launch_attn_join(p, kRows, attn_tc_grid(), st);
     return j == cudaSuccess ? NXQ_OK : cuda_fail(j, "attention join launch");
 }
 

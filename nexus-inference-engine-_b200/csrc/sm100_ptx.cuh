@@ -159,6 +159,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tmap, 
         : "memory");
 }
 
+// 3-D tiled TMA load of the box at (x, y, z).
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tmap, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+
 // 4-D tiled TMA load of the box at (x, y, z, w); out-of-range coordinates give zeros.
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tmap, int x, int y, int z, int w, uint64_t* bar) {
     asm volatile(
