@@ -40,29 +40,58 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     for (int k = 0; k < PER; ++k) {
         const int row = ((int)blockIdx.y * PER + k) * kJoinWarps + warp;
         if (row >= cut.rows) break;
-        float top = -INFINITY;
-        for (int i = lane; i < cut.pieces; i += 32) top = fmaxf(top, part_of(i)[(size_t)ROWS * p.D + row]);
+        // Outputs of piece i, eight of them asked for at a time, the first before the maxima are known.
+        auto outputs = [&](int i, float4 (&v)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v[h] = make_float4(0, 0, 0, 0);
+                if (i < cut.pieces && 4 * lane + 128 * h < p.D)
+                    v[h] = *reinterpret_cast<const float4*>(part_of(i) + (size_t)row * p.D + 4 * lane + 128 * h);
+            }
+        };
+        float4 v[8][2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) outputs(i, v[i]);
+        // Lane i has the factor of piece i0 + i; more than 32 pieces are looked at again.
+        float top = -INFINITY, mine = -INFINITY, sum = 0.0f;
+        auto statistics = [&](int i, float& m, float& l) {
+            m = -INFINITY, l = 0.0f;
+            if (i < cut.pieces) m = part_of(i)[(size_t)ROWS * p.D + row], l = part_of(i)[(size_t)ROWS * p.D + ROWS + row];
+        };
+        float l0;
+        statistics(lane, mine, l0);
+        top = mine;
+        for (int i = lane + 32; i < cut.pieces; i += 32) {
+            float m, l;
+            statistics(i, m, l);
+            top = fmaxf(top, m);
+        }
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        float sum = 0.0f;
         float acc[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-#pragma unroll 8
-        for (int i = 0; i < cut.pieces; ++i) {
-            const float* part = part_of(i);
-            const float m = part[(size_t)ROWS * p.D + row], l = part[(size_t)ROWS * p.D + ROWS + row];
-            float4 v[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+        for (int i0 = 0; i0 < cut.pieces; i0 += 32) {
+            if (i0) statistics(i0 + lane, mine, l0);
+            const float factor = mine > -INFINITY ? exp2f(mine - top) : 1.0f;  // (1: zeros, or NaN)
+            float part = l0 * factor;
+            for (int o = 16; o; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
+            sum += part;
+            const int n = cut.pieces - i0 < 32 ? cut.pieces - i0 : 32;
+            for (int j0 = 0; j0 < n; j0 += 8) {
+                if (i0 + j0)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (4 * lane + 128 * h < p.D) v[h] = *reinterpret_cast<const float4*>(part + (size_t)row * p.D + 4 * lane + 128 * h);
-            const float f = m > -INFINITY ? exp2f(m - top) : 1.0f;  // (1: zeros, or NaN)
-            sum = fmaf(l, f, sum);
+                    for (int j = 0; j < 8; ++j) outputs(i0 + j0 + j, v[j]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                acc[4 * h] = fmaf(v[h].x, f, acc[4 * h]);
-                acc[4 * h + 1] = fmaf(v[h].y, f, acc[4 * h + 1]);
-                acc[4 * h + 2] = fmaf(v[h].z, f, acc[4 * h + 2]);
-                acc[4 * h + 3] = fmaf(v[h].w, f, acc[4 * h + 3]);
+                for (int j = 0; j < 8; ++j) {
+                    const float f = __shfl_sync(0xFFFFFFFFu, factor, (j0 + j) & 31);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        acc[4 * h] = fmaf(v[j][h].x, f, acc[4 * h]);
+                        acc[4 * h + 1] = fmaf(v[j][h].y, f, acc[4 * h + 1]);
+                        acc[4 * h + 2] = fmaf(v[j][h].z, f, acc[4 * h + 2]);
+                        acc[4 * h + 3] = fmaf(v[j][h].w, f, acc[4 * h + 3]);
+                    }
+                }
             }
         }
         const int g = cut.r0 + row, t = (int)((unsigned)g / (unsigned)p.G), head = cut.head * p.G + (g - t * p.G);

@@ -99,6 +99,7 @@ template <int DP, int MT>
 struct Shape {
     static constexpr int kSlice = DP == 64 ? 32 : 16;  // keys of a unit per warp: 4 KB or more of each
     static constexpr int kKeys = kWarps * kSlice;
+    static constexpr int kStatic = 512;  // shared memory besides (Walks)
     static constexpr int kStages = DP <= 128 && MT == 1 ? 3 : 2;
     static constexpr int kRows = 16 * MT;
     static constexpr int kSliceBytes = kSlice * DP * 2;                 // a warp's keys (or values) of a unit
@@ -110,7 +111,7 @@ struct Shape {
     static constexpr int kShared0 = kJoin > (int)sizeof(PlanSmem) ? kJoin : (int)sizeof(PlanSmem);
     static constexpr int kShared = kShared0 > kQBytes ? kShared0 : kQBytes;
     static constexpr int kSmem = kRing + kShared + (kQInRegs ? 0 : kQBytes);
-    static constexpr int kCtas = 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
+    static constexpr int kCtas = 2 * (kSmem + 1024 + kStatic) <= 228 * 1024 ? 2 : 1;
 };
 
 // Swizzled offset of 16-byte chunk c of row r in a block of rows of DP 16-bit elements.
@@ -119,7 +120,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
     return (uint32_t)(r * DP * 2 + ((c ^ (r & 7)) << 4));
 }
 
-template <bool BF16, bool SPLIT, int DP, int MT>
+// MULTI: sequences may have several new tokens, so rows of an item may differ in what they see.
+template <bool BF16, bool SPLIT, bool MULTI, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using Sh = Shape<DP, MT>;
     constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kSlice = Sh::kSlice, kKeys = Sh::kKeys;
@@ -141,14 +143,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     float* const slots = reinterpret_cast<float*>(static_cast<uint8_t*>(p.work) + cuts_bytes(gridDim.x));
     if (threadIdx.x == 0) note->pieces = 0;
     plan_total<kRows, kKeys, kThreads>(p, plan);
-    const Runs runs(plan.total, gridDim.x);
-    const long long units = runs.units(blockIdx.x);
+    const long long total = plan.total, units = Runs(total, gridDim.x).units(blockIdx.x);
     if (units == 0) return;
-    plan_locate<kRows, kKeys, kThreads>(p, plan, runs.start(blockIdx.x));
+    plan_locate<kRows, kKeys, kThreads>(p, plan, Runs(total, gridDim.x).start(blockIdx.x));
 
-    W ahead, w;  // the piece being loaded, and the one being computed
+    // The piece being computed, and the one being loaded, each warp's for itself and in shared
+    // memory: registers are short.
+    __shared__ W aheads[kWarps];
+    __shared__ long long all_units;
+    static_assert(sizeof(aheads) + sizeof(all_units) <= Sh::kStatic, "");
+    W w;
     w.start(p, plan, units);
-    ahead = w;
+    W& ahead = aheads[warp];
+    if (lane == 0) ahead = w;
+    if (threadIdx.x == 0) all_units = total;
     __syncthreads();  // the plan has been read: its memory is the join's
     int au = 0;       // unit of `ahead` whose pages are looked up next
     bool more = true;
@@ -186,7 +194,10 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
         }
         if (++au == ahead.count) {
             au = 0;
-            more = ahead.next(p);
+            __syncwarp();  // (all have read it)
+            if (lane == 0) more = ahead.next(p);
+            more = __shfl_sync(0xFFFFFFFFu, more, 0);
+            __syncwarp();
         }
     };
     const uint32_t ring = smem_of(smem) + warp * kStages * 2 * Sh::kSliceBytes;
@@ -247,7 +258,6 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     bool go = true;
     while (go) {
         // Queries of the piece: rows of DP, zeros behind D and behind the item's rows.
-        if (threadIdx.x == 0) w.cut(runs, blockIdx.x, note);
         auto token_of = [&](int r) { return (int)((unsigned)(w.it.r0 + r) / (unsigned)p.G); };  // from the item's first on
         auto query_at = [&](int r) {  // row r's place in q
             const int t = token_of(r), g = w.it.r0 + r - t * p.G;
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
             // A value that not all rows see may be infinite or NaN, and its weight of zero
             // must not meet it: such elements are added to the rows that see them one by
             // one, and are zeros to the product below.
-            if (masked && w.it.p_lo != w.it.p_hi) {
+            if (MULTI && masked && w.it.p_lo != w.it.p_hi) {
                 bool bad = false;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
@@ -537,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
         }
         if (warp == 0) {
             const bool whole = w.whole();
+            if (lane == 0) w.cut(Runs(all_units, gridDim.x), blockIdx.x, note);
             float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -590,16 +601,20 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     copies_wait<0>();
 }
 
+template <int DP, int MT, bool BF16, bool SPLIT>
+auto* kernel_of(bool multi) {
+    return multi ? attn_mma_kernel<BF16, SPLIT, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, false, DP, MT>;
+}
 template <int DP, int MT>
-auto* kernel_of(bool bf16, bool split) {
-    return bf16 ? (split ? attn_mma_kernel<true, true, DP, MT> : attn_mma_kernel<true, false, DP, MT>)
-                : (split ? attn_mma_kernel<false, true, DP, MT> : attn_mma_kernel<false, false, DP, MT>);
+auto* kernel_of(bool bf16, bool split, bool multi) {
+    return bf16 ? (split ? kernel_of<DP, MT, true, true>(multi) : kernel_of<DP, MT, true, false>(multi))
+                : (split ? kernel_of<DP, MT, false, true>(multi) : kernel_of<DP, MT, false, false>(multi));
 }
 
 template <int DP, int MT>
 int set_attr() {
-    for (int i = 0; i < 4; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2), cudaFuncAttributeMaxDynamicSharedMemorySize,
+    for (int i = 0; i < 8; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2, i & 4), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    Shape<DP, MT>::kSmem);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
     }
@@ -614,7 +629,7 @@ unsigned grid_of() {
 
 template <int DP, int MT>
 cudaError_t launch(const AttnParams& p, bool bf16, cudaStream_t st) {
-    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32), grid_of<DP>(), kThreads, Shape<DP, MT>::kSmem, st, p);
+    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32, p.max_new > 1), grid_of<DP>(), kThreads, Shape<DP, MT>::kSmem, st, p);
 }
 
 }  // namespace

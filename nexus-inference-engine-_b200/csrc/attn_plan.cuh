@@ -73,10 +73,12 @@ __device__ __forceinline__ Seq launch_seq(const AttnParams& p, int s, bool* bad)
 }
 
 struct PlanSmem {
-    long long units[kPlanChunk];       // of each sequence of the chunk, per key head
+    Seq seqs[kPlanChunk];              // of the chunk looked at last
+    long long units[kPlanChunk];       // of each of them, per key head
     long long chunks[65536 / kPlanChunk];  // of each chunk
     long long total;                   // of all sequences and key heads
     // A unit's place.
+    Seq q;
     int s, head, item, off;
 };
 
@@ -90,15 +92,19 @@ __device__ __forceinline__ void plan_chunk(const AttnParams& p, PlanSmem& sm, in
     for (int i0 = 0; i0 < n; i0 += THREADS / share) {
         const int i = i0 + threadIdx.x / share, part = threadIdx.x % share;
         long long u = 0;
+        Seq q{0, 0, 0};
         if (i < n) {
             bool bad;
-            const Seq q = launch_seq(p, s0 + i, &bad);
+            q = launch_seq(p, s0 + i, &bad);
             if (bad && report && part == 0) raise_index(p.status, kIndexSeq);
             const int items = items_of<ROWS>(p, q);
             for (int j = part; j < items; j += share) u += make_item<ROWS, KEYS>(p, q, j).units;
         }
         for (int o = share / 2; o; o >>= 1) u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-        if (i < n && part == 0) sm.units[i] = u;
+        if (i < n && part == 0) {
+            sm.units[i] = u;
+            sm.seqs[i] = q;
+        }
     }
     for (int i = n + threadIdx.x; i < kPlanChunk; i += THREADS) sm.units[i] = 0;
 }
@@ -170,12 +176,12 @@ __device__ __forceinline__ void plan_locate(const AttnParams& p, PlanSmem& sm, l
         const long long per = sm.units[i];
         const int head = (int)(((unsigned long long)x | per) >> 32 ? x / per : (unsigned)x / (unsigned)per);
         x -= head * per;
-        bool bad;
-        const Seq q = launch_seq(p, c * kPlanChunk + i, &bad);
+        const Seq q = sm.seqs[i];
         const int items = items_of<ROWS>(p, q);
         const int j = warp_locate([&](int j) { return j < items ? (long long)make_item<ROWS, KEYS>(p, q, j).units : 0ll; },
                                   (items + 31) / 32 * 32, x);
         if (threadIdx.x == 0) {
+            sm.q = q;
             sm.s = c * kPlanChunk + i;
             sm.head = head;
             sm.item = j;
@@ -225,10 +231,8 @@ struct Walk {
 
     __device__ __forceinline__ void piece() { count = (int)(it.units - off < left ? it.units - off : left); }
     __device__ __forceinline__ void start(const AttnParams& p, const PlanSmem& sm, long long units) {
-        s = sm.s, head = sm.head, item = sm.item, off = sm.off;
+        q = sm.q, s = sm.s, head = sm.head, item = sm.item, off = sm.off;
         left = units;
-        bool bad;
-        q = launch_seq(p, s, &bad);
         items = items_of<ROWS>(p, q);
         it = make_item<ROWS, KEYS>(p, q, item);
         piece();

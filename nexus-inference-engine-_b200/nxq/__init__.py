@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import re
+import struct
 from pathlib import Path
 from typing import Optional
 
@@ -684,25 +685,11 @@ _LAYOUTS = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
 _SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3, "blend": 4}
 
 
-class _Heads(ctypes.Structure):
-    """nxq_heads"""
-
-    _fields_ = [("dev", _c.c_void_p), ("heads", _c.c_int), ("token_stride", _c.c_int64), ("head_stride", _c.c_int64)]
-
-
-class _Cache(ctypes.Structure):
-    """nxq_kv_cache"""
-
-    _fields_ = [("k_dev", _c.c_void_p), ("v_dev", _c.c_void_p), ("dtype", _c.c_int), ("pages", _c.c_int64),
-                ("page_size", _c.c_int), ("heads", _c.c_int), ("head_dim", _c.c_int), ("page_stride", _c.c_int64),
-                ("head_stride", _c.c_int64), ("slot_stride", _c.c_int64)]
-
-
-class _Batch(ctypes.Structure):
-    """nxq_kv_batch"""
-
-    _fields_ = [("sequences", _c.c_int), ("q_offsets_dev", _c.c_void_p), ("kv_lens_dev", _c.c_void_p),
-                ("block_table_dev", _c.c_void_p), ("table_stride", _c.c_int64), ("table_pages", _c.c_int64)]
+# The structures of these calls as bytes, which ctypes passes by address (a
+# ctypes.Structure takes three times as long to make).
+_HEADS = struct.Struct("Pi4xqq").pack      # nxq_heads: dev, heads, token_stride, head_stride
+_CACHE = struct.Struct("PPi4xqiii4xqqq").pack  # nxq_kv_cache
+_BATCH = struct.Struct("i4xPPPqq").pack    # nxq_kv_batch
 
 
 def rope_frequencies(dims: int, base: float = 10000.0, scaling: str = "plain", factor: float = 1.0,
@@ -756,37 +743,48 @@ def _on_device(what: str, name: str, t) -> int:
 
 def _rows(what: str, name: str, t, heads=None, head_dim=None, tokens=None):
     """nxq_heads of a tensor [T][heads][D] whose last dimension is contiguous."""
-    if t.dim() != 3:
-        raise _bad(f"{what}: {name} has {t.dim()} dimensions, not tokens, heads, elements")
-    T, H, D = t.shape
+    try:
+        T, H, D = t.shape
+        ts, hs, ds = t.stride()
+    except ValueError:
+        raise _bad(f"{what}: {name} has {t.dim()} dimensions, not tokens, heads, elements") from None
     if (heads is not None and H != heads) or (head_dim is not None and D != head_dim) or (tokens is not None and T != tokens):
         want = " ".join(f"[{'any' if x is None else x}]" for x in (tokens, heads, head_dim))
         raise _bad(f"{what}: {name} is {tuple(t.shape)}, not {want}")
-    _on_device(what, name, t)
-    ts, hs, ds = t.stride()
+    d = t.get_device()
+    if d < 0 or (d != _device and _device is not None):
+        raise _bad(f"{what}: {name} is on {t.device}, the library on cuda:{_device}")
     if ds != 1 and D > 1:
         raise _bad(f"{what}: the elements of {name}'s heads are not contiguous")
-    return _Heads(t.data_ptr(), H, ts, hs)
+    return _HEADS(t.data_ptr(), H, ts, hs)
 
 
 def _norm(what: str, name: str, w, head_dim: int):
     if w is None:
         return None
-    if w.dtype is not _torch.float32 or tuple(w.shape) != (head_dim,):
+    if w.dtype is not _torch.float32 or w.dim() != 1 or w.shape[0] != head_dim:
         raise _bad(f"{what}: {name} must be fp32 [{head_dim}]")
     _usable(what, name, w)
     return w.data_ptr()
 
 
-def _rows_out(what: str, out, like, dtype, stream):
-    """`out` if given (any strides of tokens and heads), else a new tensor of `like`'s shape; and its type's code."""
+def _rows_out(what: str, name: str, out, like, dtype, stream):
+    """`out` if given (any strides of tokens and heads), else a new tensor of
+    `like`'s shape; its nxq_heads and its type's code."""
     if out is None:
-        return _output(what, None, tuple(like.shape), dtype, like, stream)
-    if tuple(out.shape) != tuple(like.shape):
-        raise _bad(f"{what}: out has shape {tuple(out.shape)}, not {tuple(like.shape)}")
+        shape = like.shape
+        T, H, D = shape
+        dtype = dtype or _torch.float32
+        if stream is None or _is_current(stream, like.device):
+            out = _torch.empty_strided(shape, (H * D, D, 1), dtype=dtype, device=like.device)
+        else:
+            out, = _empty([(shape, dtype)], like.device, stream)
+        return out, _HEADS(out.data_ptr(), H, H * D, D), _float_code(what, name, dtype)
+    if out.shape != like.shape:
+        raise _bad(f"{what}: {name} has shape {tuple(out.shape)}, not {tuple(like.shape)}")
     if dtype is not None and out.dtype != dtype:
-        raise _bad(f"{what}: out is {out.dtype}, out_dtype {dtype}")
-    return out, _float_code(what, "out", out.dtype)
+        raise _bad(f"{what}: {name} is {out.dtype}, out_dtype {dtype}")
+    return out, _rows(what, name, out), _float_code(what, name, out.dtype)
 
 
 def rope(r: Optional[Rope], positions, q, k=None, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, k_out=None,
@@ -799,29 +797,31 @@ def rope(r: Optional[Rope], positions, q, k=None, q_norm=None, k_norm=None, eps:
     what = "rope"
     qr = _rows(what, "q", q)
     T, _, D = q.shape
-    code = _float_code(what, "q", q.dtype)
-    kr = ko = None
-    if k is not None:
-        kr = _rows(what, "k", k, head_dim=D, tokens=T)
-        if k.dtype != q.dtype:
-            raise _bad(f"{what}: q is {q.dtype}, k {k.dtype}")
+    xtype = q.dtype
+    code = _float_code(what, "q", xtype)
     pp, pt = None, I32
     if r is not None:
-        if positions is None or (positions.dtype is not torch.int64 and positions.dtype is not torch.int32) or tuple(positions.shape) != (T,):
+        if positions is None:
+            raise _bad(f"{what}: positions must be int32 or int64 [{T}]")
+        ptype = positions.dtype
+        if (ptype is not torch.int64 and ptype is not torch.int32) or positions.dim() != 1 or positions.shape[0] != T:
             raise _bad(f"{what}: positions must be int32 or int64 [{T}]")
         _usable(what, "positions", positions)
-        pp, pt = positions.data_ptr(), I64 if positions.dtype is torch.int64 else I32
-    qn, kn = _norm(what, "q_norm", q_norm, D), _norm(what, "k_norm", k_norm, D)
-    q_out, ycode = _rows_out(what, q_out, q, out_dtype, stream)
-    qo = _rows(what, "q_out", q_out)
+        pp, pt = positions.data_ptr(), I64 if ptype is torch.int64 else I32
+    kr = ko = kn = None
     if k is not None:
-        k_out, kcode = _rows_out(what, k_out, k, q_out.dtype, stream)
-        ko = _rows(what, "k_out", k_out)
+        kr = _rows(what, "k", k, head_dim=D, tokens=T)
+        if k.dtype is not xtype:
+            raise _bad(f"{what}: q is {xtype}, k {k.dtype}")
+        kn = _norm(what, "k_norm", k_norm, D)
     elif k_out is not None:
         raise _bad(f"{what}: k_out without k")
-    b = ctypes.byref
-    _check(lib().nxq_rope(r.handle if r is not None else None, pp, pt, T, D, b(qr), qn, b(kr) if kr else None, kn, eps, code,
-                          b(qo), b(ko) if ko else None, ycode, _stream_on(stream, q.get_device())))
+    qn = _norm(what, "q_norm", q_norm, D)
+    q_out, qo, ycode = _rows_out(what, "q_out", q_out, q, out_dtype, stream)
+    if k is not None:
+        k_out, ko, _ = _rows_out(what, "k_out", k_out, k, q_out.dtype, stream)
+    _check((_lib or lib()).nxq_rope(r.handle if r is not None else None, pp, pt, T, D, qr, qn, kr, kn, eps, code, qo, ko, ycode,
+                         _stream_on(stream, q.get_device())))
     return q_out if k is None else (q_out, k_out)
 
 
@@ -847,9 +847,10 @@ class KVCache:
         self.keys, self.values, self.order = keys, values, order
         self.pages, self.heads, self.page_size, self.head_dim = keys.shape[0], keys.shape[h], keys.shape[t], keys.shape[3]
         self.dtype, self.device = keys.dtype, keys.device
-        self._c = _Cache(keys.data_ptr(), values.data_ptr(), _FLOATS[keys.dtype], self.pages, self.page_size, self.heads,
+        lib()
+        self._c = _CACHE(keys.data_ptr(), values.data_ptr(), _FLOATS[keys.dtype], self.pages, self.page_size, self.heads,
                          self.head_dim, keys.stride(0), keys.stride(h), keys.stride(t))
-        self._ref = ctypes.byref(self._c)
+        self._scale = self.head_dim ** -0.5
 
 
 def _batch(what: str, q_offsets, kv_lens, block_table):
@@ -858,7 +859,7 @@ def _batch(what: str, q_offsets, kv_lens, block_table):
     if kv_lens.dim() != 1 or kv_lens.dtype is not i32 or kv_lens.shape[0] < 1:
         raise _bad(f"{what}: kv_lens must be int32, one for each sequence")
     S = kv_lens.shape[0]
-    if q_offsets.dtype is not i32 or tuple(q_offsets.shape) != (S + 1,):
+    if q_offsets.dtype is not i32 or q_offsets.dim() != 1 or q_offsets.shape[0] != S + 1:
         raise _bad(f"{what}: q_offsets must be int32 [{S + 1}]")
     if block_table.dtype is not i32 or block_table.dim() != 2 or block_table.shape[0] != S:
         raise _bad(f"{what}: block_table must be int32 [{S}][pages]")
@@ -866,9 +867,10 @@ def _batch(what: str, q_offsets, kv_lens, block_table):
     _usable(what, "q_offsets", q_offsets)
     _on_device(what, "block_table", block_table)
     pages = block_table.shape[1]
-    if pages > 1 and block_table.stride(1) != 1:
+    row, step = block_table.stride()
+    if pages > 1 and step != 1:
         raise _bad(f"{what}: the rows of block_table are not contiguous")
-    return _Batch(S, q_offsets.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), pages)
+    return _BATCH(S, q_offsets.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), row, pages)
 
 
 def kv_append(cache: KVCache, k, v, q_offsets, kv_lens, block_table, rope: Optional[Rope] = None, q=None, q_norm=None,
@@ -877,28 +879,26 @@ def kv_append(cache: KVCache, k, v, q_offsets, kv_lens, block_table, rope: Optio
     the cache at their positions (nxq_kv_append): sequence s has rows q_offsets[s] ..
     q_offsets[s + 1] - 1 and kv_lens[s] tokens with them.  With queries q [T][Hq][D]
     returns them normed and rotated."""
-    _torch or _load_torch()
     what = "kv_append"
-    kr = _rows(what, "k", k, heads=cache.heads, head_dim=cache.head_dim)
-    T, D = k.shape[0], cache.head_dim
+    D = cache.head_dim
+    kr = _rows(what, "k", k, heads=cache.heads, head_dim=D)
+    T, xtype = k.shape[0], k.dtype
     vr = _rows(what, "v", v, heads=cache.heads, head_dim=D, tokens=T)
-    code = _float_code(what, "k", k.dtype)
-    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    code = _float_code(what, "k", xtype)
+    if v.dtype is not xtype or (q is not None and q.dtype is not xtype):
         raise _bad(f"{what}: q, k and v are of different types")
     batch = _batch(what, q_offsets, kv_lens, block_table)
-    qn, kn = _norm(what, "q_norm", q_norm, D), _norm(what, "k_norm", k_norm, D)
-    qr = qo = None
+    kn = _norm(what, "k_norm", k_norm, D)
+    qr = qo = qn = None
     ycode = F32
     if q is not None:
         qr = _rows(what, "q", q, head_dim=D, tokens=T)
-        q_out, ycode = _rows_out(what, q_out, q, out_dtype, stream)
-        qo = _rows(what, "q_out", q_out)
+        qn = _norm(what, "q_norm", q_norm, D)
+        q_out, qo, ycode = _rows_out(what, "q_out", q_out, q, out_dtype, stream)
     elif q_out is not None:
         raise _bad(f"{what}: q_out without q")
-    b = ctypes.byref
-    _check(lib().nxq_kv_append(cache._ref, b(batch), T, b(kr), b(vr), kn, rope.handle if rope is not None else None,
-                               b(qr) if qr else None, qn, eps, code, b(qo) if qo else None, ycode,
-                               _stream_on(stream, k.get_device())))
+    _check(_lib.nxq_kv_append(cache._c, batch, T, kr, vr, kn, rope.handle if rope is not None else None, qr, qn, eps, code, qo,
+                              ycode, _stream_on(stream, k.get_device())))
     return q_out
 
 
@@ -910,21 +910,18 @@ def paged_attention(q, cache: KVCache, q_offsets, kv_lens, block_table, scale: O
     window: keys that a query sees, itself among them (0: all), besides the first
     `sinks`.  max_new: the most new tokens of any sequence, if known.  Rows of `out` that no sequence has
     are left as they are (undefined in a new tensor).  return_lse: (out, lse [T][Hq])."""
-    torch = _torch or _load_torch()
     what = "paged_attention"
     qr = _rows(what, "q", q, head_dim=cache.head_dim)
-    if q.dtype != cache.dtype:
+    if q.dtype is not cache.dtype:
         raise _bad(f"{what}: q is {q.dtype}, the cache {cache.dtype}")
     batch = _batch(what, q_offsets, kv_lens, block_table)
-    out, ycode = _rows_out(what, out, q, out_dtype, stream)
-    oh = _rows(what, "out", out)
-    lse = None
+    out, oh, ycode = _rows_out(what, "out", out, q, out_dtype, stream)
+    lse, lp = None, None
     if return_lse:
-        lse, _ = _output(what, None, tuple(q.shape[:2]), torch.float32, q, stream)
-    b = ctypes.byref
-    _check(lib().nxq_paged_attention(cache._ref, b(batch), b(qr), q.shape[0], cache.head_dim ** -0.5 if scale is None else scale,
-                                     window, sinks, max_new, b(oh), ycode, lse.data_ptr() if return_lse else None,
-                                     _stream_on(stream, q.get_device())))
+        lse, _ = _output(what, None, tuple(q.shape[:2]), _torch.float32, q, stream)
+        lp = lse.data_ptr()
+    _check(_lib.nxq_paged_attention(cache._c, batch, qr, q.shape[0], cache._scale if scale is None else scale, window, sinks,
+                                    max_new, oh, ycode, lp, _stream_on(stream, q.get_device())))
     return (out, lse) if return_lse else out
 
 
