@@ -7,12 +7,13 @@
 // sincospif (error of the fraction 2^-33 turns, about 2e-9 radians; the sum p f_i in fp32 would
 // be off by 0.06 radians at position 10^6).
 //
-// A CTA takes kTokens tokens: it finds their positions (append: their sequence, by a
+// A CTA takes one to eight tokens: it finds their positions (append: their sequence, by a
 // 32-ary search of the offsets, and their page), computes each token's dims / 2 sines and
 // cosines once into shared memory, and then walks the (token, head) pairs of queries,
 // keys and values: 16 elements per lane, as two 8-element vectors that hold whole
 // pairs in either layout, the fewest lanes (a power of two) that cover a head, so the
-// norm's sum is a few shuffles.  Heads, strides or rotated parts that 8-element
+// norm's sum is a few shuffles; the next pair's loads are in flight meanwhile, and
+// the first's before the positions are known.  Heads, strides or rotated parts that 8-element
 // vectors do not fit take one warp per head and one pair per lane.
 //
 // Bound by memory: T (heads in and out) and nothing else of size.
@@ -30,7 +31,7 @@ namespace nxq {
 
 namespace {
 
-constexpr int kRopeThreads = 256, kMaxHeadDim = 512;
+constexpr int kRopeThreads = 256, kMaxHeadDim = 512, kMaxTokensPerCta = kRopeThreads / 32;
 
 struct HeadRows {
     void* dev;
@@ -45,6 +46,7 @@ struct RopeParams {
     const uint64_t* turns;
     HeadRows in[3], out[3];  // queries, keys, values (heads 0: none); out[1], out[2] of an append are the cache
     const float* norm[3];
+    int norm_vec;  // norms are 16-byte aligned
     int x_dtype, y_dtype, c_dtype;
     const void* positions;  // nxq_rope
     int positions_type;
@@ -72,25 +74,6 @@ __device__ __forceinline__ bool store1(void* y, int dt, int64_t i, float v) {
 }
 
 // 8 consecutive elements (16-byte aligned).
-__device__ __forceinline__ void load8(const void* x, int dt, int64_t i, float (&v)[8]) {
-    if (dt == NXQ_F32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
-        const float4 a = q[0], b = q[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
-    }
-    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (dt == NXQ_F16) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[2 * j] = f.x, v[2 * j + 1] = f.y;
-        } else {
-            v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-        }
-    }
-}
 __device__ __forceinline__ bool store8(void* y, int dt, int64_t i, const float (&v)[8]) {
     if (dt == NXQ_F32) {
         float4* q = reinterpret_cast<float4*>(static_cast<float*>(y) + i);
@@ -144,26 +127,101 @@ struct Token {
     int64_t pos, slot;
 };
 
-template <int VEC, bool APPEND>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeParams p, const int tokens) {
+// The two 8-element vectors of a lane, as they lie in memory.
+template <bool X32>
+struct Raw {
+    uint4 a[X32 ? 2 : 1], b[X32 ? 2 : 1];
+};
+template <bool X32>
+__device__ __forceinline__ void fetch8(const void* x, int64_t i, uint4 (&v)[X32 ? 2 : 1]) {
+    if constexpr (X32) {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(x) + i);
+        v[0] = q[0], v[1] = q[1];
+    } else {
+        v[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + i);
+    }
+}
+template <bool X32>
+__device__ __forceinline__ void widen8(const uint4 (&q)[X32 ? 2 : 1], int dt, float (&v)[8]) {
+    if constexpr (X32) {
+        const uint32_t w[8] = {q[0].x, q[0].y, q[0].z, q[0].w, q[1].x, q[1].y, q[1].z, q[1].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    } else {
+        const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (dt == NXQ_F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                v[2 * j] = f.x, v[2 * j + 1] = f.y;
+            } else {
+                v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+            }
+        }
+    }
+}
+
+template <int VEC, bool APPEND, bool X32>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeParams p, const int tokens,
+                                                            const int splits) {
     extern __shared__ float2 sc[];  // [tokens][dims / 2] (cos, sin) * scale
-    __shared__ Token tok[8];
+    __shared__ Token tok[kMaxTokensPerCta];
     overlap_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t t0 = (int64_t)blockIdx.x * tokens;
+    const int cta = blockIdx.x / splits, split = blockIdx.x - cta * splits;  // `splits` CTAs share their tokens' heads
+    const int64_t t0 = (int64_t)cta * tokens;
     const int nt = (int)(p.T - t0 < tokens ? p.T - t0 : tokens);
+
+    // The (token, head) pairs of this thread's group of lanes, and their place in memory.
+    const int heads = p.in[0].heads + p.in[1].heads + p.in[2].heads;
+    const int L = VEC == 8 ? p.lanes : 32, group = threadIdx.x / L, u = threadIdx.x % L, groups = kRopeThreads / L * splits;
+    const unsigned mates = L == 32 ? 0xFFFFFFFFu : ((1u << L) - 1u) << (lane & ~(L - 1));  // lanes of the same head
+    struct Pair {
+        int part, head;
+        int64_t x;   // offset of the head in the part's input
+        int a, b;    // offsets of the lane's two vectors
+        bool turned;
+    };
+    auto pair_at = [&](int t, int h) {
+        Pair q{0, h, 0, 0, 0, false};
+        while (q.head >= p.in[q.part].heads) q.head -= p.in[q.part++].heads;
+        q.x = (t0 + t) * p.in[q.part].token + q.head * p.in[q.part].head;
+        const int dims = q.part == 2 ? 0 : p.dims;  // values stay
+        q.turned = u < dims / 16;
+        if (q.turned && p.layout == NXQ_ROPE_HALF)
+            q.a = 8 * u, q.b = dims / 2 + 8 * u;
+        else
+            q.a = 16 * u, q.b = q.a + 8;
+        return q;
+    };
+    auto fetch = [&](const Pair& q, Raw<X32>& r) {
+        if (q.a < p.D) fetch8<X32>(p.in[q.part].dev, q.x + q.a, r.a);
+        if (q.b < p.D) fetch8<X32>(p.in[q.part].dev, q.x + q.b, r.b);
+    };
+    auto advance = [&](int& t, int& h) {
+        for (h += groups; h >= heads; h -= heads) ++t;
+    };
+    // The first pair's loads go out before its position is known.
+    const int first = split * (kRopeThreads / L) + group;
+    int t = first / heads, h = first % heads;
+    Raw<X32> raw{};
+    Pair q{};
+    if (t < nt) {
+        q = pair_at(t, h);
+        if constexpr (VEC == 8) fetch(q, raw);
+    }
     if (APPEND) {
         if (warp < nt) {
-            const int64_t t = t0 + warp;
-            const int s = find_seq(p.b.q_off, p.b.S, t);
+            const int64_t row = t0 + warp;
+            const int s = find_seq(p.b.q_off, p.b.S, row);
             Token k{0, -1};
             if (s >= 0 && lane == 0) {
                 bool bad;
                 const Seq q = read_seq(p.b, s, p.T, &bad);
                 if (bad) {
                     raise_index(p.status, kIndexSeq);
-                } else if (t < (int64_t)q.q0 + q.n) {
-                    k.pos = (int64_t)q.len - q.n + (t - q.q0);
+                } else if (row < (int64_t)q.q0 + q.n) {
+                    k.pos = (int64_t)q.len - q.n + (row - q.q0);
                     if (k.pos < 0) {
                         raise_index(p.status, kIndexPosition);
                     } else {
@@ -178,106 +236,108 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
             if (lane == 0) tok[warp] = k;
         }
         // Offsets that descend leave no row to meet them: one CTA looks at all.
-        if (blockIdx.x == 0)
+        if (blockIdx.x == gridDim.x - 1)
             for (int s = threadIdx.x; s < p.b.S; s += kRopeThreads) {
                 bool bad;
                 read_seq(p.b, s, p.T, &bad);
                 if (bad) raise_index(p.status, kIndexSeq);
             }
     } else if ((int)threadIdx.x < nt) {
-        const int64_t t = t0 + threadIdx.x;
+        const int64_t row = t0 + threadIdx.x;
         tok[threadIdx.x] = Token{!p.turns                      ? 0
-                                 : p.positions_type == NXQ_I64 ? static_cast<const int64_t*>(p.positions)[t]
-                                                               : static_cast<const int32_t*>(p.positions)[t],
+                                 : p.positions_type == NXQ_I64 ? static_cast<const int64_t*>(p.positions)[row]
+                                                               : static_cast<const int32_t*>(p.positions)[row],
                                  0};
     }
     __syncthreads();
     const int pairs = p.dims / 2;
     for (int i = threadIdx.x; i < nt * pairs; i += kRopeThreads) {
-        const int t = i / pairs, j = i - t * pairs;
-        const uint64_t turn = (uint64_t)tok[t].pos * p.turns[j];
+        const int k = i / pairs, j = i - k * pairs;
+        const uint64_t angle = (uint64_t)tok[k].pos * p.turns[j];
         float s, c;
-        sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
-        sc[i] = make_float2(c * p.scale, s * p.scale);
+        sincospif((float)(int32_t)(angle >> 32) * 0x1p-31f, &s, &c);
+        // (Vectors: pair 8 u + j at [j][u], where the lanes of a head read it without conflicts.)
+        sc[VEC == 8 ? k * pairs + (j & 7) * (pairs >> 3) + (j >> 3) : i] = make_float2(c * p.scale, s * p.scale);
     }
     __syncthreads();
 
-    const int heads = p.in[0].heads + p.in[1].heads + p.in[2].heads;
-    const int L = VEC == 8 ? p.lanes : 32, group = threadIdx.x / L, u = threadIdx.x % L;
-    const unsigned mates = L == 32 ? 0xFFFFFFFFu : ((1u << L) - 1u) << (lane & ~(L - 1));  // lanes of the same head
     const float inv_d = 1.0f / (float)p.D;
     bool over = false;
-    for (int item0 = 0; item0 < nt * heads; item0 += kRopeThreads / L) {
-        const int item = item0 + group;
-        const bool live = item < nt * heads;
-        const int t = live ? item / heads : 0;
-        int h = live ? item - t * heads : 0, part = 0;
-        while (h >= p.in[part].heads) h -= p.in[part++].heads;
-        const bool skip = !live || (APPEND && tok[t].slot < 0);
-        const HeadRows& in = p.in[part];
-        const HeadRows& out = p.out[part];
-        const int64_t row = t0 + t, xi = row * in.token + h * in.head;
-        const bool cached = APPEND && part > 0;
-        const int64_t yi = (cached ? tok[t].slot : row * out.token) + h * out.head;
+    while (t < nt) {
+        int t1 = t, h1 = h;
+        advance(t1, h1);
+        Raw<X32> next{};
+        Pair q1{};
+        if (t1 < nt) {
+            q1 = pair_at(t1, h1);
+            if constexpr (VEC == 8) fetch(q1, next);
+        }
+        const bool skip = APPEND && tok[t].slot < 0;
+        const HeadRows& out = p.out[q.part];
+        const bool cached = APPEND && q.part > 0;
+        const int64_t yi = (cached ? tok[t].slot : (t0 + t) * out.token) + q.head * out.head;
         const int ydt = cached ? p.c_dtype : p.y_dtype;
-        const float* norm = p.norm[part];
-        const int dims = part == 2 ? 0 : p.dims;  // values stay
+        const float* norm = p.norm[q.part];
+        const int dims = q.part == 2 ? 0 : p.dims;
         const float2* cs = sc + t * pairs;
         if constexpr (VEC == 8) {
-            // Two vectors of 8: from a and from b.
-            int a, b;
-            const int turned = dims / 16;
-            if (u < turned && p.layout == NXQ_ROPE_HALF)
-                a = 8 * u, b = dims / 2 + 8 * u;
-            else
-                a = 16 * u, b = a + 8;
-            const bool has_a = !skip && a < p.D, has_b = !skip && b < p.D;
+            const bool has_a = q.a < p.D, has_b = q.b < p.D;
             float va[8], vb[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) va[j] = vb[j] = 0.0f;
-            if (has_a) load8(in.dev, p.x_dtype, xi + a, va);
-            if (has_b) load8(in.dev, p.x_dtype, xi + b, vb);
+            widen8<X32>(raw.a, p.x_dtype, va);
+            widen8<X32>(raw.b, p.x_dtype, vb);
             if (norm) {
                 float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum = fmaf(va[j], va[j], fmaf(vb[j], vb[j], sum));
-                for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
-                const float r = 1.0f / sqrtf(fmaf(sum, inv_d, p.eps));
                 if (has_a)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) va[j] = va[j] * r * norm[a + j];
+                    for (int j = 0; j < 8; ++j) sum = fmaf(va[j], va[j], sum);
                 if (has_b)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) vb[j] = vb[j] * r * norm[b + j];
+                    for (int j = 0; j < 8; ++j) sum = fmaf(vb[j], vb[j], sum);
+                for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
+                const float r = 1.0f / sqrtf(fmaf(sum, inv_d, p.eps));
+                auto scale = [&](float (&v)[8], int at) {
+                    if (p.norm_vec) {
+                        const float4 x = *reinterpret_cast<const float4*>(norm + at), y = *reinterpret_cast<const float4*>(norm + at + 4);
+                        const float w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = v[j] * r * w[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = v[j] * r * norm[at + j];
+                    }
+                };
+                if (has_a) scale(va, q.a);
+                if (has_b) scale(vb, q.b);
             }
-            if (u < turned) {
+            if (q.turned) {
                 if (p.layout == NXQ_ROPE_HALF) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) turn(va[j], vb[j], cs[8 * u + j]);
+                    for (int j = 0; j < 8; ++j) turn(va[j], vb[j], cs[j * (pairs >> 3) + u]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        turn(va[2 * j], va[2 * j + 1], cs[8 * u + j]);
-                        turn(vb[2 * j], vb[2 * j + 1], cs[8 * u + 4 + j]);
+                        turn(va[2 * j], va[2 * j + 1], cs[j * (pairs >> 3) + u]);
+                        turn(vb[2 * j], vb[2 * j + 1], cs[(4 + j) * (pairs >> 3) + u]);
                     }
                 }
             }
-            if (has_a) over |= store8(out.dev, ydt, yi + a, va);
-            if (has_b) over |= store8(out.dev, ydt, yi + b, vb);
-        } else {
-            if (skip) continue;  // (a whole warp)
+            if (has_a && !skip) over |= store8(out.dev, ydt, yi + q.a, va);
+            if (has_b && !skip) over |= store8(out.dev, ydt, yi + q.b, vb);
+            raw = next;
+        } else if (!skip) {  // (a whole warp)
+            const HeadRows& in = p.in[q.part];
             float r = 1.0f;
             if (norm) {
                 float sum = 0.0f;
                 for (int d = u; d < p.D; d += 32) {
-                    const float x = load1(in.dev, p.x_dtype, xi + d);
+                    const float x = load1(in.dev, p.x_dtype, q.x + d);
                     sum = fmaf(x, x, sum);
                 }
                 for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
                 r = 1.0f / sqrtf(fmaf(sum, inv_d, p.eps));
             }
             auto at = [&](int d) {
-                const float x = load1(in.dev, p.x_dtype, xi + d);
+                const float x = load1(in.dev, p.x_dtype, q.x + d);
                 return norm ? x * r * norm[d] : x;
             };
             for (int i = u; i < dims / 2; i += 32) {
@@ -289,6 +349,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
             }
             for (int d = dims + u; d < p.D; d += 32) over |= store1(out.dev, ydt, yi + d, at(d));
         }
+        t = t1, h = h1, q = q1;
     }
     if (over) raise_range(p.status, 4u);
 }
@@ -310,13 +371,20 @@ cudaError_t launch_rope(RopeParams& p, bool append, cudaStream_t st) {
     p.lanes = lanes;
     p.status = context_status();
     // Few tokens: a CTA for each.  Many: several share one, with fewer barriers per byte.
-    const int tokens = p.T <= 4 * (int64_t)context_sm_count() ? 1 : 4;
+    const int64_t sms = context_sm_count();
+    const int tokens = p.T <= 4 * sms ? 1 : p.T <= 32 * sms ? 4 : kMaxTokensPerCta;
+    p.norm_vec = (uintptr_t)p.norm[0] % 16 == 0 && (uintptr_t)p.norm[1] % 16 == 0;
     const size_t smem = (size_t)tokens * (p.dims / 2) * sizeof(float2);
-    const unsigned grid = (unsigned)((p.T + tokens - 1) / tokens);
+    // Fewer tokens than SMs: several CTAs for each, so that no thread has a second head to wait for.
+    const int heads = p.in[0].heads + p.in[1].heads + p.in[2].heads, per = kRopeThreads / (vec ? lanes : 32);
+    const int splits = p.T <= sms ? (heads + per - 1) / per : 1;
+    const unsigned grid = (unsigned)((p.T + tokens - 1) / tokens * splits);
     note_launches(1);
-    auto* kernel = vec ? (append ? rope_kernel<8, true> : rope_kernel<8, false>)
-                       : (append ? rope_kernel<1, true> : rope_kernel<1, false>);
-    return launch_overlapped(kernel, grid, kRopeThreads, smem, st, p, tokens);
+    const bool wide = p.x_dtype == NXQ_F32;
+    auto* kernel = !vec    ? (append ? rope_kernel<1, true, false> : rope_kernel<1, false, false>)
+                   : wide  ? (append ? rope_kernel<8, true, true> : rope_kernel<8, false, true>)
+                           : (append ? rope_kernel<8, true, false> : rope_kernel<8, false, false>);
+    return launch_overlapped(kernel, grid, kRopeThreads, smem, st, p, tokens, splits);
 }
 
 std::mutex g_ropes_mu;
