@@ -175,7 +175,10 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     const int rows = attn_mma_rows(p.D, tc ? kFewRows : most);
     const unsigned runs = attn_mma_grid(p.D);
     size_t bytes = few ? work_bytes(runs, rows, p.D) : 0;
-    if (tc && work_bytes(attn_tc_grid(), attn_tc_rows(), p.D) > bytes) bytes = work_bytes(attn_tc_grid(), attn_tc_rows(), p.D);
+    if (tc) {
+        const size_t b = work_bytes(attn_tc_grid(), attn_tc_rows(), p.D) + attn_tc_grid() * (size_t)attn_tc_rows() * p.D * sizeof(float);
+        if (b > bytes) bytes = b;
+    }
     cudaError_t e = cudaMallocAsync(&p.work, bytes, st);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync (attention workspace)");
     int rc = NXQ_OK;

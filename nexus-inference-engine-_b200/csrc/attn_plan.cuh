@@ -285,7 +285,8 @@ __device__ __forceinline__ bool any_sees(const AttnParams& p, const Item& it, in
     return j <= it.p_hi && (p.window <= 0 || j > it.p_lo - p.window || j < p.sinks);
 }
 
-// The workspace: Cut [runs], then slots [runs][2] of partial results.
+// The workspace: Cut [runs], then slots [runs][2] of partial results (then, tcgen05 kernel, fp32
+// sums [runs][ROWS][D]).
 // A partial result: [ROWS][D] fp32 sums of weights times values, then
 // [ROWS] maxima (in units of c q k) and [ROWS] sums of weights, all relative to the maximum.
 __host__ __device__ inline size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }

@@ -49,6 +49,10 @@ constexpr int kSlots = 5, kAhead = 1;
 constexpr uint32_t kTmemCols = 512;
 constexpr int kColO = 2 * kKeys;  // S_t at kKeys t, O_t at kColO + 128 t
 constexpr float kSlack = 8.0f;
+// tcgen05 sums toward zero: every accumulation loses up to 2^-23 of the sum, on average some 2^-26
+// (2500 of them, 20000 keys with SPLIT: 2.4e-5).  So every kFlush units O_t moves to fp32 sums in
+// the workspace, and begins anew.
+constexpr int flush_units(bool split) { return split ? 8 : 64; }
 constexpr int kChunkBytes = kKeys * 128, kQChunkBytes = kTile * 128;  // 64 elements of a block's keys, of a tile's rows
 
 template <int DP>
@@ -56,7 +60,7 @@ struct Shape {
     static constexpr int kChunks = DP / 64;
     static constexpr int kBlock = kChunks * kChunkBytes;    // keys, or values, of a unit
     static constexpr int kQTile = kChunks * kQChunkBytes;  // queries of a tile
-    static constexpr int kSmem = 1024 + 2 * kQTile + kSlots * kBlock + 512;
+    static constexpr int kSmem = 1024 + 2 * kQTile + kSlots * kBlock + 512 + kRows * 4;
     static_assert(sizeof(PlanSmem) <= kSlots * kBlock, "the plan is made where the ring will be");
     static_assert(kSmem <= 227 * 1024, "");
 };
@@ -168,9 +172,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* const found = abort_flag + 1;     // [slot] its values are not all finite
-    volatile int* const started = found + kSlots;   // [tile] O_t was set before its first product
+    volatile int* const anew = found + kSlots;      // [tile] the unit's product begins O_t anew
     static_assert((3 * kSlots + 2 + 6 + 2 + 1) * 8 + (2 + kSlots + 2) * 4 <= 512, "barrier area too small");
 
+    float* const moved_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [kRows]
     PlanSmem& plan = *reinterpret_cast<PlanSmem*>(ring);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const ptx::WaitCtl ctl{abort_flag, p.status};
@@ -188,7 +193,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::mbar_init(&p_full[t], 4);
             ptx::mbar_init(&o_full[t], 1);
             ptx::mbar_init(&meet[t], t ? 8 : 4);
-            started[t] = 0;
         }
         ptx::mbar_init(drain, 1);
         *abort_flag = 0;
@@ -309,9 +313,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::mma_commit(&s_full[t]);
         };
         // O_t (+)= P_t V, the values in slot i.
-        auto outputs = [&](int t, int i, bool fresh, bool last) {
+        auto outputs = [&](int t, int i, bool last) {
             const uint64_t b = vd + ((uint32_t)(i * Sh::kBlock) >> 4);
-            const uint32_t accumulate = !fresh || started[t] ? 1u : 0u;
+            const uint32_t accumulate = anew[t] ? 0u : 1u;
 #pragma unroll
             for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
 #pragma unroll
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         if (go) {
             int left = w.count;  // units of the piece from unit g on
-            bool two = w.it.rows > kTile, fresh = true;
+            bool two = w.it.rows > kTile;
             // Step g: outputs of unit g and scores of unit g + 1, tile 0's and then tile 1's: a wait for all
             // that a tile's need (different lanes for each barrier) and one go of the issuing lane.
             for (int g = -1; g < units; ++g) {
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = ptx::warp_mbar_wait(bar, ph, ctl, 64))) break;
                 ptx::tc_fence_after();
                 if (lead) {
-                    if (has_o) outputs(0, v.i, fresh, last);
+                    if (has_o) outputs(0, v.i, last);
                     if (has_s) scores(0, k.i);
                 }
                 __syncwarp();
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::tc_fence_after();
                 }
                 if (lead) {
-                    if (had) outputs(1, v.i, fresh, last);
+                    if (had) outputs(1, v.i, last);
                     if (has_o) ptx::mma_commit(&kv_empty[v.i]);
                     if (has_s && two) scores(1, k.i);
                     if (has_s) ptx::mma_commit(&kv_empty[k.i]);
@@ -370,7 +374,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p_ph1 ^= had;
                 q_ph ^= s_fresh;
                 left -= has_o;
-                fresh = s_fresh;
             }
         }
         if (lead) ptx::mma_commit(drain);
@@ -531,6 +534,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool mine = t * kTile + row < w.it.rows;
             const int pos = mine ? w.it.p_lo + tok : -1;
             float m = -INFINITY, l = 0.0f;
+            // What has left O_t, relative to the maximum that was in use then.
+            constexpr int kFlush = flush_units(SPLIT);
+            float& m_moved = moved_m[t * kTile + row];
+            auto moved_to = [&]() {
+                return reinterpret_cast<float*>(static_cast<uint8_t*>(p.work) + cuts_bytes(gridDim.x)) +
+                       2 * (size_t)gridDim.x * part_floats(kRows, p.D) + ((size_t)blockIdx.x * kRows + t * kTile + row) * p.D;
+            };
+            auto factor_moved = [&]() { return m_moved == -INFINITY ? 1.0f : exp2_fast(m_moved - m); };  // (1: zeros, or NaN)
+            auto move = [&](bool first) {
+                const float f = first ? 0.0f : factor_moved();
+                float* const moved = moved_to();
+#pragma unroll 1
+                for (int d = 0; d < DP && d < p.D; d += 8) {
+                    uint32_t o[8];
+                    ptx::tmem_ld8(to + d, o);
+                    ptx::tmem_wait_ld();
+                    if (!mine) continue;
+                    float v[8], x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[k]);
+                    if (!first) {
+                        load_f32x8(moved + d, x);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = fmaf(x[k], f, v[k]);
+                    }
+                    store_f32x8(moved + d, v);
+                }
+                m_moved = m;
+            };
             // Raises the maximum in use of rows whose new one is too far above, and corrects what
             // has been summed in unit u - 1 and before.
             auto raise_to = [&](float now, int u) {
@@ -556,6 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = ptx::warp_mbar_wait(&s_full[t], s_ph, ctl, 69))) break;
                 s_ph ^= 1u;
                 ptx::tc_fence_after();
+                bool fresh = u % kFlush == 0;
+                if (fresh && u > 0) move(u == kFlush);
                 const bool hidden = mixed(p, w.it, j0);
                 if (hidden) {
                     if (!(ok = ptx::warp_mbar_wait(&looked[r.i], (looked_ph >> r.i) & 1u, ctl, 70))) break;
@@ -574,11 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         raise_to(now, u);
                         const float base = m == -INFINITY ? 0.0f : m - kShift;
                         uint8_t* const vs = ring + r.i * Sh::kBlock;
-                        if (u == 0) {
+                        if (fresh) {
 #pragma unroll 1
                             for (int d = 0; d < DP; ++d) ptx::tmem_st1(to + d, 0u);
                             ptx::tmem_wait_st();
-                            if (row == 0) started[t] = 1;
+                            fresh = false;
                         }
 #pragma unroll 1
                         for (int k = 0; k < kKeys; ++k)
@@ -685,6 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (SPLIT) ptx::tmem_st32(ts + 64, z0);
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
+                if (row == 0) anew[t] = fresh;
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&p_full[t]);
                 const float2 a = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
@@ -694,12 +729,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = ptx::warp_mbar_wait(&o_full[t], o_ph, ctl, 73))) break;
             o_ph ^= 1u;
             ptx::tc_fence_after();
-            if (row == 0) started[t] = 0;
             const bool whole = w.whole();
             float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
             const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t token = (int64_t)w.q.q0 + w.it.t0 + tok, at = token * p.o_token + head * p.o_head;
             const bool wide = p.o_vec > 1;
+            const bool has_moved = w.count > kFlush;
+            const float f_moved = has_moved ? factor_moved() : 0.0f;
+            float* const moved = moved_to();
 #pragma unroll 1
             for (int d = 0; d < DP && d < p.D; d += 32) {
                 uint32_t o[32];
@@ -708,7 +745,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!mine) continue;
                 float v[32];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]) * f;
+                for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
+                if (has_moved)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        if (d + 8 * h >= p.D) break;
+                        float x[8];
+                        load_f32x8(moved + d + 8 * h, x);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[8 * h + k] = fmaf(x[k], f_moved, v[8 * h + k]);
+                    }
+#pragma unroll
+                for (int k = 0; k < 32; ++k) v[k] *= f;
                 if (!whole || p.y_dtype == NXQ_F32) {
                     float* const q = whole ? static_cast<float*>(p.out) + at + d : part + (int64_t)(t * kTile + row) * p.D + d;
 #pragma unroll

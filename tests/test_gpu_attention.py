@@ -69,6 +69,18 @@ def test_windows(gpu, window, sinks, D):
 
 
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("S,new,total", [(40, 1, 8000), (2, 700, 20000), (1, 3000, 3000)])
+def test_fp32_outputs_are_exact_enough(gpu, S, new, total, dt):
+    # Relative 2-norm.  A weight as two numbers of the type is off by at most 2^-17 of itself (bf16; half a step of
+    # what half a step leaves); the tensor cores sum toward zero, up to 2^-23 of the sum each, on average an eighth of
+    # that, 128 times before the sums move on (tcgen05) or once per 64 keys (250 times here): 2^-18.
+    p = Paged(gpu, [new] * S, [total] * S, 8, 2, 128, 32, DT[dt], seed=S)
+    got = p.attend(gpu, out_dtype=torch.float32)
+    want, _, _ = p.expected(y=torch.float32)
+    assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -17 + 2.0 ** -18
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("S,total", [(1, 20000), (2, 33333), (40, 900)])
 def test_split_histories(gpu, S, total, dt):
     # Few sequences: every item is cut between many runs and joined.
