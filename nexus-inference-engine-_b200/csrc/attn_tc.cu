@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
 #pragma unroll
                 for (int e = 0; e < kKeys / 16; ++e)
-                    ptx::mma_ts_f16(tmem + kColO + 128 * t, tmem + kKeys * t + 64 * h + 8 * e, b + e * (2048 >> 4), kIdO,
+                    ptx::mma_ts_f16(tmem + kColO + 128 * t, tmem + kKeys * t + 32 * (e >> 1) + 16 * h + 8 * (e & 1), b + e * (2048 >> 4), kIdO,
                                     h || e ? 1u : accumulate);
             if (last) ptx::mma_commit(&o_full[t]);
         };
@@ -646,14 +646,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (warp == kWarpSoft0 && lane == 0) found[r.i] = 0;
                     }
                 }
-                // The scores do not fit the registers beside everything else: 64 keys are read, then the other
-                // 64 and made weights, then the first 64 again.
+                // 64 keys at a time: the first for the maximum, the other for the maximum and the weights, the
+                // first again for the weights, which go over the first half of each 32 scores' columns (what
+                // their rounding leaves, SPLIT, over the other).  Loops of two rather than 128 of
+                // everything: those neither fit the registers nor a scheduler's instruction cache.
                 const int hi = pos - j0, lo = p.window > 0 ? pos - p.window - j0 : -1, sk = p.sinks - j0;
-                auto read = [&](int half, uint32_t (&s)[2][32]) {
+                uint32_t s[2][32];
+                auto read = [&](int half) {
                     ptx::tmem_ld32(ts + 64 * half, s[0]);
                     ptx::tmem_ld32(ts + 64 * half + 32, s[1]);
-                };
-                auto mask = [&](int half, uint32_t (&s)[2][32]) {
+                    ptx::tmem_wait_ld();
                     if (!hidden) return;
                     // 32 keys at a time, against the positions of the warp's rows: most are seen by all.
                     const int low = __reduce_min_sync(0xFFFFFFFFu, hi), high = __reduce_max_sync(0xFFFFFFFFu, lo);
@@ -663,14 +665,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (j + 31 > low)
 #pragma unroll
                             for (int k = 0; k < 32; ++k)
-                                if (j + k > hi) s[i][k] = 0xFF800000u;
+                                if (k > hi - j) s[i][k] = 0xFF800000u;
                         if (j <= high && j + 31 >= sk)
 #pragma unroll
                             for (int k = 0; k < 32; ++k)
-                                if (j + k <= lo && j + k >= sk) s[i][k] = 0xFF800000u;
+                                if (k <= lo - j && k >= sk - j) s[i][k] = 0xFF800000u;
                     }
                 };
-                auto largest = [&](const uint32_t (&s)[2][32]) {
+                float now = -INFINITY;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    read(half);
                     float top[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -679,44 +684,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int k = 2; k < 16; k += 2) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(x[k])), __uint_as_float(x[k + 1]));
                     }
-                    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                };
-                uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
-                // Weights of 64 keys, packed (and what the packing leaves, SPLIT).
-                auto weights = [&](const uint32_t (&s)[2][32], uint64_t c2, uint64_t b2, uint32_t (&y)[32], uint32_t (&z)[SPLIT ? 32 : 1]) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const uint32_t* q = s[k >> 4] + 2 * (k & 15);
-                        float2 x = unpair(fma2(pair(__uint_as_float(q[0]), __uint_as_float(q[1])), c2, b2));
-                        x.x = exp2_fast(x.x);
-                        x.y = exp2_fast(x.y);
-                        sum[k & 3] = add2(sum[k & 3], pair(x.x, x.y));
-                        y[k] = pack2<BF16>(x.x, x.y);
-                        if constexpr (SPLIT) z[k] = pack2<BF16>(x.x - value_of<BF16>(y[k] & 0xFFFFu), x.y - value_of<BF16>(y[k] >> 16));
-                    }
-                };
-                uint32_t s[2][32];
-                read(0, s);
-                ptx::tmem_wait_ld();
-                mask(0, s);
-                float now = largest(s);
-                read(1, s);
-                ptx::tmem_wait_ld();
-                mask(1, s);
-                now = fmaxf(now, largest(s));
+                    now = fmaxf(now, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                }
                 raise_to(now * p.c, u);
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
                 const uint64_t c2 = pair(p.c, p.c), b2 = pair(-base, -base);
-                uint32_t y1[32], z1[SPLIT ? 32 : 1], y0[32], z0[SPLIT ? 32 : 1], s0[2][32];
-                weights(s, c2, b2, y1, z1);
-                read(0, s0);
-                ptx::tmem_wait_ld();
-                ptx::tmem_st32(ts + 32, y1);
-                if constexpr (SPLIT) ptx::tmem_st32(ts + 96, z1);
-                mask(0, s0);
-                weights(s0, c2, b2, y0, z0);
-                ptx::tmem_st32(ts, y0);
-                if constexpr (SPLIT) ptx::tmem_st32(ts + 64, z0);
+                uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll 1
+                for (int half = 1; half >= 0; --half) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t y[16], z[SPLIT ? 16 : 1];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float2 x = unpair(fma2(pair(__uint_as_float(s[i][2 * k]), __uint_as_float(s[i][2 * k + 1])), c2, b2));
+                            x.x = exp2_fast(x.x);
+                            x.y = exp2_fast(x.y);
+                            sum[k & 3] = add2(sum[k & 3], pair(x.x, x.y));
+                            y[k] = pack2<BF16>(x.x, x.y);
+                            if constexpr (SPLIT)
+                                z[k] = pack2<BF16>(x.x - value_of<BF16>(y[k] & 0xFFFFu), x.y - value_of<BF16>(y[k] >> 16));
+                        }
+                        ptx::tmem_st16(ts + 64 * half + 32 * i, y);
+                        if constexpr (SPLIT) ptx::tmem_st16(ts + 64 * half + 32 * i + 16, z);
+                    }
+                    if (half) read(0);
+                }
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
                 if (row == 0) anew[t] = fresh;
