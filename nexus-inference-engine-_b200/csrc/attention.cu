@@ -12,6 +12,10 @@ namespace {
 
 using namespace attn;
 
+// Rows of a sequence and key head up to which the kernel that streams the cache is the
+// quicker one: 24 sequences of 6 new tokens over 3000, 5 query heads per key head (30
+// rows), take 88 us there and 117 on tcgen05; 32 of one over 4000 with 32 heads per key
+// head 124 and 160.
 constexpr int kFewRows = 32;
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 

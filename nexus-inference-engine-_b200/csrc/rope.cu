@@ -441,7 +441,7 @@ int check_heads(const char* what, const nxq_heads* h, int dtype) {
 int check_cache(const nxq_kv_cache* c) {
     if (!c || !c->k_dev || !c->v_dev) return fail(NXQ_ERR_ARG, "null cache");
     if (c->dtype != NXQ_F16 && c->dtype != NXQ_BF16) return fail(NXQ_ERR_ARG, "a cache of type %d (f16 or bf16)", c->dtype);
-    if (c->pages < 0 || c->pages > 0x7FFFFFFF || c->page_size < 1 || c->heads < 1 || c->heads > 65536)
+    if (c->pages < 1 || c->pages > 0x7FFFFFFF || c->page_size < 1 || c->heads < 1 || c->heads > 65536)
         return fail(NXQ_ERR_ARG, "a cache of %lld pages of %d slots, %d heads", (long long)c->pages, c->page_size, c->heads);
     if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8)
         return fail(NXQ_ERR_SHAPE, "a cache with heads of %d elements (a multiple of 8 up to 256)", c->head_dim);

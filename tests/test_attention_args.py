@@ -55,7 +55,7 @@ def test_rope_refuses_shapes():
     assert rope(k=heads(n=2), k_out=heads(n=3)) == SHAPE
 
 
-CACHES = [cache(k=0), cache(v=0), cache(dtype=nxq.F32), cache(pages=-1), cache(page=0), cache(n=0), cache(k=P + 8), cache(v=P + 2),
+CACHES = [cache(k=0), cache(v=0), cache(dtype=nxq.F32), cache(pages=-1), cache(pages=0), cache(page=0), cache(n=0), cache(k=P + 8), cache(v=P + 2),
           cache(page_stride=0), cache(head_stride=4), cache(slot_stride=-64), None]
 BATCHES = [batch(S=0), batch(S=65537), batch(q=0), batch(lens=0), batch(table=0), batch(stride=-1), batch(pages=-1), batch(q=P + 2),
            batch(lens=P + 1), batch(table=P + 3), None]
