@@ -14,6 +14,12 @@
 // of the 1390 cycles in which an SM gets 32 KB.  An item ends with the four warps'
 // states joined in shared memory.
 //
+// 64 sequences of 200 to 8000 keys, 32 heads over 8 (bf16, 1.2 GB): 200 us, 6.1 TB/s, 0.94 of the
+// copy rate; one of 131072 keys, 128 heads over 8: 99.5 us with its join, 83 at that rate.  Two
+// tiles of rows (MT = 2; 24 sequences of 2 to 6 new tokens, 5 heads per key head) take 77 us where the
+// cache's bytes take 41: a unit's chain of products, maximum, exponentials and products with two
+// warps on a scheduler, whose issue slots are 0.29 used; more warps would have too few registers (255).
+//
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8, so most units need no rescaling; an f16 cache's weights get a factor 2^7 on top,
 // which keeps small ones out of f16's subnormals (2^15 at most).  They are rounded to the

@@ -3,28 +3,33 @@
 //
 // A persistent grid of one CTA per SM, each with an equal share of the call's units
 // (attn_plan.cuh): an item is 256 rows of one (sequence, key head) as two tiles of 128, a
-// unit one block of 64 keys with its values, which both tiles share.  Roles:
+// unit one block of 128 keys with its values, which both tiles share.  Roles:
 //   warp 0      producer: keys and values by TMA, one box per page (or part of one) and 64
 //               elements, straight from the scattered pages into 128-byte-swizzled
-//               blocks [64 elements][64 keys]; ten of them in a ring
-//   warps 1, 12 issue tcgen05.mma, one for each tile: S_t = Q_t K^T (fp32 in TMEM), O_t +=
-//               P_t V with P_t from TMEM and V as it lies (its head elements contiguous)
-//   warps 2, 3  bring an item's queries into shared memory, and look through the values of
-//               units that not all rows see for any that is infinite or NaN (they take
-//               part in handing every block back: a wait by phase parity must see every phase)
+//               blocks [64 elements][128 keys]; five of them in a ring
+//   warp 1      issues tcgen05.mma: S_t = Q_t K^T (fp32 in TMEM), O_t += P_t V with P_t
+//               from TMEM and V as it lies (its head elements contiguous); one wait and one
+//               turn of the issuing lane for a tile's outputs and next scores
+//   warp 2      brings an item's queries into shared memory, and looks through the values of
+//               units that not all rows see for any that is infinite or NaN (it takes part
+//               in handing every block back: a wait by phase parity must see every phase)
 //   warps 4-7   softmax of tile 0, 8-11 of tile 1: a thread per row, so a row's maximum
 //               and sum need no shuffles; reads S_t, writes P_t over it, corrects O_t
 //               when the maximum in use is raised, and stores the outputs
-// S_t has two buffers and is issued two units ahead of the O_t += P_t V that needs it,
-// across items as well, so the softmax warps find the next scores there, and the
-// tiles, which nothing but the blocks ties together, take turns at the exponential unit.  (One buffer of 128 keys, each tile's
-// softmax beside the other's products: 4000 cycles for 128 keys, of which 1660 waiting for
-// the tile's own products.)  tcgen05.mma of one thread run in order, so S_t may be issued
-// over a P_t that is still to be read.
+// (Warp 3 only fills the group of four.)  S_t of a unit is issued behind O_t of the unit before
+// - tcgen05.mma of one thread run in order, so it may go over a P_t still to be read - and across
+// items as well.  One tile's softmax runs beside the other's products.
 //
-// Bound by the exponentials and the products alike: 128 keys are 2 x 128 x 128 exponentials,
-// 16 a cycle, 2048 cycles, and, at D = 128, about 2500 cycles of MMA (scores of 64 keys
-// take 128 + 64 rows from shared memory, 48 cycles for 32 of arithmetic).
+// What bounds it (one prompt of 8192 tokens, 32 heads over 8, D = 128: 661 to 692 us, 790 to 830
+// TFLOP/s, 0.48 of the measured GEMM rate; 330 us at that rate): a tile's chain of products, softmax,
+// products.  128 keys take both tiles 2057 cycles of tcgen05.mma (scores are bound by the reads of
+// both operands from shared memory, 64 cycles for 16 elements) and 2048 of the exponential
+// unit (16 a cycle), but some 4000 go by, 1660 of them a tile's wait for its own products; issue
+// slots are a third used.  Tried, and no faster beyond the spread between runs: blocks of 64 keys
+// with two score buffers (651 us, but 48 cycles of MMA for 32 of arithmetic), an issuing warp for
+// each tile (857), tiles that take turns at the exponentials (666), a register split by
+// setmaxnreg (spills), and one to three eighths of the exponentials as a polynomial of degree 4 on
+// the FMA units (665, 675, 707).
 //
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8 (so O_t is seldom read back), f16 ones times 2^7; rounding and SPLIT as in

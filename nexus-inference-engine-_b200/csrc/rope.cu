@@ -16,7 +16,10 @@
 // the first's before the positions are known.  Heads, strides or rotated parts that 8-element
 // vectors do not fit take one warp per head and one pair per lane.
 //
-// Bound by memory: T (heads in and out) and nothing else of size.
+// Bound by memory: T (heads in and out) and nothing else of size.  8192 tokens of 40 heads of
+// 128 (168 MB): 38.0 us, 4.4 TB/s, 0.69 of the copy rate; 16800 tokens of 64 + 8 + 8 into the
+// cache: 144 us, 4.8 TB/s, 0.74 (scattered heads in flight per lane, not instructions: issue slots are
+// 0.70 used).  One token is a launch: 3.5 us.
 #include "attention.h"
 
 #include <cuda_bf16.h>
