@@ -464,7 +464,8 @@ NXQ_API int nxq_rope(nxq_rope_t rope, const void* positions_dev, int positions_t
 /* Appends the keys and values of the batch's new tokens (T rows; k and v have the cache's
  * heads and head_dim) at their positions: keys normed and rotated as by nxq_rope, values
  * as they are, both rounded once to the cache's type.  Their queries are normed
- * and rotated on the way if q is given (q NULL: none).  rope NULL: no rotation.  q_out may be q.
+ * and rotated on the way if q is given (q NULL: none).  rope NULL: no rotation.  q_out may be
+ * q (same strides and type).
  * Two sequences must not append to the same slot.  A new token whose position is
  * negative (more new tokens than kv_lens) is reported and left out. */
 NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, int64_t T, const nxq_heads* k,
@@ -487,7 +488,7 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
  * sequence with more is left out and reported.  Scores, statistics and sums are fp32;
  * probabilities are rounded to the cache's type for the product with the values (where
  * y_dtype is NXQ_F32, to two numbers of that type, with twice its digits).  The same
- * inputs give the same bits on every call. */
+ * inputs give the same bits on every call.  out may be q (same strides and type). */
 NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads* q, int64_t T,
                                 float scale, int64_t window, int64_t sinks, int64_t max_new, const nxq_heads* out,
                                 int y_dtype, float* lse_dev, void* stream);

@@ -219,13 +219,16 @@ NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* b
     int rc;
     if ((rc = check_cache(cache)) || (rc = check_batch(batch, T))) return rc;
     if (!dtype_valid(y_dtype)) return fail(NXQ_ERR_ARG, "bad dtype");
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(NXQ_ERR_ARG, "a scale of %g (finite, above zero)", scale);
+    if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f)) return fail(NXQ_ERR_ARG, "a scale of %g (finite, above zero)", scale);
     if (window < 0 || sinks < 0 || max_new < 0)
         return fail(NXQ_ERR_ARG, "window %lld, sinks %lld, max_new %lld", (long long)window, (long long)sinks, (long long)max_new);
     if (T == 0) return NXQ_OK;
     if ((rc = check_heads("queries", q, cache->dtype)) || (rc = check_heads("output", out, y_dtype))) return rc;
     if (q->heads % cache->heads || q->heads != out->heads)
         return fail(NXQ_ERR_SHAPE, "%d query heads and %d output heads for %d key heads", q->heads, out->heads, cache->heads);
+    if (q->dev == out->dev && (y_dtype != cache->dtype || (T > 1 && q->token_stride != out->token_stride) ||
+                               (q->heads > 1 && q->head_stride != out->head_stride)))
+        return fail(NXQ_ERR_ARG, "in place with another type or other strides");
     if (T * (q->heads / cache->heads) > 0x7FFFFFFF)
         return fail(NXQ_ERR_SHAPE, "%lld rows of %d query heads per key head", (long long)T, q->heads / cache->heads);
     if (!aligned_4(lse_dev)) return fail(NXQ_ERR_ARG, "lse is not aligned to its type");

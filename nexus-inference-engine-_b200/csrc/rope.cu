@@ -3,9 +3,9 @@
 //
 // Pair i of a head at position p is turned by the angle p f_i.  f_i is held as turns
 // per position in units of 2^-64, so p f_i modulo a turn is one 64-bit product, exact
-// at any position; its upper 32 bits, as a signed fraction of a half turn, go to
-// sincospif (error of the fraction 2^-33 turns, about 2e-9 radians; the sum p f_i in fp32 would
-// be off by 0.06 radians at position 10^6).
+// at any position; its upper 32 bits, as a signed fraction of a half turn and rounded to
+// fp32, go to sincospif (off by at most 2^-25 of a half turn, 9e-8 radians; the product p f_i in
+// fp32 would be off by 0.06 radians at position 10^6).
 //
 // A CTA takes one to eight tokens: it finds their positions (append: their sequence, by a
 // 32-ary search of the offsets, and their page), computes each token's dims / 2 sines and
@@ -408,8 +408,13 @@ int take_rope(nxq_rope_t h, int D, RopeParams* p) {
     return NXQ_OK;
 }
 
-int same_heads(const char* what, const nxq_heads* in, const nxq_heads* out) {
+// In place means that a head's output lies where the head lay; other threads may not have read what
+// lies anywhere else.
+int same_heads(const char* what, const nxq_heads* in, const nxq_heads* out, int64_t T, int x_dtype, int y_dtype) {
     if (in->heads != out->heads) return fail(NXQ_ERR_SHAPE, "%s: %d heads in, %d out", what, in->heads, out->heads);
+    if (in->dev == out->dev && (x_dtype != y_dtype || (T > 1 && in->token_stride != out->token_stride) ||
+                                (in->heads > 1 && in->head_stride != out->head_stride)))
+        return fail(NXQ_ERR_ARG, "%s: in place with another type or other strides", what);
     return NXQ_OK;
 }
 
@@ -585,10 +590,10 @@ NXQ_API int nxq_rope(nxq_rope_t rope, const void* positions_dev, int positions_t
     if (T == 0) return NXQ_OK;
     int rc;
     if ((rc = check_heads("queries", q, x_dtype)) || (rc = check_heads("query outputs", q_out, y_dtype)) ||
-        (rc = same_heads("queries", q, q_out)))
+        (rc = same_heads("queries", q, q_out, T, x_dtype, y_dtype)))
         return rc;
     if (k && ((rc = check_heads("keys", k, x_dtype)) || (rc = check_heads("key outputs", k_out, y_dtype)) ||
-              (rc = same_heads("keys", k, k_out))))
+              (rc = same_heads("keys", k, k_out, T, x_dtype, y_dtype))))
         return rc;
     if (!aligned_4(q_norm) || !aligned_4(k_norm)) return fail(NXQ_ERR_ARG, "a norm is not aligned to its type");
     RopeParams p{};
@@ -628,7 +633,7 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
     if (k->heads != cache->heads || v->heads != cache->heads)
         return fail(NXQ_ERR_SHAPE, "%d key and %d value heads for a cache of %d", k->heads, v->heads, cache->heads);
     if (q && ((rc = check_heads("queries", q, x_dtype)) || (rc = check_heads("query outputs", q_out, y_dtype)) ||
-              (rc = same_heads("queries", q, q_out))))
+              (rc = same_heads("queries", q, q_out, T, x_dtype, y_dtype))))
         return rc;
     if (!aligned_4(q_norm) || !aligned_4(k_norm)) return fail(NXQ_ERR_ARG, "a norm is not aligned to its type");
     RopeParams p{};

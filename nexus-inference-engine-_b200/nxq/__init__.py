@@ -909,7 +909,7 @@ def paged_attention(q, cache: KVCache, q_offsets, kv_lens, block_table, scale: O
     q_offsets[s + 1] - 1, the last of its kv_lens[s] tokens.  scale: 1 / sqrt(D) unless given.
     window: keys that a query sees, itself among them (0: all), besides the first
     `sinks`.  max_new: the most new tokens of any sequence, if known.  Rows of `out` that no sequence has
-    are left as they are (undefined in a new tensor).  return_lse: (out, lse [T][Hq])."""
+    are left as they are (undefined in a new tensor).  out may be q.  return_lse: (out, lse [T][Hq])."""
     what = "paged_attention"
     qr = _rows(what, "q", q, head_dim=cache.head_dim)
     if q.dtype is not cache.dtype:

@@ -94,6 +94,25 @@ def test_attention_refuses(kw, code):
     assert attention(**kw) == code
 
 
+Q2 = P + 4096
+
+
+@pytest.mark.parametrize("y,other", [(nxq.F32, {}), (nxq.BF16, {}), (nxq.F16, dict(token=512)), (nxq.F16, dict(head=128))])
+def test_in_place_only_where_each_head_lay(y, other):
+    assert rope(q_out=heads(**other), y=y) == ARG
+    assert rope(q_out=heads(dev=Q2), k=heads(), k_out=heads(**other), y=y) == ARG
+    assert append(q=heads(), q_out=heads(**other), y=y) == ARG
+    assert attention(out=heads(**other), y=y) == ARG
+    # Strides that no address depends on may differ.
+    if not torch.cuda.is_available():
+        assert attention(T=1, out=heads(token=512)) in (STATE, UNSUPPORTED)
+        assert rope(T=1, q_out=heads(token=512)) in (STATE, UNSUPPORTED)
+
+
+def test_scale_beyond_fp32_with_its_logarithm():
+    assert attention(scale=3e38) == ARG
+
+
 def test_nothing_to_do_is_no_error_without_a_gpu():
     assert rope(T=0) == 0 and append(T=0) == 0 and attention(T=0) == 0
 

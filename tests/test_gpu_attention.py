@@ -293,6 +293,25 @@ def test_cache_beyond_32_bits(gpu):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D,dt", [(128, "bf16"), (64, "f16"), (192, "bf16")])
+@pytest.mark.parametrize("new,total", [([1, 1, 1], [4000, 3, 700]), ([5, 3, 6], [900, 3, 700]), ([300, 1, 129], [2100, 50, 129])])
+def test_in_place(gpu, new, total, D, dt):
+    b = Paged(gpu, new, total, 10, 2, D, 16, DT[dt], seed=D)
+    want = b.attend(gpu, out_dtype=DT[dt])
+    q = b.q.clone()
+    for _ in range(3):
+        b.q.copy_(q)
+        assert torch.equal(b.attend(gpu, out=b.q), want)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 200, 4096])
+@pytest.mark.parametrize("new", [1, 140])
+def test_odd_pages(gpu, new, page):
+    b = Paged(gpu, [new, new], [new + 333, new], 4, 2, 64, page, torch.float16, seed=page)
+    b.check(b.attend(gpu, out_dtype=torch.float16))
+    b.check(b.attend(gpu, out_dtype=torch.float16, window=100, sinks=3), window=100, sinks=3)
+
+
 def test_another_stream_and_graphs(gpu):
     # Calls on two streams at once, and two captured graphs replayed in turn and at once.
     a = Paged(gpu, [1] * 8, [3000] * 8, 8, 2, 128, 16, torch.bfloat16, seed=15)
