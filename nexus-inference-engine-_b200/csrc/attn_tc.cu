@@ -95,6 +95,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (BF16) {
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int flat = w.it.r0 + t * kTile + row, tok = (int)((unsigned)flat / (unsigned)p.G);
             const int head = w.head * p.G + (flat - tok * p.G);
             const bool mine = t * kTile + row < w.it.rows;
-            const int pos = mine ? w.it.p_lo + tok : -1;
+            const int pos = mine ? w.it.p_lo + tok : w.it.p_hi;  // (what rows behind the item's see is nobody's)
             float m = -INFINITY, l = 0.0f;
             // What has left O_t, relative to the maximum that was in use then.
             constexpr int kFlush = flush_units(SPLIT);
@@ -651,31 +653,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (warp == kWarpSoft0 && lane == 0) found[r.i] = 0;
                     }
                 }
+                // Scores that a row does not see become -inf in place, 32 keys at a time against the positions of
+                // the warp's rows (most are seen by all or by none), before and apart from the loops below: with the
+                // masks inside them, as long as they are, every unit took 500 cycles more.
+                if (hidden) {
+                    const int hi = pos - j0, lo = p.window > 0 ? pos - p.window - j0 : -1, sk = p.sinks - j0;
+                    const int hi_min = __reduce_min_sync(0xFFFFFFFFu, hi), hi_max = __reduce_max_sync(0xFFFFFFFFu, hi);
+                    const int lo_min = __reduce_min_sync(0xFFFFFFFFu, lo), lo_max = __reduce_max_sync(0xFFFFFFFFu, lo);
+#pragma unroll 1
+                    for (int j = 0; j < kKeys; j += 16) {
+                        if (j + 15 <= hi_min && (j > lo_max || j + 15 < sk)) continue;
+                        const uint32_t seen = below(hi - j + 1) & (~below(lo - j + 1) | below(sk - j));
+                        uint32_t x[16];
+                        if (j <= hi_max && (j + 15 > lo_min || j < sk)) {
+                            ptx::tmem_ld16(ts + j, x);
+                            ptx::tmem_wait_ld();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (!(seen >> k & 1)) x[k] = 0xFF800000u;
+                        ptx::tmem_st16(ts + j, x);
+                    }
+                    ptx::tmem_wait_st();
+                }
                 // 64 keys at a time: the first for the maximum, the other for the maximum and the weights, the
                 // first again for the weights, which go over the first half of each 32 scores' columns (what
                 // their rounding leaves, SPLIT, over the other).  Loops of two rather than 128 of
                 // everything: those neither fit the registers nor a scheduler's instruction cache.
-                const int hi = pos - j0, lo = p.window > 0 ? pos - p.window - j0 : -1, sk = p.sinks - j0;
                 uint32_t s[2][32];
                 auto read = [&](int half) {
                     ptx::tmem_ld32(ts + 64 * half, s[0]);
                     ptx::tmem_ld32(ts + 64 * half + 32, s[1]);
                     ptx::tmem_wait_ld();
-                    if (!hidden) return;
-                    // 32 keys at a time, against the positions of the warp's rows: most are seen by all.
-                    const int low = __reduce_min_sync(0xFFFFFFFFu, hi), high = __reduce_max_sync(0xFFFFFFFFu, lo);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int j = 64 * half + 32 * i;
-                        if (j + 31 > low)
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (k > hi - j) s[i][k] = 0xFF800000u;
-                        if (j <= high && j + 31 >= sk)
-#pragma unroll
-                            for (int k = 0; k < 32; ++k)
-                                if (k <= lo - j && k >= sk - j) s[i][k] = 0xFF800000u;
-                    }
                 };
                 float now = -INFINITY;
 #pragma unroll 1
@@ -724,15 +733,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 l += a.x + a.y;
             }
             if (!ok) break;
-            if (!(ok = ptx::warp_mbar_wait(&o_full[t], o_ph, ctl, 73))) break;
-            o_ph ^= 1u;
-            ptx::tc_fence_after();
             const bool whole = w.whole();
             float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
             const float f = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t token = (int64_t)w.q.q0 + w.it.t0 + tok, at = token * p.o_token + head * p.o_head;
             const bool wide = p.o_vec > 1;
             const bool has_moved = w.count > kFlush;
+            go = w.next(p);  // (while the last products run)
+            if (!(ok = ptx::warp_mbar_wait(&o_full[t], o_ph, ctl, 73))) break;
+            o_ph ^= 1u;
+            ptx::tc_fence_after();
             const float f_moved = has_moved ? factor_moved() : 0.0f;
             float* const moved = moved_to();
 #pragma unroll 1
@@ -803,7 +813,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p.lse[token * ((int64_t)p.Hk * p.G) + head] =
                     l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
             ptx::tc_fence_before();
-            go = w.next(p);
         }
     }
 
