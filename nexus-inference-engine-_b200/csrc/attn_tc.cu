@@ -8,8 +8,8 @@
 //               elements, straight from the scattered pages into 128-byte-swizzled
 //               blocks [64 elements][128 keys]; five of them in a ring
 //   warp 1      issues tcgen05.mma: S_t = Q_t K^T (fp32 in TMEM), O_t += P_t V with P_t
-//               from TMEM and V as it lies (its head elements contiguous); one wait and one
-//               turn of the issuing lane for a tile's outputs and next scores
+//               from TMEM and V as it lies (its head elements contiguous): the products of 64 keys
+//               as soon as their weights are there, then the other 64's and the next scores
 //   warp 2      brings an item's queries into shared memory, and looks through the values of
 //               units that not all rows see for any that is infinite or NaN (it takes part
 //               in handing every block back: a wait by phase parity must see every phase)
@@ -20,16 +20,17 @@
 // - tcgen05.mma of one thread run in order, so it may go over a P_t still to be read - and across
 // items as well.  One tile's softmax runs beside the other's products.
 //
-// What bounds it (one prompt of 8192 tokens, 32 heads over 8, D = 128: 661 to 692 us, 790 to 830
-// TFLOP/s, 0.48 of the measured GEMM rate; 330 us at that rate): a tile's chain of products, softmax,
-// products.  128 keys take both tiles 2057 cycles of tcgen05.mma (scores are bound by the reads of
-// both operands from shared memory, 64 cycles for 16 elements) and 2048 of the exponential
-// unit (16 a cycle), but some 4000 go by, 1660 of them a tile's wait for its own products; issue
-// slots are a third used.  Tried, and no faster beyond the spread between runs: blocks of 64 keys
-// with two score buffers (651 us, but 48 cycles of MMA for 32 of arithmetic), an issuing warp for
-// each tile (857), tiles that take turns at the exponentials (666), a register split by
-// setmaxnreg (spills), and one to three eighths of the exponentials as a polynomial of degree 4 on
-// the FMA units (665, 675, 707).
+// What bounds it (one prompt of 8192 tokens, 32 heads over 8, D = 128: 623 us, 880 TFLOP/s, 0.53 of
+// the measured GEMM rate; 330 us at that rate): a tile's chain of scores, softmax, products.  128
+// keys take both tiles 2057 cycles of tcgen05.mma (scores are bound by the reads of both operands
+// from shared memory, 64 cycles for 16 elements) and 2048 of the exponential unit (16 a
+// cycle), but some 3900 go by: softmax 2200, a tile's wait for its products 1000 to 1400, the
+// rest barriers.  Loops must stay short: code of seldom ways inside them costs every turn
+// its fetch (masks inside the score loops: 740 us; in a pass of their own: 624).  Tried,
+// and no faster beyond the spread between runs: blocks of 64 keys with two score buffers
+// (48 cycles of MMA for 32 of arithmetic), an issuing warp for each tile, tiles that take turns at
+// the exponentials, a register split by setmaxnreg (spills), an eighth to a half of the exponentials as
+// a polynomial of degree 4 on the FMA units, a shorter loop over the outputs.
 //
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8 (so O_t is seldom read back), f16 ones times 2^7; rounding and SPLIT as in
@@ -173,14 +174,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* const q_empty = q_full + 1;
     uint64_t* const s_full = q_empty + 1;  // [tile]
     uint64_t* const p_full = s_full + 2;   // [tile]
-    uint64_t* const o_full = p_full + 2;   // [tile] the item's products are in O_t
+    uint64_t* const p_half = p_full + 2;   // [tile] the weights of the second 64 keys, which come first
+    uint64_t* const o_full = p_half + 2;   // [tile] the item's products are in O_t
     uint64_t* const meet = o_full + 2;     // the softmax warps: of tile 0 alone, of both
     uint64_t* const drain = meet + 2;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* const found = abort_flag + 1;     // [slot] its values are not all finite
     volatile int* const anew = found + kSlots;      // [tile] the unit's product begins O_t anew
-    static_assert((3 * kSlots + 2 + 6 + 2 + 1) * 8 + (2 + kSlots + 2) * 4 <= 512, "barrier area too small");
+    static_assert((3 * kSlots + 2 + 8 + 2 + 1) * 8 + (2 + kSlots + 2) * 4 <= 512, "barrier area too small");
 
     float* const moved_m = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);  // [kRows]
     PlanSmem& plan = *reinterpret_cast<PlanSmem*>(ring);
@@ -198,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(&s_full[t], 1);
             ptx::mbar_init(&p_full[t], 4);
+            ptx::mbar_init(&p_half[t], 4);
             ptx::mbar_init(&o_full[t], 1);
             ptx::mbar_init(&meet[t], t ? 8 : 4);
         }
@@ -320,16 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::mma_commit(&s_full[t]);
         };
         // O_t (+)= P_t V, the values in slot i.
-        auto outputs = [&](int t, int i, bool last) {
+        auto outputs = [&](int t, int i, int half, bool last) {
             const uint64_t b = vd + ((uint32_t)(i * Sh::kBlock) >> 4);
             const uint32_t accumulate = anew[t] ? 0u : 1u;
 #pragma unroll
             for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
 #pragma unroll
-                for (int e = 0; e < kKeys / 16; ++e)
+                for (int e = kKeys / 32 * half; e < kKeys / 32 * (half + 1); ++e)
                     ptx::mma_ts_f16(tmem + kColO + 128 * t, tmem + kKeys * t + 32 * (e >> 1) + 16 * h + 8 * (e & 1), b + e * (2048 >> 4), kIdO,
-                                    h || e ? 1u : accumulate);
-            if (last) ptx::mma_commit(&o_full[t]);
+                                    h || e != kKeys / 32 ? 1u : accumulate);
+            if (last && !half) ptx::mma_commit(&o_full[t]);
         };
         Ring r;
         uint32_t q_ph = 0, p_ph0 = 0, p_ph1 = 0;
@@ -355,22 +358,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t* bar = has_o ? &kv_full[v.i] : &kv_full[k.i];
                 uint32_t ph = has_o ? v.ph : k.ph;
                 const int part = lane & 3;
-                if (part == 1 && has_o) bar = &p_full[0], ph = p_ph0;
-                if (part == 2 && has_s) bar = &kv_full[k.i], ph = k.ph;
-                if (part == 3 && s_fresh) bar = q_full, ph = q_ph;
+                if (part == 1 && has_o) bar = &p_half[0], ph = p_ph0;
+                if (part == 2 && !has_o && s_fresh) bar = q_full, ph = q_ph;
                 if (!(ok = ptx::warp_mbar_wait(bar, ph, ctl, 64))) break;
                 ptx::tc_fence_after();
+                if (has_o) {
+                    if (lead) outputs(0, v.i, 1, last);
+                    __syncwarp();
+                    bar = part == 1 && has_s ? &kv_full[k.i] : part == 2 && s_fresh ? q_full : &p_full[0];
+                    ph = part == 1 && has_s ? k.ph : part == 2 && s_fresh ? q_ph : p_ph0;
+                    if (!(ok = ptx::warp_mbar_wait(bar, ph, ctl, 64))) break;
+                    ptx::tc_fence_after();
+                }
                 if (lead) {
-                    if (has_o) outputs(0, v.i, last);
+                    if (has_o) outputs(0, v.i, 0, last);
                     if (has_s) scores(0, k.i);
                 }
                 __syncwarp();
                 if (had) {
+                    if (!(ok = ptx::warp_mbar_wait(&p_half[1], p_ph1, ctl, 65))) break;
+                    ptx::tc_fence_after();
+                    if (lead) outputs(1, v.i, 1, last);
+                    __syncwarp();
                     if (!(ok = ptx::warp_mbar_wait(&p_full[1], p_ph1, ctl, 65))) break;
                     ptx::tc_fence_after();
                 }
                 if (lead) {
-                    if (had) outputs(1, v.i, last);
+                    if (had) outputs(1, v.i, 0, last);
                     if (has_o) ptx::mma_commit(&kv_empty[v.i]);
                     if (has_s && two) scores(1, k.i);
                     if (has_s) ptx::mma_commit(&kv_empty[k.i]);
@@ -703,6 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 raise_to(now * p.c, u);
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
                 const uint64_t c2 = pair(p.c, p.c), b2 = pair(-base, -base);
+                if (row == 0) anew[t] = fresh;
                 uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
                 for (int half = 1; half >= 0; --half) {
@@ -722,13 +737,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ptx::tmem_st16(ts + 64 * half + 32 * i, y);
                         if constexpr (SPLIT) ptx::tmem_st16(ts + 64 * half + 32 * i + 16, z);
                     }
+                    ptx::tmem_wait_st();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(half ? &p_half[t] : &p_full[t]);
                     if (half) read(0);
                 }
-                ptx::tmem_wait_st();
-                ptx::tc_fence_before();
-                if (row == 0) anew[t] = fresh;
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&p_full[t]);
                 const float2 a = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
                 l += a.x + a.y;
             }
