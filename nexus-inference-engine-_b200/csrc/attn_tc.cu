@@ -585,9 +585,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m_moved = m;
             };
             // Raises the maximum in use of rows whose new one is too far above, and corrects what
-            // has been summed in unit u - 1 and before.
+            // has been summed in unit u - 1 and before.  A warp's rows are raised together, so rows
+            // behind the item's have no say: theirs are scores of whatever lies there.
             auto raise_to = [&](float now, int u) {
-                if (!__any_sync(0xFFFFFFFFu, now > m + kSlack || (m == -INFINITY && now > -INFINITY))) return;
+                if (!__any_sync(0xFFFFFFFFu, mine && (now > m + kSlack || (m == -INFINITY && now > -INFINITY)))) return;
                 const float to_m = fmaxf(m, now), f = m == -INFINITY ? 0.0f : exp2_fast(m - to_m);
                 m = to_m;
                 l *= f;
