@@ -554,7 +554,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int head = w.head * p.G + (flat - tok * p.G);
             const bool mine = t * kTile + row < w.it.rows;
             const int pos = mine ? w.it.p_lo + tok : w.it.p_hi;  // (what rows behind the item's see is nobody's)
-            float m = -INFINITY, l = 0.0f;
+            // The maximum in use.  A warp's rows are raised together, and rows behind the item's must have no
+            // say in that (theirs are scores of whatever lies there): nothing is above +inf.
+            float m = mine ? -INFINITY : INFINITY, l = 0.0f;
             // What has left O_t, relative to the maximum that was in use then.
             constexpr int kFlush = flush_units(SPLIT);
             float& m_moved = moved_m[t * kTile + row];
@@ -585,10 +587,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m_moved = m;
             };
             // Raises the maximum in use of rows whose new one is too far above, and corrects what
-            // has been summed in unit u - 1 and before.  A warp's rows are raised together, so rows
-            // behind the item's have no say: theirs are scores of whatever lies there.
+            // has been summed in unit u - 1 and before.
             auto raise_to = [&](float now, int u) {
-                if (!__any_sync(0xFFFFFFFFu, mine && (now > m + kSlack || (m == -INFINITY && now > -INFINITY)))) return;
+                if (!__any_sync(0xFFFFFFFFu, now > m + kSlack || (m == -INFINITY && now > -INFINITY))) return;
                 const float to_m = fmaxf(m, now), f = m == -INFINITY ? 0.0f : exp2_fast(m - to_m);
                 m = to_m;
                 l *= f;
