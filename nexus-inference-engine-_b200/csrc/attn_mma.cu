@@ -127,7 +127,12 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 }
 
 // MULTI: sequences may have several new tokens, so rows of an item may differ in what they see.
-template <bool BF16, bool SPLIT, bool MULTI, int DP, int MT>
+// FRESH: a unit's products are summed from zero and added to the outputs here.  The tensor
+// cores sum toward zero: 131072 keys in one accumulator fall short by 1.5e-4 (with SPLIT
+// 1.8e-4), by nothing that shows with fresh sums.  It costs nothing where there are registers for it (single tokens, 1.2 GB: 199 us
+// either way), which two tiles of rows over heads of 128 lack: 88 us against 78 (24
+// sequences of 2 to 6 new tokens), so those do it only in long sums (sums_fresh).
+template <bool BF16, bool SPLIT, bool MULTI, bool FRESH, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using Sh = Shape<DP, MT>;
     constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kSlice = Sh::kSlice, kKeys = Sh::kKeys;
@@ -471,21 +476,26 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                 }
             }
 #pragma unroll
-            for (int n = 0; n < kNT / 2; ++n)
+            for (int t = 0; t < kTiles; t += 2) {
+                uint32_t b[kNT / 2][4];  // tile t: keys 0-7, 8-15; tile t + 1: the same
 #pragma unroll
-                for (int t = 0; t < kTiles; t += 2) {
-                    uint32_t b[4];  // tile t: keys 0-7, 8-15; tile t + 1: the same
-                    ldsm4t(vs0 + chunk_at<DP>(16 * n + (lane & 15), t + (lane >> 4)), b);
+                for (int n = 0; n < kNT / 2; ++n) ldsm4t(vs0 + chunk_at<DP>(16 * n + (lane & 15), t + (lane >> 4)), b[n]);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        mma<BF16>(o[mt][t], pa[mt][n], b[0], b[1]);
-                        mma<BF16>(o[mt][t + 1], pa[mt][n], b[2], b[3]);
-                        if constexpr (SPLIT) {
-                            mma<BF16>(o[mt][t], pb[mt][n], b[0], b[1]);
-                            mma<BF16>(o[mt][t + 1], pb[mt][n], b[2], b[3]);
+                for (int mt = 0; mt < MT; ++mt) {
+                    float d[2][4] = {};
+#pragma unroll
+                    for (int n = 0; n < kNT / 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float(&sum)[4] = FRESH ? d[i] : o[mt][t + i];
+                            mma<BF16>(sum, pa[mt][n], b[n][2 * i], b[n][2 * i + 1]);
+                            if constexpr (SPLIT) mma<BF16>(sum, pb[mt][n], b[n][2 * i], b[n][2 * i + 1]);
                         }
-                    }
+                    if constexpr (FRESH)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o[mt][t + (i >> 2)][i & 3] += d[i >> 2][i & 3];
                 }
+            }
             if (++stage == kStages) stage = 0;
         }
 
@@ -607,20 +617,30 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
     copies_wait<0>();
 }
 
+// Whether a kernel's sums are fresh ones anyway.
+template <int DP, int MT, bool SPLIT>
+constexpr bool kAlwaysFresh = SPLIT || MT == 1 || DP <= 64;
+// Whether they must be where there is a choice: a unit (64 keys) is one sum more toward zero, 7.5e-8 of the
+// result each, and together they are to stay below a sixth of half a step of the output's type.  (No
+// sequence is longer than its row of the block table.)
+bool sums_fresh(const AttnParams& p) { return p.b.capacity / 64 > (p.y_dtype == NXQ_F16 ? 1 << 10 : 1 << 13); }
+
 template <int DP, int MT, bool BF16, bool SPLIT>
-auto* kernel_of(bool multi) {
-    return multi ? attn_mma_kernel<BF16, SPLIT, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, false, DP, MT>;
+auto* kernel_of(bool multi, bool fresh) {
+    constexpr bool kF = kAlwaysFresh<DP, MT, SPLIT>;
+    return multi ? (fresh ? attn_mma_kernel<BF16, SPLIT, true, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, true, kF, DP, MT>)
+                 : (fresh ? attn_mma_kernel<BF16, SPLIT, false, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, false, kF, DP, MT>);
 }
 template <int DP, int MT>
-auto* kernel_of(bool bf16, bool split, bool multi) {
-    return bf16 ? (split ? kernel_of<DP, MT, true, true>(multi) : kernel_of<DP, MT, true, false>(multi))
-                : (split ? kernel_of<DP, MT, false, true>(multi) : kernel_of<DP, MT, false, false>(multi));
+auto* kernel_of(bool bf16, bool split, bool multi, bool fresh) {
+    return bf16 ? (split ? kernel_of<DP, MT, true, true>(multi, fresh) : kernel_of<DP, MT, true, false>(multi, fresh))
+                : (split ? kernel_of<DP, MT, false, true>(multi, fresh) : kernel_of<DP, MT, false, false>(multi, fresh));
 }
 
 template <int DP, int MT>
 int set_attr() {
-    for (int i = 0; i < 8; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2, i & 4), cudaFuncAttributeMaxDynamicSharedMemorySize,
+    for (int i = 0; i < 16; ++i) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2, i & 4, i & 8), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                    Shape<DP, MT>::kSmem);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
     }
@@ -635,7 +655,8 @@ unsigned grid_of() {
 
 template <int DP, int MT>
 cudaError_t launch(const AttnParams& p, bool bf16, cudaStream_t st) {
-    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32, p.max_new > 1), grid_of<DP>(), kThreads, Shape<DP, MT>::kSmem, st, p);
+    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32, p.max_new > 1, sums_fresh(p)), grid_of<DP>(), kThreads,
+                            Shape<DP, MT>::kSmem, st, p);
 }
 
 }  // namespace

@@ -30,3 +30,51 @@ def test_rows_behind_a_sequence_do_not_matter(gpu, n, G, dt, D, y):
     gpu.stream_sync()
     p.check(outs[0])
     assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+
+
+# ---- long sums ------------------------------------------------------------------
+
+def long_items(gpu, D, new, dt, y):
+    """(got, want) of 16 sequences of 131072 keys whose values have a mean: as many sequences (of the same pages) as
+    the kernel has runs, so that a run sums a whole history."""
+    t, page, G, Hk = 131072, 64, 4, 1
+    runs = torch.cuda.get_device_properties(0).multi_processor_count * (1 if D > 128 else 2)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    keys = torch.randn((t // page, Hk, page, D), generator=g, device="cuda").to(DT[dt])
+    values = (1 + torch.randn((t // page, Hk, page, D), generator=g, device="cuda")).to(DT[dt])
+    q = torch.randn((runs * new, G, D), generator=g, device="cuda").to(DT[dt])
+    offsets = torch.arange(runs + 1, dtype=torch.int32, device="cuda") * new
+    lens = torch.full((runs,), t, dtype=torch.int32, device="cuda")
+    table = torch.arange(t // page, dtype=torch.int32, device="cuda").expand(runs, -1)
+    got = gpu.paged_attention(q, gpu.KVCache(keys, values), offsets, lens, table, max_new=new, out_dtype=DT[y])
+    gpu.stream_sync()
+    k, v = keys.view(t, D).double(), values.view(t, D).double()
+    see = torch.arange(t, device="cuda") <= torch.arange(t - new, t, device="cuda")[:, None]
+    pick = [s * new + i for s in range(0, 16 * (runs // 16), runs // 16) for i in range(new)]
+    want = []
+    for r in pick:
+        a = (q[r].double() @ k.T * D ** -0.5).masked_fill(~see[r % new], -math.inf)
+        want.append(torch.softmax(a, dim=-1) @ v)
+    return got[pick].double(), torch.stack(want)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("D,new", [(64, 1), (128, 1), (128, 6), (256, 1), (256, 6)])
+def test_long_items_with_fp32_outputs(gpu, D, new, dt):
+    # Relative 2-norm: a weight as two numbers of the type is off by at most 2^-17 of itself.  A unit's
+    # 16 or 32 keys are 2 or 4 sums of the tensor cores from zero on, each short by at most 2^-23 of itself: 2^-21.
+    # The units' sums and those of the weights are up to 4096 roundings to nearest, half a step each at most and of
+    # either sign, 2^6 2^-24 together, and scores (8 at most) are off by some 2^-23 of themselves, 2^-20.
+    # 2^-17 + 2^-21 + 2 2^-18 + 2^-20 at the very most; together in square far below 2^-16.
+    got, want = long_items(gpu, D, new, dt, "f32")
+    err = float((got - want).norm() / want.norm())
+    assert err <= 2.0 ** -16, f"{err:.3g}"
+
+
+@pytest.mark.parametrize("D,new", [(64, 6), (128, 1), (128, 6), (256, 1)])
+def test_long_items_are_not_short(gpu, D, new):
+    # Roundings to nearest have no preferred sign: over 8192 outputs or more, each off by half a step (2^-11) at most, their
+    # mean has a deviation of 2^-11 / 3^0.5 / 8192^0.5 = 3.1e-6, a fifth of 2^-16.  (2048 sums toward zero fell
+    # short by 1.5e-4.)
+    got, want = long_items(gpu, D, new, "f16", "f16")
+    assert abs(float((got.sum() - want.sum()) / want.sum())) <= 2.0 ** -16
