@@ -483,7 +483,8 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
  * query of the batch sees are not read, so freed pages may have any table entry and
  * unused slots any content; a value that only some queries see reaches no other
  * query, be it infinite or NaN (what an infinite value gives to those that see it is
- * infinite, or NaN with an fp32 output).
+ * infinite, or NaN with an fp32 output).  A finite output that f16
+ * does not hold (f16 outputs of a bf16 cache) is infinite, and reported as NXQ_ERR_RANGE.
  * max_new: the most new tokens that any sequence has, where the host knows it (0: T); a
  * sequence with more is left out and reported.  Scores, statistics and sums are fp32;
  * probabilities are rounded to the cache's type for the product with the values (where

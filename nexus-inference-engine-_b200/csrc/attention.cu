@@ -26,7 +26,7 @@ constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 // a row of 128 elements is one load of a warp per piece, eight of them in flight, and a
 // CTA has few rows (one item of 16 rows in 37 pieces: 88 us with 16 rows per CTA,
 // 4.0 with 4).
-template <int ROWS, int PER>
+template <int ROWS, int PER, bool BF16, int Y>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p, const int runs) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     // Piece 0 is in run r's slot 1, piece i in run r + i's slot 0.
     auto part_of = [&](int i) { return slots + (2 * (size_t)(r + i) + (i == 0 ? 1 : 0)) * floats; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool over = false;
 #pragma unroll 1
     for (int k = 0; k < PER; ++k) {
         const int row = ((int)blockIdx.y * PER + k) * kJoinWarps + warp;
@@ -108,16 +109,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
                 const int d = 4 * lane + 128 * h + e;
                 if (d >= p.D) continue;
                 const float v = acc[4 * h + e] * f;
-                if (p.y_dtype == NXQ_F32)
+                if constexpr (Y == NXQ_F32)
                     static_cast<float*>(p.out)[at + d] = v;
-                else if (p.y_dtype == NXQ_BF16)
+                else if constexpr (Y == NXQ_BF16)
                     static_cast<__nv_bfloat16*>(p.out)[at + d] = __float2bfloat16_rn(v);
                 else
-                    static_cast<__half*>(p.out)[at + d] = __float2half_rn(v);
+                    static_cast<__half*>(p.out)[at + d] = __float2half_rn(for_f16<BF16>(v, over));
             }
         if (p.lse && lane == 0)
             p.lse[token * ((int64_t)p.Hk * p.G) + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
     }
+    if (Y == NXQ_F16 && BF16 && over) raise_range(p.status, kRangeAttn);
 }
 
 template <int ROWS, int PER>
@@ -132,7 +134,12 @@ cudaError_t join(const AttnParams& p, unsigned runs, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     note_launches(1);
-    return cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, PER>, p, (int)runs);
+    // (Only f16 outputs depend on the cache's type.)
+    auto* kernel = p.y_dtype == NXQ_F32    ? attn_join_kernel<ROWS, PER, false, NXQ_F32>
+                   : p.y_dtype == NXQ_BF16 ? attn_join_kernel<ROWS, PER, false, NXQ_BF16>
+                   : p.bf16                ? attn_join_kernel<ROWS, PER, true, NXQ_F16>
+                                           : attn_join_kernel<ROWS, PER, false, NXQ_F16>;
+    return cudaLaunchKernelEx(&cfg, kernel, p, (int)runs);
 }
 
 size_t work_bytes(unsigned runs, int rows, int D) { return cuts_bytes(runs) + 2 * runs * part_floats(rows, D) * sizeof(float); }
@@ -151,6 +158,7 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     p.page_stride = cache->page_stride, p.head_stride = cache->head_stride, p.slot_stride = cache->slot_stride;
     p.Hk = cache->heads, p.G = q->heads / cache->heads, p.D = cache->head_dim;
     p.y_dtype = y_dtype;
+    p.bf16 = cache->dtype == NXQ_BF16;
     p.q_vec = (uintptr_t)q->dev % 16 == 0 && q->token_stride % 8 == 0 && q->head_stride % 8 == 0;
     const uintptr_t o_bits = (uintptr_t)out->dev |
                              (uintptr_t)(out->token_stride | out->head_stride) * (y_dtype == NXQ_F32 ? 4 : 2);

@@ -59,6 +59,7 @@ struct AttnParams {
     int64_t page_stride, head_stride, slot_stride;
     int Hk, G, D;      // key heads, query heads per key head, elements of a head
     int y_dtype;
+    int bf16;          // the cache's type
     int q_vec, o_vec;  // rows of q (of the output) are multiples of 16 bytes, at such an address (o_vec 2: of 32)
     int page_shift;    // log2 of the page size, or -1
     int page_align;    // the largest power of two that divides the page size

@@ -132,9 +132,11 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 // 1.8e-4), by nothing that shows with fresh sums.  It costs nothing where there are registers for it (single tokens, 1.2 GB: 199 us
 // either way), which two tiles of rows over heads of 128 lack: 88 us against 78 (24
 // sequences of 2 to 6 new tokens), so those do it only in long sums (sums_fresh).
-template <bool BF16, bool SPLIT, bool MULTI, bool FRESH, int DP, int MT>
+// Y: the outputs' type (SPLIT: fp32).
+template <bool BF16, int Y, bool MULTI, bool FRESH, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kernel(const __grid_constant__ AttnParams p) {
     using Sh = Shape<DP, MT>;
+    constexpr bool SPLIT = Y == NXQ_F32;
     constexpr int kRows = Sh::kRows, kStages = Sh::kStages, kSlice = Sh::kSlice, kKeys = Sh::kKeys;
     constexpr int kChunks = DP / 8, kSteps = DP / 16, kTiles = DP / 8, kNT = kSlice / 8;
     constexpr float kShift = BF16 ? 0.0f : 7.0f;
@@ -563,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
         }
         if (warp == 0) {
             const bool whole = w.whole();
+            bool over = false;
             if (lane == 0) w.cut(Runs(all_units, gridDim.x), blockIdx.x, note);
             float* const part = whole ? nullptr : slots + (2ll * blockIdx.x + w.slot()) * part_floats(kRows, p.D);
 #pragma unroll
@@ -580,12 +583,13 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                         for (int tt = 0; tt < kTiles; ++tt) {
                             const int d = 8 * tt + 2 * (lane & 3);
                             if (d >= p.D) break;
-                            const float x = o[mt][tt][2 * h] * f, y = o[mt][tt][2 * h + 1] * f;
-                            if (p.y_dtype == NXQ_F32) {
+                            float x = o[mt][tt][2 * h] * f, y = o[mt][tt][2 * h + 1] * f;
+                            if constexpr (Y == NXQ_F32) {
                                 float* e = static_cast<float*>(p.out) + at + d;
                                 e[0] = x, e[1] = y;
                             } else {
-                                const uint32_t two = p.y_dtype == NXQ_BF16 ? pack2<true>(x, y) : pack2<false>(x, y);
+                                if constexpr (Y == NXQ_F16) x = for_f16<BF16>(x, over), y = for_f16<BF16>(y, over);
+                                const uint32_t two = pack2<Y == NXQ_BF16>(x, y);
                                 uint16_t* e = static_cast<uint16_t*>(p.out) + at + d;
                                 if (p.o_vec) {
                                     *reinterpret_cast<uint32_t*>(e) = two;
@@ -610,6 +614,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DP, MT>::kCtas) attn_mma_kerne
                         }
                     }
                 }
+            if (Y == NXQ_F16 && BF16 && over) raise_range(p.status, kRangeAttn);
         }
         __syncthreads();  // the join's memory is the next piece's queries'
         go = w.next(p);
@@ -625,25 +630,31 @@ constexpr bool kAlwaysFresh = SPLIT || MT == 1 || DP <= 64;
 // sequence is longer than its row of the block table.)
 bool sums_fresh(const AttnParams& p) { return p.b.capacity / 64 > (p.y_dtype == NXQ_F16 ? 1 << 10 : 1 << 13); }
 
-template <int DP, int MT, bool BF16, bool SPLIT>
+template <int DP, int MT, bool BF16, int Y>
 auto* kernel_of(bool multi, bool fresh) {
-    constexpr bool kF = kAlwaysFresh<DP, MT, SPLIT>;
-    return multi ? (fresh ? attn_mma_kernel<BF16, SPLIT, true, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, true, kF, DP, MT>)
-                 : (fresh ? attn_mma_kernel<BF16, SPLIT, false, true, DP, MT> : attn_mma_kernel<BF16, SPLIT, false, kF, DP, MT>);
+    constexpr bool kF = kAlwaysFresh<DP, MT, Y == NXQ_F32>;
+    return multi ? (fresh ? attn_mma_kernel<BF16, Y, true, true, DP, MT> : attn_mma_kernel<BF16, Y, true, kF, DP, MT>)
+                 : (fresh ? attn_mma_kernel<BF16, Y, false, true, DP, MT> : attn_mma_kernel<BF16, Y, false, kF, DP, MT>);
+}
+template <int DP, int MT, bool BF16>
+auto* kernel_of(int y, bool multi, bool fresh) {
+    return y == NXQ_F32   ? kernel_of<DP, MT, BF16, NXQ_F32>(multi, fresh)
+           : y == NXQ_F16 ? kernel_of<DP, MT, BF16, NXQ_F16>(multi, fresh)
+                          : kernel_of<DP, MT, BF16, NXQ_BF16>(multi, fresh);
 }
 template <int DP, int MT>
-auto* kernel_of(bool bf16, bool split, bool multi, bool fresh) {
-    return bf16 ? (split ? kernel_of<DP, MT, true, true>(multi, fresh) : kernel_of<DP, MT, true, false>(multi, fresh))
-                : (split ? kernel_of<DP, MT, false, true>(multi, fresh) : kernel_of<DP, MT, false, false>(multi, fresh));
+auto* kernel_of(bool bf16, int y, bool multi, bool fresh) {
+    return bf16 ? kernel_of<DP, MT, true>(y, multi, fresh) : kernel_of<DP, MT, false>(y, multi, fresh);
 }
 
 template <int DP, int MT>
 int set_attr() {
-    for (int i = 0; i < 16; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, i & 2, i & 4, i & 8), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   Shape<DP, MT>::kSmem);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
-    }
+    for (const int y : {NXQ_F32, NXQ_F16, NXQ_BF16})
+        for (int i = 0; i < 8; ++i) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP, MT>(i & 1, y, i & 2, i & 4),
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP, MT>::kSmem);
+            if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_mma)");
+        }
     return NXQ_OK;
 }
 
@@ -655,7 +666,7 @@ unsigned grid_of() {
 
 template <int DP, int MT>
 cudaError_t launch(const AttnParams& p, bool bf16, cudaStream_t st) {
-    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype == NXQ_F32, p.max_new > 1, sums_fresh(p)), grid_of<DP>(), kThreads,
+    return launch_overlapped(kernel_of<DP, MT>(bf16, p.y_dtype, p.max_new > 1, sums_fresh(p)), grid_of<DP>(), kThreads,
                             Shape<DP, MT>::kSmem, st, p);
 }
 

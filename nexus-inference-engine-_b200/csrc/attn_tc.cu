@@ -154,11 +154,13 @@ struct Ring {
 // page's slots whether any row sees them or not).
 __device__ __forceinline__ bool mixed(const AttnParams& p, const Item& it, int j0) { return !all_see(p, it, j0, kKeys); }
 
-template <bool BF16, bool SPLIT, int DP>
+// Y: the outputs' type (SPLIT: fp32).
+template <bool BF16, int Y, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap, const int box,
                    const int q_boxes) {
+    constexpr bool SPLIT = Y == NXQ_F32;
     using Sh = Shape<DP>;
     using W = Walk<kRows, kKeys>;
     constexpr float kShift = BF16 ? 0.0f : 7.0f;
@@ -761,6 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::tc_fence_after();
             const float f_moved = has_moved ? factor_moved() : 0.0f;
             float* const moved = moved_to();
+            bool over = false;
 #pragma unroll 1
             for (int d = 0; d < DP && d < p.D; d += 32) {
                 uint32_t o[32];
@@ -781,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                 for (int k = 0; k < 32; ++k) v[k] *= f;
-                if (!whole || p.y_dtype == NXQ_F32) {
+                if (!whole || Y == NXQ_F32) {
                     float* const q = whole ? static_cast<float*>(p.out) + at + d : part + (int64_t)(t * kTile + row) * p.D + d;
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
@@ -793,12 +796,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int k = 0; k < 8; ++k) q[8 * h + k] = v[8 * h + k];
                         }
                     }
-                } else {
+                } else if constexpr (Y != NXQ_F32) {
+                    if constexpr (Y == NXQ_F16)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = for_f16<BF16>(v[k], over);
                     uint16_t* const q = static_cast<uint16_t*>(p.out) + at + d;
                     uint32_t y[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        y[k] = p.y_dtype == NXQ_BF16 ? pack2<true>(v[2 * k], v[2 * k + 1]) : pack2<false>(v[2 * k], v[2 * k + 1]);
+                    for (int k = 0; k < 16; ++k) y[k] = pack2<Y == NXQ_BF16>(v[2 * k], v[2 * k + 1]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (d + 16 * h >= p.D) break;
@@ -821,6 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            if (Y == NXQ_F16 && BF16 && over) raise_range(p.status, kRangeAttn);
             if (mine && !whole) {
                 part[(int64_t)kRows * p.D + t * kTile + row] = m == -INFINITY ? m : m - kShift;
                 part[(int64_t)kRows * p.D + kRows + t * kTile + row] = l;
@@ -841,18 +847,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int DP>
-auto* kernel_of(bool bf16, bool split) {
-    return bf16 ? (split ? attn_tc_kernel<true, true, DP> : attn_tc_kernel<true, false, DP>)
-                : (split ? attn_tc_kernel<false, true, DP> : attn_tc_kernel<false, false, DP>);
+auto* kernel_of(bool bf16, int y) {
+    return y == NXQ_F32   ? (bf16 ? attn_tc_kernel<true, NXQ_F32, DP> : attn_tc_kernel<false, NXQ_F32, DP>)
+           : y == NXQ_F16 ? (bf16 ? attn_tc_kernel<true, NXQ_F16, DP> : attn_tc_kernel<false, NXQ_F16, DP>)
+                          : (bf16 ? attn_tc_kernel<true, NXQ_BF16, DP> : attn_tc_kernel<false, NXQ_BF16, DP>);
 }
 
 template <int DP>
 int set_attr() {
-    for (int i = 0; i < 4; ++i) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP>(i & 1, i & 2), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   Shape<DP>::kSmem);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_tc)");
-    }
+    for (const int y : {NXQ_F32, NXQ_F16, NXQ_BF16})
+        for (const bool bf16 : {false, true}) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel_of<DP>(bf16, y), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       Shape<DP>::kSmem);
+            if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute (attn_tc)");
+        }
     return NXQ_OK;
 }
 
@@ -903,7 +911,7 @@ unsigned attn_tc_grid() { return (unsigned)context_sm_count(); }
 
 int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st) {
     const int box = box_rows(cache->page_size);
-    const bool bf = cache->dtype == NXQ_BF16, split = p.y_dtype == NXQ_F32;
+    const bool bf = cache->dtype == NXQ_BF16;
     CUtensorMap k, v, q{};
     int rc;
     if ((rc = cache_map(&k, cache, cache->k_dev, box)) || (rc = cache_map(&v, cache, cache->v_dev, box))) return rc;
@@ -913,9 +921,9 @@ int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st) {
     const int q_boxes = kTile % p.G == 0 && p.q_vec && p.q_head > 0 && p.q_token > 0 && p.q_head < far && p.q_token < far;
     if (q_boxes && (rc = query_map(&q, p, bf))) return rc;
     note_launches(1);
-    const cudaError_t e = p.D <= 64 ? launch_overlapped(kernel_of<64>(bf, split), attn_tc_grid(), kThreads, Shape<64>::kSmem, st,
+    const cudaError_t e = p.D <= 64 ? launch_overlapped(kernel_of<64>(bf, p.y_dtype), attn_tc_grid(), kThreads, Shape<64>::kSmem, st,
                                                         p, k, v, q, box, q_boxes)
-                                    : launch_overlapped(kernel_of<128>(bf, split), attn_tc_grid(), kThreads, Shape<128>::kSmem,
+                                    : launch_overlapped(kernel_of<128>(bf, p.y_dtype), attn_tc_grid(), kThreads, Shape<128>::kSmem,
                                                         st, p, k, v, q, box, q_boxes);
     if (e != cudaSuccess) return cuda_fail(e, "attention launch (tcgen05)");
     const cudaError_t j = launch_attn_join(p, kRows, attn_tc_grid(), st);

@@ -142,11 +142,12 @@ int report_status(const DeviceStatus& st) {
     if (st.code == kStatusRange) {
         static const char* const what[] = {"?", "the f16 conversion of fp32/bf16 activations",
                                            "the RMSNorm prologue", "the decode GEMV's activation staging",
-                                           "an f16 output of a rotation or an f16 cache"};
+                                           "an f16 output of a rotation or an f16 cache",
+                                           "an f16 output of attention"};
         return fail(NXQ_ERR_RANGE,
                     "an activation of magnitude >= 65520 reached %s: it is outside the f16 range the "
                     "tensor-core kernels compute in (results of that call are not finite)",
-                    what[st.where < 5 ? st.where : 0]);
+                    what[st.where < 6 ? st.where : 0]);
     }
     if (st.code == kStatusIndex) {
         static const char* const what[] = {"an index", "a token id of an embedding lookup",

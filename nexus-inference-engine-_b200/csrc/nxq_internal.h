@@ -82,6 +82,7 @@ __device__ __forceinline__ void raise_host_flag(DeviceStatus* st) {
     }
 }
 // Records a range error (first error wins; `where` names the conversion).
+constexpr unsigned kRangeAttn = 5u;
 __device__ __forceinline__ void raise_range(DeviceStatus* st, unsigned where) {
     if (st && atomicCAS(&st->code, 0u, kStatusRange) == 0u) {
         st->where = where;

@@ -78,3 +78,32 @@ def test_long_items_are_not_short(gpu, D, new):
     # short by 1.5e-4.)
     got, want = long_items(gpu, D, new, "f16", "f16")
     assert abs(float((got.sum() - want.sum()) / want.sum())) <= 2.0 ** -16
+
+
+# ---- f16 outputs that a finite value does not fit ----------------------------------
+
+@pytest.mark.parametrize("Hk,new,total", [(2, [1, 1, 1], [20, 5, 9]), (1, [1], [20000]), (1, [60], [60]), (1, [200], [3000])],
+                         ids=["whole", "joined", "whole-chunk", "joined-chunk"])
+def test_f16_outputs_out_of_range_are_reported(gpu, new, total, Hk):
+    p = Paged(gpu, new, total, 4 * Hk, Hk, 64, 16, torch.bfloat16, seed=1)
+    for v in p.v:
+        v.fill_(70144.0)
+    p.store()
+    for y in (torch.float32, torch.bfloat16):  # (weights and output off by half a step each: 70144 (1 - 2^-8)^2 = 69597)
+        assert bool((p.attend(gpu, out_dtype=y) > 69500).all())
+        gpu.stream_sync()
+    assert bool((p.attend(gpu, out_dtype=torch.float16) == math.inf).all())
+    with pytest.raises(gpu.NxqError) as e:
+        gpu.stream_sync()
+    assert e.value.name == "ERR_RANGE" and "attention" in str(e.value)
+    # 65024 (1 + 2^-8) = 65278 has an f16 form still, and an output of infinite values is no error.
+    for v in (65024.0, math.inf):
+        for x in p.v:
+            x.fill_(v)
+        p.store()
+        got = p.attend(gpu, out_dtype=torch.float16)
+        gpu.stream_sync()
+        if v == math.inf:
+            assert not torch.isfinite(got).any()
+        else:  # half a step of the weights, half a step of the output (16)
+            assert float((got.double() - v).abs().max()) <= v * 2.0 ** -8 + 16
