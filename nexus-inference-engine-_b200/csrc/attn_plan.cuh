@@ -291,10 +291,14 @@ __device__ __forceinline__ bool any_sees(const AttnParams& p, const Item& it, in
 // [ROWS] maxima (in units of c q k) and [ROWS] sums of weights, all relative to the maximum.
 __host__ __device__ inline size_t part_floats(int rows, int D) { return (size_t)rows * (D + 2); }
 
-// An output on its way to f16: a finite one of a bf16 cache that f16 does not hold is reported.
+// An output on its way to f16.  A finite one beyond that type is the largest value where the cache
+// is f16 (the average of f16 values lies among them, but weights rounded to f16 put it up to 2^-11
+// of itself outside), and is reported where it is bf16.
 template <bool BF16>
 __device__ __forceinline__ float for_f16(float x, bool& over) {
-    if constexpr (BF16) over |= f16_overflows(x);
+    if (!f16_overflows(x)) return x;
+    if constexpr (!BF16) return copysignf(65504.0f, x);
+    over = true;
     return x;
 }
 

@@ -107,3 +107,26 @@ def test_f16_outputs_out_of_range_are_reported(gpu, new, total, Hk):
             assert not torch.isfinite(got).any()
         else:  # half a step of the weights, half a step of the output (16)
             assert float((got.double() - v).abs().max()) <= v * 2.0 ** -8 + 16
+
+
+@pytest.mark.parametrize("S,new,total", [(100, 1, 1280), (100, 8, 1280), (40, 64, 4000)])
+def test_largest_f16_values(gpu, S, new, total):
+    # The average of f16 values lies among them.  Here one key has almost all weight, 2^5 to 2^7 times that of the key which
+    # sets the maximum in use, and its weight rounded to f16 may be up to 2^-11 of itself too large: 65536 of
+    # 65504, which has no f16 form.
+    p = Paged(gpu, [new] * S, [total] * S, 8, 2, 64, 16, torch.float16, seed=1)
+    p.q.zero_()
+    p.q[..., 0] = 28 + 12 * torch.rand(p.q.shape[:2], generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    for k, v in zip(p.k, p.v):
+        k.zero_()
+        k[..., 0] = -4
+        k[::128, :, 0] = 1
+        k[7 * 128 + 5, :, 0] = 2
+        v.fill_(65504.0)
+        v[:, 1] = -65504.0
+    p.store()
+    got = p.attend(gpu, out_dtype=torch.float16)
+    gpu.stream_sync()
+    top = got.abs().double()
+    assert bool((top <= 65504).all()) and bool((top >= 65504 * (1 - 2.0 ** -11) - 16).all())
+    assert bool((got[:, :4] > 0).all()) and bool((got[:, 4:] < 0).all())
