@@ -11,8 +11,9 @@
 //               from TMEM and V as it lies (its head elements contiguous): the products of 64 keys
 //               as soon as their weights are there, then the other 64's and the next scores
 //   warp 2      brings an item's queries into shared memory, and looks through the values of
-//               units that not all rows see for any that is infinite or NaN (it takes part
-//               in handing every block back: a wait by phase parity must see every phase)
+//               units that not all rows see for any that is infinite or NaN, and clears those that
+//               no row sees (it takes part in handing every block back: a wait by phase parity
+//               must see every phase)
 //   warps 4-7   softmax of tile 0, 8-11 of tile 1: a thread per row, so a row's maximum
 //               and sum need no shuffles; reads S_t, writes P_t over it, corrects O_t
 //               when the maximum in use is raised, and stores the outputs
@@ -479,14 +480,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (!(ok = ptx::warp_mbar_wait(&kv_full[r.i], r.ph, ctl, 68))) break;
                     if (mixed(p, it, j0)) {
-                        // The largest magnitude, NaN above all, among the keys that not all rows see: behind
-                        // the first row's position, or up to where the last row's window begins.
-                        const int behind = it.p_lo + 1 - j0, before = p.window > 0 ? it.p_hi - p.window + 1 - j0 : 0;
-                        const uint8_t* const block = ring + r.i * Sh::kBlock;
+                        // Keys `behind` .. end - 1 and those before `before`, but for sinks, are seen by some rows only: the
+                        // largest magnitude of their values, NaN above all.  Keys from `end` on and before `gone` are
+                        // seen by none: what lies there (the rest of a page; tokens that left the window) is zeros to
+                        // the product if it is not finite.
+                        const bool windowed = p.window > 0;
+                        const int behind = it.p_lo + 1 - j0, end = it.p_hi + 1 - j0, sinks = windowed ? p.sinks - j0 : 0;
+                        const int gone = windowed ? it.p_lo - p.window + 1 - j0 : 0, before = windowed ? it.p_hi - p.window + 1 - j0 : 0;
+                        uint8_t* const block = ring + r.i * Sh::kBlock;
                         uint32_t big = 0;
+                        bool cleared = false;
                         auto look = [&](int from, int to) {
                             from = from > 0 ? from : 0, to = to < kKeys ? to : kKeys;
-#pragma unroll 4
+                            if (from >= to) return;  // (8 * from would pass 31 bits with 2^30 sinks)
+#pragma unroll 1
                             for (int i = 8 * from + lane; i < 8 * to; i += 32)
 #pragma unroll
                                 for (int c = 0; c < Sh::kChunks; ++c) {
@@ -494,8 +501,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     big = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(big, v.x), v.y), v.z), v.w);
                                 }
                         };
-                        look(0, before);
-                        look(behind > before ? behind : before, kKeys);
+                        look(gone > sinks ? gone : sinks, before);
+                        look(behind, end);
+                        // (Boxes without a key that a row sees are zeros already.)
+                        const int upto = (sinks + box - 1) & -box, whole = gone & -box;
+#pragma unroll 1
+                        for (int part = windowed ? 0 : 2; part < 3; ++part) {
+                            int from = part == 0 ? sinks : part == 1 ? (whole > sinks ? whole : sinks) : end;
+                            int to = part == 0 ? (upto < gone ? upto : gone) : part == 1 ? gone : (end + box - 1) & -box;
+                            from = from > 0 ? from : 0, to = to < kKeys ? to : kKeys;
+                            if (from >= to) continue;
+#pragma unroll 1
+                            for (int i = 8 * from + lane; i < 8 * to; i += 32)
+#pragma unroll
+                                for (int c = 0; c < Sh::kChunks; ++c) {
+                                    uint4* const at = reinterpret_cast<uint4*>(block + c * kChunkBytes + 16 * i);
+                                    const uint4 v = *at;
+                                    const uint32_t top = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(v.x & 0x7FFF7FFFu, v.y), v.z), v.w);
+                                    if (not_finite<BF16>(top & 0xFFFFu) || not_finite<BF16>(top >> 16)) {
+                                        *at = make_uint4(0u, 0u, 0u, 0u);
+                                        cleared = true;
+                                    }
+                                }
+                        }
+                        if (cleared) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         const bool bad = __any_sync(0xFFFFFFFFu, not_finite<BF16>(big & 0xFFFFu) || not_finite<BF16>(big >> 16));
                         if (lane == 0) {
                             if (bad) found[r.i] = 1;

@@ -130,3 +130,51 @@ def test_largest_f16_values(gpu, S, new, total):
     top = got.abs().double()
     assert bool((top <= 65504).all()) and bool((top >= 65504 * (1 - 2.0 ** -11) - 16).all())
     assert bool((got[:, :4] > 0).all()) and bool((got[:, 4:] < 0).all())
+
+
+# ---- what unused slots hold -----------------------------------------------------
+
+def fastest(call):
+    """Least device time of 10 calls, of 7 tries."""
+    best = math.inf
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(10):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64)])
+def test_unused_slots_cost_nothing(gpu, dt, D, window, sinks):
+    # Values that no query sees may be NaN without a look at each of them: neither bits nor time change.
+    n, total = 130, 1985
+    p = Paged(gpu, [n], [total], 32, 8, D, 64, DT[dt], seed=3, fill=0.0)
+    kw = dict(window=window, sinks=sinks, out_dtype=DT[dt])
+    out = torch.empty_like(p.q)
+    want = p.attend(gpu, **kw).clone()
+    clean = fastest(lambda: p.attend(gpu, **kw, out=out))
+    pages, slots = p.places(0)
+    for x in (p.keys, p.values):
+        seen = p.view(x)[pages, slots].clone()
+        x.fill_(math.nan)
+        if window:
+            seen[sinks:total - n - window + 1] = math.nan
+        p.view(x)[pages, slots] = seen
+    full = fastest(lambda: p.attend(gpu, **kw, out=out))
+    gpu.stream_sync()
+    assert torch.equal(out, want)
+    assert full <= 2 * clean, f"{full * 100:.0f} us, {clean * 100:.0f} with zeros in unused slots"
+
+
+@pytest.mark.parametrize("new", [1, 130])
+@pytest.mark.parametrize("sinks", [2**30, 2**40])
+def test_everything_is_a_sink(gpu, sinks, new):
+    p = Paged(gpu, [new], [new + 700], 8, 2, 64, 32, torch.bfloat16, seed=4)
+    want = p.attend(gpu)
+    assert torch.equal(p.attend(gpu, window=50, sinks=sinks), want)
+    gpu.stream_sync()
