@@ -604,16 +604,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t o[8];
                     ptx::tmem_ld8(to + d, o);
                     ptx::tmem_wait_ld();
-                    if (!mine) continue;
-                    float v[8], x[8];
+                    if (mine) {
+                        float v[8], x[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[k]);
-                    if (!first) {
-                        load_f32x8(moved + d, x);
+                        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[k]);
+                        if (!first) {
+                            load_f32x8(moved + d, x);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = fmaf(x[k], f, v[k]);
+                            for (int k = 0; k < 8; ++k) v[k] = fmaf(x[k], f, v[k]);
+                        }
+                        store_f32x8(moved + d, v);
                     }
-                    store_f32x8(moved + d, v);
+                    __syncwarp();
                 }
                 m_moved = m;
             };
@@ -658,6 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float x = __uint_as_float(ptx::tmem_ld1(ts + k));
                             ptx::tmem_wait_ld();
                             if (sees(p, pos, j0 + k)) now = fmaxf(now, x * p.c);
+                            __syncwarp();
                         }
                         raise_to(now, u);
                         const float base = m == -INFINITY ? 0.0f : m - kShift;
@@ -679,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 float x = __uint_as_float(ptx::tmem_ld1(ts + k)), o = __uint_as_float(ptx::tmem_ld1(to + d));
                                 ptx::tmem_wait_ld();
                                 if (sees(p, pos, j0 + k)) o += exp2_fast(fmaf(x, p.c, -base)) * value_of<BF16>(bits);
+                                __syncwarp();
                                 ptx::tmem_st1(to + d, __float_as_uint(o));
                                 ptx::tmem_wait_st();
                             }
@@ -751,6 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
                 const uint64_t c2 = pair(p.c, p.c), b2 = pair(-base, -base);
                 if (row == 0) anew[t] = fresh;
+                __syncwarp();
                 uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll 1
                 for (int half = 1; half >= 0; --half) {
@@ -774,6 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ptx::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(half ? &p_half[t] : &p_full[t]);
+                    __syncwarp();
                     if (half) read(0);
                 }
                 const float2 a = unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
@@ -798,62 +804,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t o[32];
                 ptx::tmem_ld32(to + d, o);
                 ptx::tmem_wait_ld();
-                if (!mine) continue;
-                float v[32];
+                if (mine) {
+                    float v[32];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
-                if (has_moved)
+                    for (int k = 0; k < 32; ++k) v[k] = __uint_as_float(o[k]);
+                    if (has_moved)
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        if (d + 8 * h >= p.D) break;
-                        float x[8];
-                        load_f32x8(moved + d + 8 * h, x);
+                        for (int h = 0; h < 4; ++h) {
+                            if (d + 8 * h >= p.D) break;
+                            float x[8];
+                            load_f32x8(moved + d + 8 * h, x);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[8 * h + k] = fmaf(x[k], f_moved, v[8 * h + k]);
-                    }
-#pragma unroll
-                for (int k = 0; k < 32; ++k) v[k] *= f;
-                if (!whole || Y == NXQ_F32) {
-                    float* const q = whole ? static_cast<float*>(p.out) + at + d : part + (int64_t)(t * kTile + row) * p.D + d;
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        if (d + 8 * h >= p.D) break;
-                        if (!whole || wide) {
-                            store_f32x8(q + 8 * h, v + 8 * h);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) q[8 * h + k] = v[8 * h + k];
+                            for (int k = 0; k < 8; ++k) v[8 * h + k] = fmaf(x[k], f_moved, v[8 * h + k]);
                         }
-                    }
-                } else if constexpr (Y != NXQ_F32) {
-                    if constexpr (Y == NXQ_F16)
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = for_f16<BF16>(v[k], over);
-                    uint16_t* const q = static_cast<uint16_t*>(p.out) + at + d;
-                    uint32_t y[16];
+                    for (int k = 0; k < 32; ++k) v[k] *= f;
+                    if (!whole || Y == NXQ_F32) {
+                        float* const q = whole ? static_cast<float*>(p.out) + at + d : part + (int64_t)(t * kTile + row) * p.D + d;
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) y[k] = pack2<Y == NXQ_BF16>(v[2 * k], v[2 * k + 1]);
+                        for (int h = 0; h < 4; ++h) {
+                            if (d + 8 * h >= p.D) break;
+                            if (!whole || wide) {
+                                store_f32x8(q + 8 * h, v + 8 * h);
+                            } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (d + 16 * h >= p.D) break;
-                        if (wide && d + 16 * h + 16 <= p.D) {
-                            store_f32x8(reinterpret_cast<float*>(q + 16 * h), reinterpret_cast<const float*>(y + 8 * h));
-                        } else {
+                                for (int k = 0; k < 8; ++k) q[8 * h + k] = v[8 * h + k];
+                            }
+                        }
+                    } else if constexpr (Y != NXQ_F32) {
+                        if constexpr (Y == NXQ_F16)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                if (d + 16 * h + 8 * e >= p.D) break;
-                                const uint32_t* z = y + 8 * h + 4 * e;
-                                uint16_t* const to_y = q + 16 * h + 8 * e;
-                                if (p.o_vec) {
-                                    *reinterpret_cast<uint4*>(to_y) = make_uint4(z[0], z[1], z[2], z[3]);
-                                } else {
+                            for (int k = 0; k < 32; ++k) v[k] = for_f16<BF16>(v[k], over);
+                        uint16_t* const q = static_cast<uint16_t*>(p.out) + at + d;
+                        uint32_t y[16];
 #pragma unroll
-                                    for (int k = 0; k < 8; ++k) to_y[k] = (uint16_t)(z[k >> 1] >> (16 * (k & 1)));
+                        for (int k = 0; k < 16; ++k) y[k] = pack2<Y == NXQ_BF16>(v[2 * k], v[2 * k + 1]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (d + 16 * h >= p.D) break;
+                            if (wide && d + 16 * h + 16 <= p.D) {
+                                store_f32x8(reinterpret_cast<float*>(q + 16 * h), reinterpret_cast<const float*>(y + 8 * h));
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    if (d + 16 * h + 8 * e >= p.D) break;
+                                    const uint32_t* z = y + 8 * h + 4 * e;
+                                    uint16_t* const to_y = q + 16 * h + 8 * e;
+                                    if (p.o_vec) {
+                                        *reinterpret_cast<uint4*>(to_y) = make_uint4(z[0], z[1], z[2], z[3]);
+                                    } else {
+#pragma unroll
+                                        for (int k = 0; k < 8; ++k) to_y[k] = (uint16_t)(z[k >> 1] >> (16 * (k & 1)));
+                                    }
                                 }
                             }
                         }
                     }
                 }
+                __syncwarp();
             }
             if (Y == NXQ_F16 && BF16 && over) raise_range(p.status, kRangeAttn);
             if (mine && !whole) {
@@ -863,6 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (mine && whole && p.lse)
                 p.lse[token * ((int64_t)p.Hk * p.G) + head] =
                     l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
+            __syncwarp();
             ptx::tc_fence_before();
         }
     }
