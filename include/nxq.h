@@ -480,10 +480,11 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
  * first `sinks` tokens j < sinks.  window 0: all.  A query that sees no key (its position is
  * negative) gives zeros.  lse_dev (or NULL): [T][heads] fp32, the natural logarithm
  * of sum_j exp(scale * q k_j), -inf where no key is seen.  Keys and values that no
- * query of the batch sees are not read, so freed pages may have any table entry and
- * unused slots any content; a value that only some queries see reaches no other
- * query, be it infinite or NaN (what an infinite value gives to those that see it is
- * infinite, or NaN with an fp32 output).  A finite output that f16
+ * query of the batch sees reach no result, and the table entries of pages without a key
+ * that is seen are not read, so freed pages may have any entry and unused slots any
+ * content; a value that only some queries see reaches no other query, be it
+ * infinite or NaN.  (An infinite value makes the outputs of those that see it infinite or
+ * NaN: NaN where its weight rounds to zero, or the output is fp32.)  A finite output that f16
  * does not hold (f16 outputs of a bf16 cache) is infinite, and reported as NXQ_ERR_RANGE.
  * max_new: the most new tokens that any sequence has, where the host knows it (0: T); a
  * sequence with more is left out and reported.  Scores, statistics and sums are fp32;

@@ -178,3 +178,20 @@ def test_everything_is_a_sink(gpu, sinks, new):
     want = p.attend(gpu)
     assert torch.equal(p.attend(gpu, window=50, sinks=sinks), want)
     gpu.stream_sync()
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 6, 140])
+def test_infinite_values_of_no_weight(gpu, new, dt):
+    # exp(-200) is zero in every type: zero times infinity is NaN.  Whatever it is, it is not finite, and other elements are.
+    p = Paged(gpu, [new], [new + 300], 8, 2, 64, 32, DT[dt], seed=5)
+    p.q[..., 0] = 40
+    p.k[0][3, :, 0] = -40
+    p.v[0][3, :, 7] = math.inf
+    p.store()
+    for y in (DT[dt], torch.float32):
+        got = p.attend(gpu, out_dtype=y)
+        gpu.stream_sync()
+        assert not torch.isfinite(got[..., 7]).any()
+        got[..., 7] = 0
+        assert torch.isfinite(got).all()
