@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -195,3 +196,39 @@ def test_infinite_values_of_no_weight(gpu, new, dt):
         assert not torch.isfinite(got[..., 7]).any()
         got[..., 7] = 0
         assert torch.isfinite(got).all()
+
+
+# ---- many sequences -----------------------------------------------------------------
+
+@pytest.mark.parametrize("S,lengths", [(700, [0, 1, 40, 70]), (1500, [1, 1, 1, 1, 1, 1, 2, 40]), (257, [33, 65])])
+def test_chunks_of_many_sequences(gpu, S, lengths):
+    # More than one chunk of the plan (256), all for the kernel of many rows, or for both.
+    rng = random.Random(S)
+    new = [rng.choice(lengths) for _ in range(S)]
+    p = Paged(gpu, new, [n + rng.randrange(0, 90) for n in new], 8, 2, 64, 16, torch.float16, seed=3)
+    got, lse = p.attend(gpu, return_lse=True)
+    gpu.stream_sync()
+    p.check(got, lse)
+
+
+def test_most_sequences(gpu):
+    # 65536 sequences over the same page, the last of them a chunk.
+    S, n, t, Hk, G, D = 65536, 40, 50, 1, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    keys, values = (torch.randn((1, Hk, 64, D), generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn((S - 1 + n, G, D), generator=g, device="cuda").half()
+    offsets = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    offsets[S] = S - 1 + n
+    lens = torch.full((S,), t, dtype=torch.int32, device="cuda")
+    table = torch.zeros((S, 1), dtype=torch.int32, device="cuda")
+    k, v = keys[0, 0, :t].double(), values[0, 0, :t].double()
+    pos = torch.full((S - 1 + n,), t - 1, device="cuda")
+    pos[S - 1:] = torch.arange(t - n, t, device="cuda")
+    a = q.double() @ k.T * D ** -0.5
+    a.masked_fill_(torch.arange(t, device="cuda") > pos[:, None, None], -math.inf)
+    want = torch.softmax(a, dim=-1) @ v
+    for max_new in (0, n):
+        got = gpu.paged_attention(q, gpu.KVCache(keys, values), offsets, lens, table, max_new=max_new, out_dtype=torch.float32)
+        gpu.stream_sync()
+        # Weights as two f16 numbers (2^-22), scores and sums of 64 in fp32: well below 2^-16 of the values' magnitude.
+        assert float((got.double() - want).abs().max()) <= 2.0 ** -16 * float(v.abs().max())
