@@ -489,7 +489,8 @@ NXQ_API int nxq_kv_append(const nxq_kv_cache* cache, const nxq_kv_batch* batch, 
  * max_new: the most new tokens that any sequence has, where the host knows it (0: T); a
  * sequence with more is left out and reported.  Scores, statistics and sums are fp32;
  * probabilities are rounded to the cache's type for the product with the values (where
- * y_dtype is NXQ_F32, to two numbers of that type, with twice its digits).  The same
+ * y_dtype is NXQ_F32, to two numbers of that type, with twice its digits).  Sums are
+ * divided last: finite values beyond some 2^100 (bf16) may give infinite outputs.  The same
  * inputs give the same bits on every call.  out may be q (same strides and type). */
 NXQ_API int nxq_paged_attention(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads* q, int64_t T,
                                 float scale, int64_t window, int64_t sinks, int64_t max_new, const nxq_heads* out,

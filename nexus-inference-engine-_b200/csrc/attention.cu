@@ -14,8 +14,8 @@ using namespace attn;
 
 // Rows of a sequence and key head up to which the kernel that streams the cache is the
 // quicker one: 24 sequences of 6 new tokens over 3000, 5 query heads per key head (30
-// rows), take 88 us there and 117 on tcgen05; 32 of one over 4000 with 32 heads per key
-// head 124 and 160.
+// rows), take 75 us there and 98 on tcgen05, of 8 new tokens (40 rows) 126 and 98; 32 of
+// one over 4000 with 32 heads over one 30.6 and 31.5.
 constexpr int kFewRows = 32;
 constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32;
 
@@ -178,9 +178,12 @@ int attend(const nxq_kv_cache* cache, const nxq_kv_batch* batch, const nxq_heads
     p.first = 1;
     // Sequences of up to kFewRows rows per key head go to the kernel that streams the cache, those
     // with more to the tcgen05 kernel, each by a launch that leaves the others out.  Where the
-    // average is above kFewRows the tcgen05 kernel takes them all: beside chunks of that
-    // size, single tokens cost it no more than their bytes, and the second pair of
-    // launches would cost some 5 us.
+    // average is above kFewRows the tcgen05 kernel takes them all.  What that gives depends on
+    // the histories, which the host does not know (32 heads over 8 of 128; all on tcgen05, then
+    // both): 64 single tokens over 1000 beside a chunk of 512 105 and 123 us, 32 over 4000 beside
+    // 2048 232 and 235, but 32 over 4000 beside 512 171 and 160, 64 over 4000 beside 600 304 and 259;
+    // on the other side of the rule, 64 over 4000 beside 128 297 and 235, 128 over 2000 beside 256
+    // 299 and 246.
     const int64_t most = (int64_t)p.max_new * p.G;
     const bool tc = most > kFewRows && attn_tc_supported(cache);
     const bool few = !tc || T * p.G <= (int64_t)kFewRows * p.b.S;

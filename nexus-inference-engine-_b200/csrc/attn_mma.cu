@@ -14,17 +14,19 @@
 // of the 1390 cycles in which an SM gets 32 KB.  An item ends with the four warps'
 // states joined in shared memory.
 //
-// 64 sequences of 200 to 8000 keys, 32 heads over 8 (bf16, 1.2 GB): 200 us, 6.1 TB/s, 0.94 of the
-// copy rate; one of 131072 keys, 128 heads over 8: 99.5 us with its join, 83 at that rate.  Two
-// tiles of rows (MT = 2; 24 sequences of 2 to 6 new tokens, 5 heads per key head) take 77 us where the
+// 64 sequences of 200 to 8000 keys, 32 heads over 8 (bf16, 1.2 GB): 199 us, 6.1 TB/s, 0.94 of the
+// copy rate; one of 131072 keys, 128 heads over 8: 101 us with its join, 83 at that rate.  Two
+// tiles of rows (MT = 2; 24 sequences of 2 to 6 new tokens, 5 heads per key head) take 78 us where the
 // cache's bytes take 41: a unit's chain of products, maximum, exponentials and products with two
 // warps on a scheduler, whose issue slots are 0.29 used; more warps would have too few registers (255).
 //
 // Weights are relative to a maximum that is raised only when a score passes it by
 // 2^8, so most units need no rescaling; an f16 cache's weights get a factor 2^7 on top,
 // which keeps small ones out of f16's subnormals (2^15 at most).  They are rounded to the
-// cache's type for the product with the values; where the output is fp32 (SPLIT) what
-// the rounding leaves goes through a second product, so that they keep twice its digits.
+// cache's type for the product with the values, which takes both operands in one type: bf16
+// outputs are off by 0.0023 of their size (their own rounding alone 0.0017), f16 by 0.00029 (0.00021).
+// Where the output is fp32 (SPLIT) what the rounding leaves goes through a second product, so that
+// they keep twice its digits (203 us instead of 199, two tiles of rows 86 instead of 78).
 #include "attn_plan.cuh"
 
 #include <cuda_bf16.h>

@@ -21,7 +21,7 @@
 // - tcgen05.mma of one thread run in order, so it may go over a P_t still to be read - and across
 // items as well.  One tile's softmax runs beside the other's products.
 //
-// What bounds it (one prompt of 8192 tokens, 32 heads over 8, D = 128: 623 us, 880 TFLOP/s, 0.53 of
+// What bounds it (one prompt of 8192 tokens, 32 heads over 8, D = 128: 602 us, 913 TFLOP/s, 0.55 of
 // the measured GEMM rate; 330 us at that rate): a tile's chain of scores, softmax, products.  128
 // keys take both tiles 2057 cycles of tcgen05.mma (scores are bound by the reads of both operands
 // from shared memory, 64 cycles for 16 elements) and 2048 of the exponential unit (16 a
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int boxes = kKeys / box, b = lane % boxes, chunk = lane / boxes;
         const bool mine = chunk < Sh::kChunks;
         // Where a unit's box of this lane lies.  The page entries of keys are asked for a unit
-        // ahead (a load of some 700 cycles, twice a unit, was what the ring waited for: 2235
-        // cycles for 64 keys), and values take the places of their keys two units before.
+        // ahead (a load of some 700 cycles, twice a unit, was what the ring waited for), and values
+        // take the places of their keys two units before.
         struct Place {
             int page, slot, head;
         };
@@ -954,7 +954,8 @@ int attn_tc(const AttnParams& p, const nxq_kv_cache* cache, cudaStream_t st) {
     int rc;
     if ((rc = cache_map(&k, cache, cache->k_dev, box)) || (rc = cache_map(&v, cache, cache->v_dev, box))) return rc;
     // Queries by TMA where tiles hold whole tokens and rows are such that a tensor map takes them; by
-    // 16-byte copies of two warps otherwise (10000 cycles for an item, against 2000).
+    // 16-byte copies of one warp otherwise (4096 tokens, 8 key heads of 128: 4 query heads for each
+    // 207 us, 8 364; 3 280, 5 412, 7 547).
     const int64_t far = (int64_t)1 << 38;
     const int q_boxes = kTile % p.G == 0 && p.q_vec && p.q_head > 0 && p.q_token > 0 && p.q_head < far && p.q_token < far;
     if (q_boxes && (rc = query_map(&q, p, bf))) return rc;
