@@ -671,21 +671,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ptx::tmem_wait_st();
                             fresh = false;
                         }
+                        // (A lane looks at 8 elements; the pieces found are gone through by all.)
+                        constexpr int kPer = DP / 8;
+                        auto piece_at = [&](int i) {
+                            return vs + (i % kPer >> 3) * kChunkBytes + i / kPer * 128 + (((i % kPer & 7) ^ (i / kPer & 7)) << 4);
+                        };
 #pragma unroll 1
-                        for (int k = 0; k < kKeys; ++k)
+                        for (int i = lane; i < kKeys * kPer; i += 32) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(piece_at(i));
+                            const uint32_t top = max_abs2<BF16>(max_abs2<BF16>(max_abs2<BF16>(v.x & 0x7FFF7FFFu, v.y), v.z), v.w);
+                            uint32_t hits = __ballot_sync(0xFFFFFFFFu, not_finite<BF16>(top & 0xFFFFu) || not_finite<BF16>(top >> 16));
 #pragma unroll 1
-                            for (int d = 0; d < DP; ++d) {
-                                const uint32_t bits = *(reinterpret_cast<const uint16_t*>(
-                                                            vs + (d >> 6) * kChunkBytes + k * 128 +
-                                                            ((((d >> 3) & 7) ^ (k & 7)) << 4)) + (d & 7));
-                                if (!not_finite<BF16>(bits)) continue;  // (the same in all lanes)
-                                float x = __uint_as_float(ptx::tmem_ld1(ts + k)), o = __uint_as_float(ptx::tmem_ld1(to + d));
-                                ptx::tmem_wait_ld();
-                                if (sees(p, pos, j0 + k)) o += exp2_fast(fmaf(x, p.c, -base)) * value_of<BF16>(bits);
-                                __syncwarp();
-                                ptx::tmem_st1(to + d, __float_as_uint(o));
-                                ptx::tmem_wait_st();
+                            for (; hits; hits &= hits - 1) {
+                                const int j = i - lane + __ffs(hits) - 1, k = j / kPer;
+#pragma unroll 1
+                                for (int e = 0; e < 8; ++e) {
+                                    const uint32_t bits = reinterpret_cast<const uint16_t*>(piece_at(j))[e];
+                                    if (!not_finite<BF16>(bits)) continue;  // (the same in all lanes)
+                                    const int d = j % kPer * 8 + e;
+                                    float x = __uint_as_float(ptx::tmem_ld1(ts + k)), o = __uint_as_float(ptx::tmem_ld1(to + d));
+                                    ptx::tmem_wait_ld();
+                                    if (sees(p, pos, j0 + k)) o += exp2_fast(fmaf(x, p.c, -base)) * value_of<BF16>(bits);
+                                    __syncwarp();
+                                    ptx::tmem_st1(to + d, __float_as_uint(o));
+                                    ptx::tmem_wait_st();
+                                }
                             }
+                        }
                         // Everybody has read them; then everybody has cleared them.
                         for (int both = 0; both < 2 && ok; ++both) {
                             __syncwarp();

@@ -172,6 +172,24 @@ def test_unused_slots_cost_nothing(gpu, dt, D, window, sinks):
     assert full <= 2 * clean, f"{full * 100:.0f} us, {clean * 100:.0f} with zeros in unused slots"
 
 
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64)])
+def test_one_infinite_value_costs_little(gpu, dt, D):
+    # One that some queries see and others do not: it is added where it is seen, without a look at each other element by all.
+    p = Paged(gpu, [130], [1985], 32, 8, D, 64, DT[dt], seed=3, fill=0.0)
+    out = torch.empty_like(p.q)
+    call = lambda: p.attend(gpu, out_dtype=DT[dt], out=out)  # noqa: E731
+    call()
+    want, clean = out.clone(), fastest(call)
+    p.v[0][1980, 0, 3] = math.inf
+    p.store()
+    one = fastest(call)
+    gpu.stream_sync()
+    seen = torch.zeros_like(out, dtype=torch.bool)
+    seen[1980 - 1855:, :4, 3] = True  # positions from 1980 on, the query heads of key head 0
+    assert bool((out[seen] == math.inf).all()) and torch.equal(out[~seen], want[~seen])
+    assert one <= 2 * clean, f"{one * 100:.0f} us, {clean * 100:.0f} without"
+
+
 @pytest.mark.parametrize("new", [1, 130])
 @pytest.mark.parametrize("sinks", [2**30, 2**40])
 def test_everything_is_a_sink(gpu, sinks, new):
